@@ -1,0 +1,154 @@
+// Rows of bfloat16 or float32 to microscaled 4-bit floating point and back (formats: mxfp4.cuh).
+//
+// For a block of 32 neighbours with largest size a: e = floor(log2 a) - 2, code = the nearest E2M1 value to x 2^-e (ties to the
+// even code, above 6 to 6), scale = 2^e.  The power of two makes the multiplication exact, so a code is one rounding away from x.
+// Four lanes share a block (eight elements each: a 16-byte load of bfloat16), sixteen lanes the four blocks whose scales are one
+// word; two exchanges find a block's largest.  The kernels are bound by bytes.
+#include "mxfp4.cuh"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+__device__ __forceinline__ void load_8(const bf16* p, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ void load_8(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+// Sixteen lanes a group of four blocks.  Groups behind a row's end, up to the next 256 elements, write zero scales.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                           long long rows, long long width, long long tiles_of_a_row) {
+    pdl_wait();
+    const long long groups = rows * tiles_of_a_row;
+    const int lane16 = threadIdx.x & 15;
+    const long long step = (long long)gridDim.x * (THREADS / 16);
+    for (long long first = (long long)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 5) * 2; first < groups; first += step) {      // the same for a whole warp
+        const long long group = first + ((threadIdx.x >> 4) & 1);
+        const long long row = group / tiles_of_a_row, q = group - row * tiles_of_a_row;
+        const long long column = q * 128 + lane16 * 8;
+        const bool inside = group < groups && column < width;
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (inside) load_8(x + row * width + column, v);
+        uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        const uint32_t byte = mx_scale_byte(largest);
+        const uint32_t word = byte == 255u ? 0u : mx_encode_8(v, mx_inverse(byte));
+        if (inside) *reinterpret_cast<uint32_t*>(codes + row * (width >> 1) + (column >> 1)) = word;
+        uint32_t four = byte << (8 * (lane16 >> 2));
+        four |= __shfl_xor_sync(0xffffffffu, four, 4);
+        four |= __shfl_xor_sync(0xffffffffu, four, 8);
+        if (lane16 == 0 && group < groups) *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(row, q, tiles_of_a_row)) = four;
+    }
+}
+
+__device__ __forceinline__ void store_8(bf16* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);       // exact: one bit of mantissa
+        w[i] = *reinterpret_cast<uint32_t*>(&pair);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
+                                                             long long rows, long long width, long long tiles_of_a_row) {
+    pdl_wait();
+    const long long eighths = width >> 3, total = rows * eighths;
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
+        const long long row = i / eighths, part = i - row * eighths;
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + i * 4);
+        const float scale = mx_scale(scales[mx_scale_offset(row, part >> 4, tiles_of_a_row) + ((part >> 2) & 3)]);
+        uint32_t h[4];
+        mx_decode_8(word, h);
+        float v[8];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const float2 pair = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
+            v[2 * p] = pair.x * scale;
+            v[2 * p + 1] = pair.y * scale;
+        }
+        store_8(out + i * 8, v);
+    }
+}
+
+// Scales [rows, width / 32] of a matrix from elsewhere into tiles; the codes of blocks whose scale is not a number become 0 (a
+// product that multiplies a block's sum by its scale then gives NaN however it does so).
+__global__ void __launch_bounds__(THREADS) scales_to_tiles_kernel(const uint8_t* __restrict__ plain, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                  long long rows, long long width, long long tiles_of_a_row) {
+    pdl_wait();
+    const long long total = rows * tiles_of_a_row * 4, blocks = width / MX_BLOCK;
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
+        const long long row = i / (tiles_of_a_row * 4), block = i - row * tiles_of_a_row * 4;
+        const uint8_t byte = block < blocks ? plain[row * blocks + block] : (uint8_t)0;
+        if (byte == 255) *reinterpret_cast<uint4*>(codes + row * (width >> 1) + block * 16) = make_uint4(0, 0, 0, 0);
+        scales[mx_scale_offset(row, block >> 2, tiles_of_a_row) + (block & 3)] = byte;
+    }
+}
+
+// Blocks of a launch over `items` threads of work: loops over them where that is more than 16 blocks an SM.
+int blocks_for(long long items) {
+    const long long want = (items + THREADS - 1) / THREADS, most = (long long)mrs_sm_count() * 64;
+    return (int)(want < most ? want : most);
+}
+
+bool bad_sizes(long long rows, long long width) { return rows < 0 || width <= 0 || width % MX_BLOCK || rows > (1ll << 40) / width; }
+
+}  // namespace
+
+// Bytes of a matrix's scales.
+MRS_EXPORT long long mrs_mxfp4_scale_bytes(long long rows, long long width) {
+    return (rows + 127) / 128 * mx_tiles_of_a_row(width) * MX_TILE_BYTES;
+}
+
+// x [rows, width] bfloat16 (`is_bf16`) or float32 on 16-byte boundaries, width a multiple of 32.
+MRS_EXPORT int mrs_mxfp4_quantise(int is_bf16, const void* x, void* codes, void* scales, long long rows, long long width, void* stream) {
+    if (rows == 0) return 0;
+    if (bad_sizes(rows, width) || !x || !codes || !scales || (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
+    const long long tiles = mx_tiles_of_a_row(width);
+    const int blocks = blocks_for(rows * tiles * 16);
+    if (is_bf16) MRS_LAUNCH(quantise_kernel<bf16>, blocks, THREADS, 0, stream, (const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles);
+    else MRS_LAUNCH(quantise_kernel<float>, blocks, THREADS, 0, stream, (const float*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles);
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+MRS_EXPORT int mrs_mxfp4_dequantise(int is_bf16, const void* codes, const void* scales, void* out, long long rows, long long width, void* stream) {
+    if (rows == 0) return 0;
+    if (bad_sizes(rows, width) || !out || !codes || !scales || (((uintptr_t)out | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
+    const long long tiles = mx_tiles_of_a_row(width);
+    const int blocks = blocks_for(rows * (width >> 3));
+    if (is_bf16) MRS_LAUNCH(dequantise_kernel<bf16>, blocks, THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (bf16*)out, rows, width, tiles);
+    else MRS_LAUNCH(dequantise_kernel<float>, blocks, THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (float*)out, rows, width, tiles);
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+MRS_EXPORT int mrs_mxfp4_scales_to_tiles(const void* plain, void* codes, void* scales, long long rows, long long width, void* stream) {
+    if (rows == 0) return 0;
+    if (bad_sizes(rows, width) || !plain || !codes || !scales || (((uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
+    const long long tiles = mx_tiles_of_a_row(width);
+    MRS_LAUNCH(scales_to_tiles_kernel, blocks_for(rows * tiles * 4), THREADS, 0, stream, (const uint8_t*)plain, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles);
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+MRS_EXPORT const char* mrs_mxfp4_error_string(int code) {
+    if (code == MRS_BAD_ARGUMENT) return "arguments outside what the kernels support (width no multiple of 32, unaligned base)";
+    return cudaGetErrorString((cudaError_t)code);
+}

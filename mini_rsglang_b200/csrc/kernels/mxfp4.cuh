@@ -1,0 +1,57 @@
+// Matrices in microscaled 4-bit floating point (MXFP4): how they lie in memory, and the steps between floats and codes.
+//
+// An element is a sign, two bits of exponent and one of mantissa (E2M1): 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, codes
+// 0 to 7 and 8 to 15.  32 neighbours of a row (a block) share a power of two, held as its exponent + 127 in a byte (E8M0; 255: not
+// a number).  In memory:
+//   codes   [rows, width / 2]: element 2 j of a row in the low half of byte j, element 2 j + 1 in the high half; what bulk tensor
+//           copies bring into shared memory as the tensor cores read it;
+//   scales  in tiles of 128 rows x 4 blocks (512 bytes), the tile of rows r / 128 and blocks b / 4 at tile index
+//           (r / 128) * tiles_of_a_row + b / 4, a scale at byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of its tile: what
+//           one copy into tensor memory takes.  A row of tiles covers a multiple of 256 elements; scales behind the row's end are 0.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+constexpr int MX_BLOCK = 32;
+constexpr int MX_TILE_BYTES = 512;
+
+__host__ __device__ __forceinline__ long long mx_tiles_of_a_row(long long width) { return (width + 255) / 256 * 2; }
+
+// Where the four scales of row r's blocks 4 q to 4 q + 3 lie.
+__device__ __forceinline__ size_t mx_scale_offset(long long r, long long q, long long tiles_of_a_row) {
+    return (size_t)((r >> 7) * tiles_of_a_row + q) * MX_TILE_BYTES + (size_t)((r & 31) * 16 + ((r >> 5) & 3) * 4);
+}
+
+// Eight floats times `inverse` to eight codes, the first in the lowest bits: to the nearest, ties to the even code, above 6 to 6.
+__device__ __forceinline__ uint32_t mx_encode_8(const float (&v)[8], float inverse) {
+    uint32_t r;
+    asm("{\n .reg .b8 b0, b1, b2, b3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+        " mov.b32 %0, {b0, b1, b2, b3};\n}"
+        : "=r"(r)
+        : "f"(v[0] * inverse), "f"(v[1] * inverse), "f"(v[2] * inverse), "f"(v[3] * inverse), "f"(v[4] * inverse),
+          "f"(v[5] * inverse), "f"(v[6] * inverse), "f"(v[7] * inverse));
+    return r;
+}
+
+// Eight codes to four pairs of halfs (exact).
+__device__ __forceinline__ void mx_decode_8(uint32_t codes, uint32_t (&h)[4]) {
+    asm("{\n .reg .b8 b0, b1, b2, b3;\n mov.b32 {b0, b1, b2, b3}, %4;\n"
+        " cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n cvt.rn.f16x2.e2m1x2 %2, b2;\n cvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(codes));
+}
+
+// The scale byte of a block whose largest element has the float bits `largest` (sign off): its exponent less two, so that the
+// largest lies in [4, 8) times the scale; 255 for a block with an infinity or NaN in it.
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t largest) {
+    const int exponent = (int)(largest >> 23);
+    return exponent == 255 ? 255u : (uint32_t)max(exponent - 2, 0);
+}
+// 2^-(byte - 127) for bytes up to 252: an ordinary number.
+__device__ __forceinline__ float mx_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^(byte - 127); byte 0 is under the ordinary numbers, byte 255 gives NaN.
+__device__ __forceinline__ float mx_scale(uint32_t byte) {
+    return __uint_as_float(byte == 255u ? 0x7FC00000u : max(byte << 23, 0x00400000u));
+}

@@ -2557,3 +2557,191 @@ def concat_rows(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> None:
     _need(out, None, "joined rows", (rows, 2 * width))
     _check(rotary_library().mrs_concat_rows(_is_bf16(out.dtype), a.data_ptr(), b.data_ptr(), out.data_ptr(), rows, width, _stream()),
            "concat_rows")
+
+
+# ------------------------------------------------------------------------------------------------
+# matrices in microscaled 4-bit floating point (MXFP4)
+# ------------------------------------------------------------------------------------------------
+MXFP4_BLOCK = 32               # neighbours of a row that share a power of two
+_MXFP4_SIGNATURES = {
+    "mrs_mxfp4_quantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
+    "mrs_mxfp4_dequantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
+    "mrs_mxfp4_scales_to_tiles": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
+    "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+}
+_mxfp4_lib = None
+
+
+def mxfp4_library() -> ctypes.CDLL:
+    global _mxfp4_lib
+    if _mxfp4_lib is None:
+        if not torch.cuda.is_available():
+            raise BackendError("no CUDA device: the engine has no CPU path")
+        from .csrc.build import mxfp4_kernel_library
+
+        lib = _typed(mxfp4_kernel_library(), _MXFP4_SIGNATURES)
+        lib.mrs_mxfp4_error_string.argtypes = [_c_int]
+        lib.mrs_mxfp4_error_string.restype = ctypes.c_char_p
+        _mxfp4_lib = lib
+    return _mxfp4_lib
+
+
+def _mxfp4_check(code: int, what: str) -> None:
+    global launch_count
+    launch_count += 1
+    if code != 0:
+        raise BackendError(f"{what}: {mxfp4_library().mrs_mxfp4_error_string(code).decode()} (code {code})")
+
+
+class _OnDevice:
+    """The tensor's device as the current one, where it is not (`torch.cuda.device` costs microseconds)."""
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+class Mxfp4:
+    """A matrix [rows, width] in microscaled 4-bit floating point: for every element a sign, two bits of exponent and one of
+    mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), for every 32 neighbours of a row one power of two.
+
+    `codes` uint8 [rows, width / 2] (element 2 j in the low half of byte j), `scales` uint8 in the tiles that the tensor
+    cores read (`csrc/kernels/mxfp4.cuh`).  `settled`: the matrix was there before anything that is still queued, and nothing
+    writes it any more, so that a product may fetch it while the kernel before still runs."""
+
+    __slots__ = ("codes", "scales", "rows", "width", "settled")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int, settled: bool = False):
+        self.codes, self.scales, self.rows, self.width, self.settled = codes, scales, int(rows), int(width), bool(settled)
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return (self.rows, self.width)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def bytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def block_scales(self) -> torch.Tensor:
+        """The scale bytes [rows, width / 32]: a block's exponent + 127, 255 for a block that is not a number."""
+        row_tiles, tiles = -(-self.rows // 128), -(-self.width // 256) * 2
+        by_row = self.scales.view(row_tiles, tiles, 32, 4, 4).permute(0, 3, 2, 1, 4)   # row tile, row / 32, row % 32, tile, block
+        return by_row.reshape(row_tiles * 128, tiles * 4)[:self.rows, :self.width // MXFP4_BLOCK].contiguous()
+
+
+def _mxfp4_sizes(rows: int, width: int, what: str) -> None:
+    if width <= 0 or width % MXFP4_BLOCK:
+        raise InvalidRequest(f"{what}: rows of {width} elements; 4-bit rows are whole blocks of {MXFP4_BLOCK}")
+    if rows >= 1 << 31 or width > 1 << 30:
+        raise InvalidRequest(f"{what}: {rows} rows of {width} elements are too many")
+
+
+def _mxfp4_buffers(rows: int, width: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    tile_rows, tiles = -(-rows // 128), -(-width // 256) * 2
+    return (torch.empty((rows, width // 2), dtype=torch.uint8, device=device),
+            torch.empty(tile_rows * tiles * 512, dtype=torch.uint8, device=device))
+
+
+def _mxfp4_aligned(t: torch.Tensor, what: str) -> None:
+    if t.data_ptr() % 16:
+        raise InvalidRequest(f"{what}: the tensor does not begin on a 16-byte boundary")
+
+
+def mxfp4_quantise(x: torch.Tensor) -> Mxfp4:
+    """Rows [rows, width] of bfloat16 or float32 in 4 bits.  A block's power of two is 2^(floor(log2 of its largest size) - 2); an
+    element becomes the nearest of the fifteen values times it, ties to the one with an even code, sizes above 6 times it 6 times it.
+    A block with an infinity or NaN in it is not a number as a whole."""
+    if x.dim() != 2:
+        raise InvalidRequest(f"mxfp4_quantise: a tensor of {x.dim()} dimensions, expected rows")
+    rows, width = x.shape
+    _mxfp4_sizes(rows, width, "mxfp4_quantise")
+    bf16 = _is_bf16(x.dtype)
+    _need(x, None, "mxfp4_quantise input")
+    _mxfp4_aligned(x, "mxfp4_quantise input")
+    with _OnDevice(x.device):
+        codes, scales = _mxfp4_buffers(rows, width, x.device)
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, width, _stream()),
+                     "mxfp4_quantise")
+    return Mxfp4(codes, scales, rows, width)
+
+
+def mxfp4_dequantise(matrix: Mxfp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """What the codes stand for, in bfloat16 or float32 (both hold every such value; a scale beyond 2^125 may make bfloat16's and
+    float32's infinity of a code)."""
+    bf16 = _is_bf16(dtype)
+    _need(matrix.codes, torch.uint8, "mxfp4 codes", (matrix.rows, matrix.width // 2))
+    with _OnDevice(matrix.device):
+        out = torch.empty((matrix.rows, matrix.width), dtype=dtype, device=matrix.device)
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_dequantise(bf16, matrix.codes.data_ptr(), matrix.scales.data_ptr(), out.data_ptr(),
+                                                          matrix.rows, matrix.width, _stream()), "mxfp4_dequantise")
+    return out
+
+
+def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
+    """A matrix from elsewhere: `codes` uint8 [rows, width / 2], element 2 j of a row in the low half of byte j, and `scales` uint8
+    [rows, width / 32], a block's exponent + 127 (255: not a number).  Takes copies, and waits until they are made: what it
+    returns is settled.  For loading weights, not for a step."""
+    if codes.dim() != 2 or scales.dim() != 2:
+        raise InvalidRequest("mxfp4_matrix: codes [rows, width / 2] and scales [rows, width / 32]")
+    rows, width = codes.shape[0], 2 * codes.shape[1]
+    _mxfp4_sizes(rows, width, "mxfp4_matrix")
+    if tuple(scales.shape) != (rows, width // MXFP4_BLOCK):
+        raise InvalidRequest(f"mxfp4_matrix: scales {tuple(scales.shape)}, expected {(rows, width // MXFP4_BLOCK)}")
+    _need(codes, torch.uint8, "mxfp4 codes")
+    _need(scales, torch.uint8, "mxfp4 scales")
+    if scales.device != codes.device:
+        raise InvalidRequest("mxfp4_matrix: codes and scales are on different devices")
+    with _OnDevice(codes.device):
+        _, tiles = _mxfp4_buffers(rows, width, codes.device)
+        held = codes.clone()
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_scales_to_tiles(scales.data_ptr(), held.data_ptr(), tiles.data_ptr(), rows, width, _stream()),
+                     "mxfp4_matrix")
+        torch.cuda.current_stream().synchronize()
+    return Mxfp4(held, tiles, rows, width, settled=True)
+
+
+def mxfp4_few_rows_ranges(n: int, k: int, sms: int) -> tuple[int, int]:
+    """(ranges of K within a CTA, CTAs of a cluster) of the product for few rows with [n, k] weights.  A warp takes 16 rows and one
+    range; the ranges are as many as give every SM 16 warps, a stage of 256 elements at least each."""
+    stages, groups = -(-k // 256), -(-n // 16)
+    parts = cluster = 1
+    while parts < 8 and groups * parts < 16 * sms and parts * 2 <= stages:
+        parts *= 2
+    while cluster < 8 and groups * parts * cluster < 16 * sms and parts * cluster * 2 <= stages:
+        cluster *= 2
+    return parts, cluster
+
+
+def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool = False, ranges: tuple[int, int] | None = None) -> None:
+    """out[M, N] = x[M, K] . weight[N, K]^T; x bfloat16, weight in 4 bits, sums in float32, `out` bfloat16 or float32.  With `quantise`
+    x's rows are brought to 4 bits first, as `mxfp4_quantise` does."""
+    if x.dim() != 2 or out.dim() != 2:
+        raise InvalidRequest("mxfp4_gemm: input and output are rows")
+    m, k = x.shape
+    n = weight.rows
+    if k != weight.width:
+        raise InvalidRequest(f"mxfp4_gemm: rows of {k} elements against weights of {weight.width}")
+    if out.dtype not in (torch.bfloat16, torch.float32):
+        raise InvalidRequest("mxfp4_gemm: out must be bfloat16 or float32")
+    _need(x, torch.bfloat16, "mxfp4_gemm input")
+    _need(out, None, "mxfp4_gemm out", (m, n))
+    if x.device != weight.device or out.device != x.device:
+        raise InvalidRequest("mxfp4_gemm: input, weights and output are on different devices")
+    if m == 0 or n == 0:
+        return
+    _mxfp4_aligned(x, "mxfp4_gemm input")
+    with _OnDevice(x.device):
+        parts, cluster = ranges if ranges is not None else mxfp4_few_rows_ranges(n, k, sm_count(x.device))
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_few_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
+                                                        int(out.dtype is torch.float32), m, n, k, int(bool(quantise)), parts, cluster,
+                                                        int(weight.settled), _stream()), "mxfp4_gemm")

@@ -1,0 +1,126 @@
+"""Matrices in microscaled 4-bit floating point on the GPU: quantisation against the definition in 64 bits, products against
+64-bit sums of the same values."""
+import math
+
+import pytest
+import torch
+
+from mini_rsglang_b200 import kernels
+from mini_rsglang_b200.errors import InvalidRequest
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+VALUES = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+def block_exponent(largest):
+    """floor(log2) - 2 of 64-bit sizes, from their exponents; blocks of zeros as the smallest."""
+    field = (largest.double().view(torch.int64) >> 52) - 1023 - 2
+    return field.clamp(-127, 125)
+
+
+def power_of_two(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def plain_quantise(x):
+    """(values float64, scale bytes) of rows by the definition."""
+    rows, width = x.shape
+    blocks = x.double().view(rows, width // 32, 32)
+    finite = blocks.isfinite().all(dim=2, keepdim=True)
+    safe = torch.where(finite, blocks, torch.zeros_like(blocks))
+    e = block_exponent(safe.abs().amax(dim=2, keepdim=True))
+    power = power_of_two(e)
+    size = (safe / power).abs()
+    grid = torch.tensor(VALUES, dtype=torch.float64, device=x.device)
+    best = torch.zeros_like(size)
+    for i in range(1, 8):
+        middle = (grid[i - 1] + grid[i]) / 2
+        best = torch.where((size > middle) | ((size == middle) & (i % 2 == 0)), grid[i], best)
+    value = best * torch.sign(safe) * power
+    value = torch.where(finite, value, torch.full_like(value, math.nan))
+    byte = torch.where(finite, e + 127, torch.full_like(e, 255))
+    return value.view(rows, width), byte.view(rows, width // 32).to(torch.uint8)
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0)) and torch.equal(a.isnan(), b.isnan())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(0, 64), (1, 32), (1, 4096), (3, 96), (5, 160), (127, 288), (129, 224), (300, 1056)])
+def test_quantise_is_the_definition(dtype, rows, width):
+    g = torch.Generator(device=DEV).manual_seed(rows * 5 + width)
+    x = torch.randn(rows, width, device=DEV, generator=g) * torch.exp2(torch.randint(-40, 40, (rows, width), device=DEV, generator=g) / 4)
+    x = x.to(dtype)
+    q = kernels.mxfp4_quantise(x)
+    values, bytes_ = plain_quantise(x) if rows else (torch.empty(0, width, dtype=torch.float64, device=DEV), torch.empty(0, width // 32, dtype=torch.uint8, device=DEV))
+    assert q.shape == (rows, width)
+    assert torch.equal(q.block_scales(), bytes_)
+    for out in (torch.bfloat16, torch.float32):
+        assert torch.equal(kernels.mxfp4_dequantise(q, out).double(), values)
+
+
+def test_quantise_of_ties_ends_of_the_range_and_what_is_not_finite():
+    """Every tie, both signs, in blocks of every power of two; zeros; the smallest and largest floats; infinities and NaN."""
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.96875, 4.0, 0.2490234375, 0.251953125, 0.0, 2.484375, 5.03125])
+    block = torch.cat([ties, -ties])
+    x = block[None, :].double() * power_of_two(torch.arange(-126, 125))[:, None]
+    x = torch.cat([x, torch.zeros(1, 32), torch.full((1, 32), -0.0), torch.full((1, 32), 2.0 ** -149), torch.full((1, 32), 1e-39),
+                   torch.full((1, 32), 3.3e38)]).float().to(DEV)
+    bad = torch.randn(4, 32, device=DEV)
+    bad[0, 3], bad[1, 31], bad[2, 0], bad[3, 7] = math.inf, math.nan, -math.inf, 3.4028234663852886e38
+    x = torch.cat([x, bad]).contiguous()
+    values, bytes_ = plain_quantise(x)
+    q = kernels.mxfp4_quantise(x)
+    assert torch.equal(q.block_scales(), bytes_)
+    assert same(kernels.mxfp4_dequantise(q, torch.float32).double(), values)
+    assert same(kernels.mxfp4_dequantise(q, torch.bfloat16).double(), values)
+    # two blocks of a row: what is not finite stays in its own
+    wide = torch.cat([bad, bad.flip(1).nan_to_num(1.0, 1.0, 1.0)], dim=1).contiguous()
+    values, bytes_ = plain_quantise(wide)
+    q = kernels.mxfp4_quantise(wide)
+    assert torch.equal(q.block_scales(), bytes_) and same(kernels.mxfp4_dequantise(q, torch.float32).double(), values)
+
+
+def random_matrix(g, n, k, spread=3):
+    """A matrix of every code with scales of different sizes, its 64-bit values, and its plain layout."""
+    codes = torch.randint(0, 256, (n, k // 2), device=DEV, generator=g, dtype=torch.uint8)
+    scales = torch.randint(127 - spread - 5, 127 + spread - 5, (n, k // 32), device=DEV, generator=g, dtype=torch.uint8)
+    return codes, scales, plain_values(codes, scales)
+
+
+def plain_values(codes, scales):
+    n, k = codes.shape[0], codes.shape[1] * 2
+    table = torch.tensor(VALUES + [-v for v in VALUES], dtype=torch.float64, device=codes.device)
+    value = torch.stack([table[(codes & 15).long()], table[(codes >> 4).long()]], dim=2).view(n, k // 32, 32)
+    power = power_of_two(scales.long() - 127).view(n, k // 32, 1)
+    power = torch.where(scales.view(n, k // 32, 1) == 255, torch.full_like(power, math.nan), power)
+    return (value * power).view(n, k)
+
+
+def close_to_sums(out, want, size, k, what):
+    """Products of a bfloat16 and a 4-bit value are exact in float32.  32 of them are added by the tensor cores and joined by
+    k / 32 float32 additions, at most 2^-24 of the running sum of sizes each; the tensor cores' own additions of 32 (64 with 4-bit
+    inputs on both sides) count one each.  bfloat16 results are rounded once more."""
+    limit = size * (k / 32 + 64) * 2.0 ** -24
+    if out.dtype is torch.bfloat16:
+        limit = limit + (want.abs() + limit) * 2.0 ** -8
+    off = (out.double() - want).abs()
+    assert (off <= limit + 1e-45).all(), f"{what}: {(off / (limit + 1e-45)).max().item():.3f} of the limit"
+
+
+@pytest.mark.parametrize("quantise", [False, True])
+@pytest.mark.parametrize("m", [0, 1, 2, 7, 8, 9, 15, 16, 17, 33, 64, 100, 129, 257])
+@pytest.mark.parametrize("n,k", [(1, 32), (16, 64), (129, 96), (40, 4096), (300, 1056), (257, 2336), (1000, 512)])
+def test_product_over_the_sizes(m, n, k, quantise):
+    g = torch.Generator(device=DEV).manual_seed(m * 131 + n + k)
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    values = plain_quantise(x)[0] if quantise and m else x.double()
+    want, size = values @ w.T, values.abs() @ w.abs().T
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((m, n), float("nan"), device=DEV, dtype=dtype)
+        kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+        close_to_sums(out, want, size, k, f"{m} x {n} x {k}")

@@ -1,0 +1,70 @@
+"""What the 4-bit entry points refuse before anything is launched; host arithmetic of their launches.  No GPU."""
+import pytest
+import torch
+
+from mini_rsglang_b200 import kernels
+from mini_rsglang_b200.errors import BackendError, InvalidRequest
+
+
+def matrix(rows, width):
+    return kernels.Mxfp4(*kernels._mxfp4_buffers(rows, width, "cpu"), rows, width)
+
+
+@pytest.mark.parametrize("shape", [(4, 33), (4, 16), (4, 0), (32,), (2, 2, 32)])
+def test_quantise_refuses_rows_that_are_no_whole_blocks(shape):
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_quantise(torch.zeros(shape))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.int32])
+def test_quantise_refuses_other_types(dtype):
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_quantise(torch.zeros(4, 32, dtype=dtype))
+
+
+def test_nothing_runs_without_a_gpu():
+    with pytest.raises(BackendError):
+        kernels.mxfp4_quantise(torch.zeros(4, 32))
+    with pytest.raises(BackendError):
+        kernels.mxfp4_dequantise(matrix(4, 32))
+    with pytest.raises(BackendError):
+        kernels.mxfp4_matrix(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8))
+    with pytest.raises(BackendError):
+        kernels.mxfp4_gemm(torch.zeros(2, 64, dtype=torch.bfloat16), matrix(8, 64), torch.zeros(2, 8))
+
+
+def test_dequantise_refuses_other_types():
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_dequantise(matrix(4, 32), torch.float16)
+
+
+@pytest.mark.parametrize("codes,scales", [((4, 16), (4, 2)), ((4, 16), (3, 1)), ((4, 17), (4, 1)), ((4, 16), (4,)), ((64,), (4, 1)), ((4, 0), (4, 0))])
+def test_matrix_refuses_sizes_that_do_not_match(codes, scales):
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_matrix(torch.zeros(codes, dtype=torch.uint8), torch.zeros(scales, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("x,out,dtype", [((2, 96), (2, 8), torch.float32), ((2, 64, 1), (2, 8), torch.float32),
+                                         ((2, 64), (16,), torch.float32), ((2, 64), (2, 8), torch.float16)])
+def test_product_refuses_sizes_and_types(x, out, dtype):
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_gemm(torch.zeros(x, dtype=torch.bfloat16), matrix(8, 64), torch.zeros(out, dtype=dtype))
+
+
+def test_block_scales_reads_the_tiles():
+    """A scale lies at byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of tile (r / 128, b / 4)."""
+    for rows, width in ((1, 32), (129, 288), (300, 1056)):
+        m = matrix(rows, width)
+        want = torch.randint(0, 256, (rows, width // 32), dtype=torch.uint8)
+        tiles = -(-width // 256) * 2
+        for r in range(rows):
+            for b in range(width // 32):
+                m.scales[(r // 128 * tiles + b // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4] = want[r, b]
+        assert torch.equal(m.block_scales(), want)
+    assert matrix(0, 64).block_scales().shape == (0, 2)
+
+
+@pytest.mark.parametrize("n,k", [(1, 32), (128, 4096), (6144, 4096), (24576, 4096), (5120, 17408), (151936, 1024), (40, 65536)])
+def test_ranges_are_what_the_kernel_takes(n, k):
+    parts, cluster = kernels.mxfp4_few_rows_ranges(n, k, 148)
+    assert parts in (1, 2, 4, 8) and cluster in (1, 2, 4, 8) and (parts * cluster == 1 or parts * cluster <= -(-k // 256))
