@@ -190,7 +190,7 @@ PARALLEL_KERNEL_SOURCES = ("parallel_elementwise.cu",)
 DELTA_KERNEL_SOURCES = ("delta_rule.cu",)
 LINEAR_SCAN_KERNEL_SOURCES = ("linear_scan.cu",)
 ROTARY_KERNEL_SOURCES = ("rotary_store.cu", "stream_entry.cu")
-MXFP4_KERNEL_SOURCES = ("mxfp4.cu", "mxfp4_few.cu")
+MXFP4_KERNEL_SOURCES = ("mxfp4.cu", "mxfp4_few.cu", "mxfp4_tc.cu")
 
 
 def _kernel_group(key: str, name: str, sources: tuple[str, ...]) -> ctypes.CDLL:

@@ -8,35 +8,52 @@
 // of a block as its K indices of two MMAs and the same eight elements of x.  A block's two MMAs start from zero, and their sums are
 // multiplied by the block's power of two as they join the row's float32 sums: products of halfs are exact, every sum is float32.
 //
-// x as halfs.  A CTA brings its part of x into the halfs' range by one power of two, which goes into the scales again.
-// Where that loses a bit of any element (more than 2^32 between the sizes of two), or x has an element that is not finite, or the
-// power is beyond [2^-20, 2^15], the CTA multiplies in bfloat16 instead, whose codes take more steps to make: the same sums.
+// One CTA of 16 warps an SM takes an equal share of the groups of 16 rows and keeps x in shared memory for all of them.  Its
+// (group, stage of 256 elements) pairs, group by group, are cut into 16 equal runs, one a warp: a warp's first and last group may
+// be shared with its neighbours, whose sums meet in shared memory in the order of K.  Where x does not fit, the CTAs of a cluster
+// take a range of K each and their sums meet in the ranges' order.  A result does not depend on timing.
 //
-// Ranges of K: the `parts` warps that share a CTA's rows, times the CTAs of a cluster; their sums meet in shared memory, added
-// in the ranges' order, so that a result does not depend on timing.
+// x as halfs.  A CTA brings its part of x into the halfs' range by one power of two (for up to 128 pieces of 256 elements at a time),
+// which goes into the scales again.  Where that could lose a bit of any element (2^29 and more between the sizes of two), or x has an
+// element that is not finite, or the power is beyond [2^-20, 2^15], the CTA multiplies in bfloat16 instead, whose codes take more
+// steps to make: the same products and sums.
 #include "mxfp4.cuh"
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int WARPS = 16, THREADS = WARPS * 32;
 constexpr int STAGE_K = 256;                       // elements of K a stage: 128 bytes a row
 constexpr int CODE_BYTES = 16 * 128, SCALE_BYTES = 16 * 8, STAGE_BYTES = CODE_BYTES + SCALE_BYTES;
-constexpr int RING = 4;
-constexpr int SEGMENT = 2048;                      // elements of K of x in shared memory at a time
+constexpr int RING = 3;
+constexpr int FACTOR_BYTES = 16 * 8 * 4;           // a stage's scales as floats
 constexpr int X_PAD = 64;                          // bytes behind a row of x: two rows then fill all banks
+constexpr int HELD = 8;                            // pieces of 256 elements of x that a warp holds while their power is found
+constexpr int MAX_BATCHES = 64;
+constexpr int SMEM_MOST = 227 * 1024 - 1024;
+constexpr int ROUND_GROUPS = 16;                   // groups whose sums wait for the cluster's others at a time
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy_16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy_4(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+__device__ __forceinline__ void copy_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
+// d = a . b, and d += a . b
 template <bool HALFS>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (HALFS)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+template <bool HALFS>
+__device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (HALFS)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -54,279 +71,357 @@ __device__ __forceinline__ uint32_t as_bf16_pair(uint32_t halfs) {
 
 struct Shapes {
     int M, N, K;
-    int parts;              // warps that share a CTA's rows, a range of K each: 1, 2, 4 or 8
-    int cluster;            // CTAs that share them
-    int segment;            // elements of K of x that shared memory holds
+    int cluster;            // CTAs that share their groups, a range of K each
+    int x_stages;           // the longest of these ranges, in stages
     int early;              // w was there before the kernel before this one: it may be fetched while that runs
 };
 
-// Ranges of K in stages: range r of `ranges`.
-__device__ __forceinline__ int range_start(int stages, int ranges, int r) { return (int)((long long)stages * r / ranges); }
+__device__ __forceinline__ int range_start(int count, int ranges, int r) { return (int)((long long)count * r / ranges); }
 
-// Stages [from, to) of one warp's rows joined to its sums; `x_smem` holds elements of K from stage `x_from` on.
+__device__ __forceinline__ uint32_t shared_word(uint32_t address) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+    return v;
+}
+
+// One stage of a warp's rows joined to its sums.  `factors`: room for the stage's scales as floats.
 template <int NT, bool HALFS>
-__device__ __forceinline__ void stage_products(const unsigned char* stage, const unsigned char* x_stage, int x_pitch, float factor,
-                                               float (&sums)[NT][4]) {
+__device__ __forceinline__ void stage_products(uint32_t stage, float* factors, const unsigned char* x_stage, int x_pitch, float factor,
+                                               int live, float (&sums)[NT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const unsigned char* codes = stage + g * 128 + t * 4;
-    const uint2 scale_low = *reinterpret_cast<const uint2*>(stage + CODE_BYTES + g * 8);
-    const uint2 scale_high = *reinterpret_cast<const uint2*>(stage + CODE_BYTES + (g + 8) * 8);
-    const unsigned char* x_row = x_stage + g * x_pitch + t * 16;
+    {
+        // lane: row lane / 2, blocks 4 (lane % 2) to 4 (lane % 2) + 3.  Byte 0 is 2^-127; byte 255, not a number, stands beside codes of 0:
+        // infinity times a sum of 0 is NaN.
+        const uint32_t word = shared_word(stage + CODE_BYTES + lane * 4);
+        float4 f;
+        f.x = __uint_as_float(max((word << 23) & 0x7F800000u, 0x00400000u)) * factor;
+        f.y = __uint_as_float(max((word << 15) & 0x7F800000u, 0x00400000u)) * factor;
+        f.z = __uint_as_float(max((word << 7) & 0x7F800000u, 0x00400000u)) * factor;
+        f.w = __uint_as_float(max((word >> 1) & 0x7F800000u, 0x00400000u)) * factor;
+        *reinterpret_cast<float4*>(factors + lane * 4) = f;
+        __syncwarp();
+    }
+    const uint32_t codes = stage + g * 128 + g * 16 + t * 4;                  // stages are multiples of 128 bytes: block b lies 16 b xor-ed further
+    const unsigned char* x_rows[NT];                                         // tokens that are not there read the first: nobody stores their sums
 #pragma unroll
-    for (int b = 0; b < STAGE_K / MX_BLOCK; ++b) {
-        const int place = (b ^ g) * 16;
-        uint32_t low[4], high[4];
-        mx_decode_8(*reinterpret_cast<const uint32_t*>(codes + place), low);
-        mx_decode_8(*reinterpret_cast<const uint32_t*>(codes + place + 8 * 128), high);
-        if constexpr (!HALFS) {
+    for (int n = 0; n < NT; ++n) x_rows[n] = x_stage + (n * 8 + g < live ? n * 8 + g : 0) * x_pitch + t * 16;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) low[i] = as_bf16_pair(low[i]), high[i] = as_bf16_pair(high[i]);
-        }
-        const uint32_t word_low = b < 4 ? scale_low.x : scale_low.y, word_high = b < 4 ? scale_high.x : scale_high.y;
-        const int shift = 23 - 8 * (b & 3);
-        const uint32_t bits_low = (shift >= 0 ? word_low << (shift & 31) : word_low >> (-shift & 31)) & 0x7F800000u;
-        const uint32_t bits_high = (shift >= 0 ? word_high << (shift & 31) : word_high >> (-shift & 31)) & 0x7F800000u;
-        // byte 0 is 2^-127; byte 255, not a number, stands beside codes of 0: infinity times the sum of 0 is NaN
-        const float s_low = __uint_as_float(max(bits_low, 0x00400000u)) * factor, s_high = __uint_as_float(max(bits_high, 0x00400000u)) * factor;
-        const uint32_t a0[4] = {low[0], high[0], low[1], high[1]}, a1[4] = {low[2], high[2], low[3], high[3]};
+    for (int half = 0; half < 2; ++half) {
+        const float4 f_low = *reinterpret_cast<const float4*>(factors + g * 8 + half * 4);
+        const float4 f_high = *reinterpret_cast<const float4*>(factors + (g + 8) * 8 + half * 4);
+        const float s_low[4] = {f_low.x, f_low.y, f_low.z, f_low.w}, s_high[4] = {f_high.x, f_high.y, f_high.z, f_high.w};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const uint4 xs = *reinterpret_cast<const uint4*>(x_row + (size_t)n * 8 * x_pitch + b * 64);
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma<HALFS>(d, a0, xs.x, xs.y);
-            mma<HALFS>(d, a1, xs.z, xs.w);
-            sums[n][0] = fmaf(d[0], s_low, sums[n][0]);
-            sums[n][1] = fmaf(d[1], s_low, sums[n][1]);
-            sums[n][2] = fmaf(d[2], s_high, sums[n][2]);
-            sums[n][3] = fmaf(d[3], s_high, sums[n][3]);
+        for (int i = 0; i < 4; ++i) {
+            const int b = half * 4 + i;
+            uint32_t low[4], high[4];
+            mx_decode_8(shared_word(codes ^ (b * 16)), low);
+            mx_decode_8(shared_word((codes ^ (b * 16)) + 8 * 128), high);
+            if constexpr (!HALFS) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) low[j] = as_bf16_pair(low[j]), high[j] = as_bf16_pair(high[j]);
+            }
+            const uint32_t a0[4] = {low[0], high[0], low[1], high[1]}, a1[4] = {low[2], high[2], low[3], high[3]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint4 xs = *reinterpret_cast<const uint4*>(x_rows[n] + b * 64);
+                float d[4];
+                mma_first<HALFS>(d, a0, xs.x, xs.y);
+                mma_more<HALFS>(d, a1, xs.z, xs.w);
+                sums[n][0] = fmaf(d[0], s_low[i], sums[n][0]);
+                sums[n][1] = fmaf(d[1], s_low[i], sums[n][1]);
+                sums[n][2] = fmaf(d[2], s_high[i], sums[n][2]);
+                sums[n][3] = fmaf(d[3], s_high[i], sums[n][3]);
+            }
         }
     }
 }
 
-// Eight elements of x as pairs of bfloat16; with QUANTISE what their 4-bit codes stand for (four lanes a block).
-template <bool QUANTISE>
-__device__ __forceinline__ uint4 load_x(const bf16* x, bool there) {
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (there) raw = *reinterpret_cast<const uint4*>(x);
-    if constexpr (QUANTISE) {
-        uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        float v[8];
-        uint32_t largest = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-            largest = max(largest, max(__float_as_uint(v[2 * i]) & 0x7FFFFFFFu, __float_as_uint(v[2 * i + 1]) & 0x7FFFFFFFu));
-        }
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        const uint32_t byte = mx_scale_byte(largest);
-        const float scale = mx_scale(byte);
-        uint32_t h[4];
-        mx_decode_8(byte == 255u ? 0u : mx_encode_8(v, mx_inverse(byte)), h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 pair = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
-            __nv_bfloat162 rounded = __floats2bfloat162_rn(pair.x * scale, pair.y * scale);       // exact
-            w[i] = *reinterpret_cast<uint32_t*>(&rounded);
-        }
-        raw = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    return raw;
-}
-
-// x[tokens][from, from + count) into shared memory, `rows` rows (those behind M and what lies behind K as zeros).  Returns whether
-// they lie there as halfs, times 2^(15 - e) (`factor` = 2^(e - 15)), or, where that would lose a bit, as they are (`factor` = 1).
-template <bool QUANTISE>
-__device__ bool bring_x(const bf16* __restrict__ x, unsigned char* x_smem, int x_pitch, int rows, int first_token, const Shapes& s, int from,
-                        int count, uint32_t* scratch, float& factor) {
-    const int chunks = count >> 3, total = rows * chunks;
+// Eight elements of x, pairs of bfloat16, as what their 4-bit codes stand for (four lanes a block).
+__device__ __forceinline__ uint4 through_codes(uint4 raw) {
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float v[8];
     uint32_t largest = 0;
-    for (int base = 0; base < total; base += THREADS) {                       // whole warps: a block's four lanes stay together
-        const int i = base + threadIdx.x, row = i / chunks, column = (i - row * chunks) * 8;
-        const bool there = i < total && first_token + row < s.M && from + column < s.K;
-        const uint4 raw = load_x<QUANTISE>(x + (size_t)(first_token + row) * s.K + from + column, there);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) largest = max(largest, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
-        if (i < total) *reinterpret_cast<uint4*>(x_smem + (size_t)row * x_pitch + column * 2) = raw;
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        largest = max(largest, max(__float_as_uint(v[2 * i]) & 0x7FFFFFFFu, __float_as_uint(v[2 * i + 1]) & 0x7FFFFFFFu));
     }
-    largest = __reduce_max_sync(0xffffffffu, largest);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = largest;
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    const uint32_t byte = mx_scale_byte(largest);
+    const float scale = mx_scale(byte);
+    uint32_t h[4];
+    mx_decode_8(byte == 255u ? 0u : mx_encode_8(v, mx_inverse(byte)), h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 pair = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+        __nv_bfloat162 rounded = __floats2bfloat162_rn(pair.x * scale, pair.y * scale);       // exact
+        w[i] = *reinterpret_cast<uint32_t*>(&rounded);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Stages [from, to) of x's rows first_token .. + live into shared memory (what lies behind K as zeros), `to - from` times `live` pieces of
+// 256 elements, at most HELD a warp.  Returns the factor 2^(e - 15) of elements that lie there as halfs times 2^(15 - e), or 0 where
+// that might lose a bit and they lie there as they are.
+template <bool QUANTISE>
+__device__ __forceinline__ float bring_x(const bf16* __restrict__ x, unsigned char* x_smem, int x_pitch, int live, int first_token, const Shapes& s,
+                                         int from, int to, int x_from, uint32_t* scratch) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = (to - from) * live;
+    uint4 held[HELD];
+    uint32_t largest = 0;                                                     // a pair
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * WARPS + warp, stage = i / live, row = i - stage * live, column = (from + stage) * STAGE_K + lane * 8;
+        held[j] = make_uint4(0, 0, 0, 0);
+        if (i < pieces && column < s.K) held[j] = *reinterpret_cast<const uint4*>(x + (size_t)(first_token + row) * s.K + column);
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        if (j * WARPS + warp >= pieces) break;                                // the same for the whole warp
+        if constexpr (QUANTISE) held[j] = through_codes(held[j]);
+        const uint32_t w[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) largest = __viaddmax_s16x2(w[p] & 0x7FFF7FFFu, 0u, largest);
+    }
+    largest = __reduce_max_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16));
+    if (lane == 0) scratch[warp] = largest;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) largest = max(largest, scratch[w]);
     const int field = (int)(largest >> 7), e = largest == 0 ? 0 : field - 127;
-    bool exact = field != 255 && e >= -20 && e <= 15;
-    if (exact) {
-        const float up = __uint_as_float((uint32_t)(127 + 15 - e) << 23);
-        for (int i = threadIdx.x; i < total; i += THREADS) {
-            const int row = i / chunks, column = (i - row * chunks) * 8;
-            uint4* place = reinterpret_cast<uint4*>(x_smem + (size_t)row * x_pitch + column * 2);
-            const uint4 raw = *place;
-            uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const bool asked = e >= -20 && e <= 15;                                   // the same for the whole CTA; not with infinities or NaN
+    bool exact = asked;
+    if (asked) {
+        // a half's exponent field is the element's less that of the largest, plus 30; its mantissa the element's seven bits, then zeros
+        const uint32_t down = (uint32_t)(-((e + 127 - 30) << 7)) & 0xFFFFu, both = down | down << 16;
+        uint32_t lost = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float a = __uint_as_float(w[j] << 16) * up, b = __uint_as_float(w[j] & 0xFFFF0000u) * up;
-                __half2 pair = __floats2half2_rn(a, b);
-                const float2 back = __half22float2(pair);
-                exact = exact && back.x == a && back.y == b;
-                w[j] = *reinterpret_cast<uint32_t*>(&pair);
+        for (int j = 0; j < HELD; ++j) {
+            const int i = j * WARPS + warp, stage = i / live, row = i - stage * live;
+            if (i >= pieces) break;
+            const uint32_t w[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
+            uint32_t h[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const uint32_t size = w[p] & 0x7FFF7FFFu, r = __viaddmax_s16x2(size, both, 0u);
+                lost |= (size + 0x7FFF7FFFu) & ~(r + 0x7F807F80u);            // highest bit of each half: not 0, and below the halfs' smallest ordinary number
+                h[p] = (r << 3) | (w[p] & 0x80008000u);
             }
-            *place = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(x_smem + row * x_pitch + (from - x_from + stage) * (STAGE_K * 2) + lane * 16) = make_uint4(h[0], h[1], h[2], h[3]);
         }
+        exact = (lost & 0x80008000u) == 0;
     }
-    const bool asked = field != 255 && e >= -20 && e <= 15;                   // the same for the whole CTA
-    exact = !__syncthreads_or(!exact);
-    factor = exact ? __uint_as_float((uint32_t)(127 + e - 15) << 23) : 1.0f;
-    if (!exact && asked) {                                                     // overwritten above: read again
-        for (int base = 0; base < total; base += THREADS) {
-            const int i = base + threadIdx.x, row = i / chunks, column = (i - row * chunks) * 8;
-            const bool there = i < total && first_token + row < s.M && from + column < s.K;
-            const uint4 raw = load_x<QUANTISE>(x + (size_t)(first_token + row) * s.K + from + column, there);
-            if (i < total) *reinterpret_cast<uint4*>(x_smem + (size_t)row * x_pitch + column * 2) = raw;
-        }
-        __syncthreads();
+    if (!__syncthreads_or(!exact)) return __uint_as_float((uint32_t)(127 + e - 15) << 23);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * WARPS + warp, stage = i / live, row = i - stage * live;
+        if (i < pieces) *reinterpret_cast<uint4*>(x_smem + row * x_pitch + (from - x_from + stage) * (STAGE_K * 2) + lane * 16) = held[j];
     }
-    return exact;
+    return 0.0f;
 }
 
 template <int NT, bool QUANTISE, typename Out>
-__global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes,
+__global__ void __launch_bounds__(THREADS, 1) few_rows_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, Out* __restrict__ out, const Shapes s) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t scratch[WARPS];
+    __shared__ float x_factors[MAX_BATCHES];
+    constexpr int TOKENS = NT * 8, GROUP_SUMS = TOKENS * 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int groups = WARPS / s.parts, rows_of_cta = groups * 16;
-    const int rank = blockIdx.x % s.cluster, tile = blockIdx.x / s.cluster;
-    const int group = warp / s.parts, part = warp - group * s.parts;
-    const long long row0 = (long long)tile * rows_of_cta + group * 16;
-    const int first_token = blockIdx.y * (NT * 8);
+    const int rank = blockIdx.x % s.cluster, share = blockIdx.x / s.cluster, shares = gridDim.x / s.cluster;
+    const int groups = (s.N + 15) >> 4;
+    const int group_from = range_start(groups, shares, share), group_to = range_start(groups, shares, share + 1);
+    const int first_token = blockIdx.y * TOKENS, live = min(TOKENS, s.M - first_token);
     const int stages = (s.K + STAGE_K - 1) / STAGE_K;
-    const int cta_from = range_start(stages, s.cluster, rank), cta_to = range_start(stages, s.cluster, rank + 1);
+    const int k_from = range_start(stages, s.cluster, rank), k_to = range_start(stages, s.cluster, rank + 1), depth = k_to - k_from;
+    const int batch_stages = HELD * WARPS / live;                             // of x, whose power is found together
 
-    unsigned char* ring = smem + warp * (RING * STAGE_BYTES);
-    unsigned char* x_smem = smem + WARPS * RING * STAGE_BYTES;
-    float* partial = reinterpret_cast<float*>(x_smem);                       // x is done with when the sums meet
-    const int x_pitch = s.segment * 2 + X_PAD;
+    unsigned char* place = smem;
+    const uint32_t ring = smem_address(place + warp * (RING * STAGE_BYTES));
+    place += WARPS * RING * STAGE_BYTES;
+    float* factors = reinterpret_cast<float*>(place + warp * FACTOR_BYTES);
+    place += WARPS * FACTOR_BYTES;
+    float* pieces = reinterpret_cast<float*>(place);                          // [warp][its first group, its last][token][row]
+    place += WARPS * 2 * GROUP_SUMS * 4;
+    float* whole = reinterpret_cast<float*>(place);                           // [group of the round][token][row], for the cluster
+    if (s.cluster > 1) place += ROUND_GROUPS * GROUP_SUMS * 4;
+    unsigned char* x_smem = place;
+    const int x_pitch = s.x_stages * (STAGE_K * 2) + X_PAD;
 
+    // Without a cluster one round takes all of the CTA's groups.
+    const int round_groups = s.cluster > 1 ? ROUND_GROUPS : group_to - group_from;
     const long long code_pitch = s.K >> 1, tiles_of_a_row = mx_tiles_of_a_row(s.K);
-    // A stage of this warp's rows: four 16-byte copies and one of four scales a lane.
-    auto fetch = [&](int stage, int slot) {
-        const uint32_t base = smem_address(ring + slot * STAGE_BYTES);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int q = j * 32 + lane, r = q >> 3, c = q & 7;
-            const bool there = row0 + r < s.N && stage * 128 + c * 16 < code_pitch;
-            copy_16(base + r * 128 + ((c ^ (r & 7)) << 4), there ? codes + (row0 + r) * code_pitch + stage * 128 + c * 16 : codes, there);
-        }
-        const long long r = row0 + (lane >> 1);
-        const bool there = r < s.N;
-        copy_4(base + CODE_BYTES + lane * 4, there ? scales + mx_scale_offset(r, stage * 2 + (lane & 1), tiles_of_a_row) : scales, there);
-    };
+    const uint32_t even = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);                  // rows lane / 8 and + 8 of a stage
+    const uint32_t odd = (4 + (lane >> 3)) * 128 + (((lane & 7) ^ (4 + (lane >> 3))) << 4);       // rows lane / 8 + 4 and + 12
 
-    float sums[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) sums[n][0] = sums[n][1] = sums[n][2] = sums[n][3] = 0.0f;
+    bool waited = false;
+    for (int first = group_from; first < group_to; first += round_groups) {
+        const int count = min(round_groups, group_to - first), units = count * depth;
+        const int unit_from = range_start(units, WARPS, warp), unit_to = range_start(units, WARPS, warp + 1);
 
-    if (!s.early) pdl_wait();
-    // this CTA's stages in segments of x; within a segment warp `part` takes stages part, part + parts, ...
-    const int segment_stages = s.segment / STAGE_K;
-    int next = cta_from + part, fetched = 0, used = 0;          // the next stage to fetch: this warp's walk through the CTA's range
-    auto fetch_next = [&]() {
-        if (next < cta_to) {
-            fetch(next, fetched % RING);
-            next += s.parts;
-        }
-        ++fetched;
-        copy_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < RING - 1; ++i) fetch_next();
-    pdl_launch_dependents();
-    if (s.early) pdl_wait();
-    // the segments are multiples of `parts` stages long, so a warp's walk through the range meets every segment in step
-    for (int from = cta_from; from < cta_to; from += segment_stages) {
-        const int to = min(from + segment_stages, cta_to);
-        float factor;
-        if (from > cta_from) __syncthreads();
-        const bool halfs = bring_x<QUANTISE>(x, x_smem, x_pitch, NT * 8, first_token, s, from * STAGE_K, (to - from) * STAGE_K, scratch, factor);
-        for (int stage = from + part; stage < to; stage += s.parts) {
-            copy_wait<RING - 2>();
-            __syncwarp();
-            fetch_next();
-            const unsigned char* slot = ring + (used % RING) * STAGE_BYTES;
-            const unsigned char* x_stage = x_smem + (stage - from) * (STAGE_K * 2);
-            if (halfs) stage_products<NT, true>(slot, x_stage, x_pitch, factor, sums);
-            else stage_products<NT, false>(slot, x_stage, x_pitch, factor, sums);
-            ++used;
-            __syncwarp();
-        }
-    }
-    copy_wait<0>();
-    __syncthreads();
+        // The copies' walk through this warp's units: four 16-byte copies and one of four scales a lane.  Rows behind N and columns behind K
+        // are copies of the last (their sums are not stored; x is 0 there): nothing is read out of range.
+        int copy_group = depth ? first + unit_from / depth : 0, copy_stage = k_from + (depth ? unit_from % depth : 0), left = unit_to - unit_from;
+        uint32_t copy_offset = 0, used_offset = 0;
+        const uint8_t *from0, *from1, *from2, *from3, *from_scales;
+        auto start_group = [&]() {
+            const long long row = (long long)copy_group * 16 + (lane >> 3), last = s.N - 1;
+            const uint8_t* base = codes + (long long)copy_stage * 128 + (lane & 7) * 16;
+            from0 = base + min(row, last) * code_pitch;
+            from1 = base + min(row + 4, last) * code_pitch;
+            from2 = base + min(row + 8, last) * code_pitch;
+            from3 = base + min(row + 12, last) * code_pitch;
+            from_scales = scales + mx_scale_offset(min((long long)copy_group * 16 + (lane >> 1), last), copy_stage * 2 + (lane & 1), tiles_of_a_row);
+        };
+        auto copy_next = [&]() {
+            if (left > 0) {
+                const uint32_t base = ring + copy_offset;
+                const int behind = max(copy_stage * 128 + (lane & 7) * 16 + 16 - (int)code_pitch, 0);      // 0 but at the end of rows that end inside a stage
+                copy_16(base + even, from0 - behind);
+                copy_16(base + odd, from1 - behind);
+                copy_16(base + even + 8 * 128, from2 - behind);
+                copy_16(base + odd + 8 * 128, from3 - behind);
+                copy_4(base + CODE_BYTES + lane * 4, from_scales);
+                from0 += 128, from1 += 128, from2 += 128, from3 += 128;
+                from_scales += 2 * MX_TILE_BYTES;
+                --left;
+                if (++copy_stage == k_to) {
+                    ++copy_group;
+                    copy_stage = k_from;
+                    if (left > 0) start_group();
+                }
+            }
+            copy_offset = copy_offset + STAGE_BYTES == RING * STAGE_BYTES ? 0 : copy_offset + STAGE_BYTES;
+            copy_commit();
+        };
+        if (left > 0) start_group();
 
-    // the ranges' sums [part][token][row of the CTA] meet
-    const int tokens = NT * 8, plane = tokens * rows_of_cta;
-    {
-        float* mine = partial + part * plane + group * 16;
-        const int g = lane >> 2, t = lane & 3;
+        if (!waited && !s.early) pdl_wait();
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            mine[(n * 8 + 2 * t) * rows_of_cta + g] = sums[n][0];
-            mine[(n * 8 + 2 * t + 1) * rows_of_cta + g] = sums[n][1];
-            mine[(n * 8 + 2 * t) * rows_of_cta + g + 8] = sums[n][2];
-            mine[(n * 8 + 2 * t + 1) * rows_of_cta + g + 8] = sums[n][3];
+        for (int i = 0; i < RING - 1; ++i) copy_next();
+        if (!waited) {
+            pdl_launch_dependents();
+            if (s.early) pdl_wait();
+            waited = true;
+            for (int b = k_from; b < k_to; b += batch_stages) {
+                const float factor = bring_x<QUANTISE>(x, x_smem, x_pitch, live, first_token, s, b, min(b + batch_stages, k_to), k_from, scratch);
+                if (threadIdx.x == 0) x_factors[(b - k_from) / batch_stages] = factor;
+            }
+            __syncthreads();
         }
-    }
-    if (s.cluster > 1) {
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    } else {
-        __syncthreads();
-    }
-    const int live = min(tokens, s.M - first_token) * rows_of_cta;
-    const uint32_t base = smem_address(partial);
-    for (int i = rank * THREADS + threadIdx.x; i < live; i += s.cluster * THREADS) {
-        const int token = i / rows_of_cta, row = i - token * rows_of_cta;
-        const long long n = (long long)tile * rows_of_cta + row;
-        float sum = 0.0f;
-        for (int c = 0; c < s.cluster; ++c) {
-            uint32_t there;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(base + i * 4), "r"(c));
-            for (int p = 0; p < s.parts; ++p) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there + p * plane * 4) : "memory");
-                sum += v;
+
+        int group = depth ? first + unit_from / depth : 0, stage = depth ? unit_from % depth : 0;        // of the CTA's range
+        for (int unit = unit_from; unit < unit_to; ++group, stage = 0) {
+            const int stop = min(unit + depth - stage, unit_to);               // of this warp's piece of the group
+            const bool alone = stage == 0 && stop - unit == depth;
+            float sums[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sums[n][0] = sums[n][1] = sums[n][2] = sums[n][3] = 0.0f;
+            const int slot = unit == unit_from ? 0 : 1;
+            int batch = stage / batch_stages, batch_end = (batch + 1) * batch_stages;
+            float factor = x_factors[batch];
+            const unsigned char* x_stage = x_smem + stage * (STAGE_K * 2);
+            for (; unit < stop; ++unit, ++stage, x_stage += STAGE_K * 2) {
+                if (stage == batch_end) {
+                    factor = x_factors[++batch];
+                    batch_end += batch_stages;
+                }
+                copy_wait<RING - 2>();
+                __syncwarp();
+                copy_next();
+                if (factor != 0.0f) stage_products<NT, true>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
+                else stage_products<NT, false>(ring + used_offset, factors, x_stage, x_pitch, 1.0f, live, sums);
+                used_offset = used_offset + STAGE_BYTES == RING * STAGE_BYTES ? 0 : used_offset + STAGE_BYTES;
+                __syncwarp();
+            }
+            const int g = lane >> 2, t = lane & 3;
+            if (alone && s.cluster == 1) {                                      // these sums are the results
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int token = n * 8 + 2 * t + (i & 1);
+                        const long long row = (long long)group * 16 + g + (i >> 1) * 8;
+                        if (token < live && row < s.N) out[(size_t)(first_token + token) * s.N + row] = from_float<Out>(sums[n][i]);
+                    }
+            } else {
+                float* mine = alone ? whole + (group - first) * GROUP_SUMS : pieces + (warp * 2 + slot) * GROUP_SUMS;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mine[(n * 8 + 2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = sums[n][i];
             }
         }
-        if (n < s.N) out[(size_t)(first_token + token) * s.N + n] = from_float<Out>(sum);
-    }
-    if (s.cluster > 1) {                                          // a CTA's sums stay until its cluster has read them
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        copy_wait<0>();
+        __syncthreads();
+
+        // groups that several warps share: their pieces in the order of K.  Unit u belongs to warp ((u + 1) * WARPS - 1) / units.
+        for (int index = warp; index < count; index += WARPS) {
+            const int begin = index * depth;
+            const int low = units ? (int)(((long long)(begin + 1) * WARPS - 1) / units) : 0, high = units ? (int)(((long long)(begin + depth) * WARPS - 1) / units) : 0;
+            if (units && low == high) continue;
+            const float* first_piece = pieces + (low * 2 + (range_start(units, WARPS, low) >= begin ? 0 : 1)) * GROUP_SUMS;
+            for (int i = lane; i < live * 16; i += 32) {
+                float sum = 0.0f;
+                if (units) {
+                    sum = first_piece[i];
+                    for (int w = low + 1; w <= high; ++w)
+                        if (range_start(units, WARPS, w) < range_start(units, WARPS, w + 1)) sum += pieces[w * 2 * GROUP_SUMS + i];
+                }
+                const long long row = (long long)(first + index) * 16 + (i & 15);
+                if (s.cluster > 1) whole[index * GROUP_SUMS + i] = sum;
+                else if (row < s.N) out[(size_t)(first_token + (i >> 4)) * s.N + row] = from_float<Out>(sum);
+            }
+        }
+        if (s.cluster > 1) {
+            asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+            const uint32_t base = smem_address(whole);
+            for (int i = rank * THREADS + threadIdx.x; i < count * live * 16; i += s.cluster * THREADS) {
+                const int index = i / (live * 16), within = i - index * (live * 16);
+                float sum = 0.0f;
+                for (int c = 0; c < s.cluster; ++c) {
+                    uint32_t there;
+                    float v;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(base + (index * GROUP_SUMS + within) * 4), "r"(c));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+                    sum += v;
+                }
+                const long long row = (long long)(first + index) * 16 + (within & 15);
+                if (row < s.N) out[(size_t)(first_token + (within >> 4)) * s.N + row] = from_float<Out>(sum);
+            }
+            asm volatile("barrier.cluster.arrive.release;" ::: "memory");        // a CTA's sums stay until its cluster has read them
+            asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        }
     }
 }
 
+// Bytes of shared memory; 0 where x does not fit.
+size_t shared_bytes(int tokens, int x_stages, int live, int cluster) {
+    const size_t bytes = (size_t)WARPS * (RING * STAGE_BYTES + FACTOR_BYTES) + (size_t)WARPS * 2 * tokens * 16 * 4 +
+                         (cluster > 1 ? (size_t)ROUND_GROUPS * tokens * 16 * 4 : 0) + (size_t)live * ((size_t)x_stages * STAGE_K * 2 + X_PAD);
+    const int batch = HELD * WARPS / live;
+    return bytes > SMEM_MOST || (x_stages + batch - 1) / batch > MAX_BATCHES ? 0 : bytes;
+}
+
 template <int NT, bool QUANTISE, typename Out>
-int launch(const void* x, const void* codes, const void* scales, void* out, Shapes s, void* stream) {
-    const int groups = WARPS / s.parts;
-    const int stages = (s.K + STAGE_K - 1) / STAGE_K, of_cta = (stages + s.cluster - 1) / s.cluster;
-    const int most = SEGMENT / STAGE_K;                           // a multiple of every count of parts
-    s.segment = (of_cta < most ? of_cta : most) * STAGE_K;
-    const size_t x_bytes = (size_t)NT * 8 * (s.segment * 2 + X_PAD), sum_bytes = (size_t)WARPS * 16 * NT * 8 * 4;
-    const size_t bytes = (size_t)WARPS * RING * STAGE_BYTES + (x_bytes > sum_bytes ? x_bytes : sum_bytes);
+int launch(const void* x, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
+    const int stages = (s.K + STAGE_K - 1) / STAGE_K;
+    s.x_stages = (stages + s.cluster - 1) / s.cluster;
+    const size_t bytes = shared_bytes(NT * 8, s.x_stages, s.M < NT * 8 ? s.M : NT * 8, s.cluster);
+    if (!bytes) return MRS_BAD_ARGUMENT;
     static PerDevice configured;
     if (!configured.get()) {
-        const size_t all = (size_t)WARPS * RING * STAGE_BYTES + (size_t)NT * 8 * (SEGMENT * 2 + X_PAD);
-        cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<NT, QUANTISE, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)all);
+        cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<NT, QUANTISE, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
         if (e != cudaSuccess) return (int)e;
         configured.set(1);
     }
-    const long long rows = groups * 16, tiles = ((long long)s.N + rows - 1) / rows;
-    if (tiles * s.cluster > 0x7FFFFFFFll) return MRS_BAD_ARGUMENT;
+    const int groups = (s.N + 15) / 16, most_shares = (ctas / s.cluster) > 1 ? ctas / s.cluster : 1;
+    const int shares = groups < most_shares ? groups : most_shares;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(tiles * s.cluster), (unsigned)((s.M + NT * 8 - 1) / (NT * 8)));
+    config.gridDim = dim3((unsigned)(shares * s.cluster), (unsigned)((s.M + NT * 8 - 1) / (NT * 8)));
     config.blockDim = dim3(THREADS);
     config.dynamicSmemBytes = bytes;
     config.stream = (cudaStream_t)stream;
@@ -344,26 +439,31 @@ int launch(const void* x, const void* codes, const void* scales, void* out, Shap
 }
 
 template <int NT, typename Out>
-int launch_x(const void* x, const void* codes, const void* scales, void* out, const Shapes& s, int quantise, void* stream) {
-    return quantise ? launch<NT, true, Out>(x, codes, scales, out, s, stream) : launch<NT, false, Out>(x, codes, scales, out, s, stream);
+int launch_x(const void* x, const void* codes, const void* scales, void* out, const Shapes& s, int quantise, int ctas, void* stream) {
+    return quantise ? launch<NT, true, Out>(x, codes, scales, out, s, ctas, stream) : launch<NT, false, Out>(x, codes, scales, out, s, ctas, stream);
 }
 
 }  // namespace
 
-// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16; w as in mxfp4.cuh; `parts` 1, 2, 4 or 8, `cluster` 1, 2, 4 or 8 ranges of K.
-// `early`: nothing that still runs when this kernel starts writes w.
-MRS_EXPORT int mrs_mxfp4_few_rows(const void* x, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int quantise,
-                                  int parts, int cluster, int early, void* stream) {
-    if (M == 0 || N == 0) return 0;
-    if (M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || M > 65535 * 8 || !x || !codes || !scales || !out) return MRS_BAD_ARGUMENT;
-    if ((((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1))) return MRS_BAD_ARGUMENT;
-    if ((parts != 1 && parts != 2 && parts != 4 && parts != 8) || (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8)) return MRS_BAD_ARGUMENT;
-    Shapes s = {M, N, K, parts, cluster, 0, early};
-    if (M <= 8) return out_f32 ? launch_x<1, float>(x, codes, scales, out, s, quantise, stream) : launch_x<1, bf16>(x, codes, scales, out, s, quantise, stream);
-    return out_f32 ? launch_x<2, float>(x, codes, scales, out, s, quantise, stream) : launch_x<2, bf16>(x, codes, scales, out, s, quantise, stream);
+// CTAs of a cluster (1, 2, 4 or 8) whose shared memory holds their ranges of up to 16 rows (tokens of 8 at a time for up to 8) of
+// K elements; 0 where none does.
+MRS_EXPORT int mrs_mxfp4_few_rows_cluster(int M, int K) {
+    const int tokens = M <= 8 ? 8 : 16, stages = (K + STAGE_K - 1) / STAGE_K;
+    for (int c = 1; c <= 8; c *= 2)
+        if (shared_bytes(tokens, (stages + c - 1) / c, M < tokens ? M : tokens, c)) return c;
+    return 0;
 }
 
-MRS_EXPORT const char* mrs_mxfp4_few_error_string(int code) {
-    if (code == MRS_BAD_ARGUMENT) return "arguments outside what the kernel supports (K no multiple of 32, unaligned base, ranges)";
-    return cudaGetErrorString((cudaError_t)code);
+// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16; w as in mxfp4.cuh; `cluster` 1, 2, 4 or 8 ranges of K; `ctas`: the GPU's
+// SMs.  `early`: nothing that still runs when this kernel starts writes w.
+MRS_EXPORT int mrs_mxfp4_few_rows(const void* x, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int quantise,
+                                  int cluster, int ctas, int early, void* stream) {
+    if (M == 0 || N == 0) return 0;
+    if (M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || M > 65535 * 8 || ctas < 1 || !x || !codes || !scales || !out) return MRS_BAD_ARGUMENT;
+    if ((((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1))) return MRS_BAD_ARGUMENT;
+    if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return MRS_BAD_ARGUMENT;
+    Shapes s = {M, N, K, cluster, 0, early};
+    if (M <= 8)
+        return out_f32 ? launch_x<1, float>(x, codes, scales, out, s, quantise, ctas, stream) : launch_x<1, bf16>(x, codes, scales, out, s, quantise, ctas, stream);
+    return out_f32 ? launch_x<2, float>(x, codes, scales, out, s, quantise, ctas, stream) : launch_x<2, bf16>(x, codes, scales, out, s, quantise, ctas, stream);
 }

@@ -2568,6 +2568,10 @@ _MXFP4_SIGNATURES = {
     "mrs_mxfp4_dequantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_scales_to_tiles": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_few_rows_cluster": [_c_int, _c_int],
+    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_take_error": [ctypes.POINTER(ctypes.c_uint)],
 }
 _mxfp4_lib = None
 
@@ -2583,6 +2587,7 @@ def mxfp4_library() -> ctypes.CDLL:
         lib.mrs_mxfp4_error_string.argtypes = [_c_int]
         lib.mrs_mxfp4_error_string.restype = ctypes.c_char_p
         _mxfp4_lib = lib
+        _register_error_word("mxfp4", lib, "mrs_mxfp4")
     return _mxfp4_lib
 
 
@@ -2710,21 +2715,21 @@ def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
     return Mxfp4(held, tiles, rows, width, settled=True)
 
 
-def mxfp4_few_rows_ranges(n: int, k: int, sms: int) -> tuple[int, int]:
-    """(ranges of K within a CTA, CTAs of a cluster) of the product for few rows with [n, k] weights.  A warp takes 16 rows and one
-    range; the ranges are as many as give every SM 16 warps, a stage of 256 elements at least each."""
-    stages, groups = -(-k // 256), -(-n // 16)
-    parts = cluster = 1
-    while parts < 8 and groups * parts < 16 * sms and parts * 2 <= stages:
-        parts *= 2
-    while cluster < 8 and groups * parts * cluster < 16 * sms and parts * cluster * 2 <= stages:
-        cluster *= 2
-    return parts, cluster
+def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
+    """How a product is launched: ("few", CTAs of a cluster) or ("many", tokens of a tile, CTAs of a cluster)."""
+    if m <= (4 if quantise else 8):
+        cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
+        if cluster:
+            return ("few", cluster)
+    tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128 if m <= 128 else 256
+    tiles = -(-n // 128) * -(-m // tokens)
+    return ("many", tokens, 4 if tiles * 4 <= sms and k >= 1024 else 2 if tiles * 2 <= sms and k >= 512 else 1)
 
 
-def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool = False, ranges: tuple[int, int] | None = None) -> None:
+def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool = False, plan: tuple | None = None) -> None:
     """out[M, N] = x[M, K] . weight[N, K]^T; x bfloat16, weight in 4 bits, sums in float32, `out` bfloat16 or float32.  With `quantise`
-    x's rows are brought to 4 bits first, as `mxfp4_quantise` does."""
+    x's rows are brought to 4 bits first, as `mxfp4_quantise` does.  `plan`: another than `mxfp4_plan` only for measurements and tests."""
+    global launch_count
     if x.dim() != 2 or out.dim() != 2:
         raise InvalidRequest("mxfp4_gemm: input and output are rows")
     m, k = x.shape
@@ -2740,8 +2745,21 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
     if m == 0 or n == 0:
         return
     _mxfp4_aligned(x, "mxfp4_gemm input")
+    lib = mxfp4_library()
+    out_f32, early = int(out.dtype is torch.float32), int(weight.settled)
     with _OnDevice(x.device):
-        parts, cluster = ranges if ranges is not None else mxfp4_few_rows_ranges(n, k, sm_count(x.device))
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_few_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
-                                                        int(out.dtype is torch.float32), m, n, k, int(bool(quantise)), parts, cluster,
-                                                        int(weight.settled), _stream()), "mxfp4_gemm")
+        if plan is None:
+            plan = mxfp4_plan(m, n, k, quantise, sm_count(x.device))
+        if plan[0] == "few":
+            code = lib.mrs_mxfp4_few_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32, m, n, k,
+                                          int(bool(quantise)), plan[1], sm_count(x.device), early, _stream())
+        elif quantise:
+            codes, scales = _mxfp4_buffers(m, k, x.device)
+            launch_count += 1
+            code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k, _stream())
+            code = code or lib.mrs_mxfp4_both_rows(codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+                                                   out.data_ptr(), out_f32, m, n, k, plan[1], plan[2], early, _stream())
+        else:
+            code = lib.mrs_mxfp4_weights_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32,
+                                              m, n, k, plan[1], plan[2], early, _stream())
+        _mxfp4_check(code, "mxfp4_gemm")

@@ -100,10 +100,11 @@ def plain_values(codes, scales):
 
 
 def close_to_sums(out, want, size, k, what):
-    """Products of a bfloat16 and a 4-bit value are exact in float32.  32 of them are added by the tensor cores and joined by
-    k / 32 float32 additions, at most 2^-24 of the running sum of sizes each; the tensor cores' own additions of 32 (64 with 4-bit
-    inputs on both sides) count one each.  bfloat16 results are rounded once more."""
-    limit = size * (k / 32 + 64) * 2.0 ** -24
+    """Products of a bfloat16 and a 4-bit value are exact in float32.  The tensor cores add 16 (32 or 64 with 4 bits on both sides) of
+    them to a sum at a time; an addition that cuts off instead of rounding loses up to 2^-23 of the sum of sizes so far, and joining
+    blocks, ranges and pieces is float32 additions of 2^-24 each: k / 16 + 16 times 2^-23 covers both.  bfloat16 results are rounded
+    once more, by 2^-9 of their power of two or less: 2^-8 of themselves."""
+    limit = size * (k / 16 + 16) * 2.0 ** -23
     if out.dtype is torch.bfloat16:
         limit = limit + (want.abs() + limit) * 2.0 ** -8
     off = (out.double() - want).abs()
@@ -124,3 +125,29 @@ def test_product_over_the_sizes(m, n, k, quantise):
         out = torch.full((m, n), float("nan"), device=DEV, dtype=dtype)
         kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
         close_to_sums(out, want, size, k, f"{m} x {n} x {k}")
+
+
+PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 1), ("many", 16, 3), ("many", 32, 1), ("many", 64, 2), ("many", 128, 1), ("many", 128, 4),
+         ("many", 256, 1), ("many", 256, 8)]
+
+
+@pytest.mark.parametrize("quantise", [False, True])
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080)])
+def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
+    if plan[0] == "many" and plan[1] < 128 and m > plan[1]:
+        pytest.skip("tiles of fewer than 128 tokens hold all of them")
+    if plan[0] == "few" and plan[1] < kernels.mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k):
+        pytest.skip("these rows do not fit the shared memory of so few CTAs")
+    g = torch.Generator(device=DEV).manual_seed(m * 31 + n * 7 + k)
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    values = plain_quantise(x)[0] if quantise else x.double()
+    want, size = values @ w.T, values.abs() @ w.abs().T
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((m, n), float("nan"), device=DEV, dtype=dtype)
+        kernels.mxfp4_gemm(x, weight, out, quantise=quantise, plan=plan)
+        torch.cuda.synchronize()
+        kernels.check_device_errors(certain=True)
+        close_to_sums(out, want, size, k, f"{m} x {n} x {k} {plan}")

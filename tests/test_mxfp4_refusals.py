@@ -62,9 +62,3 @@ def test_block_scales_reads_the_tiles():
                 m.scales[(r // 128 * tiles + b // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4] = want[r, b]
         assert torch.equal(m.block_scales(), want)
     assert matrix(0, 64).block_scales().shape == (0, 2)
-
-
-@pytest.mark.parametrize("n,k", [(1, 32), (128, 4096), (6144, 4096), (24576, 4096), (5120, 17408), (151936, 1024), (40, 65536)])
-def test_ranges_are_what_the_kernel_takes(n, k):
-    parts, cluster = kernels.mxfp4_few_rows_ranges(n, k, 148)
-    assert parts in (1, 2, 4, 8) and cluster in (1, 2, 4, 8) and (parts * cluster == 1 or parts * cluster <= -(-k // 256))
