@@ -4,6 +4,8 @@
 // even code, above 6 to 6), scale = 2^e.  The power of two makes the multiplication exact, so a code is one rounding away from x.
 // Four lanes share a block (eight elements each: a 16-byte load of bfloat16), sixteen lanes the four blocks whose scales are one
 // word; two exchanges find a block's largest.  The kernels are bound by bytes.
+#include <limits.h>
+
 #include "mxfp4.cuh"
 
 namespace {
@@ -104,6 +106,85 @@ __global__ void __launch_bounds__(THREADS) scales_to_tiles_kernel(const uint8_t*
     }
 }
 
+// The smallest and the largest scale byte of the blocks that are not all zeros, into range[0] and range[1] (which begin as 256 and -1).
+__global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int* __restrict__ range,
+                                                              long long rows, long long width, long long tiles_of_a_row) {
+    pdl_wait();
+    const long long blocks = width / MX_BLOCK, total = rows * blocks;
+    int low = 256, high = -1;
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
+        const long long row = i / blocks, block = i - row * blocks;
+        const int byte = scales[mx_scale_offset(row, block >> 2, tiles_of_a_row) + (block & 3)];
+        const uint4 c = *reinterpret_cast<const uint4*>(codes + i * 16);
+        if (((c.x | c.y | c.z | c.w) & 0x77777777u) != 0u || byte == 255) low = min(low, byte), high = max(high, byte);
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if ((threadIdx.x & 31) == 0) {
+        atomicMin(&range[0], low);
+        atomicMax(&range[1], high);
+    }
+}
+
+// Rows of bfloat16 as halfs times a power of two of the row's own: row r holds x 2^-exponents[r], its largest in [2^15, 2^16).  An element's
+// exponent field becomes itself less that of the largest, plus 30, its mantissa its seven bits and three zeros: exact, but for elements
+// 2^30 and more below the largest, rows below 2^-96 and what is not finite; exponents[r] is then HALFS_LOST and the row is not to be used.
+constexpr int HELD = 4;
+constexpr int HALFS_LOST = INT_MIN;
+__global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __restrict__ x, uint16_t* __restrict__ halfs, int* __restrict__ exponents,
+                                                                long long width) {
+    __shared__ uint32_t scratch[THREADS / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long row = blockIdx.x;
+    const uint4* from = reinterpret_cast<const uint4*>(x + row * width);
+    uint4* to = reinterpret_cast<uint4*>(halfs + row * width);
+    const int chunks = (int)(width >> 3);
+    uint4 held[HELD];
+    uint32_t largest = 0;
+    auto widen = [&](const uint4& v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) largest = __viaddmax_s16x2(w[p] & 0x7FFF7FFFu, 0u, largest);
+    };
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * THREADS + threadIdx.x;
+        held[j] = i < chunks ? from[i] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) widen(held[j]);
+    for (int i = HELD * THREADS + threadIdx.x; i < chunks; i += THREADS) widen(from[i]);
+    largest = __reduce_max_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16));
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) largest = max(largest, scratch[w]);
+    const int field = (int)(largest >> 7);
+    const bool zeros = largest == 0, ordinary = field >= 31 && field < 255;
+    const uint32_t down = zeros || !ordinary ? 0u : (uint32_t)(-((field - 30) << 7)) & 0xFFFFu, both = down | down << 16;
+    uint32_t lost = 0;
+    auto convert = [&](const uint4& v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const uint32_t size = w[p] & 0x7FFF7FFFu, r = __viaddmax_s16x2(size, both, 0u);
+            lost |= (size + 0x7FFF7FFFu) & ~(r + 0x7F807F80u);                // highest bit of each half: not 0, and below the halfs' smallest ordinary number
+            h[p] = (r << 3) | (w[p] & 0x80008000u);
+        }
+        return make_uint4(h[0], h[1], h[2], h[3]);
+    };
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * THREADS + threadIdx.x;
+        if (i < chunks) to[i] = convert(held[j]);
+    }
+    for (int i = HELD * THREADS + threadIdx.x; i < chunks; i += THREADS) to[i] = convert(from[i]);
+    const bool bad = __syncthreads_or((lost & 0x80008000u) != 0u) || !(zeros || ordinary);
+    if (threadIdx.x == 0) exponents[row] = bad ? HALFS_LOST : zeros ? 0 : field - 127 - 15;
+}
+
 // Blocks of a launch over `items` threads of work: loops over them where that is more than 16 blocks an SM.
 int blocks_for(long long items) {
     const long long want = (items + THREADS - 1) / THREADS, most = (long long)mrs_sm_count() * 64;
@@ -145,6 +226,23 @@ MRS_EXPORT int mrs_mxfp4_scales_to_tiles(const void* plain, void* codes, void* s
     if (bad_sizes(rows, width) || !plain || !codes || !scales || (((uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
     const long long tiles = mx_tiles_of_a_row(width);
     MRS_LAUNCH(scales_to_tiles_kernel, blocks_for(rows * tiles * 4), THREADS, 0, stream, (const uint8_t*)plain, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles);
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+// range: two ints, 256 and -1 to begin with.
+MRS_EXPORT int mrs_mxfp4_scale_range(const void* codes, const void* scales, void* range, long long rows, long long width, void* stream) {
+    if (rows == 0) return 0;
+    if (bad_sizes(rows, width) || !range || !codes || !scales || (((uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)range & 3)) return MRS_BAD_ARGUMENT;
+    MRS_LAUNCH(scale_range_kernel, blocks_for(rows * (width / MX_BLOCK)), THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (int*)range, rows, width,
+               mx_tiles_of_a_row(width));
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+// x [rows, width] bfloat16 to halfs [rows, width] and exponents [rows] int32; width a multiple of 8.
+MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* exponents, long long rows, long long width, void* stream) {
+    if (rows == 0) return 0;
+    if (bad_sizes(rows, width) || rows > 0x7FFFFFFF || !x || !halfs || !exponents || (((uintptr_t)x | (uintptr_t)halfs) & 15) || ((uintptr_t)exponents & 3)) return MRS_BAD_ARGUMENT;
+    MRS_LAUNCH(rows_to_halfs_kernel, (unsigned)rows, THREADS, 0, stream, (const bf16*)x, (uint16_t*)halfs, (int*)exponents, width);
     MRS_RETURN_LAUNCH_STATUS();
 }
 

@@ -1,15 +1,23 @@
 // Products of many rows with a matrix in microscaled 4-bit floating point on the tcgen05 tensor cores: out[m, n] = sum_k x[m, k] w[n, k],
-// float32 sums.  A CTA takes 128 rows of w (the M of the MMA, so that a few tokens fill a narrow N) and up to 256 tokens; the CTAs
-// of a cluster share a tile with a range of K each, and their sums meet in the ranges' order.
+// float32 sums.  A tile is 128 rows of w (the M of the MMA, so that a few tokens fill a narrow N) and up to 192 tokens.  CTAs walk
+// through tiles, neighbours through the tokens of the same weights, with two accumulators in tensor memory: a tile's results are
+// stored while the next tile's MMAs run.  With few tiles the CTAs of a cluster share one with a range of K each, and their sums meet
+// in the ranges' order.
 //
 //   weights_kernel   x in bfloat16.  Bulk tensor copies bring 128 x 256 codes (128-byte swizzle) and their scales into a ring, x in
-//                    pieces of 64 elements into another.  Eight warps make bfloat16 of the codes, a thread a row: code to half, half to
-//                    float32, times the block's power of two, two floats to a pair of bfloat16 (every step exact), into tensor memory as
-//                    the A operand; no shared memory is written for them.  One thread issues kind::f16 MMAs with A in tensor memory.
+//                    pieces of 128 elements into another.  Sixteen warps make the A operand of the codes, a thread a row and 64
+//                    elements, in tensor memory; no shared memory is written for it.  One thread issues kind::f16 MMAs.
+//                    Making A is what a scheduler has to do for each MMA: halfs are a conversion and a multiplication for two codes (9
+//                    clocks for eight codes of a warp), bfloat16 goes through float32 (21 clocks).  So x comes as halfs, times a
+//                    power of two a row, from a kernel before (mxfp4.cu), and w becomes halfs times one power of two of the matrix;
+//                    both powers go into the results.  All of it is exact: where a row of x does not fit the halfs' range without
+//                    losing a bit, or the matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead.
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
 //                    tensor memory (tcgen05.cp) stage by stage.
 //
 // Every wait is bounded (tma.cuh).
+#include <limits.h>
+
 #include "mxfp4.cuh"
 #include "tcgen05.cuh"
 
@@ -18,8 +26,6 @@ namespace {
 constexpr int BM = 128;                            // rows of w of a tile
 constexpr int STAGE_K = 256;                       // elements of K of a stage of codes: 128 bytes a row
 constexpr int CODE_BYTES = BM * 128, SCALE_BYTES = 2 * MX_TILE_BYTES;
-constexpr int WORKERS = 8;                         // warps that make bfloat16 and store results
-constexpr int THREADS = 64 + WORKERS * 32;
 constexpr int TMEM_COLUMNS = 512;
 constexpr int MOST_BYTES = 226 * 1024;             // of shared memory a CTA may have
 constexpr size_t ALONE_BYTES = 208 * 1024;         // with so much no other CTA that uses tensor memory fits the SM
@@ -31,6 +37,22 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// A whole warp's bounded wait, whose outcome is the same for the whole warp and whose loop the compiler does not see: what the warp walks
+// through stays in uniform registers, which the MMA and copy instructions take their operands from.  (With the loop of mbar_wait and
+// breaks lane by lane a step of MMAs took 510 clocks to issue, with this one XXX.)
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p, q;\n .reg .u64 start, now;\n"
+                 " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+                 " mov.u64 start, %%clock64;\n"
+                 "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+                 " mov.u64 now, %%clock64;\n sub.u64 now, now, start;\n setp.lt.u64 q, now, %3;\n @q bra AGAIN;\n"
+                 "DONE:\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "n"(MRS_WAIT_CYCLES) : "memory");
+    if (__all_sync(0xffffffffu, done != 0u)) return true;
+    mrs_raise(MRS_ERR_BARRIER_TIMEOUT);
+    return false;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
@@ -39,80 +61,131 @@ __device__ __forceinline__ void cluster_sync() {
 struct Shapes {
     int M, N, K;
     int token_tiles;
-    int cluster;
+    long long tiles;
+    int cluster;            // CTAs that share a tile; each then takes one tile only
     int early;              // w was there before the kernel before this one: it may be fetched while that runs
     long long w_tiles_of_a_row, x_row_tiles;
+    const int* x_exponents; // of x as halfs, a row each; null: x is bfloat16
+    int w_exponent;         // halfs are made of w times 2^-w_exponent
 };
 
-// The accumulator's results (lane: row of w, column: token) to memory; `sums` is shared memory for TOKENS x 128 floats, used by clusters only.
-// Called by every thread of the CTA; the workers read the accumulator.
-template <int TOKENS, typename Out>
-__device__ __forceinline__ void store_results(uint32_t tmem, float* sums, Out* __restrict__ out, const Shapes& s, long long n0, int token0, int rank,
-                                              bool empty) {
-    constexpr int STEP = TOKENS < 32 ? 16 : 32;
-    constexpr int GROUPS = TOKENS / STEP < 2 ? 1 : 2;                          // of four warps, that share the columns
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// What a CTA walks through: its tiles, and its range of K.
+struct Walk {
+    long long tile, step;
+    int rank, from, to;
+    __device__ __forceinline__ Walk(const Shapes& s) {
+        rank = blockIdx.x % s.cluster, tile = blockIdx.x / s.cluster, step = gridDim.x / s.cluster;
+        const int stages = (s.K + STAGE_K - 1) / STAGE_K;
+        from = range_start(stages, s.cluster, rank), to = range_start(stages, s.cluster, rank + 1);
+    }
+};
+
+// An accumulator's results (lane: row of w, column: token) to memory, or, with a cluster, into `sums` (TOKENS x 128 floats of shared
+// memory).  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes are those of its number modulo 4.
+template <int TOKENS, int WARPS, typename Out>
+__device__ __forceinline__ void store_accumulator(uint32_t accumulator, float* sums, Out* __restrict__ out, const Shapes& s, long long n0, int token0, int index,
+                                                  bool empty, bool halfs = false) {
+    constexpr int STEP = TOKENS < 32 ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
+    const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
     const int live = min(TOKENS, s.M - token0);
-    if (warp >= 2 && (warp - 2) >> 2 < GROUPS) {
-        const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;
-        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-        const long long n = n0 + row;
+    const uint32_t acc = accumulator + ((uint32_t)(quarter * 32) << 16);
+    const long long n = n0 + row;
 #pragma unroll 1
-        for (int c = group * STEP; c < TOKENS; c += GROUPS * STEP) {
-            if (c >= live) break;
-            float v[STEP];
-            if (!empty) {
-                if constexpr (STEP == 16) tmem_load_16_async(acc + c, v);
-                else tmem_load_32_async(acc + c, v);
-                tmem_load_wait();
-            } else {
+    for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
+        float v[STEP];
+        if (!empty) {
+            if constexpr (STEP == 16) tmem_load_16_async(acc + c, v);
+            else tmem_load_32_async(acc + c, v);
+            tmem_load_wait();
+        } else {
 #pragma unroll
-                for (int e = 0; e < STEP; ++e) v[e] = 0.0f;
-            }
-            if (s.cluster == 1) {
-                if (n < s.N) {
+            for (int e = 0; e < STEP; ++e) v[e] = 0.0f;
+        }
+        if (halfs) {                               // the rows' powers of two, all in the floats' range
+#pragma unroll
+            for (int e = 0; e < STEP; ++e)
+                v[e] *= __uint_as_float((uint32_t)(127 + s.w_exponent + (c + e < live ? __ldg(s.x_exponents + token0 + c + e) : -s.w_exponent)) << 23);
+        }
+        if (s.cluster == 1) {
+            if (n < s.N) {
+                Out* place = out + (size_t)(token0 + c) * s.N + n;
+                if (c + STEP <= live) {
+#pragma unroll
+                    for (int e = 0; e < STEP; ++e) place[(size_t)e * s.N] = from_float<Out>(v[e]);
+                } else {
 #pragma unroll
                     for (int e = 0; e < STEP; ++e)
-                        if (c + e < live) out[(size_t)(token0 + c + e) * s.N + n] = from_float<Out>(v[e]);
+                        if (c + e < live) place[(size_t)e * s.N] = from_float<Out>(v[e]);
                 }
-            } else {
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < STEP; ++e) sums[(c + e) * BM + row] = v[e];
-            }
+            for (int e = 0; e < STEP; ++e) sums[(c + e) * BM + row] = v[e];
         }
     }
-    if (s.cluster > 1) {
-        cluster_sync();
-        const uint32_t base = smem_u32(sums);
-        for (int i = rank * THREADS + threadIdx.x; i < live * BM; i += s.cluster * THREADS) {
-            float sum = 0.0f;
-            for (int c = 0; c < s.cluster; ++c) {
-                uint32_t there;
-                float v;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(base + i * 4), "r"(c));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-                sum += v;
-            }
-            const long long n = n0 + (i & (BM - 1));
-            if (n < s.N) out[(size_t)(token0 + i / BM) * s.N + n] = from_float<Out>(sum);
+}
+
+// The cluster's sums of a tile, in the order of the ranges of K, to memory.  Every thread of every CTA.
+template <int TOKENS, int THREADS, typename Out>
+__device__ __forceinline__ void join_cluster(const float* sums, Out* __restrict__ out, const Shapes& s, long long n0, int token0, int rank) {
+    const int live = min(TOKENS, s.M - token0);
+    cluster_sync();
+    const uint32_t base = smem_u32(sums);
+    for (int i = rank * THREADS + threadIdx.x; i < live * BM; i += s.cluster * THREADS) {
+        float sum = 0.0f;
+        for (int c = 0; c < s.cluster; ++c) {
+            uint32_t there;
+            float v;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(base + i * 4), "r"(c));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+            sum += v;
         }
-        cluster_sync();                            // a CTA's sums stay until its cluster has read them
+        const long long n = n0 + (i & (BM - 1));
+        if (n < s.N) out[(size_t)(token0 + i / BM) * s.N + n] = from_float<Out>(sum);
     }
+    cluster_sync();                            // a CTA's sums stay until its cluster has read them
 }
 
 // ------------------------------------------------------------------------------------------
 // x in bfloat16
 // ------------------------------------------------------------------------------------------
-constexpr int STEP_K = 64;                         // elements of K of a piece of x and of a buffer of A
-constexpr int A_BUFFERS = 8, A_COLUMNS = STEP_K / 2, A_FIRST = 256;
-constexpr int W_STAGES = 4, X_STAGES = 4;
+constexpr int STEP_K = 128;                        // elements of K of a piece of x and of a buffer of A: eight MMAs
+constexpr int HALF_K = 64;                         // a 128-byte row of x, and what one thread makes of its row at a time
+constexpr int STAGE_STEPS = STAGE_K / STEP_K;
+constexpr int MAKERS = 16, STORERS = 4;            // warps that make bfloat16, and that store results
+constexpr int W_THREADS = (3 + MAKERS + STORERS) * 32;
+constexpr int A_COLUMNS = STEP_K / 2;
+constexpr int W_STAGES = 4;
 template <int TOKENS> constexpr int x_bytes() { return TOKENS * STEP_K * 2; }
+template <int TOKENS> constexpr int x_stages() { return TOKENS > 128 ? 3 : 4; }
+template <int TOKENS> constexpr int a_first() { return TOKENS > 128 ? 2 * TOKENS : 256; }            // columns before it: two accumulators
+template <int TOKENS> constexpr int a_buffers() { return (TMEM_COLUMNS - a_first<TOKENS>()) / A_COLUMNS; }
 template <int TOKENS> constexpr size_t weights_smem() {
-    return 1024 + (size_t)W_STAGES * (CODE_BYTES + SCALE_BYTES) + (size_t)X_STAGES * x_bytes<TOKENS>() + 512;
+    return 1024 + (size_t)W_STAGES * (CODE_BYTES + SCALE_BYTES) + (size_t)x_stages<TOKENS>() * x_bytes<TOKENS>() + 512;
 }
 
-// 32 codes of a row and their scale as 16 pairs of bfloat16.
-__device__ __forceinline__ void decode_block(uint4 codes, float scale, uint32_t* words) {
+// 32 codes of a row as 16 pairs of halfs, times 2^(byte - 127 - w_exponent); only blocks of zeros have powers beyond [-23, 13].
+__device__ __forceinline__ void decode_block_halfs(uint4 codes, uint32_t byte, int w_exponent, uint32_t* words) {
+    const int d = max(min((int)byte - 127 - w_exponent, 15), -24);
+    const uint32_t bits = d >= -14 ? (uint32_t)(d + 15) << 10 : 1u << (d + 24), both = bits | bits << 16;
+    const __half2 scale = *reinterpret_cast<const __half2*>(&both);
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t h[4];
+        mx_decode_8(w[i], h);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const __half2 pair = __hmul2(*reinterpret_cast<const __half2*>(&h[p]), scale);
+            words[i * 4 + p] = *reinterpret_cast<const uint32_t*>(&pair);
+        }
+    }
+}
+// 32 codes of a row and their scale byte as 16 pairs of bfloat16.
+__device__ __forceinline__ void decode_block(uint4 codes, uint32_t byte, uint32_t* words) {
+    // 2^(byte - 127) as bfloat16: byte 0 under the ordinary numbers, byte 255 not a number
+    const uint32_t bits = byte == 0u ? 0x0040u : byte == 255u ? 0x7FC0u : byte << 7, both = bits | bits << 16;
+    const __nv_bfloat162 scale = *reinterpret_cast<const __nv_bfloat162*>(&both);
     const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -121,8 +194,8 @@ __device__ __forceinline__ void decode_block(uint4 codes, float scale, uint32_t*
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             const float2 v = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
-            __nv_bfloat162 pair = __floats2bfloat162_rn(v.x * scale, v.y * scale);
-            words[i * 4 + p] = *reinterpret_cast<uint32_t*>(&pair);
+            const __nv_bfloat162 pair = __hmul2(__floats2bfloat162_rn(v.x, v.y), scale);
+            words[i * 4 + p] = *reinterpret_cast<const uint32_t*>(&pair);
         }
     }
 }
@@ -136,10 +209,12 @@ __device__ __forceinline__ void tmem_store_32_words(uint32_t address, const uint
 }
 
 template <int TOKENS, typename Out>
-__global__ void __launch_bounds__(THREADS, 1) weights_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
-                                                             const uint8_t* __restrict__ scales, Out* __restrict__ out, const Shapes s) {
+__global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                                                               const __grid_constant__ CUtensorMap halfs_map, const uint8_t* __restrict__ scales,
+                                                               Out* __restrict__ out, const Shapes s) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int A_FIRST = a_first<TOKENS>(), A_BUFFERS = a_buffers<TOKENS>(), ACCUMULATOR = A_FIRST / 2, X_STAGES = x_stages<TOKENS>();
     unsigned char* w_ring = smem;
     unsigned char* x_ring = w_ring + W_STAGES * CODE_BYTES;
     unsigned char* s_ring = x_ring + X_STAGES * x_bytes<TOKENS>();
@@ -150,29 +225,31 @@ __global__ void __launch_bounds__(THREADS, 1) weights_kernel(const __grid_consta
     uint64_t* a_full = x_empty + X_STAGES;
     uint64_t* a_empty = a_full + A_BUFFERS;
     uint64_t* acc_full = a_empty + A_BUFFERS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % s.cluster, tile = blockIdx.x / s.cluster;
-    const int token0 = tile % s.token_tiles * TOKENS, n_tile = tile / s.token_tiles;
-    const int stages = (s.K + STAGE_K - 1) / STAGE_K, steps = (s.K + STEP_K - 1) / STEP_K;
-    const int from = range_start(stages, s.cluster, rank), to = range_start(stages, s.cluster, rank + 1);
-    const int step_from = from * (STAGE_K / STEP_K), step_to = min(to * (STAGE_K / STEP_K), steps);
+    const Walk walk(s);
+    // the range's stages; the last stage of K may hold fewer steps
+    const int steps = min(walk.to * STAGE_STEPS, (s.K + STEP_K - 1) / STEP_K) - walk.from * STAGE_STEPS;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < W_STAGES; ++i) {
             mbar_init(&w_full[i], 1);
-            mbar_init(&w_empty[i], WORKERS);
+            mbar_init(&w_empty[i], MAKERS);
         }
         for (int i = 0; i < X_STAGES; ++i) {
             mbar_init(&x_full[i], 1);
             mbar_init(&x_empty[i], 1);
         }
         for (int i = 0; i < A_BUFFERS; ++i) {
-            mbar_init(&a_full[i], 4);
+            mbar_init(&a_full[i], 8);
             mbar_init(&a_empty[i], 1);
         }
-        mbar_init(acc_full, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], STORERS);
+        }
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -185,100 +262,156 @@ __global__ void __launch_bounds__(THREADS, 1) weights_kernel(const __grid_consta
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
 
+    // The codes' first stages are on their way before anything else; then, once the kernel before has ended, whether all of x is there as
+    // halfs whose powers, with the matrix's, are ordinary floats.
+    const int ahead = s.early && walk.tile < s.tiles ? min(W_STAGES, walk.to - walk.from) : 0;
+    auto load_codes = [&](int n_tile, int stage, int slot) {
+        mbar_arrive_expect_tx(&w_full[slot], CODE_BYTES + SCALE_BYTES);
+        tma_load_2d(w_ring + slot * CODE_BYTES, &w_map, &w_full[slot], stage * 128, n_tile * BM);
+        bulk_load(s_ring + slot * SCALE_BYTES, scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &w_full[slot]);
+    };
+    if (warp == 2 + MAKERS + STORERS) {
+        if (elect_one())
+            for (int i = 0; i < ahead; ++i) load_codes((int)(walk.tile / s.token_tiles), walk.from + i, i);
+        __syncwarp();
+    }
+    pdl_wait();
+    bool halfs = false;
+    if (s.x_exponents) {
+        bool fit = true;
+        for (int i = threadIdx.x; i < s.M; i += W_THREADS) {
+            const int e = s.x_exponents[i];
+            fit = fit && e != INT_MIN && e + s.w_exponent >= -126 && e + s.w_exponent <= 127;
+        }
+        halfs = __syncthreads_and(fit);
+    }
+
+    // Codes and x come by the hands of two warps: a wait for the makers must not hold up x, whose pieces free up MMA by MMA.
     if (warp == 0) {
         const bool leader = elect_one();
-        if (!s.early) pdl_wait();
-        bool waited = !s.early, alive = true;
-        int w_next = from, x_next = step_from;
-        // codes run ahead of x by as much as their ring holds
-        while (alive && (w_next < to || x_next < step_to)) {
-            if (w_next < to && (w_next - from < W_STAGES || x_next >= (w_next - W_STAGES + 1) * (STAGE_K / STEP_K) || x_next >= step_to)) {
-                const int i = (w_next - from) % W_STAGES;
-                if (!(alive = mbar_wait(&w_empty[i], (((w_next - from) / W_STAGES) & 1) ^ 1))) break;
+        const CUtensorMap* map = halfs ? &halfs_map : &x_map;
+        bool alive = true;
+        int slot = 0;
+        uint32_t phase = 1;
+        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step) {
+            const int token0 = (int)(tile % s.token_tiles) * TOKENS;
+            for (int step = 0; step < steps; ++step) {
+                if (!(alive = warp_wait(&x_empty[slot], phase))) break;
                 if (leader) {
-                    mbar_arrive_expect_tx(&w_full[i], CODE_BYTES + SCALE_BYTES);
-                    tma_load_2d(w_ring + i * CODE_BYTES, &w_map, &w_full[i], w_next * 128, n_tile * BM);
-                    bulk_load(s_ring + i * SCALE_BYTES, scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * w_next) * MX_TILE_BYTES, SCALE_BYTES, &w_full[i]);
+                    mbar_arrive_expect_tx(&x_full[slot], x_bytes<TOKENS>());
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_2d(x_ring + slot * x_bytes<TOKENS>() + h * (TOKENS * 128), map, &x_full[slot], (walk.from * STAGE_STEPS + step) * STEP_K + h * HALF_K,
+                                    token0);
                 }
                 __syncwarp();
-                ++w_next;
-                continue;
+                if (++slot == X_STAGES) slot = 0, phase ^= 1;
             }
-            if (!waited) {
-                pdl_wait();
-                waited = true;
-            }
-            const int i = (x_next - step_from) % X_STAGES;
-            if (!(alive = mbar_wait(&x_empty[i], (((x_next - step_from) / X_STAGES) & 1) ^ 1))) break;
-            if (leader) {
-                mbar_arrive_expect_tx(&x_full[i], x_bytes<TOKENS>());
-                tma_load_2d(x_ring + i * x_bytes<TOKENS>(), &x_map, &x_full[i], x_next * STEP_K, token0);
-            }
-            __syncwarp();
-            ++x_next;
         }
-        if (!waited) pdl_wait();
-    } else if (warp == 1) {
-        pdl_wait();
+    } else if (warp == 2 + MAKERS + STORERS) {
         const bool leader = elect_one();
-        constexpr uint32_t idesc = umma_idesc_bf16_f32(BM, TOKENS);
         bool alive = true;
-        for (int step = step_from; step < step_to && alive; ++step) {
-            const int index = step - step_from, b = index % A_BUFFERS, i = index % X_STAGES;
-            if (!(alive = mbar_wait(&x_full[i], (index / X_STAGES) & 1))) break;
-            if (!(alive = mbar_wait(&a_full[b], (index / A_BUFFERS) & 1))) break;
+        int slot = 0;
+        uint32_t phase = 1;
+        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step) {
+            const int n_tile = (int)(tile / s.token_tiles);
+            for (int stage = walk.from; stage < walk.to; ++stage) {
+                if (!(alive = warp_wait(&w_empty[slot], phase))) break;
+                if (leader && (stage - walk.from >= ahead || tile != walk.tile)) load_codes(n_tile, stage, slot);
+                __syncwarp();
+                if (++slot == W_STAGES) slot = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        const bool leader = elect_one();
+        const uint32_t idesc = umma_idesc_bf16_f32(BM, TOKENS) & (halfs ? ~((1u << 7) | (1u << 10)) : ~0u);      // both operands halfs, or both bfloat16
+        bool alive = true;
+        int x_slot = 0, a_slot = 0, round = 0;
+        uint32_t x_phase = 0, a_phase = 0;
+        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step, ++round) {
+            const int buffer = round & 1;
+            if (!(alive = warp_wait(&acc_empty[buffer], ((round >> 1) & 1) ^ 1))) break;
             tcgen05_fence_after_sync();
-            const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + i * x_bytes<TOKENS>()));
-            const uint32_t a_tmem = tmem + A_FIRST + b * A_COLUMNS;
-            if (leader) {
-#pragma unroll
-                for (int k = 0; k < STEP_K / 16; ++k) umma_bf16_a_tmem(tmem, a_tmem + 8 * k, b_desc + 2 * k, idesc, index > 0 || k > 0);
-                umma_commit(&x_empty[i]);
-                umma_commit(&a_empty[b]);
-            }
-            __syncwarp();
-        }
-        if (leader) umma_commit(acc_full);
-        __syncwarp();
-    } else {
-        pdl_wait();
-        const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;
-        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        bool alive = true;
-        for (int stage = from; stage < to && alive; ++stage) {
-            const int i = (stage - from) % W_STAGES;
-            if (!(alive = mbar_wait(&w_full[i], ((stage - from) / W_STAGES) & 1))) break;
-            const unsigned char* codes = w_ring + i * CODE_BYTES + row * 128;
-            const unsigned char* scale_tiles = s_ring + i * SCALE_BYTES + lane * 16 + quarter * 4;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {                            // steps `group` and 2 + group of the stage
-                const int within = half * 2 + group, step = stage * (STAGE_K / STEP_K) + within, index = step - step_from;
-                if (step >= step_to) break;
-                const uint32_t four = *reinterpret_cast<const uint32_t*>(scale_tiles + half * MX_TILE_BYTES) >> (group * 16);
-                const uint4 first = *reinterpret_cast<const uint4*>(codes + (((within * 2) ^ (row & 7)) << 4));
-                const uint4 second = *reinterpret_cast<const uint4*>(codes + (((within * 2 + 1) ^ (row & 7)) << 4));
-                uint32_t words[32];
-                decode_block(first, mx_scale(four & 255u), words);
-                decode_block(second, mx_scale((four >> 8) & 255u), words + 16);
-                const int b = index % A_BUFFERS;
-                if (!(alive = mbar_wait(&a_empty[b], ((index / A_BUFFERS) & 1) ^ 1))) break;
-                __syncwarp();
+            const uint32_t d_tmem = tmem + buffer * ACCUMULATOR;
+            for (int step = 0; step < steps; ++step) {
+                if (!(alive = warp_wait(&x_full[x_slot], x_phase))) break;
+                if (!(alive = warp_wait(&a_full[a_slot], a_phase))) break;
                 tcgen05_fence_after_sync();
-                tmem_store_32_words(lanes + A_FIRST + b * A_COLUMNS, words);
-                tmem_store_wait();
-                tcgen05_fence_before_sync();
+                const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + x_slot * x_bytes<TOKENS>()));
+                const uint32_t a_tmem = tmem + A_FIRST + a_slot * A_COLUMNS;
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < STEP_K / 16; ++k)
+                        umma_bf16_a_tmem(d_tmem, a_tmem + 8 * k, b_desc + (k >> 2) * (TOKENS * 128 / 16) + 2 * (k & 3), idesc, step > 0 || k > 0);
+                    umma_commit(&x_empty[x_slot]);
+                    umma_commit(&a_empty[a_slot]);
+                }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[b]);
+                if (++x_slot == X_STAGES) x_slot = 0, x_phase ^= 1;
+                if (++a_slot == A_BUFFERS) a_slot = 0, a_phase ^= 1;
             }
+            if (leader) umma_commit(&acc_full[buffer]);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&w_empty[i]);
         }
-        mbar_wait(acc_full, 0);
-        __syncwarp();
-        tcgen05_fence_after_sync();
+    } else if (warp < 2 + MAKERS) {
+        const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;        // group: a stage's quarter of K
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + A_FIRST;
+        const uint32_t first_chunk = ((group * 2) ^ (row & 7)) << 4, second_chunk = ((group * 2 + 1) ^ (row & 7)) << 4;
+        const int scale_place = (group >> 1) * MX_TILE_BYTES + lane * 16 + quarter * 4 + (group & 1) * 2;
+        bool alive = true;
+        int w_slot = 0, round = 0;
+        uint32_t w_phase = 0;
+        long long before = 0;                                                                    // steps of the tiles before
+        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step, ++round, before += steps) {
+            for (int stage = 0; stage < walk.to - walk.from; ++stage) {
+                if (!(alive = warp_wait(&w_full[w_slot], w_phase))) break;
+                const int step = stage * STAGE_STEPS + (group >> 1);
+                if (step < steps) {
+                    const unsigned char* codes = w_ring + w_slot * CODE_BYTES + row * 128;
+                    const uint32_t two = *reinterpret_cast<const uint16_t*>(s_ring + w_slot * SCALE_BYTES + scale_place);
+                    const uint4 first = *reinterpret_cast<const uint4*>(codes + first_chunk);
+                    const uint4 second = *reinterpret_cast<const uint4*>(codes + second_chunk);
+                    uint32_t words[32];
+                    if (halfs) {
+                        decode_block_halfs(first, two & 255u, s.w_exponent, words);
+                        decode_block_halfs(second, two >> 8, s.w_exponent, words + 16);
+                    } else {
+                        decode_block(first, two & 255u, words);
+                        decode_block(second, two >> 8, words + 16);
+                    }
+                    const long long index = before + step;
+                    const int b = (int)(index % A_BUFFERS);
+                    if (!(alive = warp_wait(&a_empty[b], (uint32_t)((index / A_BUFFERS) & 1) ^ 1))) break;
+                    __syncwarp();
+                    tcgen05_fence_after_sync();
+                    tmem_store_32_words(lanes + b * A_COLUMNS + (group & 1) * (A_COLUMNS / 2), words);
+                    tmem_store_wait();
+                    tcgen05_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&a_full[b]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&w_empty[w_slot]);
+                if (++w_slot == W_STAGES) w_slot = 0, w_phase ^= 1;
+            }
+        }
+    } else {
+        int round = 0;
+        for (long long tile = walk.tile; tile < s.tiles; tile += walk.step, ++round) {
+            const int buffer = round & 1;
+            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
+            tcgen05_fence_after_sync();
+            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, reinterpret_cast<float*>(smem), out, s, tile / s.token_tiles * BM,
+                                                    (int)(tile % s.token_tiles) * TOKENS, warp - 2 - MAKERS, steps <= 0, halfs);
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buffer]);
+        }
     }
     __syncwarp();
-    store_results<TOKENS, Out>(tmem, reinterpret_cast<float*>(smem), out, s, (long long)n_tile * BM, token0, rank, step_from >= step_to);
+    if (s.cluster > 1)
+        join_cluster<TOKENS, W_THREADS, Out>(reinterpret_cast<const float*>(smem), out, s, walk.tile / s.token_tiles * BM, (int)(walk.tile % s.token_tiles) * TOKENS,
+                                             walk.rank);
     tcgen05_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
@@ -313,15 +446,17 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t columns, uint32_t smem_a
 }
 
 constexpr int B_STAGES = 4;
+constexpr int B_STORERS = 8, B_THREADS = 64 + B_STORERS * 32;
 template <int TOKENS> constexpr int token_blocks() { return TOKENS > 128 ? 2 : 1; }            // tiles of scales of the tokens
 template <int TOKENS> constexpr int both_stage_bytes() { return CODE_BYTES + TOKENS * 128 + SCALE_BYTES * (1 + token_blocks<TOKENS>()); }
 template <int TOKENS> constexpr size_t both_smem() { return 1024 + (size_t)B_STAGES * both_stage_bytes<TOKENS>() + 256; }
-constexpr int SCALES_FIRST = 256, SCALE_COLUMNS = 32;      // tensor memory columns of a stage's scales (up to 8 + 16 used)
+// Tensor memory: two accumulators of up to 192 columns, then a stage's scales in 32 columns: 2 x 4 of w, 2 x 8 of the tokens.
+constexpr int B_ACCUMULATOR = 192, SCALES_FIRST = 2 * B_ACCUMULATOR, SCALE_COLUMNS = 32;
 
 template <int TOKENS, typename Out>
-__global__ void __launch_bounds__(THREADS, 1) both_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
-                                                          const uint8_t* __restrict__ w_scales, const uint8_t* __restrict__ x_scales, Out* __restrict__ out,
-                                                          const Shapes s) {
+__global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                                                            const uint8_t* __restrict__ w_scales, const uint8_t* __restrict__ x_scales, Out* __restrict__ out,
+                                                            const Shapes s) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* w_ring = smem;
@@ -331,20 +466,22 @@ __global__ void __launch_bounds__(THREADS, 1) both_kernel(const __grid_constant_
     uint64_t* full = reinterpret_cast<uint64_t*>(s_ring + B_STAGES * STAGE_SCALES);
     uint64_t* empty = full + B_STAGES;
     uint64_t* acc_full = empty + B_STAGES;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
-    const int warp = threadIdx.x >> 5;
-    const int rank = blockIdx.x % s.cluster, tile = blockIdx.x / s.cluster;
-    const int token0 = tile % s.token_tiles * TOKENS, n_tile = tile / s.token_tiles;
-    const int stages = (s.K + STAGE_K - 1) / STAGE_K;
-    const int from = range_start(stages, s.cluster, rank), to = range_start(stages, s.cluster, rank + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Walk walk(s);
+    const int depth = walk.to - walk.from;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < B_STAGES; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        mbar_init(acc_full, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], B_STORERS);
+        }
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -359,71 +496,97 @@ __global__ void __launch_bounds__(THREADS, 1) both_kernel(const __grid_constant_
 
     if (warp == 0) {
         const bool leader = elect_one();
-        // w first, as far as the ring goes, then x once the kernel before has ended
-        const int ahead = s.early ? min(B_STAGES, to - from) : 0;
-        auto load_w = [&](int stage, int i) {
+        // the first stages of w, as far as the ring goes, before the kernel before has ended
+        const int ahead = s.early && walk.tile < s.tiles ? min(B_STAGES, depth) : 0;
+        auto load_w = [&](int n_tile, int stage, int i) {
             mbar_arrive_expect_tx(&full[i], CODE_BYTES + TOKENS * 128 + STAGE_SCALES);
             tma_load_2d(w_ring + i * CODE_BYTES, &w_map, &full[i], stage * 128, n_tile * BM);
             bulk_load(s_ring + i * STAGE_SCALES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[i]);
         };
         if (leader)
-            for (int i = 0; i < ahead; ++i) load_w(from + i, i);
+            for (int i = 0; i < ahead; ++i) load_w((int)(walk.tile / s.token_tiles), walk.from + i, i);
         __syncwarp();
         pdl_wait();
         bool alive = true;
-        for (int stage = from; stage < to && alive; ++stage) {
-            const int index = stage - from, i = index % B_STAGES;
-            if (!(alive = mbar_wait(&empty[i], ((index / B_STAGES) & 1) ^ 1))) break;
-            if (leader) {
-                if (index >= ahead) load_w(stage, i);
-                tma_load_2d(x_ring + i * TOKENS * 128, &x_map, &full[i], stage * 128, token0);
+        int slot = 0;
+        uint32_t phase = 1;
+        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step) {
+            const int token0 = (int)(tile % s.token_tiles) * TOKENS, n_tile = (int)(tile / s.token_tiles);
+            for (int index = 0; index < depth; ++index) {
+                const int stage = walk.from + index;
+                if (!(alive = warp_wait(&empty[slot], phase))) break;
+                if (leader) {
+                    if (index >= ahead || tile != walk.tile) load_w(n_tile, stage, slot);
+                    tma_load_2d(x_ring + slot * TOKENS * 128, &x_map, &full[slot], stage * 128, token0);
 #pragma unroll
-                for (int t = 0; t < token_blocks<TOKENS>(); ++t) {
-                    const long long row_tile = min((long long)(token0 >> 7) + t, s.x_row_tiles - 1);      // a tile behind the last token: nobody stores its sums
-                    bulk_load(s_ring + i * STAGE_SCALES + SCALE_BYTES * (1 + t), x_scales + ((size_t)row_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES,
-                              SCALE_BYTES, &full[i]);
+                    for (int t = 0; t < token_blocks<TOKENS>(); ++t) {
+                        const long long row_tile = min((long long)(token0 >> 7) + t, s.x_row_tiles - 1);      // a tile behind the last token: nobody stores its sums
+                        bulk_load(s_ring + slot * STAGE_SCALES + SCALE_BYTES * (1 + t),
+                                  x_scales + ((size_t)row_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[slot]);
+                    }
                 }
+                __syncwarp();
+                if (++slot == B_STAGES) slot = 0, phase ^= 1;
             }
-            __syncwarp();
         }
     } else if (warp == 1) {
         pdl_wait();
         const bool leader = elect_one();
         bool alive = true;
-        for (int stage = from; stage < to && alive; ++stage) {
-            const int index = stage - from, i = index % B_STAGES;
-            if (!(alive = mbar_wait(&full[i], (index / B_STAGES) & 1))) break;
+        int slot = 0, round = 0;
+        uint32_t phase = 0;
+        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step, ++round) {
+            const int buffer = round & 1;
+            if (!(alive = warp_wait(&acc_empty[buffer], ((round >> 1) & 1) ^ 1))) break;
             tcgen05_fence_after_sync();
-            const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(w_ring + i * CODE_BYTES));
-            const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + i * TOKENS * 128));
-            const uint32_t scales = smem_u32(s_ring + i * STAGE_SCALES);
-            const uint32_t columns = tmem + SCALES_FIRST + i * SCALE_COLUMNS;
-            if (leader) {
+            const uint32_t d_tmem = tmem + buffer * B_ACCUMULATOR;
+            // tiles of 192 tokens begin in the middle of a tile of scales every other time: two columns, 64 tokens, further in
+            const uint32_t shift = TOKENS == 192 ? (((uint32_t)(tile % s.token_tiles) * TOKENS) & 127u) / 32 : 0u;
+            for (int index = 0; index < depth; ++index) {
+                if (!(alive = warp_wait(&full[slot], phase))) break;
+                tcgen05_fence_after_sync();
+                const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(w_ring + slot * CODE_BYTES));
+                const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + slot * TOKENS * 128));
+                const uint32_t scales = smem_u32(s_ring + slot * STAGE_SCALES);
+                const uint32_t columns = tmem + SCALES_FIRST + slot * SCALE_COLUMNS;
+                if (leader) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {                                   // 128 elements of K
-                    scales_to_tmem(columns + q * 4, scales + q * MX_TILE_BYTES);
+                    for (int q = 0; q < 2; ++q) {                                   // 128 elements of K
+                        scales_to_tmem(columns + q * 4, scales + q * MX_TILE_BYTES);
 #pragma unroll
-                    for (int t = 0; t < token_blocks<TOKENS>(); ++t)
-                        scales_to_tmem(columns + 8 + q * 8 + t * 4, scales + SCALE_BYTES * (1 + t) + q * MX_TILE_BYTES);
+                        for (int t = 0; t < token_blocks<TOKENS>(); ++t)
+                            scales_to_tmem(columns + 8 + q * 8 + t * 4, scales + SCALE_BYTES * (1 + t) + q * MX_TILE_BYTES);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_mxf4(d_tmem, a_desc + 2 * k, b_desc + 2 * k, mxf4_idesc(BM, TOKENS, (k & 1) * 2), columns + (k >> 1) * 4,
+                                  columns + 8 + (k >> 1) * 8 + shift, index > 0 || k > 0);
+                    umma_commit(&empty[slot]);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_mxf4(tmem, a_desc + 2 * k, b_desc + 2 * k, mxf4_idesc(BM, TOKENS, (k & 1) * 2), columns + (k >> 1) * 4, columns + 8 + (k >> 1) * 8,
-                              index > 0 || k > 0);
-                umma_commit(&empty[i]);
+                __syncwarp();
+                if (++slot == B_STAGES) slot = 0, phase ^= 1;
             }
+            if (leader) umma_commit(&acc_full[buffer]);
             __syncwarp();
         }
-        if (leader) umma_commit(acc_full);
-        __syncwarp();
     } else {
         pdl_wait();
-        mbar_wait(acc_full, 0);
-        __syncwarp();
-        tcgen05_fence_after_sync();
+        int round = 0;
+        for (long long tile = walk.tile; tile < s.tiles; tile += walk.step, ++round) {
+            const int buffer = round & 1;
+            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
+            tcgen05_fence_after_sync();
+            store_accumulator<TOKENS, B_STORERS, Out>(tmem + buffer * B_ACCUMULATOR, reinterpret_cast<float*>(smem), out, s, tile / s.token_tiles * BM,
+                                                      (int)(tile % s.token_tiles) * TOKENS, warp - 2, depth <= 0);
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buffer]);
+        }
     }
     __syncwarp();
-    store_results<TOKENS, Out>(tmem, reinterpret_cast<float*>(smem), out, s, (long long)n_tile * BM, token0, rank, from >= to);
+    if (s.cluster > 1)
+        join_cluster<TOKENS, B_THREADS, Out>(reinterpret_cast<const float*>(smem), out, s, walk.tile / s.token_tiles * BM, (int)(walk.tile % s.token_tiles) * TOKENS,
+                                             walk.rank);
     tcgen05_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
@@ -445,19 +608,20 @@ int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, long 
 }
 
 template <typename... KernelArgs, typename... Args>
-int launch_cluster(void (*kernel)(KernelArgs...), PerDevice& configured, long long ctas, int cluster, size_t smem, void* stream, Args... args) {
+int launch_cluster(void (*kernel)(KernelArgs...), PerDevice& configured, int threads, long long tiles, int sms, int cluster, size_t smem, void* stream, Args... args) {
     if (!configured.get()) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BYTES);
         if (e != cudaSuccess) return (int)e;
         configured.set(1);
     }
+    const long long ctas = cluster > 1 ? tiles * cluster : tiles < sms ? tiles : sms;
     if (ctas > 0x7FFFFFFFll) return MRS_BAD_ARGUMENT;
     // A CTA that waits for its cluster keeps its tensor memory meanwhile: clusters that wait for one another's would wait for good, so they
     // take whole SMs.
     if (cluster > 1 && smem < ALONE_BYTES) smem = ALONE_BYTES;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)ctas);
-    config.blockDim = dim3(THREADS);
+    config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attributes[2];
@@ -473,19 +637,21 @@ int launch_cluster(void (*kernel)(KernelArgs...), PerDevice& configured, long lo
 }
 
 template <int TOKENS, typename Out>
-int launch_weights(const void* x, const void* codes, const void* scales, void* out, Shapes s, void* stream) {
-    CUtensorMap w_map, x_map;
+int launch_weights(const void* x, const void* x_halfs, const void* codes, const void* scales, void* out, Shapes s, int sms, void* stream) {
+    CUtensorMap w_map, x_map, halfs_map;
     int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
-    if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, STEP_K, TOKENS);
+    if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, HALF_K, TOKENS);
+    halfs_map = x_map;
+    if (!code && s.x_exponents) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, HALF_K, TOKENS);
     if (code) return code;
     static PerDevice configured;
     s.token_tiles = (s.M + TOKENS - 1) / TOKENS;
-    const long long tiles = (long long)((s.N + BM - 1) / BM) * s.token_tiles;
-    return launch_cluster(weights_kernel<TOKENS, Out>, configured, tiles * s.cluster, s.cluster, weights_smem<TOKENS>(), stream, w_map, x_map,
+    s.tiles = (long long)((s.N + BM - 1) / BM) * s.token_tiles;
+    return launch_cluster(weights_kernel<TOKENS, Out>, configured, W_THREADS, s.tiles, sms, s.cluster, weights_smem<TOKENS>(), stream, w_map, x_map, halfs_map,
                           (const uint8_t*)scales, (Out*)out, s);
 }
 template <int TOKENS, typename Out>
-int launch_both(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, Shapes s, void* stream) {
+int launch_both(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, Shapes s, int sms, void* stream) {
     CUtensorMap w_map, x_map;
     int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
     if (!code) code = make_map(&x_map, x_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.M, 128, TOKENS);
@@ -493,8 +659,8 @@ int launch_both(const void* x_codes, const void* x_scales, const void* codes, co
     static PerDevice configured;
     s.token_tiles = (s.M + TOKENS - 1) / TOKENS;
     s.x_row_tiles = (s.M + 127) / 128;
-    const long long tiles = (long long)((s.N + BM - 1) / BM) * s.token_tiles;
-    return launch_cluster(both_kernel<TOKENS, Out>, configured, tiles * s.cluster, s.cluster, both_smem<TOKENS>(), stream, w_map, x_map,
+    s.tiles = (long long)((s.N + BM - 1) / BM) * s.token_tiles;
+    return launch_cluster(both_kernel<TOKENS, Out>, configured, B_THREADS, s.tiles, sms, s.cluster, both_smem<TOKENS>(), stream, w_map, x_map,
                           (const uint8_t*)scales, (const uint8_t*)x_scales, (Out*)out, s);
 }
 
@@ -506,27 +672,29 @@ bool bad(const void* x, const void* codes, const void* scales, const void* out, 
 
 }  // namespace
 
-// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16; w as in mxfp4.cuh.  `tokens` (16, 32, 64, 128, 256): of a tile, below 128 only
-// if they are all; `cluster` 1 to 8 ranges of K.  `early`: nothing that still runs when this kernel starts writes w.
-MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int tokens,
-                                      int cluster, int early, void* stream) {
+// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16, also as halfs with exponents (mxfp4.cu) or null; w as in mxfp4.cuh, whose blocks
+// other than zeros have scales of 2^(w_exponent - 23) to 2^(w_exponent + 13) if halfs are given.  `tokens` (16, 32, 64, 128, 192): of a tile, below 128 only
+// if they are all; `cluster` 1 to 8 ranges of K; `ctas`: the GPU's SMs.  `early`: nothing that still runs when this kernel starts writes w.
+MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const void* x_exponents, int w_exponent, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int tokens,
+                                      int cluster, int ctas, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
     if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, cluster)) return MRS_BAD_ARGUMENT;
-    const Shapes s = {M, N, K, 0, cluster, early, mx_tiles_of_a_row(K), 0};
-#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_weights<T, float>(x, codes, scales, out, s, stream) : launch_weights<T, bf16>(x, codes, scales, out, s, stream)
-    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(256);
+    if ((x_halfs == nullptr) != (x_exponents == nullptr) || ((uintptr_t)x_halfs & 15) || ((uintptr_t)x_exponents & 3)) return MRS_BAD_ARGUMENT;
+    const Shapes s = {M, N, K, 0, 0, cluster, early, mx_tiles_of_a_row(K), 0, (const int*)x_exponents, w_exponent};
+#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_weights<T, float>(x, x_halfs, codes, scales, out, s, ctas, stream) : launch_weights<T, bf16>(x, x_halfs, codes, scales, out, s, ctas, stream)
+    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
 #undef MRS_TOKENS
     return MRS_BAD_ARGUMENT;
 }
 
 // The same with x in 4 bits.
 MRS_EXPORT int mrs_mxfp4_both_rows(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K,
-                                   int tokens, int cluster, int early, void* stream) {
+                                   int tokens, int cluster, int ctas, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
     if (bad(x_codes, codes, scales, out, out_f32, M, N, K, tokens, cluster) || !x_scales || ((uintptr_t)x_scales & 15)) return MRS_BAD_ARGUMENT;
-    const Shapes s = {M, N, K, 0, cluster, early, mx_tiles_of_a_row(K), 0};
-#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_both<T, float>(x_codes, x_scales, codes, scales, out, s, stream) : launch_both<T, bf16>(x_codes, x_scales, codes, scales, out, s, stream)
-    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(256);
+    const Shapes s = {M, N, K, 0, 0, cluster, early, mx_tiles_of_a_row(K), 0, nullptr, 0};
+#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_both<T, float>(x_codes, x_scales, codes, scales, out, s, ctas, stream) : launch_both<T, bf16>(x_codes, x_scales, codes, scales, out, s, ctas, stream)
+    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
 #undef MRS_TOKENS
     return MRS_BAD_ARGUMENT;
 }

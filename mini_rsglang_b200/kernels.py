@@ -2569,8 +2569,10 @@ _MXFP4_SIGNATURES = {
     "mrs_mxfp4_scales_to_tiles": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
     "mrs_mxfp4_few_rows_cluster": [_c_int, _c_int],
-    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
-    "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_scale_range": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
+    "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
+    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
     "mrs_mxfp4_take_error": [ctypes.POINTER(ctypes.c_uint)],
 }
 _mxfp4_lib = None
@@ -2618,13 +2620,28 @@ class Mxfp4:
     mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), for every 32 neighbours of a row one power of two.
 
     `codes` uint8 [rows, width / 2] (element 2 j in the low half of byte j), `scales` uint8 in the tiles that the tensor
-    cores read (`csrc/kernels/mxfp4.cuh`).  `settled`: the matrix was there before anything that is still queued, and nothing
-    writes it any more, so that a product may fetch it while the kernel before still runs."""
+    cores read (`csrc/kernels/mxfp4.cuh`).  `settled` (`settle()`): the matrix was there before anything that is still queued, and
+    nothing writes it any more, so that a product may fetch it while the kernel before still runs; `half_exponent` is then the
+    power by which all of it fits halfs exactly, or None."""
 
-    __slots__ = ("codes", "scales", "rows", "width", "settled")
+    __slots__ = ("codes", "scales", "rows", "width", "settled", "half_exponent")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int, settled: bool = False):
-        self.codes, self.scales, self.rows, self.width, self.settled = codes, scales, int(rows), int(width), bool(settled)
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int):
+        self.codes, self.scales, self.rows, self.width = codes, scales, int(rows), int(width)
+        self.settled, self.half_exponent = False, None
+
+    def settle(self) -> "Mxfp4":
+        """Waits until the matrix is there and takes note of its scales' range.  For weights, once: products of settled weights are
+        faster.  Whoever writes the tensors afterwards has to make a matrix anew."""
+        with _OnDevice(self.device):
+            span = torch.tensor([256, -1], dtype=torch.int32, device=self.device)
+            _mxfp4_check(mxfp4_library().mrs_mxfp4_scale_range(self.codes.data_ptr(), self.scales.data_ptr(), span.data_ptr(), self.rows, self.width,
+                                                               _stream()), "mxfp4_scale_range")
+            low, high = span.tolist()                        # waits for the stream
+        # halfs hold 0.5 times 2^-23 to 6 times 2^13
+        self.half_exponent = None if high == 255 or high - low > 36 else max(high, 0) - 127 - 13
+        self.settled = True
+        return self
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -2711,8 +2728,7 @@ def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
         held = codes.clone()
         _mxfp4_check(mxfp4_library().mrs_mxfp4_scales_to_tiles(scales.data_ptr(), held.data_ptr(), tiles.data_ptr(), rows, width, _stream()),
                      "mxfp4_matrix")
-        torch.cuda.current_stream().synchronize()
-    return Mxfp4(held, tiles, rows, width, settled=True)
+    return Mxfp4(held, tiles, rows, width).settle()
 
 
 def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
@@ -2721,7 +2737,10 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
         if cluster:
             return ("few", cluster)
-    tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128 if m <= 128 else 256
+    if m <= 128:
+        tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128
+    else:
+        tokens = min((128, 192), key=lambda t: -(-(-(-n // 128) * -(-m // t)) // sms) * t)
     tiles = -(-n // 128) * -(-m // tokens)
     return ("many", tokens, 4 if tiles * 4 <= sms and k >= 1024 else 2 if tiles * 2 <= sms and k >= 512 else 1)
 
@@ -2758,8 +2777,15 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
             launch_count += 1
             code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k, _stream())
             code = code or lib.mrs_mxfp4_both_rows(codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                                   out.data_ptr(), out_f32, m, n, k, plan[1], plan[2], early, _stream())
+                                                   out.data_ptr(), out_f32, m, n, k, plan[1], plan[2], sm_count(x.device), early, _stream())
         else:
-            code = lib.mrs_mxfp4_weights_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32,
-                                              m, n, k, plan[1], plan[2], early, _stream())
+            halfs = exponents = None
+            code = 0
+            if weight.half_exponent is not None:
+                halfs = torch.empty((m, k), dtype=torch.float16, device=x.device)
+                exponents = torch.empty(m, dtype=torch.int32, device=x.device)
+                launch_count += 1
+                code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), halfs.data_ptr(), exponents.data_ptr(), m, k, _stream())
+            code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), _ptr(halfs), _ptr(exponents), weight.half_exponent or 0, weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32,
+                                              m, n, k, plan[1], plan[2], sm_count(x.device), early, _stream())
         _mxfp4_check(code, "mxfp4_gemm")

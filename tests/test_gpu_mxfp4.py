@@ -128,12 +128,12 @@ def test_product_over_the_sizes(m, n, k, quantise):
 
 
 PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 1), ("many", 16, 3), ("many", 32, 1), ("many", 64, 2), ("many", 128, 1), ("many", 128, 4),
-         ("many", 256, 1), ("many", 256, 8)]
+         ("many", 192, 1), ("many", 192, 8)]
 
 
 @pytest.mark.parametrize("quantise", [False, True])
 @pytest.mark.parametrize("plan", PLANS)
-@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080)])
+@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96), (400, 2500, 512)])
 def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
     if plan[0] == "many" and plan[1] < 128 and m > plan[1]:
         pytest.skip("tiles of fewer than 128 tokens hold all of them")
@@ -151,3 +151,92 @@ def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
         torch.cuda.synchronize()
         kernels.check_device_errors(certain=True)
         close_to_sums(out, want, size, k, f"{m} x {n} x {k} {plan}")
+
+
+SOME_PLANS = [("few", 1), ("few", 2), ("many", 64, 1), ("many", 128, 2), ("many", 192, 1)]
+
+
+def check_product(x, weight, w, quantise, plan, what):
+    """Against the 64-bit product of the values: not a number where that is none, infinities as they are, the rest within the bound."""
+    values = plain_quantise(x)[0] if quantise else x.double()
+    want = values @ w.T
+    finite = want.isfinite()
+    out = torch.full((x.shape[0], w.shape[0]), 7.0, device=DEV)
+    kernels.mxfp4_gemm(x, weight, out, quantise=quantise, plan=plan)
+    assert torch.equal(out.isnan(), want.isnan()), what
+    assert torch.equal(out[want.isinf()], want[want.isinf()].float()), what
+    size = values.abs().nan_to_num(0, 0, 0) @ w.abs().nan_to_num(0, 0, 0).T
+    close_to_sums(out[finite], want[finite], size[finite], x.shape[1], what)
+
+
+@pytest.mark.parametrize("quantise", [False, True])
+@pytest.mark.parametrize("plan", SOME_PLANS)
+@pytest.mark.parametrize("kind", ["wide", "tiny", "huge", "zeros", "infinite", "one_row"])
+def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
+    """Elements of very different sizes in a row and in neighbouring rows, the ends of bfloat16's range, rows of zeros, infinities
+    and NaN beside ordinary rows: exact products whatever the range, and nothing of one row in another."""
+    m, n, k = 11, 150, 800
+    g = torch.Generator(device=DEV).manual_seed(len(kind))
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g)
+    if kind == "wide":
+        x = x * torch.exp2(torch.randint(-50, 50, (m, k), device=DEV, generator=g).float())
+    elif kind == "tiny":
+        x = x * 2.0 ** -118
+    elif kind == "huge":
+        x = x * 2.0 ** 100
+        x[3] *= 2.0 ** -180
+    elif kind == "zeros":
+        x[::2] = 0.0
+        x[1, 5:] = 0.0
+    elif kind == "infinite":
+        x[2, 7], x[5, 300], x[8, 799] = math.inf, math.nan, -math.inf
+    elif kind == "one_row":
+        x[4, 10] = 1e30
+        weight_column = (codes[:, 5] & 0xF0)                # column 10 of every row is 0: what is left of that row is its small elements
+        codes = codes.clone()
+        codes[:, 5] = weight_column
+        weight, w = kernels.mxfp4_matrix(codes, scales), plain_values(codes, scales)
+    check_product(x.bfloat16(), weight, w, quantise, plan, kind)
+
+
+@pytest.mark.parametrize("quantise", [False, True])
+@pytest.mark.parametrize("plan", SOME_PLANS)
+@pytest.mark.parametrize("kind", ["wide", "nan", "zero_blocks", "small", "large", "unsettled"])
+def test_scales_of_every_size(kind, plan, quantise):
+    m, n, k = 9, 260, 544
+    g = torch.Generator(device=DEV).manual_seed(len(kind) + 50)
+    codes, scales, w = random_matrix(g, n, k)
+    if kind == "wide":
+        scales = torch.randint(60, 190, scales.shape, device=DEV, generator=g, dtype=torch.uint8)
+    elif kind == "nan":
+        scales[7, 3], scales[200, 16], scales[259, 0] = 255, 255, 255
+    elif kind == "zero_blocks":
+        codes = codes.view(n, k // 32, 16).clone()
+        codes[::3, 1], codes[5], codes[6, 2] = 0, 0x88, 0x80
+        scales[::3, 1], scales[5] = 250, 0
+        codes = codes.view(n, k // 2)
+    elif kind == "small":
+        scales = torch.randint(2, 20, scales.shape, device=DEV, generator=g, dtype=torch.uint8)
+    elif kind == "large":
+        scales = torch.randint(200, 230, scales.shape, device=DEV, generator=g, dtype=torch.uint8)
+    w = plain_values(codes, scales)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    if kind == "unsettled":
+        weight = kernels.mxfp4_quantise(w.float())
+        w = plain_quantise(w.float())[0]
+        assert not weight.settled
+    check_product(x, weight, w, quantise, plan, kind)
+    if kind == "nan":
+        assert torch.equal(weight.block_scales(), scales) and kernels.mxfp4_dequantise(weight).isnan().sum().item() == 96
+
+
+@pytest.mark.parametrize("rows,width,low,high", [(5, 64, 100, 137), (200, 96, 100, 136), (3, 32, 255, 255)])
+def test_settle_knows_what_halfs_hold(rows, width, low, high):
+    codes = torch.full((rows, width // 2), 0x17, device=DEV, dtype=torch.uint8)
+    scales = torch.full((rows, width // 32), low, device=DEV, dtype=torch.uint8)
+    scales[-1, -1] = high
+    weight = kernels.mxfp4_matrix(codes, scales)
+    assert weight.settled and weight.half_exponent == (None if high == 255 or high - low > 36 else high - 140)
