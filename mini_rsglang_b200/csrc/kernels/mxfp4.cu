@@ -12,6 +12,11 @@ namespace {
 
 constexpr int THREADS = 256;
 
+// What the kernel after this one counts with, set to zero on the way.
+__device__ __forceinline__ void clear(int* zeros, int count) {
+    for (int i = blockIdx.x * THREADS + threadIdx.x; i < count; i += gridDim.x * THREADS) zeros[i] = 0;
+}
+
 __device__ __forceinline__ void load_8(const bf16* p, float (&v)[8]) {
     const uint4 raw = *reinterpret_cast<const uint4*>(p);
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -29,8 +34,10 @@ __device__ __forceinline__ void load_8(const float* p, float (&v)[8]) {
 // Sixteen lanes a group of four blocks.  Groups behind a row's end, up to the next 256 elements, write zero scales.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                           long long rows, long long width, long long tiles_of_a_row) {
+                                                           long long rows, long long width, long long tiles_of_a_row, int* __restrict__ zeros, int zero_count) {
+    pdl_launch_dependents();
     pdl_wait();
+    clear(zeros, zero_count);
     const long long groups = rows * tiles_of_a_row;
     const int lane16 = threadIdx.x & 15;
     const long long step = (long long)gridDim.x * (THREADS / 16);
@@ -132,10 +139,11 @@ __global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __r
 constexpr int HELD = 4;
 constexpr int HALFS_LOST = INT_MIN;
 __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __restrict__ x, uint16_t* __restrict__ halfs, int* __restrict__ exponents,
-                                                                long long width) {
+                                                                long long width, int* __restrict__ zeros, int zero_count) {
     __shared__ uint32_t scratch[THREADS / 32];
     pdl_launch_dependents();
     pdl_wait();
+    clear(zeros, zero_count);
     const long long row = blockIdx.x;
     const uint4* from = reinterpret_cast<const uint4*>(x + row * width);
     uint4* to = reinterpret_cast<uint4*>(halfs + row * width);
@@ -161,8 +169,8 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) largest = max(largest, scratch[w]);
     const int field = (int)(largest >> 7);
-    const bool zeros = largest == 0, ordinary = field >= 31 && field < 255;
-    const uint32_t down = zeros || !ordinary ? 0u : (uint32_t)(-((field - 30) << 7)) & 0xFFFFu, both = down | down << 16;
+    const bool empty = largest == 0, ordinary = field >= 31 && field < 255;
+    const uint32_t down = empty || !ordinary ? 0u : (uint32_t)(-((field - 30) << 7)) & 0xFFFFu, both = down | down << 16;
     uint32_t lost = 0;
     auto convert = [&](const uint4& v) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -181,8 +189,8 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
         if (i < chunks) to[i] = convert(held[j]);
     }
     for (int i = HELD * THREADS + threadIdx.x; i < chunks; i += THREADS) to[i] = convert(from[i]);
-    const bool bad = __syncthreads_or((lost & 0x80008000u) != 0u) || !(zeros || ordinary);
-    if (threadIdx.x == 0) exponents[row] = bad ? HALFS_LOST : zeros ? 0 : field - 127 - 15;
+    const bool bad = __syncthreads_or((lost & 0x80008000u) != 0u) || !(empty || ordinary);
+    if (threadIdx.x == 0) exponents[row] = bad ? HALFS_LOST : empty ? 0 : field - 127 - 15;
 }
 
 // Blocks of a launch over `items` threads of work: loops over them where that is more than 16 blocks an SM.
@@ -200,14 +208,14 @@ MRS_EXPORT long long mrs_mxfp4_scale_bytes(long long rows, long long width) {
     return (rows + 127) / 128 * mx_tiles_of_a_row(width) * MX_TILE_BYTES;
 }
 
-// x [rows, width] bfloat16 (`is_bf16`) or float32 on 16-byte boundaries, width a multiple of 32.
-MRS_EXPORT int mrs_mxfp4_quantise(int is_bf16, const void* x, void* codes, void* scales, long long rows, long long width, void* stream) {
+// x [rows, width] bfloat16 (`is_bf16`) or float32 on 16-byte boundaries, width a multiple of 32.  `zeros`: `zero_count` ints that are set to 0, or null.
+MRS_EXPORT int mrs_mxfp4_quantise(int is_bf16, const void* x, void* codes, void* scales, long long rows, long long width, void* zeros, int zero_count, void* stream) {
     if (rows == 0) return 0;
-    if (bad_sizes(rows, width) || !x || !codes || !scales || (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
+    if (bad_sizes(rows, width) || (zero_count && !zeros) || !x || !codes || !scales || (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
     const long long tiles = mx_tiles_of_a_row(width);
     const int blocks = blocks_for(rows * tiles * 16);
-    if (is_bf16) MRS_LAUNCH(quantise_kernel<bf16>, blocks, THREADS, 0, stream, (const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles);
-    else MRS_LAUNCH(quantise_kernel<float>, blocks, THREADS, 0, stream, (const float*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles);
+    if (is_bf16) MRS_LAUNCH(quantise_kernel<bf16>, blocks, THREADS, 0, stream, (const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles, (int*)zeros, zero_count);
+    else MRS_LAUNCH(quantise_kernel<float>, blocks, THREADS, 0, stream, (const float*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles, (int*)zeros, zero_count);
     MRS_RETURN_LAUNCH_STATUS();
 }
 
@@ -238,11 +246,12 @@ MRS_EXPORT int mrs_mxfp4_scale_range(const void* codes, const void* scales, void
     MRS_RETURN_LAUNCH_STATUS();
 }
 
-// x [rows, width] bfloat16 to halfs [rows, width] and exponents [rows] int32; width a multiple of 8.
-MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* exponents, long long rows, long long width, void* stream) {
+// x [rows, width] bfloat16 to halfs [rows, width] and exponents [rows] int32.  `zeros`: `zero_count` ints that are set to 0, or null.
+MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* exponents, long long rows, long long width, void* zeros, int zero_count,
+                                       void* stream) {
     if (rows == 0) return 0;
-    if (bad_sizes(rows, width) || rows > 0x7FFFFFFF || !x || !halfs || !exponents || (((uintptr_t)x | (uintptr_t)halfs) & 15) || ((uintptr_t)exponents & 3)) return MRS_BAD_ARGUMENT;
-    MRS_LAUNCH(rows_to_halfs_kernel, (unsigned)rows, THREADS, 0, stream, (const bf16*)x, (uint16_t*)halfs, (int*)exponents, width);
+    if (bad_sizes(rows, width) || (zero_count && !zeros) || rows > 0x7FFFFFFF || !x || !halfs || !exponents || (((uintptr_t)x | (uintptr_t)halfs) & 15) || ((uintptr_t)exponents & 3)) return MRS_BAD_ARGUMENT;
+    MRS_LAUNCH(rows_to_halfs_kernel, (unsigned)rows, THREADS, 0, stream, (const bf16*)x, (uint16_t*)halfs, (int*)exponents, width, (int*)zeros, zero_count);
     MRS_RETURN_LAUNCH_STATUS();
 }
 

@@ -1,8 +1,8 @@
 // Products of many rows with a matrix in microscaled 4-bit floating point on the tcgen05 tensor cores: out[m, n] = sum_k x[m, k] w[n, k],
-// float32 sums.  A tile is 128 rows of w (the M of the MMA, so that a few tokens fill a narrow N) and up to 192 tokens.  CTAs walk
-// through tiles, neighbours through the tokens of the same weights, with two accumulators in tensor memory: a tile's results are
-// stored while the next tile's MMAs run.  With few tiles the CTAs of a cluster share one with a range of K each, and their sums meet
-// in the ranges' order.
+// float32 sums.  A tile is 128 rows of w (the M of the MMA, so that a few tokens fill a narrow N) and up to 192 tokens.  All tiles' stages
+// of 256 elements of K, tile by tile, are cut into equal runs, one a CTA and SM.  A CTA has two accumulators in tensor memory: a tile's
+// results are stored while the next tile's MMAs run.  A tile at the end of a run is shared: its CTAs leave their sums in scratch
+// memory, and the last to do so adds them in the order of K, so that a result does not depend on timing.
 //
 //   weights_kernel   x in bfloat16.  Bulk tensor copies bring 128 x 256 codes (128-byte swizzle) and their scales into a ring, x in
 //                    pieces of 128 elements into another.  Sixteen warps make the A operand of the codes, a thread a row and 64
@@ -27,10 +27,6 @@ constexpr int BM = 128;                            // rows of w of a tile
 constexpr int STAGE_K = 256;                       // elements of K of a stage of codes: 128 bytes a row
 constexpr int CODE_BYTES = BM * 128, SCALE_BYTES = 2 * MX_TILE_BYTES;
 constexpr int TMEM_COLUMNS = 512;
-constexpr int MOST_BYTES = 226 * 1024;             // of shared memory a CTA may have
-constexpr size_t ALONE_BYTES = 208 * 1024;         // with so much no other CTA that uses tensor memory fits the SM
-
-__device__ __forceinline__ int range_start(int count, int ranges, int r) { return (int)((long long)count * r / ranges); }
 
 // Untiled copy of a multiple of 16 bytes, both sides on 16-byte boundaries.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -53,97 +49,100 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     mrs_raise(MRS_ERR_BARRIER_TIMEOUT);
     return false;
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 struct Shapes {
     int M, N, K;
-    int token_tiles;
-    long long tiles;
-    int cluster;            // CTAs that share a tile; each then takes one tile only
-    int early;              // w was there before the kernel before this one: it may be fetched while that runs
+    int token_tiles, depth;     // stages of a tile
+    int units, grain;           // stages of all tiles; those that stay together
+    int early;                  // w was there before the kernel before this one: it may be fetched while that runs
     long long w_tiles_of_a_row, x_row_tiles;
-    const int* x_exponents; // of x as halfs, a row each; null: x is bfloat16
-    int w_exponent;         // halfs are made of w times 2^-w_exponent
+    const int* x_exponents;     // of x as halfs, a row each; null: x is bfloat16
+    int w_exponent;             // halfs are made of w times 2^-w_exponent
+    float* scratch;             // with a grain of 1, for every CTA the sums of its first and of its last tile, where these are shared
+    int* arrived;               // for every tile how many CTAs have left their sums; zeros to begin with
 };
 
-// What a CTA walks through: its tiles, and its range of K.
+// A CTA's run of units, tile by tile: [from, to) are the stages of the tile at hand.
 struct Walk {
-    long long tile, step;
-    int rank, from, to;
-    __device__ __forceinline__ Walk(const Shapes& s) {
-        rank = blockIdx.x % s.cluster, tile = blockIdx.x / s.cluster, step = gridDim.x / s.cluster;
-        const int stages = (s.K + STAGE_K - 1) / STAGE_K;
-        from = range_start(stages, s.cluster, rank), to = range_start(stages, s.cluster, rank + 1);
+    int next, end, tile, from, to;
+    __device__ __forceinline__ explicit Walk(const Shapes& s) : next(start(s, blockIdx.x)), end(start(s, blockIdx.x + 1)), tile(0), from(0), to(0) {}
+    __device__ static __forceinline__ int start(const Shapes& s, int cta) { return (int)((long long)(s.units / s.grain) * cta / gridDim.x) * s.grain; }
+    __device__ static __forceinline__ int owner(const Shapes& s, int unit) { return (int)(((long long)(unit + 1) * gridDim.x - 1) / s.units); }
+    __device__ __forceinline__ bool step(const Shapes& s) {
+        if (next >= end) return false;
+        tile = next / s.depth;
+        from = next - tile * s.depth;
+        to = min(s.depth, from + end - next);
+        next += to - from;
+        return true;
     }
 };
 
-// An accumulator's results (lane: row of w, column: token) to memory, or, with a cluster, into `sums` (TOKENS x 128 floats of shared
-// memory).  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes are those of its number modulo 4.
+// An accumulator's results (lane: row of w, column: token) to memory.  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes
+// are those of its number modulo 4.  `halfs`: the rows' powers of two go into them.  A tile that other CTAs share goes through scratch
+// memory; `flag` is a word of shared memory.
 template <int TOKENS, int WARPS, typename Out>
-__device__ __forceinline__ void store_accumulator(uint32_t accumulator, float* sums, Out* __restrict__ out, const Shapes& s, long long n0, int token0, int index,
-                                                  bool empty, bool halfs = false) {
+__device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag) {
     constexpr int STEP = TOKENS < 32 ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
     const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
-    const int live = min(TOKENS, s.M - token0);
+    const int token0 = walk.tile % s.token_tiles * TOKENS, live = min(TOKENS, s.M - token0);
     const uint32_t acc = accumulator + ((uint32_t)(quarter * 32) << 16);
-    const long long n = n0 + row;
+    const long long n = (long long)(walk.tile / s.token_tiles) * BM + row;
+    const bool whole = walk.from == 0 && walk.to == s.depth;
+    auto finish = [&](int c, float (&v)[STEP]) {
+        if (halfs) {                               // powers of two in the floats' range
+#pragma unroll
+            for (int e = 0; e < STEP; ++e)
+                v[e] *= __uint_as_float((uint32_t)(127 + s.w_exponent + (c + e < live ? __ldcg(s.x_exponents + token0 + c + e) : -s.w_exponent)) << 23);
+        }
+        if (n < s.N) {
+            Out* place = out + (size_t)(token0 + c) * s.N + n;
+            if (c + STEP <= live) {
+#pragma unroll
+                for (int e = 0; e < STEP; ++e) place[(size_t)e * s.N] = from_float<Out>(v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < STEP; ++e)
+                    if (c + e < live) place[(size_t)e * s.N] = from_float<Out>(v[e]);
+            }
+        }
+    };
+    float* mine = s.scratch + ((size_t)blockIdx.x * 2 + (walk.from == 0 ? 1 : 0)) * (TOKENS * BM) + row;
 #pragma unroll 1
     for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
         float v[STEP];
-        if (!empty) {
-            if constexpr (STEP == 16) tmem_load_16_async(acc + c, v);
-            else tmem_load_32_async(acc + c, v);
-            tmem_load_wait();
+        if constexpr (STEP == 16) tmem_load_16_async(acc + c, v);
+        else tmem_load_32_async(acc + c, v);
+        tmem_load_wait();
+        if (whole) {
+            finish(c, v);
         } else {
 #pragma unroll
-            for (int e = 0; e < STEP; ++e) v[e] = 0.0f;
-        }
-        if (halfs) {                               // the rows' powers of two, all in the floats' range
-#pragma unroll
-            for (int e = 0; e < STEP; ++e)
-                v[e] *= __uint_as_float((uint32_t)(127 + s.w_exponent + (c + e < live ? __ldg(s.x_exponents + token0 + c + e) : -s.w_exponent)) << 23);
-        }
-        if (s.cluster == 1) {
-            if (n < s.N) {
-                Out* place = out + (size_t)(token0 + c) * s.N + n;
-                if (c + STEP <= live) {
-#pragma unroll
-                    for (int e = 0; e < STEP; ++e) place[(size_t)e * s.N] = from_float<Out>(v[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < STEP; ++e)
-                        if (c + e < live) place[(size_t)e * s.N] = from_float<Out>(v[e]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < STEP; ++e) sums[(c + e) * BM + row] = v[e];
+            for (int e = 0; e < STEP; ++e) __stcg(mine + (c + e) * BM, v[e]);
         }
     }
-}
-
-// The cluster's sums of a tile, in the order of the ranges of K, to memory.  Every thread of every CTA.
-template <int TOKENS, int THREADS, typename Out>
-__device__ __forceinline__ void join_cluster(const float* sums, Out* __restrict__ out, const Shapes& s, long long n0, int token0, int rank) {
-    const int live = min(TOKENS, s.M - token0);
-    cluster_sync();
-    const uint32_t base = smem_u32(sums);
-    for (int i = rank * THREADS + threadIdx.x; i < live * BM; i += s.cluster * THREADS) {
-        float sum = 0.0f;
-        for (int c = 0; c < s.cluster; ++c) {
-            uint32_t there;
-            float v;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(base + i * 4), "r"(c));
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-            sum += v;
+    if (whole) return;
+    const int first = Walk::owner(s, walk.tile * s.depth), last = Walk::owner(s, (walk.tile + 1) * s.depth - 1);
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+    if (index == 0 && (threadIdx.x & 31) == 0) *flag = atomicAdd(s.arrived + walk.tile, 1) == last - first;
+    asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+    const bool finisher = *flag != 0;
+    asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");               // the flag is read by all before it is written again
+    if (!finisher) return;
+    __threadfence();
+#pragma unroll 1
+    for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
+        float v[STEP];
+        for (int cta = first; cta <= last; ++cta) {                             // the first has the tile's first stages, at the end of its run
+            const float* from = s.scratch + ((size_t)cta * 2 + (cta == first ? 1 : 0)) * (TOKENS * BM) + row + c * BM;
+            float piece[STEP];
+#pragma unroll
+            for (int e = 0; e < STEP; ++e) piece[e] = __ldcg(from + e * BM);
+#pragma unroll
+            for (int e = 0; e < STEP; ++e) v[e] = cta == first ? piece[e] : v[e] + piece[e];
         }
-        const long long n = n0 + (i & (BM - 1));
-        if (n < s.N) out[(size_t)(token0 + i / BM) * s.N + n] = from_float<Out>(sum);
+        finish(c, v);
     }
-    cluster_sync();                            // a CTA's sums stay until its cluster has read them
 }
 
 // ------------------------------------------------------------------------------------------
@@ -227,11 +226,13 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     uint64_t* acc_full = a_empty + A_BUFFERS;
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    int* flag = reinterpret_cast<int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Walk walk(s);
-    // the range's stages; the last stage of K may hold fewer steps
-    const int steps = min(walk.to * STAGE_STEPS, (s.K + STEP_K - 1) / STEP_K) - walk.from * STAGE_STEPS;
+    Walk walk(s);
+    // Steps of the tile at hand.  Every stage has two, also where K ends in its first (the second is made of zeros): the warps that
+    // make one of them then use every second buffer of A in turn, and are never more than one use of a buffer behind.
+    auto steps_of = [&]() { return (walk.to - walk.from) * STAGE_STEPS; };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < W_STAGES; ++i) {
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
 
     // The codes' first stages are on their way before anything else; then, once the kernel before has ended, whether all of x is there as
     // halfs whose powers, with the matrix's, are ordinary floats.
-    const int ahead = s.early && walk.tile < s.tiles ? min(W_STAGES, walk.to - walk.from) : 0;
+    const int ahead = s.early ? min(W_STAGES, walk.end - walk.next) : 0;
     auto load_codes = [&](int n_tile, int stage, int slot) {
         mbar_arrive_expect_tx(&w_full[slot], CODE_BYTES + SCALE_BYTES);
         tma_load_2d(w_ring + slot * CODE_BYTES, &w_map, &w_full[slot], stage * 128, n_tile * BM);
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     };
     if (warp == 2 + MAKERS + STORERS) {
         if (elect_one())
-            for (int i = 0; i < ahead; ++i) load_codes((int)(walk.tile / s.token_tiles), walk.from + i, i);
+            for (int i = 0; i < ahead; ++i) load_codes((walk.next + i) / s.depth / s.token_tiles, (walk.next + i) % s.depth, i);
         __syncwarp();
     }
     pdl_wait();
@@ -293,8 +294,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         bool alive = true;
         int slot = 0;
         uint32_t phase = 1;
-        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step) {
-            const int token0 = (int)(tile % s.token_tiles) * TOKENS;
+        while (alive && walk.step(s)) {
+            const int token0 = walk.tile % s.token_tiles * TOKENS, steps = steps_of();
             for (int step = 0; step < steps; ++step) {
                 if (!(alive = warp_wait(&x_empty[slot], phase))) break;
                 if (leader) {
@@ -313,12 +314,15 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         bool alive = true;
         int slot = 0;
         uint32_t phase = 1;
-        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step) {
-            const int n_tile = (int)(tile / s.token_tiles);
-            for (int stage = walk.from; stage < walk.to; ++stage) {
-                if (!(alive = warp_wait(&w_empty[slot], phase))) break;
-                if (leader && (stage - walk.from >= ahead || tile != walk.tile)) load_codes(n_tile, stage, slot);
-                __syncwarp();
+        int count = 0;
+        while (alive && walk.step(s)) {
+            const int n_tile = walk.tile / s.token_tiles;
+            for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
+                if (count >= ahead) {                     // not even the wait before: the makers may be through with those stages
+                    if (!(alive = warp_wait(&w_empty[slot], phase))) break;
+                    if (leader) load_codes(n_tile, stage, slot);
+                    __syncwarp();
+                }
                 if (++slot == W_STAGES) slot = 0, phase ^= 1;
             }
         }
@@ -328,8 +332,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         bool alive = true;
         int x_slot = 0, a_slot = 0, round = 0;
         uint32_t x_phase = 0, a_phase = 0;
-        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step, ++round) {
-            const int buffer = round & 1;
+        for (; alive && walk.step(s); ++round) {
+            const int buffer = round & 1, steps = steps_of();
             if (!(alive = warp_wait(&acc_empty[buffer], ((round >> 1) & 1) ^ 1))) break;
             tcgen05_fence_after_sync();
             const uint32_t d_tmem = tmem + buffer * ACCUMULATOR;
@@ -358,60 +362,47 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + A_FIRST;
         const uint32_t first_chunk = ((group * 2) ^ (row & 7)) << 4, second_chunk = ((group * 2 + 1) ^ (row & 7)) << 4;
         const int scale_place = (group >> 1) * MX_TILE_BYTES + lane * 16 + quarter * 4 + (group & 1) * 2;
-        bool alive = true;
-        int w_slot = 0, round = 0;
+        int w_slot = 0;
         uint32_t w_phase = 0;
-        long long before = 0;                                                                    // steps of the tiles before
-        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step, ++round, before += steps) {
-            for (int stage = 0; stage < walk.to - walk.from; ++stage) {
-                if (!(alive = warp_wait(&w_full[w_slot], w_phase))) break;
-                const int step = stage * STAGE_STEPS + (group >> 1);
-                if (step < steps) {
-                    const unsigned char* codes = w_ring + w_slot * CODE_BYTES + row * 128;
-                    const uint32_t two = *reinterpret_cast<const uint16_t*>(s_ring + w_slot * SCALE_BYTES + scale_place);
-                    const uint4 first = *reinterpret_cast<const uint4*>(codes + first_chunk);
-                    const uint4 second = *reinterpret_cast<const uint4*>(codes + second_chunk);
-                    uint32_t words[32];
-                    if (halfs) {
-                        decode_block_halfs(first, two & 255u, s.w_exponent, words);
-                        decode_block_halfs(second, two >> 8, s.w_exponent, words + 16);
-                    } else {
-                        decode_block(first, two & 255u, words);
-                        decode_block(second, two >> 8, words + 16);
-                    }
-                    const long long index = before + step;
-                    const int b = (int)(index % A_BUFFERS);
-                    if (!(alive = warp_wait(&a_empty[b], (uint32_t)((index / A_BUFFERS) & 1) ^ 1))) break;
-                    __syncwarp();
-                    tcgen05_fence_after_sync();
-                    tmem_store_32_words(lanes + b * A_COLUMNS + (group & 1) * (A_COLUMNS / 2), words);
-                    tmem_store_wait();
-                    tcgen05_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&a_full[b]);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&w_empty[w_slot]);
-                if (++w_slot == W_STAGES) w_slot = 0, w_phase ^= 1;
+        for (int step = group >> 1; step < (walk.end - walk.next) * STAGE_STEPS; step += STAGE_STEPS) {          // of the CTA's run
+            if (!warp_wait(&w_full[w_slot], w_phase)) break;
+            const unsigned char* codes = w_ring + w_slot * CODE_BYTES + row * 128;
+            const uint32_t two = *reinterpret_cast<const uint16_t*>(s_ring + w_slot * SCALE_BYTES + scale_place);
+            const uint4 first = *reinterpret_cast<const uint4*>(codes + first_chunk);
+            const uint4 second = *reinterpret_cast<const uint4*>(codes + second_chunk);
+            uint32_t words[32];
+            if (halfs) {
+                decode_block_halfs(first, two & 255u, s.w_exponent, words);
+                decode_block_halfs(second, two >> 8, s.w_exponent, words + 16);
+            } else {
+                decode_block(first, two & 255u, words);
+                decode_block(second, two >> 8, words + 16);
             }
+            const int b = step % A_BUFFERS;
+            if (!warp_wait(&a_empty[b], ((step / A_BUFFERS) & 1) ^ 1)) break;
+            __syncwarp();
+            tcgen05_fence_after_sync();
+            tmem_store_32_words(lanes + b * A_COLUMNS + (group & 1) * (A_COLUMNS / 2), words);
+            tmem_store_wait();
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[b]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&w_empty[w_slot]);
+            if (++w_slot == W_STAGES) w_slot = 0, w_phase ^= 1;
         }
     } else {
-        int round = 0;
-        for (long long tile = walk.tile; tile < s.tiles; tile += walk.step, ++round) {
+        for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, reinterpret_cast<float*>(smem), out, s, tile / s.token_tiles * BM,
-                                                    (int)(tile % s.token_tiles) * TOKENS, warp - 2 - MAKERS, steps <= 0, halfs);
+            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2 - MAKERS, halfs, flag);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
         }
     }
     __syncwarp();
-    if (s.cluster > 1)
-        join_cluster<TOKENS, W_THREADS, Out>(reinterpret_cast<const float*>(smem), out, s, walk.tile / s.token_tiles * BM, (int)(walk.tile % s.token_tiles) * TOKENS,
-                                             walk.rank);
     tcgen05_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
@@ -468,10 +459,10 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
     uint64_t* acc_full = empty + B_STAGES;
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    int* flag = reinterpret_cast<int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Walk walk(s);
-    const int depth = walk.to - walk.from;
+    Walk walk(s);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < B_STAGES; ++i) {
@@ -497,26 +488,25 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
     if (warp == 0) {
         const bool leader = elect_one();
         // the first stages of w, as far as the ring goes, before the kernel before has ended
-        const int ahead = s.early && walk.tile < s.tiles ? min(B_STAGES, depth) : 0;
+        const int ahead = s.early ? min(B_STAGES, walk.end - walk.next) : 0;
         auto load_w = [&](int n_tile, int stage, int i) {
             mbar_arrive_expect_tx(&full[i], CODE_BYTES + TOKENS * 128 + STAGE_SCALES);
             tma_load_2d(w_ring + i * CODE_BYTES, &w_map, &full[i], stage * 128, n_tile * BM);
             bulk_load(s_ring + i * STAGE_SCALES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[i]);
         };
         if (leader)
-            for (int i = 0; i < ahead; ++i) load_w((int)(walk.tile / s.token_tiles), walk.from + i, i);
+            for (int i = 0; i < ahead; ++i) load_w((walk.next + i) / s.depth / s.token_tiles, (walk.next + i) % s.depth, i);
         __syncwarp();
         pdl_wait();
         bool alive = true;
-        int slot = 0;
+        int slot = 0, count = 0;
         uint32_t phase = 1;
-        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step) {
-            const int token0 = (int)(tile % s.token_tiles) * TOKENS, n_tile = (int)(tile / s.token_tiles);
-            for (int index = 0; index < depth; ++index) {
-                const int stage = walk.from + index;
+        while (alive && walk.step(s)) {
+            const int token0 = walk.tile % s.token_tiles * TOKENS, n_tile = walk.tile / s.token_tiles;
+            for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
                 if (!(alive = warp_wait(&empty[slot], phase))) break;
                 if (leader) {
-                    if (index >= ahead || tile != walk.tile) load_w(n_tile, stage, slot);
+                    if (count >= ahead) load_w(n_tile, stage, slot);
                     tma_load_2d(x_ring + slot * TOKENS * 128, &x_map, &full[slot], stage * 128, token0);
 #pragma unroll
                     for (int t = 0; t < token_blocks<TOKENS>(); ++t) {
@@ -535,14 +525,14 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
         bool alive = true;
         int slot = 0, round = 0;
         uint32_t phase = 0;
-        for (long long tile = walk.tile; tile < s.tiles && alive; tile += walk.step, ++round) {
+        for (; alive && walk.step(s); ++round) {
             const int buffer = round & 1;
             if (!(alive = warp_wait(&acc_empty[buffer], ((round >> 1) & 1) ^ 1))) break;
             tcgen05_fence_after_sync();
             const uint32_t d_tmem = tmem + buffer * B_ACCUMULATOR;
             // tiles of 192 tokens begin in the middle of a tile of scales every other time: two columns, 64 tokens, further in
-            const uint32_t shift = TOKENS == 192 ? (((uint32_t)(tile % s.token_tiles) * TOKENS) & 127u) / 32 : 0u;
-            for (int index = 0; index < depth; ++index) {
+            const uint32_t shift = TOKENS == 192 ? (((uint32_t)(walk.tile % s.token_tiles) * TOKENS) & 127u) / 32 : 0u;
+            for (int index = 0; index < walk.to - walk.from; ++index) {
                 if (!(alive = warp_wait(&full[slot], phase))) break;
                 tcgen05_fence_after_sync();
                 const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(w_ring + slot * CODE_BYTES));
@@ -571,22 +561,17 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
         }
     } else {
         pdl_wait();
-        int round = 0;
-        for (long long tile = walk.tile; tile < s.tiles; tile += walk.step, ++round) {
+        for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, B_STORERS, Out>(tmem + buffer * B_ACCUMULATOR, reinterpret_cast<float*>(smem), out, s, tile / s.token_tiles * BM,
-                                                      (int)(tile % s.token_tiles) * TOKENS, warp - 2, depth <= 0);
+            store_accumulator<TOKENS, B_STORERS, Out>(tmem + buffer * B_ACCUMULATOR, out, s, walk, warp - 2, false, flag);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
         }
     }
     __syncwarp();
-    if (s.cluster > 1)
-        join_cluster<TOKENS, B_THREADS, Out>(reinterpret_cast<const float*>(smem), out, s, walk.tile / s.token_tiles * BM, (int)(walk.tile % s.token_tiles) * TOKENS,
-                                             walk.rank);
     tcgen05_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
@@ -607,37 +592,29 @@ int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, long 
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : MRS_TENSOR_MAP_FAILED;
 }
 
+// Tiles and units of a product; false where they are too many, or more CTAs are asked for than have work.
+template <int TOKENS> bool lay_out(Shapes& s, int ctas) {
+    s.depth = (s.K + STAGE_K - 1) / STAGE_K;
+    s.token_tiles = (s.M + TOKENS - 1) / TOKENS;
+    const long long units = (long long)((s.N + BM - 1) / BM) * s.token_tiles * s.depth;
+    if (units > 0x7FFFFFFF) return false;
+    s.units = (int)units;
+    s.grain = s.scratch ? 1 : s.depth;
+    return ctas <= s.units / s.grain;
+}
+
 template <typename... KernelArgs, typename... Args>
-int launch_cluster(void (*kernel)(KernelArgs...), PerDevice& configured, int threads, long long tiles, int sms, int cluster, size_t smem, void* stream, Args... args) {
+int launch_run(void (*kernel)(KernelArgs...), PerDevice& configured, int threads, int ctas, size_t smem, void* stream, Args... args) {
     if (!configured.get()) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BYTES);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
         configured.set(1);
     }
-    const long long ctas = cluster > 1 ? tiles * cluster : tiles < sms ? tiles : sms;
-    if (ctas > 0x7FFFFFFFll) return MRS_BAD_ARGUMENT;
-    // A CTA that waits for its cluster keeps its tensor memory meanwhile: clusters that wait for one another's would wait for good, so they
-    // take whole SMs.
-    if (cluster > 1 && smem < ALONE_BYTES) smem = ALONE_BYTES;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)ctas);
-    config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = smem;
-    config.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attributes[2];
-    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[0].val.programmaticStreamSerializationAllowed = 1;
-    attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = cluster, attributes[1].val.clusterDim.y = 1, attributes[1].val.clusterDim.z = 1;
-    config.attrs = attributes;
-    config.numAttrs = 2;
-    cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<KernelArgs>(args)...);
-    if (e != cudaSuccess) return (int)e;
-    return (int)cudaGetLastError();
+    return mrs_launch(kernel, dim3(ctas), dim3(threads), smem, (cudaStream_t)stream, args...);
 }
 
 template <int TOKENS, typename Out>
-int launch_weights(const void* x, const void* x_halfs, const void* codes, const void* scales, void* out, Shapes s, int sms, void* stream) {
+int launch_weights(const void* x, const void* x_halfs, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
     CUtensorMap w_map, x_map, halfs_map;
     int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
     if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, HALF_K, TOKENS);
@@ -645,42 +622,45 @@ int launch_weights(const void* x, const void* x_halfs, const void* codes, const 
     if (!code && s.x_exponents) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, HALF_K, TOKENS);
     if (code) return code;
     static PerDevice configured;
-    s.token_tiles = (s.M + TOKENS - 1) / TOKENS;
-    s.tiles = (long long)((s.N + BM - 1) / BM) * s.token_tiles;
-    return launch_cluster(weights_kernel<TOKENS, Out>, configured, W_THREADS, s.tiles, sms, s.cluster, weights_smem<TOKENS>(), stream, w_map, x_map, halfs_map,
-                          (const uint8_t*)scales, (Out*)out, s);
+    if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
+    return launch_run(weights_kernel<TOKENS, Out>, configured, W_THREADS, ctas, weights_smem<TOKENS>(), stream, w_map, x_map, halfs_map, (const uint8_t*)scales,
+                      (Out*)out, s);
 }
 template <int TOKENS, typename Out>
-int launch_both(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, Shapes s, int sms, void* stream) {
+int launch_both(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
     CUtensorMap w_map, x_map;
     int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
     if (!code) code = make_map(&x_map, x_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.M, 128, TOKENS);
     if (code) return code;
     static PerDevice configured;
-    s.token_tiles = (s.M + TOKENS - 1) / TOKENS;
     s.x_row_tiles = (s.M + 127) / 128;
-    s.tiles = (long long)((s.N + BM - 1) / BM) * s.token_tiles;
-    return launch_cluster(both_kernel<TOKENS, Out>, configured, B_THREADS, s.tiles, sms, s.cluster, both_smem<TOKENS>(), stream, w_map, x_map,
-                          (const uint8_t*)scales, (const uint8_t*)x_scales, (Out*)out, s);
+    if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
+    return launch_run(both_kernel<TOKENS, Out>, configured, B_THREADS, ctas, both_smem<TOKENS>(), stream, w_map, x_map, (const uint8_t*)scales,
+                      (const uint8_t*)x_scales, (Out*)out, s);
 }
 
-bool bad(const void* x, const void* codes, const void* scales, const void* out, int out_f32, int M, int N, int K, int tokens, int cluster) {
+bool bad(const void* x, const void* codes, const void* scales, const void* out, int out_f32, int M, int N, int K, int tokens, int ctas, const void* scratch,
+         const void* arrived) {
     return M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || !x || !codes || !scales || !out ||
-           (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1)) || cluster < 1 || cluster > 8 ||
-           (tokens < 128 && M > tokens);
+           (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1)) || ctas < 1 || (tokens < 128 && M > tokens) ||
+           (scratch == nullptr) != (arrived == nullptr) || (((uintptr_t)scratch | (uintptr_t)arrived) & 3);
 }
 
 }  // namespace
 
 // out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16, also as halfs with exponents (mxfp4.cu) or null; w as in mxfp4.cuh, whose blocks
-// other than zeros have scales of 2^(w_exponent - 23) to 2^(w_exponent + 13) if halfs are given.  `tokens` (16, 32, 64, 128, 192): of a tile, below 128 only
-// if they are all; `cluster` 1 to 8 ranges of K; `ctas`: the GPU's SMs.  `early`: nothing that still runs when this kernel starts writes w.
-MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const void* x_exponents, int w_exponent, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int tokens,
-                                      int cluster, int ctas, int early, void* stream) {
+// other than zeros have scales of 2^(w_exponent - 23) to 2^(w_exponent + 13) if halfs are given.  `tokens` (16, 32, 64, 128, 192): of a tile,
+// below 128 only if they are all.  `ctas`: at most the GPU's SMs and the stages of 256 elements of K of all tiles.  With `scratch` (2 ctas
+// x tokens x 128 floats) and `arrived` (an int a tile, zero) the stages are cut into equal runs, without whole tiles are.  `early`: nothing
+// that still runs when this kernel starts writes w.
+MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const void* x_exponents, int w_exponent, const void* codes, const void* scales,
+                                      void* out, int out_f32, int M, int N, int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
-    if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, cluster)) return MRS_BAD_ARGUMENT;
+    if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived)) return MRS_BAD_ARGUMENT;
     if ((x_halfs == nullptr) != (x_exponents == nullptr) || ((uintptr_t)x_halfs & 15) || ((uintptr_t)x_exponents & 3)) return MRS_BAD_ARGUMENT;
-    const Shapes s = {M, N, K, 0, 0, cluster, early, mx_tiles_of_a_row(K), 0, (const int*)x_exponents, w_exponent};
+    Shapes s = {};
+    s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K);
+    s.x_exponents = (const int*)x_exponents, s.w_exponent = w_exponent, s.scratch = (float*)scratch, s.arrived = (int*)arrived;
 #define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_weights<T, float>(x, x_halfs, codes, scales, out, s, ctas, stream) : launch_weights<T, bf16>(x, x_halfs, codes, scales, out, s, ctas, stream)
     MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
 #undef MRS_TOKENS
@@ -688,11 +668,12 @@ MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const 
 }
 
 // The same with x in 4 bits.
-MRS_EXPORT int mrs_mxfp4_both_rows(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K,
-                                   int tokens, int cluster, int ctas, int early, void* stream) {
+MRS_EXPORT int mrs_mxfp4_both_rows(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, int out_f32, int M, int N,
+                                   int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
-    if (bad(x_codes, codes, scales, out, out_f32, M, N, K, tokens, cluster) || !x_scales || ((uintptr_t)x_scales & 15)) return MRS_BAD_ARGUMENT;
-    const Shapes s = {M, N, K, 0, 0, cluster, early, mx_tiles_of_a_row(K), 0, nullptr, 0};
+    if (bad(x_codes, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived) || !x_scales || ((uintptr_t)x_scales & 15)) return MRS_BAD_ARGUMENT;
+    Shapes s = {};
+    s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
 #define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_both<T, float>(x_codes, x_scales, codes, scales, out, s, ctas, stream) : launch_both<T, bf16>(x_codes, x_scales, codes, scales, out, s, ctas, stream)
     MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
 #undef MRS_TOKENS

@@ -2564,15 +2564,16 @@ def concat_rows(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> None:
 # ------------------------------------------------------------------------------------------------
 MXFP4_BLOCK = 32               # neighbours of a row that share a power of two
 _MXFP4_SIGNATURES = {
-    "mrs_mxfp4_quantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
+    "mrs_mxfp4_quantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_dequantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_scales_to_tiles": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
     "mrs_mxfp4_few_rows_cluster": [_c_int, _c_int],
     "mrs_mxfp4_scale_range": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
-    "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
-    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
-    "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
+    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp,
+                               _c_int, _c_vp],
+    "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_take_error": [ctypes.POINTER(ctypes.c_uint)],
 }
 _mxfp4_lib = None
@@ -2692,8 +2693,8 @@ def mxfp4_quantise(x: torch.Tensor) -> Mxfp4:
     _mxfp4_aligned(x, "mxfp4_quantise input")
     with _OnDevice(x.device):
         codes, scales = _mxfp4_buffers(rows, width, x.device)
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, width, _stream()),
-                     "mxfp4_quantise")
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, width, None, 0,
+                                                        _stream()), "mxfp4_quantise")
     return Mxfp4(codes, scales, rows, width)
 
 
@@ -2732,17 +2733,24 @@ def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
 
 
 def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
-    """How a product is launched: ("few", CTAs of a cluster) or ("many", tokens of a tile, CTAs of a cluster)."""
+    """How a product is launched: ("few", CTAs of a cluster) or ("many", tokens of a tile, CTAs, whether tiles may be shared)."""
     if m <= (4 if quantise else 8):
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
         if cluster:
             return ("few", cluster)
-    if m <= 128:
-        tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128
-    else:
-        tokens = min((128, 192), key=lambda t: -(-(-(-n // 128) * -(-m // t)) // sms) * t)
-    tiles = -(-n // 128) * -(-m // tokens)
-    return ("many", tokens, 4 if tiles * 4 <= sms and k >= 1024 else 2 if tiles * 2 <= sms and k >= 512 else 1)
+    tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128 if m <= 128 else 192
+    return mxfp4_many_plan(m, n, k, tokens, sms)
+
+
+def mxfp4_many_plan(m: int, n: int, k: int, tokens: int, sms: int, shared: bool | None = None) -> tuple:
+    """Tiles of 128 rows of weights x `tokens`, on as many CTAs as there are SMs."""
+    tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
+    if shared is None:
+        rounds = -(-tiles // sms)
+        shared = tiles < 0.9 * rounds * sms and depth > 1
+    if not shared:
+        return ("many", tokens, min(tiles, sms), False)
+    return ("many", tokens, min(sms, max(tiles, tiles * depth // 3)), True)
 
 
 def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool = False, plan: tuple | None = None) -> None:
@@ -2772,20 +2780,25 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
         if plan[0] == "few":
             code = lib.mrs_mxfp4_few_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32, m, n, k,
                                           int(bool(quantise)), plan[1], sm_count(x.device), early, _stream())
-        elif quantise:
-            codes, scales = _mxfp4_buffers(m, k, x.device)
-            launch_count += 1
-            code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k, _stream())
-            code = code or lib.mrs_mxfp4_both_rows(codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                                   out.data_ptr(), out_f32, m, n, k, plan[1], plan[2], sm_count(x.device), early, _stream())
         else:
-            halfs = exponents = None
-            code = 0
-            if weight.half_exponent is not None:
+            _, tokens, ctas, shared = plan
+            scratch = arrived = None
+            tiles = -(-n // 128) * -(-m // tokens)
+            if shared:
+                scratch = torch.empty(2 * ctas * tokens * 128, dtype=torch.float32, device=x.device)
+                arrived = torch.empty(tiles, dtype=torch.int32, device=x.device)              # set to zero by the kernel before the product
+            launch_count += 1
+            if quantise:
+                codes, scales = _mxfp4_buffers(m, k, x.device)
+                code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k, _ptr(arrived), tiles if shared else 0, _stream())
+                code = code or lib.mrs_mxfp4_both_rows(codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+                                                       out.data_ptr(), out_f32, m, n, k, tokens, ctas, _ptr(scratch), _ptr(arrived), early, _stream())
+            else:
                 halfs = torch.empty((m, k), dtype=torch.float16, device=x.device)
                 exponents = torch.empty(m, dtype=torch.int32, device=x.device)
-                launch_count += 1
-                code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), halfs.data_ptr(), exponents.data_ptr(), m, k, _stream())
-            code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), _ptr(halfs), _ptr(exponents), weight.half_exponent or 0, weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32,
-                                              m, n, k, plan[1], plan[2], sm_count(x.device), early, _stream())
+                code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), halfs.data_ptr(), exponents.data_ptr(), m, k, _ptr(arrived), tiles if shared else 0, _stream())
+                fits = weight.half_exponent is not None
+                code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), halfs.data_ptr() if fits else None, exponents.data_ptr() if fits else None,
+                                                          weight.half_exponent or 0, weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
+                                                          out_f32, m, n, k, tokens, ctas, _ptr(scratch), _ptr(arrived), early, _stream())
         _mxfp4_check(code, "mxfp4_gemm")

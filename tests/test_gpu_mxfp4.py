@@ -127,8 +127,16 @@ def test_product_over_the_sizes(m, n, k, quantise):
         close_to_sums(out, want, size, k, f"{m} x {n} x {k}")
 
 
-PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 1), ("many", 16, 3), ("many", 32, 1), ("many", 64, 2), ("many", 128, 1), ("many", 128, 4),
-         ("many", 192, 1), ("many", 192, 8)]
+PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 5, False), ("many", 16, 7, True), ("many", 32, 1, False), ("many", 64, 3, True), ("many", 128, 148, False),
+         ("many", 128, 148, True), ("many", 128, 11, True), ("many", 192, 148, False), ("many", 192, 9, True)]
+
+
+def fitting(plan, m, n, k):
+    """The plan with no more CTAs than have work."""
+    if plan[0] == "few":
+        return plan
+    tiles = -(-n // 128) * -(-m // plan[1])
+    return (*plan[:2], min(plan[2], tiles * -(-k // 256) if plan[3] else tiles), plan[3])
 
 
 @pytest.mark.parametrize("quantise", [False, True])
@@ -147,13 +155,13 @@ def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
     want, size = values @ w.T, values.abs() @ w.abs().T
     for dtype in (torch.float32, torch.bfloat16):
         out = torch.full((m, n), float("nan"), device=DEV, dtype=dtype)
-        kernels.mxfp4_gemm(x, weight, out, quantise=quantise, plan=plan)
+        kernels.mxfp4_gemm(x, weight, out, quantise=quantise, plan=fitting(plan, m, n, k))
         torch.cuda.synchronize()
         kernels.check_device_errors(certain=True)
         close_to_sums(out, want, size, k, f"{m} x {n} x {k} {plan}")
 
 
-SOME_PLANS = [("few", 1), ("few", 2), ("many", 64, 1), ("many", 128, 2), ("many", 192, 1)]
+SOME_PLANS = [("few", 1), ("few", 2), ("many", 64, 2, False), ("many", 128, 3, True), ("many", 192, 2, True)]
 
 
 def check_product(x, weight, w, quantise, plan, what):
