@@ -39,49 +39,64 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     uint32_t done;
     asm volatile("{\n .reg .pred p, q;\n .reg .u64 start, now;\n"
-                 " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+                 " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n @p bra DONE;\n"
                  " mov.u64 start, %%clock64;\n"
-                 "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+                 "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n @p bra DONE;\n"
                  " mov.u64 now, %%clock64;\n sub.u64 now, now, start;\n setp.lt.u64 q, now, %3;\n @q bra AGAIN;\n"
                  "DONE:\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "n"(MRS_WAIT_CYCLES) : "memory");
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "n"(MRS_WAIT_CYCLES), "r"(1000000u) : "memory");       // asleep for up to a millisecond a try
     if (__all_sync(0xffffffffu, done != 0u)) return true;
     mrs_raise(MRS_ERR_BARRIER_TIMEOUT);
     return false;
 }
+
 struct Shapes {
     int M, N, K;
     int token_tiles, depth;     // stages of a tile
-    int units, grain;           // stages of all tiles; those that stay together
+    int units;                  // stages of all tiles
     int early;                  // w was there before the kernel before this one: it may be fetched while that runs
     long long w_tiles_of_a_row, x_row_tiles;
     const int* x_exponents;     // of x as halfs, a row each; null: x is bfloat16
     int w_exponent;             // halfs are made of w times 2^-w_exponent
-    float* scratch;             // with a grain of 1, for every CTA the sums of its first and of its last tile, where these are shared
+    float* scratch;             // where tiles are shared, for every CTA the sums of its first and of its last tile
     int* arrived;               // for every tile how many CTAs have left their sums; zeros to begin with
 };
 
-// A CTA's run of units, tile by tile: [from, to) are the stages of the tile at hand.
+// A CTA's tiles; [from, to) are the stages of the tile at hand.  Shared tiles: the CTA's run of units.  Whole ones: every gridDim.x-th, so
+// that CTAs at work at the same time write neighbouring columns and read neighbouring weights.
 struct Walk {
-    int next, end, tile, from, to;
-    __device__ __forceinline__ explicit Walk(const Shapes& s) : next(start(s, blockIdx.x)), end(start(s, blockIdx.x + 1)), tile(0), from(0), to(0) {}
-    __device__ static __forceinline__ int start(const Shapes& s, int cta) { return (int)((long long)(s.units / s.grain) * cta / gridDim.x) * s.grain; }
+    int first, total, done, tile, from, to;        // `total` stages from unit `first` on (whole tiles: of this CTA's own)
+    __device__ __forceinline__ explicit Walk(const Shapes& s) : done(0), tile(0), from(0), to(0) {
+        if (s.scratch) {
+            first = start(s, blockIdx.x);
+            total = start(s, blockIdx.x + 1) - first;
+        } else {
+            first = 0;
+            total = ((s.units / s.depth - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * s.depth;
+        }
+    }
+    __device__ static __forceinline__ int start(const Shapes& s, int cta) { return (int)((long long)s.units * cta / gridDim.x); }
     __device__ static __forceinline__ int owner(const Shapes& s, int unit) { return (int)(((long long)(unit + 1) * gridDim.x - 1) / s.units); }
+    __device__ __forceinline__ int tile_of(const Shapes& s, int position) const {
+        const int index = (first + position) / s.depth;
+        return s.scratch ? index : (int)blockIdx.x + index * (int)gridDim.x;
+    }
+    __device__ __forceinline__ int stage_of(const Shapes& s, int position) const { return (first + position) % s.depth; }
     __device__ __forceinline__ bool step(const Shapes& s) {
-        if (next >= end) return false;
-        tile = next / s.depth;
-        from = next - tile * s.depth;
-        to = min(s.depth, from + end - next);
-        next += to - from;
+        if (done >= total) return false;
+        tile = tile_of(s, done);
+        from = stage_of(s, done);
+        to = min(s.depth, from + total - done);
+        done += to - from;
         return true;
     }
 };
 
 // An accumulator's results (lane: row of w, column: token) to memory.  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes
-// are those of its number modulo 4.  `halfs`: the rows' powers of two go into them.  A tile that other CTAs share goes through scratch
-// memory; `flag` is a word of shared memory.
+// are those of its number modulo 4.  `halfs`: the rows' powers of two go into them (`factors`: 32 floats of shared memory for each warp).  A
+// tile that other CTAs share goes through scratch memory; `flag` is a word of shared memory.
 template <int TOKENS, int WARPS, typename Out>
-__device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag) {
+__device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors) {
     constexpr int STEP = TOKENS < 32 ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
     const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
     const int token0 = walk.tile % s.token_tiles * TOKENS, live = min(TOKENS, s.M - token0);
@@ -89,10 +104,16 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
     const long long n = (long long)(walk.tile / s.token_tiles) * BM + row;
     const bool whole = walk.from == 0 && walk.to == s.depth;
     auto finish = [&](int c, float (&v)[STEP]) {
-        if (halfs) {                               // powers of two in the floats' range
+        if (halfs) {                               // powers of two in the floats' range, a lane each, by way of shared memory
+            const int lane = threadIdx.x & 31;
+            __syncwarp();
+            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (c + lane < live ? __ldcg(s.x_exponents + token0 + c + lane) : -s.w_exponent)) << 23);
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < STEP; ++e)
-                v[e] *= __uint_as_float((uint32_t)(127 + s.w_exponent + (c + e < live ? __ldcg(s.x_exponents + token0 + c + e) : -s.w_exponent)) << 23);
+            for (int e = 0; e < STEP; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(factors + e);
+                v[e] *= f.x, v[e + 1] *= f.y, v[e + 2] *= f.z, v[e + 3] *= f.w;
+            }
         }
         if (n < s.N) {
             Out* place = out + (size_t)(token0 + c) * s.N + n;
@@ -106,7 +127,9 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
             }
         }
     };
-    float* mine = s.scratch + ((size_t)blockIdx.x * 2 + (walk.from == 0 ? 1 : 0)) * (TOKENS * BM) + row;
+    // a CTA's sums of a shared tile: [column / 4][row] of four columns
+    auto place_of = [&](int cta, bool head) { return reinterpret_cast<float4*>(s.scratch + ((size_t)cta * 2 + (head ? 1 : 0)) * (TOKENS * BM)) + row; };
+    float4* mine = place_of(blockIdx.x, walk.from == 0);
 #pragma unroll 1
     for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
         float v[STEP];
@@ -117,7 +140,7 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
             finish(c, v);
         } else {
 #pragma unroll
-            for (int e = 0; e < STEP; ++e) __stcg(mine + (c + e) * BM, v[e]);
+            for (int e = 0; e < STEP; e += 4) __stcg(mine + ((c + e) >> 2) * BM, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
         }
     }
     if (whole) return;
@@ -133,13 +156,19 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
 #pragma unroll 1
     for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
         float v[STEP];
-        for (int cta = first; cta <= last; ++cta) {                             // the first has the tile's first stages, at the end of its run
-            const float* from = s.scratch + ((size_t)cta * 2 + (cta == first ? 1 : 0)) * (TOKENS * BM) + row + c * BM;
-            float piece[STEP];
+#pragma unroll 1
+        for (int cta = first; cta <= last; ++cta) {                             // in the order of K; the first's is at the end of its run
+            const float4* from = place_of(cta, cta == first) + (c >> 2) * BM;
+            float4 piece[STEP / 4];
 #pragma unroll
-            for (int e = 0; e < STEP; ++e) piece[e] = __ldcg(from + e * BM);
+            for (int e = 0; e < STEP / 4; ++e) piece[e] = __ldcg(from + e * BM);
 #pragma unroll
-            for (int e = 0; e < STEP; ++e) v[e] = cta == first ? piece[e] : v[e] + piece[e];
+            for (int e = 0; e < STEP / 4; ++e) {
+                v[4 * e] = cta == first ? piece[e].x : v[4 * e] + piece[e].x;
+                v[4 * e + 1] = cta == first ? piece[e].y : v[4 * e + 1] + piece[e].y;
+                v[4 * e + 2] = cta == first ? piece[e].z : v[4 * e + 2] + piece[e].z;
+                v[4 * e + 3] = cta == first ? piece[e].w : v[4 * e + 3] + piece[e].w;
+            }
         }
         finish(c, v);
     }
@@ -148,19 +177,20 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
 // ------------------------------------------------------------------------------------------
 // x in bfloat16
 // ------------------------------------------------------------------------------------------
-constexpr int STEP_K = 128;                        // elements of K of a piece of x and of a buffer of A: eight MMAs
-constexpr int HALF_K = 64;                         // a 128-byte row of x, and what one thread makes of its row at a time
-constexpr int STAGE_STEPS = STAGE_K / STEP_K;
+constexpr int PIECE_K = 64;                        // a 128-byte row of x, and what one thread makes of its row at a time
+// Elements of K of a step: a buffer of A and a slot of x.  The issuing warp's waits and commits cost some 400 clocks a step beside the
+// warps that make A, as much as 40 MMAs of 16 tokens or 4 of 192; tensor memory bounds the steps of wide tiles.
+template <int TOKENS> constexpr int step_k() { return TOKENS <= 64 ? 256 : 128; }
 constexpr int MAKERS = 16, STORERS = 4;            // warps that make bfloat16, and that store results
 constexpr int W_THREADS = (3 + MAKERS + STORERS) * 32;
-constexpr int A_COLUMNS = STEP_K / 2;
-constexpr int W_STAGES = 4;
-template <int TOKENS> constexpr int x_bytes() { return TOKENS * STEP_K * 2; }
+template <int TOKENS> constexpr int a_columns() { return step_k<TOKENS>() / 2; }
+template <int TOKENS> constexpr int x_bytes() { return TOKENS * step_k<TOKENS>() * 2; }
 template <int TOKENS> constexpr int x_stages() { return TOKENS > 128 ? 3 : 4; }
+template <int TOKENS> constexpr int w_stages() { return TOKENS > 128 ? 4 : TOKENS > 32 ? 5 : 8; }      // as many as fit
 template <int TOKENS> constexpr int a_first() { return TOKENS > 128 ? 2 * TOKENS : 256; }            // columns before it: two accumulators
-template <int TOKENS> constexpr int a_buffers() { return (TMEM_COLUMNS - a_first<TOKENS>()) / A_COLUMNS; }
+template <int TOKENS> constexpr int a_buffers() { return (TMEM_COLUMNS - a_first<TOKENS>()) / a_columns<TOKENS>(); }
 template <int TOKENS> constexpr size_t weights_smem() {
-    return 1024 + (size_t)W_STAGES * (CODE_BYTES + SCALE_BYTES) + (size_t)x_stages<TOKENS>() * x_bytes<TOKENS>() + 512;
+    return 1024 + (size_t)w_stages<TOKENS>() * (CODE_BYTES + SCALE_BYTES) + (size_t)x_stages<TOKENS>() * x_bytes<TOKENS>() + 512;
 }
 
 // 32 codes of a row as 16 pairs of halfs, times 2^(byte - 127 - w_exponent); only blocks of zeros have powers beyond [-23, 13].
@@ -213,7 +243,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
                                                                Out* __restrict__ out, const Shapes s) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    constexpr int A_FIRST = a_first<TOKENS>(), A_BUFFERS = a_buffers<TOKENS>(), ACCUMULATOR = A_FIRST / 2, X_STAGES = x_stages<TOKENS>();
+    constexpr int A_FIRST = a_first<TOKENS>(), A_BUFFERS = a_buffers<TOKENS>(), ACCUMULATOR = A_FIRST / 2, X_STAGES = x_stages<TOKENS>(), W_STAGES = w_stages<TOKENS>();
+    constexpr int STEP_K = step_k<TOKENS>(), STAGE_STEPS = STAGE_K / STEP_K, STEP_PIECES = STEP_K / PIECE_K, A_COLUMNS = a_columns<TOKENS>();
     unsigned char* w_ring = smem;
     unsigned char* x_ring = w_ring + W_STAGES * CODE_BYTES;
     unsigned char* s_ring = x_ring + X_STAGES * x_bytes<TOKENS>();
@@ -227,11 +258,12 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     int* flag = reinterpret_cast<int*>(tmem_slot + 1);
+    __shared__ __align__(16) float factors[STORERS * 32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Walk walk(s);
-    // Steps of the tile at hand.  Every stage has two, also where K ends in its first (the second is made of zeros): the warps that
-    // make one of them then use every second buffer of A in turn, and are never more than one use of a buffer behind.
+    // Steps of the tile at hand.  Every stage has all of its steps, also where K ends before (these are made of zeros): the warps that
+    // make a step then use the buffers of A in turn, and are never more than one use of a buffer behind.
     auto steps_of = [&]() { return (walk.to - walk.from) * STAGE_STEPS; };
 
     if (threadIdx.x == 0) {
@@ -244,7 +276,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
             mbar_init(&x_empty[i], 1);
         }
         for (int i = 0; i < A_BUFFERS; ++i) {
-            mbar_init(&a_full[i], 8);
+            mbar_init(&a_full[i], 4 * STEP_PIECES);
             mbar_init(&a_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -265,7 +297,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
 
     // The codes' first stages are on their way before anything else; then, once the kernel before has ended, whether all of x is there as
     // halfs whose powers, with the matrix's, are ordinary floats.
-    const int ahead = s.early ? min(W_STAGES, walk.end - walk.next) : 0;
+    const int ahead = s.early ? min(W_STAGES, walk.total) : 0;
     auto load_codes = [&](int n_tile, int stage, int slot) {
         mbar_arrive_expect_tx(&w_full[slot], CODE_BYTES + SCALE_BYTES);
         tma_load_2d(w_ring + slot * CODE_BYTES, &w_map, &w_full[slot], stage * 128, n_tile * BM);
@@ -273,7 +305,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     };
     if (warp == 2 + MAKERS + STORERS) {
         if (elect_one())
-            for (int i = 0; i < ahead; ++i) load_codes((walk.next + i) / s.depth / s.token_tiles, (walk.next + i) % s.depth, i);
+            for (int i = 0; i < ahead; ++i) load_codes(walk.tile_of(s, i) / s.token_tiles, walk.stage_of(s, i), i);
         __syncwarp();
     }
     pdl_wait();
@@ -301,9 +333,9 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
                 if (leader) {
                     mbar_arrive_expect_tx(&x_full[slot], x_bytes<TOKENS>());
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        tma_load_2d(x_ring + slot * x_bytes<TOKENS>() + h * (TOKENS * 128), map, &x_full[slot], (walk.from * STAGE_STEPS + step) * STEP_K + h * HALF_K,
-                                    token0);
+                    for (int h = 0; h < STEP_PIECES; ++h)
+                        tma_load_2d(x_ring + slot * x_bytes<TOKENS>() + h * (TOKENS * 128), map, &x_full[slot],
+                                    (walk.from * STAGE_STEPS + step) * STEP_K + h * PIECE_K, token0);
                 }
                 __syncwarp();
                 if (++slot == X_STAGES) slot = 0, phase ^= 1;
@@ -364,7 +396,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         const int scale_place = (group >> 1) * MX_TILE_BYTES + lane * 16 + quarter * 4 + (group & 1) * 2;
         int w_slot = 0;
         uint32_t w_phase = 0;
-        for (int step = group >> 1; step < (walk.end - walk.next) * STAGE_STEPS; step += STAGE_STEPS) {          // of the CTA's run
+        for (int step = group / STEP_PIECES; step < walk.total * STAGE_STEPS; step += STAGE_STEPS) {          // of the CTA's run
             if (!warp_wait(&w_full[w_slot], w_phase)) break;
             const unsigned char* codes = w_ring + w_slot * CODE_BYTES + row * 128;
             const uint32_t two = *reinterpret_cast<const uint16_t*>(s_ring + w_slot * SCALE_BYTES + scale_place);
@@ -382,7 +414,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
             if (!warp_wait(&a_empty[b], ((step / A_BUFFERS) & 1) ^ 1)) break;
             __syncwarp();
             tcgen05_fence_after_sync();
-            tmem_store_32_words(lanes + b * A_COLUMNS + (group & 1) * (A_COLUMNS / 2), words);
+            tmem_store_32_words(lanes + b * A_COLUMNS + group % STEP_PIECES * (PIECE_K / 2), words);
             tmem_store_wait();
             tcgen05_fence_before_sync();
             __syncwarp();
@@ -396,7 +428,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2 - MAKERS, halfs, flag);
+            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2 - MAKERS, halfs, flag, factors + (warp - 2 - MAKERS) * 32);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
@@ -436,13 +468,14 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t columns, uint32_t smem_a
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(columns), "l"(desc) : "memory");
 }
 
-constexpr int B_STAGES = 4;
-constexpr int B_STORERS = 8, B_THREADS = 64 + B_STORERS * 32;
+constexpr int B_STORERS = 12, B_THREADS = (3 + B_STORERS) * 32;
+// as many stages as shared memory holds, and tensor memory of their scales
+template <int TOKENS> constexpr int b_stages() { return TOKENS > 128 ? 5 : TOKENS > 64 ? 6 : TOKENS > 32 ? 8 : 9; }
 template <int TOKENS> constexpr int token_blocks() { return TOKENS > 128 ? 2 : 1; }            // tiles of scales of the tokens
 template <int TOKENS> constexpr int both_stage_bytes() { return CODE_BYTES + TOKENS * 128 + SCALE_BYTES * (1 + token_blocks<TOKENS>()); }
-template <int TOKENS> constexpr size_t both_smem() { return 1024 + (size_t)B_STAGES * both_stage_bytes<TOKENS>() + 256; }
-// Tensor memory: two accumulators of up to 192 columns, then a stage's scales in 32 columns: 2 x 4 of w, 2 x 8 of the tokens.
-constexpr int B_ACCUMULATOR = 192, SCALES_FIRST = 2 * B_ACCUMULATOR, SCALE_COLUMNS = 32;
+template <int TOKENS> constexpr size_t both_smem() { return 1024 + (size_t)b_stages<TOKENS>() * both_stage_bytes<TOKENS>() + 256; }
+// Tensor memory: two accumulators, then a stage's scales in 24 columns: 2 x 4 of w, 2 x 8 of the tokens.
+constexpr int SCALE_COLUMNS = 24;
 
 template <int TOKENS, typename Out>
 __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
@@ -450,10 +483,12 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
                                                             const Shapes s) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int STAGE_SCALES = SCALE_BYTES * (1 + token_blocks<TOKENS>()), B_STAGES = b_stages<TOKENS>();
+    constexpr int B_ACCUMULATOR = TOKENS > 128 ? TOKENS : 128, SCALES_FIRST = 2 * B_ACCUMULATOR;
+    static_assert(SCALES_FIRST + B_STAGES * SCALE_COLUMNS <= TMEM_COLUMNS, "tensor memory");
     unsigned char* w_ring = smem;
     unsigned char* x_ring = w_ring + B_STAGES * CODE_BYTES;
     unsigned char* s_ring = x_ring + B_STAGES * TOKENS * 128;
-    constexpr int STAGE_SCALES = SCALE_BYTES * (1 + token_blocks<TOKENS>());
     uint64_t* full = reinterpret_cast<uint64_t*>(s_ring + B_STAGES * STAGE_SCALES);
     uint64_t* empty = full + B_STAGES;
     uint64_t* acc_full = empty + B_STAGES;
@@ -466,7 +501,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < B_STAGES; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 2);
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -485,35 +520,46 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
 
+    // w and x come by the hands of two warps, each with its scales: four or five copies a stage took one warp some 600 clocks.
     if (warp == 0) {
         const bool leader = elect_one();
-        // the first stages of w, as far as the ring goes, before the kernel before has ended
-        const int ahead = s.early ? min(B_STAGES, walk.end - walk.next) : 0;
-        auto load_w = [&](int n_tile, int stage, int i) {
-            mbar_arrive_expect_tx(&full[i], CODE_BYTES + TOKENS * 128 + STAGE_SCALES);
-            tma_load_2d(w_ring + i * CODE_BYTES, &w_map, &full[i], stage * 128, n_tile * BM);
-            bulk_load(s_ring + i * STAGE_SCALES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[i]);
-        };
-        if (leader)
-            for (int i = 0; i < ahead; ++i) load_w((walk.next + i) / s.depth / s.token_tiles, (walk.next + i) % s.depth, i);
-        __syncwarp();
         pdl_wait();
         bool alive = true;
-        int slot = 0, count = 0;
+        int slot = 0;
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
-            const int token0 = walk.tile % s.token_tiles * TOKENS, n_tile = walk.tile / s.token_tiles;
-            for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
+            const int token0 = walk.tile % s.token_tiles * TOKENS;
+            const uint8_t* tile_scales = x_scales + (size_t)(token0 >> 7) * s.w_tiles_of_a_row * MX_TILE_BYTES;
+            // a tile behind the last token: nobody stores its sums
+            const size_t second = (token0 >> 7) + 1 < s.x_row_tiles ? (size_t)s.w_tiles_of_a_row * MX_TILE_BYTES : 0;
+            for (int stage = walk.from; stage < walk.to; ++stage) {
                 if (!(alive = warp_wait(&empty[slot], phase))) break;
                 if (leader) {
-                    if (count >= ahead) load_w(n_tile, stage, slot);
+                    mbar_arrive_expect_tx(&full[slot], TOKENS * 128 + SCALE_BYTES * token_blocks<TOKENS>());
                     tma_load_2d(x_ring + slot * TOKENS * 128, &x_map, &full[slot], stage * 128, token0);
 #pragma unroll
-                    for (int t = 0; t < token_blocks<TOKENS>(); ++t) {
-                        const long long row_tile = min((long long)(token0 >> 7) + t, s.x_row_tiles - 1);      // a tile behind the last token: nobody stores its sums
-                        bulk_load(s_ring + slot * STAGE_SCALES + SCALE_BYTES * (1 + t),
-                                  x_scales + ((size_t)row_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[slot]);
-                    }
+                    for (int t = 0; t < token_blocks<TOKENS>(); ++t)
+                        bulk_load(s_ring + slot * STAGE_SCALES + SCALE_BYTES * (1 + t), tile_scales + t * second + (size_t)stage * SCALE_BYTES, SCALE_BYTES, &full[slot]);
+                }
+                __syncwarp();
+                if (++slot == B_STAGES) slot = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == 2 + B_STORERS) {
+        const bool leader = elect_one();
+        if (!s.early) pdl_wait();
+        bool alive = true;
+        int slot = 0;
+        uint32_t phase = 1;
+        while (alive && walk.step(s)) {
+            const int n_tile = walk.tile / s.token_tiles;
+            const uint8_t* tile_scales = w_scales + (size_t)n_tile * s.w_tiles_of_a_row * MX_TILE_BYTES;
+            for (int stage = walk.from; stage < walk.to; ++stage) {
+                if (!(alive = warp_wait(&empty[slot], phase))) break;
+                if (leader) {
+                    mbar_arrive_expect_tx(&full[slot], CODE_BYTES + SCALE_BYTES);
+                    tma_load_2d(w_ring + slot * CODE_BYTES, &w_map, &full[slot], stage * 128, n_tile * BM);
+                    bulk_load(s_ring + slot * STAGE_SCALES, tile_scales + (size_t)stage * SCALE_BYTES, SCALE_BYTES, &full[slot]);
                 }
                 __syncwarp();
                 if (++slot == B_STAGES) slot = 0, phase ^= 1;
@@ -565,7 +611,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, B_STORERS, Out>(tmem + buffer * B_ACCUMULATOR, out, s, walk, warp - 2, false, flag);
+            store_accumulator<TOKENS, B_STORERS, Out>(tmem + buffer * B_ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
@@ -599,8 +645,7 @@ template <int TOKENS> bool lay_out(Shapes& s, int ctas) {
     const long long units = (long long)((s.N + BM - 1) / BM) * s.token_tiles * s.depth;
     if (units > 0x7FFFFFFF) return false;
     s.units = (int)units;
-    s.grain = s.scratch ? 1 : s.depth;
-    return ctas <= s.units / s.grain;
+    return ctas <= (s.scratch ? s.units : s.units / s.depth);
 }
 
 template <typename... KernelArgs, typename... Args>
@@ -617,9 +662,9 @@ template <int TOKENS, typename Out>
 int launch_weights(const void* x, const void* x_halfs, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
     CUtensorMap w_map, x_map, halfs_map;
     int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
-    if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, HALF_K, TOKENS);
+    if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
     halfs_map = x_map;
-    if (!code && s.x_exponents) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, HALF_K, TOKENS);
+    if (!code && s.x_exponents) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
     if (code) return code;
     static PerDevice configured;
     if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
