@@ -17,85 +17,147 @@ __device__ __forceinline__ void clear(int* zeros, int count) {
     for (int i = blockIdx.x * THREADS + threadIdx.x; i < count; i += gridDim.x * THREADS) zeros[i] = 0;
 }
 
-__device__ __forceinline__ void load_8(const bf16* p, float (&v)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+// Eight elements as they come from memory, the float bits of their largest size, and they themselves.
+struct Eight {
+    uint4 raw;
+    __device__ __forceinline__ void load(const bf16* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ uint32_t largest_of_block() const {            // of 32 elements: four lanes; two sizes a word
+        uint32_t m = __viaddmax_s16x2(raw.x & 0x7FFF7FFFu, 0u, raw.y & 0x7FFF7FFFu);
+        m = __viaddmax_s16x2(raw.z & 0x7FFF7FFFu, 0u, m);
+        m = __viaddmax_s16x2(raw.w & 0x7FFF7FFFu, 0u, m);
+        m = __viaddmax_s16x2(__shfl_xor_sync(0xffffffffu, m, 1), 0u, m);
+        m = __viaddmax_s16x2(__shfl_xor_sync(0xffffffffu, m, 2), 0u, m);
+        return max(m << 16, m & 0xFFFF0000u);
     }
-}
-__device__ __forceinline__ void load_8(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+struct EightFloats {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
+    __device__ __forceinline__ uint32_t largest_of_block() const {
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
+};
+template <typename T> struct EightOf { typedef Eight Type; };
+template <> struct EightOf<float> { typedef EightFloats Type; };
 
-// Sixteen lanes a group of four blocks.  Groups behind a row's end, up to the next 256 elements, write zero scales.
+// A warp takes UNROLL stretches of 256 elements, one after the other in a row and then in the next, all loads first: with one load of
+// 16 bytes a thread in flight and a division for each, 2,048 x 17,408 bfloat16 took XXX us.  Stretches that reach over a row's end
+// write zero scales there.
+template <typename T> constexpr int unroll() { return sizeof(T) == 2 ? 4 : 2; }
+
+struct Stretch {
+    unsigned row, index;               // of its row
+    __device__ __forceinline__ Stretch(unsigned stretch, unsigned of_a_row) : row(stretch / of_a_row), index(stretch - row * of_a_row) {}
+    __device__ __forceinline__ void next(unsigned of_a_row) {
+        if (++index == of_a_row) index = 0, ++row;
+    }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                           long long rows, long long width, long long tiles_of_a_row, int* __restrict__ zeros, int zero_count) {
+                                                           unsigned rows, unsigned width, unsigned of_a_row, int* __restrict__ zeros, int zero_count) {
+    constexpr int UNROLL = unroll<T>();
     pdl_launch_dependents();
     pdl_wait();
     clear(zeros, zero_count);
-    const long long groups = rows * tiles_of_a_row;
-    const int lane16 = threadIdx.x & 15;
-    const long long step = (long long)gridDim.x * (THREADS / 16);
-    for (long long first = (long long)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 5) * 2; first < groups; first += step) {      // the same for a whole warp
-        const long long group = first + ((threadIdx.x >> 4) & 1);
-        const long long row = group / tiles_of_a_row, q = group - row * tiles_of_a_row;
-        const long long column = q * 128 + lane16 * 8;
-        const bool inside = group < groups && column < width;
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (inside) load_8(x + row * width + column, v);
-        uint32_t largest = 0;
+    const unsigned lane = threadIdx.x & 31, half = lane >> 4, warps = gridDim.x * (THREADS / 32);
+    const unsigned stretches = rows * of_a_row;
+    for (unsigned first = (blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * UNROLL; first < stretches; first += warps * UNROLL) {
+        typename EightOf<T>::Type held[UNROLL];
+        Stretch at(first, of_a_row);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        const uint32_t byte = mx_scale_byte(largest);
-        const uint32_t word = byte == 255u ? 0u : mx_encode_8(v, mx_inverse(byte));
-        if (inside) *reinterpret_cast<uint32_t*>(codes + row * (width >> 1) + (column >> 1)) = word;
-        uint32_t four = byte << (8 * (lane16 >> 2));
-        four |= __shfl_xor_sync(0xffffffffu, four, 4);
-        four |= __shfl_xor_sync(0xffffffffu, four, 8);
-        if (lane16 == 0 && group < groups) *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(row, q, tiles_of_a_row)) = four;
+        for (int u = 0; u < UNROLL; ++u, at.next(of_a_row)) {
+            const unsigned column = at.index * 256 + lane * 8;
+            held[u] = {};
+            if (first + u < stretches && column < width) held[u].load(x + (size_t)at.row * width + column);
+        }
+        at = Stretch(first, of_a_row);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u, at.next(of_a_row)) {
+            if (first + u >= stretches) break;                                 // the same for the whole warp
+            const unsigned column = at.index * 256 + lane * 8;
+            const uint32_t byte = mx_scale_byte(held[u].largest_of_block());
+            float v[8];
+            held[u].values(v);
+            const uint32_t word = byte == 255u ? 0u : mx_encode_8(v, mx_inverse(byte));
+            if (column < width) *reinterpret_cast<uint32_t*>(codes + (size_t)at.row * (width >> 1) + (column >> 1)) = word;
+            uint32_t four = byte << (8 * ((lane >> 2) & 3));
+            four |= __shfl_xor_sync(0xffffffffu, four, 4);
+            four |= __shfl_xor_sync(0xffffffffu, four, 8);
+            if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(at.row, at.index * 2 + half, of_a_row * 2)) = four;
+        }
     }
 }
 
-__device__ __forceinline__ void store_8(bf16* p, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);       // exact: one bit of mantissa
-        w[i] = *reinterpret_cast<uint32_t*>(&pair);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void store_8(float* p, const float (&v)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-
+// The same stretches back.  A lane makes what one 16-byte store takes: eight bfloat16, or four floats of each half of the stretch.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
-                                                             long long rows, long long width, long long tiles_of_a_row) {
+                                                             unsigned rows, unsigned width, unsigned of_a_row) {
+    constexpr int UNROLL = 4, EACH = sizeof(T) == 2 ? 8 : 4, PARTS = 8 / EACH;
+    pdl_launch_dependents();
     pdl_wait();
-    const long long eighths = width >> 3, total = rows * eighths;
-    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-        const long long row = i / eighths, part = i - row * eighths;
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + i * 4);
-        const float scale = mx_scale(scales[mx_scale_offset(row, part >> 4, tiles_of_a_row) + ((part >> 2) & 3)]);
-        uint32_t h[4];
-        mx_decode_8(word, h);
-        float v[8];
+    const unsigned lane = threadIdx.x & 31, warps = gridDim.x * (THREADS / 32);
+    const unsigned stretches = rows * of_a_row;
+    for (unsigned first = (blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * UNROLL; first < stretches; first += warps * UNROLL) {
+        uint32_t word[UNROLL][PARTS], byte[UNROLL][PARTS];
+        Stretch at(first, of_a_row);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const float2 pair = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
-            v[2 * p] = pair.x * scale;
-            v[2 * p + 1] = pair.y * scale;
-        }
-        store_8(out + i * 8, v);
+        for (int u = 0; u < UNROLL; ++u, at.next(of_a_row))
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const unsigned within = p * 128 + lane * EACH, column = at.index * 256 + within;
+                word[u][p] = byte[u][p] = 0;
+                if (first + u < stretches && column < width) {
+                    const uint8_t* from = codes + (size_t)at.row * (width >> 1) + (column >> 1);
+                    word[u][p] = EACH == 8 ? *reinterpret_cast<const uint32_t*>(from) : *reinterpret_cast<const uint16_t*>(from);
+                    byte[u][p] = scales[mx_scale_offset(at.row, at.index * 2 + (within >> 7), of_a_row * 2) + ((within >> 5) & 3)];
+                }
+            }
+        at = Stretch(first, of_a_row);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u, at.next(of_a_row))
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const unsigned column = at.index * 256 + p * 128 + lane * EACH;
+                if (first + u >= stretches || column >= width) continue;
+                const float scale = mx_scale(byte[u][p]);
+                uint32_t h[EACH / 2];
+                if constexpr (EACH == 8) mx_decode_8(word[u][p], h);
+                else mx_decode_4(word[u][p], h);
+                float v[EACH];
+#pragma unroll
+                for (int i = 0; i < EACH / 2; ++i) {
+                    const float2 pair = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+                    v[2 * i] = pair.x * scale;
+                    v[2 * i + 1] = pair.y * scale;
+                }
+                T* to = out + (size_t)at.row * width + column;
+                if constexpr (EACH == 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);       // exact: one bit of mantissa
+                        w[i] = *reinterpret_cast<uint32_t*>(&pair);
+                    }
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
     }
 }
 
@@ -193,13 +255,16 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
     if (threadIdx.x == 0) exponents[row] = bad ? HALFS_LOST : empty ? 0 : field - 127 - 15;
 }
 
-// Blocks of a launch over `items` threads of work: loops over them where that is more than 16 blocks an SM.
+// Blocks of a launch over `items` threads of work: they loop where that is more than 64 blocks an SM.
 int blocks_for(long long items) {
     const long long want = (items + THREADS - 1) / THREADS, most = (long long)mrs_sm_count() * 64;
-    return (int)(want < most ? want : most);
+    return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-bool bad_sizes(long long rows, long long width) { return rows < 0 || width <= 0 || width % MX_BLOCK || rows > (1ll << 40) / width; }
+// (rows x stretches of 256 elements are counted in 32 bits)
+bool bad_sizes(long long rows, long long width) {
+    return rows < 0 || width <= 0 || width % MX_BLOCK || width > (1ll << 30) || rows > (1ll << 31) || rows * ((width + 255) / 256) > (1ll << 31);
+}
 
 }  // namespace
 
@@ -212,20 +277,24 @@ MRS_EXPORT long long mrs_mxfp4_scale_bytes(long long rows, long long width) {
 MRS_EXPORT int mrs_mxfp4_quantise(int is_bf16, const void* x, void* codes, void* scales, long long rows, long long width, void* zeros, int zero_count, void* stream) {
     if (rows == 0) return 0;
     if (bad_sizes(rows, width) || (zero_count && !zeros) || !x || !codes || !scales || (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
-    const long long tiles = mx_tiles_of_a_row(width);
-    const int blocks = blocks_for(rows * tiles * 16);
-    if (is_bf16) MRS_LAUNCH(quantise_kernel<bf16>, blocks, THREADS, 0, stream, (const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles, (int*)zeros, zero_count);
-    else MRS_LAUNCH(quantise_kernel<float>, blocks, THREADS, 0, stream, (const float*)x, (uint8_t*)codes, (uint8_t*)scales, rows, width, tiles, (int*)zeros, zero_count);
+    const unsigned of_a_row = (unsigned)((width + 255) / 256);
+    const long long threads = rows * of_a_row * 32;
+    if (is_bf16)
+        MRS_LAUNCH(quantise_kernel<bf16>, blocks_for(threads / unroll<bf16>()), THREADS, 0, stream, (const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, (unsigned)rows,
+                   (unsigned)width, of_a_row, (int*)zeros, zero_count);
+    else
+        MRS_LAUNCH(quantise_kernel<float>, blocks_for(threads / unroll<float>()), THREADS, 0, stream, (const float*)x, (uint8_t*)codes, (uint8_t*)scales, (unsigned)rows,
+                   (unsigned)width, of_a_row, (int*)zeros, zero_count);
     MRS_RETURN_LAUNCH_STATUS();
 }
 
 MRS_EXPORT int mrs_mxfp4_dequantise(int is_bf16, const void* codes, const void* scales, void* out, long long rows, long long width, void* stream) {
     if (rows == 0) return 0;
     if (bad_sizes(rows, width) || !out || !codes || !scales || (((uintptr_t)out | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
-    const long long tiles = mx_tiles_of_a_row(width);
-    const int blocks = blocks_for(rows * (width >> 3));
-    if (is_bf16) MRS_LAUNCH(dequantise_kernel<bf16>, blocks, THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (bf16*)out, rows, width, tiles);
-    else MRS_LAUNCH(dequantise_kernel<float>, blocks, THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (float*)out, rows, width, tiles);
+    const unsigned of_a_row = (unsigned)((width + 255) / 256);
+    const int blocks = blocks_for(rows * of_a_row * 8);
+    if (is_bf16) MRS_LAUNCH(dequantise_kernel<bf16>, blocks, THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (bf16*)out, (unsigned)rows, (unsigned)width, of_a_row);
+    else MRS_LAUNCH(dequantise_kernel<float>, blocks, THREADS, 0, stream, (const uint8_t*)codes, (const uint8_t*)scales, (float*)out, (unsigned)rows, (unsigned)width, of_a_row);
     MRS_RETURN_LAUNCH_STATUS();
 }
 

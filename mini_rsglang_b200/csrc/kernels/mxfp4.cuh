@@ -36,11 +36,19 @@ __device__ __forceinline__ uint32_t mx_encode_8(const float (&v)[8], float inver
     return r;
 }
 
-// Eight codes to four pairs of halfs (exact).
+// Eight codes to four pairs of halfs (exact).  All four have to be used: where the compiler (nvcc 12.9) finds a byte of the unpacked word
+// without a use it makes zeros of the others; for four codes there is mx_decode_4.
 __device__ __forceinline__ void mx_decode_8(uint32_t codes, uint32_t (&h)[4]) {
     asm("{\n .reg .b8 b0, b1, b2, b3;\n mov.b32 {b0, b1, b2, b3}, %4;\n"
         " cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n cvt.rn.f16x2.e2m1x2 %2, b2;\n cvt.rn.f16x2.e2m1x2 %3, b3;\n}"
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(codes));
+}
+
+// The four codes of the lowest 16 bits to two pairs of halfs (exact).
+__device__ __forceinline__ void mx_decode_4(uint32_t codes, uint32_t (&h)[2]) {
+    asm("{\n .reg .b8 b0, b1;\n .reg .b16 low;\n cvt.u16.u32 low, %2;\n mov.b16 {b0, b1}, low;\n"
+        " cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n}"
+        : "=r"(h[0]), "=r"(h[1]) : "r"(codes));
 }
 
 // The scale byte of a block whose largest element has the float bits `largest` (sign off): its exponent less two, so that the

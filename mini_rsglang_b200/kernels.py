@@ -2665,7 +2665,7 @@ class Mxfp4:
 def _mxfp4_sizes(rows: int, width: int, what: str) -> None:
     if width <= 0 or width % MXFP4_BLOCK:
         raise InvalidRequest(f"{what}: rows of {width} elements; 4-bit rows are whole blocks of {MXFP4_BLOCK}")
-    if rows >= 1 << 31 or width > 1 << 30:
+    if width > 1 << 30 or rows * -(-width // 256) > 1 << 31:
         raise InvalidRequest(f"{what}: {rows} rows of {width} elements are too many")
 
 
