@@ -42,6 +42,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--no-prefix-cache", action="store_true",
                    help="do not share the cache pages of equal first tokens between requests")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--weight-format", choices=["held", "mxfp4"], default="held",
+                   help="mxfp4: projections of attention and dense feed-forwards in 4-bit floating point")
+    p.add_argument("--activation-format", choices=["held", "mxfp4"], default="held", help="mxfp4: what they read in 4 bits too")
     p.add_argument("--num-pages", type=int, default=None, help="size of the page pool (overrides --kv-mib)")
     p.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                    help="take only config.json from --model and draw the weights on the device from this seed "
@@ -79,7 +82,8 @@ def build_parser() -> argparse.ArgumentParser:
 def runtime_config(args) -> RuntimeConfig:
     return RuntimeConfig(max_seq_len=args.max_seq_len, page_size=args.page_size, prefill_budget=args.prefill_budget,
                          max_running=args.max_running, max_waiting=args.max_waiting,
-                         prefix_cache=not args.no_prefix_cache)
+                         prefix_cache=not args.no_prefix_cache, weight_format=args.weight_format,
+                         activation_format=args.activation_format)
 
 
 def load_engine(args, limits: RuntimeConfig):

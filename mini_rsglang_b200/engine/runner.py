@@ -113,7 +113,11 @@ class ModelRunner:
                                  f"{config.max_position_embeddings}")
         self.config, self.runtime, self.limits = config, runtime, limits
         self.device = runtime.device
+        if runtime.weight_format != "held" and not runtime.is_bf16:
+            raise InvalidRequest("weights in 4 bits are for serving in bfloat16; the 32-bit path keeps every bit")
         self.model = Model(spec or model_spec_for(config), tensors, runtime)
+        if runtime.weight_format != "held" and not self.model.projections_in_4_bits():
+            raise InvalidRequest("this model has no projection that can be held in 4 bits (grouped-query attention, dense feed-forwards)")
         kv_needs, state_needs = self.model.kv_needs(), self.model.state_needs()
         keys, group_of = plan_groups(kv_needs)
         if not keys:                       # a model without paged caches still has block tables of width 0
@@ -169,12 +173,17 @@ class ModelRunner:
         self.h2d_bytes = 0      # bytes of batch metadata copied to the device so far
 
     # ------------------------------------------------------------------ construction
+    @staticmethod
+    def _runtime(device, dtype, limits: RuntimeConfig) -> Runtime:
+        limits.validate()
+        return Runtime(torch.device(device), resolve_dtype(dtype), limits.page_size, limits.weight_format, limits.activation_format)
+
     @classmethod
     def load(cls, folder: str, dtype="bfloat16", device="cuda:0", limits: RuntimeConfig | None = None,
              kv_bytes: int | None = None, num_pages: int | None = None) -> "ModelRunner":
         config = load_config(folder)
         spec = model_spec_for(config)
-        runtime = Runtime(torch.device(device), resolve_dtype(dtype), (limits or RuntimeConfig()).page_size)
+        runtime = cls._runtime(device, dtype, limits or RuntimeConfig())
         tensors = load_weights(folder, spec.weight_specs(), runtime.dtype, runtime.device, spec.ignorable_weights)
         return cls(config, tensors, runtime, limits or RuntimeConfig(), kv_bytes, num_pages, spec)
 
@@ -183,7 +192,7 @@ class ModelRunner:
                     kv_bytes: int | None = None, num_pages: int | None = None) -> "ModelRunner":
         """A model with seeded random weights drawn on the device (no files)."""
         spec = model_spec_for(config)
-        runtime = Runtime(torch.device(device), resolve_dtype(dtype), (limits or RuntimeConfig()).page_size)
+        runtime = cls._runtime(device, dtype, limits or RuntimeConfig())
         tensors = random_weights(spec.weight_specs(), seed, runtime.dtype, runtime.device)
         return cls(config, tensors, runtime, limits or RuntimeConfig(), kv_bytes, num_pages, spec)
 

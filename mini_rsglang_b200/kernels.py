@@ -7,6 +7,7 @@ or without the compiled library, they raise `BackendError`."""
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 
@@ -2604,8 +2605,11 @@ def _mxfp4_check(code: int, what: str) -> None:
 class _OnDevice:
     """The tensor's device as the current one, where it is not (`torch.cuda.device` costs microseconds)."""
 
+    __slots__ = ("guard",)
+
     def __init__(self, device: torch.device):
-        self.guard = None if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        index = device.index
+        self.guard = None if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:
@@ -2616,33 +2620,25 @@ class _OnDevice:
             self.guard.__exit__(*exc)
 
 
+def _mxfp4_bytes(rows: int, width: int) -> tuple[int, int]:
+    """(bytes of codes, bytes of scales): scales in tiles of 128 rows x 4 blocks, an even number of tiles a row."""
+    return rows * (width >> 1), -(-rows // 128) * (-(-width // 256) * 1024)
+
+
 class Mxfp4:
     """A matrix [rows, width] in microscaled 4-bit floating point: for every element a sign, two bits of exponent and one of
     mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), for every 32 neighbours of a row one power of two.
 
-    `codes` uint8 [rows, width / 2] (element 2 j in the low half of byte j), `scales` uint8 in the tiles that the tensor
-    cores read (`csrc/kernels/mxfp4.cuh`).  `settled` (`settle()`): the matrix was there before anything that is still queued, and
-    nothing writes it any more, so that a product may fetch it while the kernel before still runs; `half_exponent` is then the
-    power by which all of it fits halfs exactly, or None."""
+    `data` uint8 holds the codes [rows, width / 2] (element 2 j in the low half of byte j) and behind them the scales in the tiles
+    that the tensor cores read (`csrc/kernels/mxfp4.cuh`).  `settled` (`settle()`): the matrix was there before anything
+    that is still queued, and nothing writes it any more, so that a product may fetch it while the kernel before still runs;
+    `half_exponent` is then the power by which all of it fits halfs exactly, or None."""
 
-    __slots__ = ("codes", "scales", "rows", "width", "settled", "half_exponent")
+    __slots__ = ("data", "rows", "width", "settled", "half_exponent")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int):
-        self.codes, self.scales, self.rows, self.width = codes, scales, int(rows), int(width)
+    def __init__(self, data: torch.Tensor, rows: int, width: int):
+        self.data, self.rows, self.width = data, rows, width
         self.settled, self.half_exponent = False, None
-
-    def settle(self) -> "Mxfp4":
-        """Waits until the matrix is there and takes note of its scales' range.  For weights, once: products of settled weights are
-        faster.  Whoever writes the tensors afterwards has to make a matrix anew."""
-        with _OnDevice(self.device):
-            span = torch.tensor([256, -1], dtype=torch.int32, device=self.device)
-            _mxfp4_check(mxfp4_library().mrs_mxfp4_scale_range(self.codes.data_ptr(), self.scales.data_ptr(), span.data_ptr(), self.rows, self.width,
-                                                               _stream()), "mxfp4_scale_range")
-            low, high = span.tolist()                        # waits for the stream
-        # halfs hold 0.5 times 2^-23 to 6 times 2^13
-        self.half_exponent = None if high == 255 or high - low > 36 else max(high, 0) - 127 - 13
-        self.settled = True
-        return self
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -2650,10 +2646,36 @@ class Mxfp4:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[:_mxfp4_bytes(self.rows, self.width)[0]].view(self.rows, self.width // 2)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[_mxfp4_bytes(self.rows, self.width)[0]:]
+
+    def addresses(self) -> tuple[int, int]:
+        """Of the codes and of the scales."""
+        base = self.data.data_ptr()
+        return base, base + self.rows * (self.width >> 1)
 
     def bytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.data.numel()
+
+    def settle(self) -> "Mxfp4":
+        """Waits until the matrix is there and takes note of its scales' range.  For weights, once: products of settled weights are
+        faster.  Whoever writes the data afterwards has to make a matrix anew.  Not while a graph is recorded."""
+        with _OnDevice(self.device):
+            span = torch.tensor([256, -1], dtype=torch.int32, device=self.device)
+            codes, scales = self.addresses()
+            _mxfp4_check(mxfp4_library().mrs_mxfp4_scale_range(codes, scales, span.data_ptr(), self.rows, self.width, _stream()), "mxfp4_scale_range")
+            low, high = span.tolist()                        # waits for the stream
+        # halfs hold 0.5 times 2^-23 to 6 times 2^13
+        self.half_exponent = None if high == 255 or high - low > 36 else max(high, 0) - 127 - 13
+        self.settled = True
+        return self
 
     def block_scales(self) -> torch.Tensor:
         """The scale bytes [rows, width / 32]: a block's exponent + 127, 255 for a block that is not a number."""
@@ -2669,14 +2691,12 @@ def _mxfp4_sizes(rows: int, width: int, what: str) -> None:
         raise InvalidRequest(f"{what}: {rows} rows of {width} elements are too many")
 
 
-def _mxfp4_buffers(rows: int, width: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    tile_rows, tiles = -(-rows // 128), -(-width // 256) * 2
-    return (torch.empty((rows, width // 2), dtype=torch.uint8, device=device),
-            torch.empty(tile_rows * tiles * 512, dtype=torch.uint8, device=device))
+def _mxfp4_empty(rows: int, width: int, device) -> Mxfp4:
+    return Mxfp4(torch.empty(sum(_mxfp4_bytes(rows, width)), dtype=torch.uint8, device=device), rows, width)
 
 
 def _mxfp4_aligned(t: torch.Tensor, what: str) -> None:
-    if t.data_ptr() % 16:
+    if t.data_ptr() & 15:
         raise InvalidRequest(f"{what}: the tensor does not begin on a 16-byte boundary")
 
 
@@ -2692,21 +2712,21 @@ def mxfp4_quantise(x: torch.Tensor) -> Mxfp4:
     _need(x, None, "mxfp4_quantise input")
     _mxfp4_aligned(x, "mxfp4_quantise input")
     with _OnDevice(x.device):
-        codes, scales = _mxfp4_buffers(rows, width, x.device)
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, width, None, 0,
-                                                        _stream()), "mxfp4_quantise")
-    return Mxfp4(codes, scales, rows, width)
+        out = _mxfp4_empty(rows, width, x.device)
+        codes, scales = out.addresses()
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes, scales, rows, width, None, 0, _stream()), "mxfp4_quantise")
+    return out
 
 
 def mxfp4_dequantise(matrix: Mxfp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """What the codes stand for, in bfloat16 or float32 (both hold every such value; a scale beyond 2^125 may make bfloat16's and
     float32's infinity of a code)."""
     bf16 = _is_bf16(dtype)
-    _need(matrix.codes, torch.uint8, "mxfp4 codes", (matrix.rows, matrix.width // 2))
+    _need(matrix.data, torch.uint8, "mxfp4 matrix")
     with _OnDevice(matrix.device):
         out = torch.empty((matrix.rows, matrix.width), dtype=dtype, device=matrix.device)
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_dequantise(bf16, matrix.codes.data_ptr(), matrix.scales.data_ptr(), out.data_ptr(),
-                                                          matrix.rows, matrix.width, _stream()), "mxfp4_dequantise")
+        codes, scales = matrix.addresses()
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_dequantise(bf16, codes, scales, out.data_ptr(), matrix.rows, matrix.width, _stream()), "mxfp4_dequantise")
     return out
 
 
@@ -2725,13 +2745,14 @@ def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
     if scales.device != codes.device:
         raise InvalidRequest("mxfp4_matrix: codes and scales are on different devices")
     with _OnDevice(codes.device):
-        _, tiles = _mxfp4_buffers(rows, width, codes.device)
-        held = codes.clone()
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_scales_to_tiles(scales.data_ptr(), held.data_ptr(), tiles.data_ptr(), rows, width, _stream()),
-                     "mxfp4_matrix")
-    return Mxfp4(held, tiles, rows, width).settle()
+        out = _mxfp4_empty(rows, width, codes.device)
+        out.codes.copy_(codes)
+        held, tiles = out.addresses()
+        _mxfp4_check(mxfp4_library().mrs_mxfp4_scales_to_tiles(scales.data_ptr(), held, tiles, rows, width, _stream()), "mxfp4_matrix")
+    return out.settle()
 
 
+@functools.lru_cache(maxsize=4096)
 def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
     """How a product is launched: ("few", CTAs of a cluster) or ("many", tokens of a tile, CTAs, whether tiles may be shared)."""
     if m <= (4 if quantise else 8):
@@ -2774,31 +2795,33 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
     _mxfp4_aligned(x, "mxfp4_gemm input")
     lib = mxfp4_library()
     out_f32, early = int(out.dtype is torch.float32), int(weight.settled)
+    w_codes, w_scales = weight.addresses()
     with _OnDevice(x.device):
+        sms = sm_count(x.device)
         if plan is None:
-            plan = mxfp4_plan(m, n, k, quantise, sm_count(x.device))
+            plan = mxfp4_plan(m, n, k, bool(quantise), sms)
         if plan[0] == "few":
-            code = lib.mrs_mxfp4_few_rows(x.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), out_f32, m, n, k,
-                                          int(bool(quantise)), plan[1], sm_count(x.device), early, _stream())
+            code = lib.mrs_mxfp4_few_rows(x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early,
+                                          _stream())
         else:
+            # one buffer: what x becomes, then, where tiles are shared, their sums and their counts (set to zero by the kernel before the product)
             _, tokens, ctas, shared = plan
-            scratch = arrived = None
-            tiles = -(-n // 128) * -(-m // tokens)
-            if shared:
-                scratch = torch.empty(2 * ctas * tokens * 128, dtype=torch.float32, device=x.device)
-                arrived = torch.empty(tiles, dtype=torch.int32, device=x.device)              # set to zero by the kernel before the product
+            tiles = -(-n // 128) * -(-m // tokens) if shared else 0
+            x_bytes, side_bytes = _mxfp4_bytes(m, k) if quantise else (2 * m * k, -(-m // 4) * 16)
+            scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
+            work = torch.empty(x_bytes + side_bytes + scratch_bytes + 4 * tiles, dtype=torch.uint8, device=x.device)
+            made = work.data_ptr()
+            side, scratch = made + x_bytes, made + x_bytes + side_bytes if shared else None
+            arrived = scratch + scratch_bytes if shared else None
+            stream = _stream()
             launch_count += 1
             if quantise:
-                codes, scales = _mxfp4_buffers(m, k, x.device)
-                code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k, _ptr(arrived), tiles if shared else 0, _stream())
-                code = code or lib.mrs_mxfp4_both_rows(codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                                       out.data_ptr(), out_f32, m, n, k, tokens, ctas, _ptr(scratch), _ptr(arrived), early, _stream())
+                code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), made, side, m, k, arrived, tiles, stream)
+                code = code or lib.mrs_mxfp4_both_rows(made, side, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived,
+                                                       early, stream)
             else:
-                halfs = torch.empty((m, k), dtype=torch.float16, device=x.device)
-                exponents = torch.empty(m, dtype=torch.int32, device=x.device)
-                code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), halfs.data_ptr(), exponents.data_ptr(), m, k, _ptr(arrived), tiles if shared else 0, _stream())
                 fits = weight.half_exponent is not None
-                code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), halfs.data_ptr() if fits else None, exponents.data_ptr() if fits else None,
-                                                          weight.half_exponent or 0, weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
-                                                          out_f32, m, n, k, tokens, ctas, _ptr(scratch), _ptr(arrived), early, _stream())
+                code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, m, k, arrived, tiles, stream)
+                code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), made if fits else None, side if fits else None, weight.half_exponent or 0, w_codes,
+                                                          w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived, early, stream)
         _mxfp4_check(code, "mxfp4_gemm")

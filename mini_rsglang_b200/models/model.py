@@ -5,6 +5,7 @@ from __future__ import annotations
 import torch
 
 from ..parts.base import BranchSum, Normed, Prenormed, Runtime
+from ..parts.linear import FourBitWeight
 from .spec import ModelSpec
 
 
@@ -67,6 +68,21 @@ class Model:
                     total += t.numel() * t.element_size()
         return total
 
+    def projections_in_4_bits(self) -> int:
+        """Matrices that are held in 4 bits."""
+        seen, count, waiting = set(), 0, [self.embedding, *self.stream_entries, *self.blocks, self.final_norm, self.head]
+        while waiting:
+            part = waiting.pop()
+            if id(part) in seen:
+                continue
+            seen.add(id(part))
+            for value in vars(part).values():
+                if isinstance(value, FourBitWeight):
+                    count += 1
+                elif hasattr(value, "bind") and hasattr(value, "weight_specs"):
+                    waiting.append(value)
+        return count
+
     def forward(self, ctx, storage) -> torch.Tensor | None:
         """Runs the step's tokens through every layer; float32 logits [wanted, vocab], or None
         when no logits are wanted (the head is then skipped, as in the reference,
@@ -122,6 +138,8 @@ def _tensors_of(part, seen=None):
     for value in vars(part).values():
         if isinstance(value, torch.Tensor):
             out.append(value)
+        elif isinstance(value, FourBitWeight):
+            out.append(value.matrix.data)
         elif hasattr(value, "bind") and hasattr(value, "weight_specs"):
             out += _tensors_of(value, seen)
     return out

@@ -17,7 +17,7 @@ from .. import kernels
 from ..errors import InvalidRequest
 from ..weights.spec import WeightSpec
 from .base import MIXERS, NORMS, POSITION_ENCODINGS, KVNeed, Mixer, PartSpec, Prenormed, StepFacts, observing
-from .linear import few_rows, linear
+from .linear import few_rows, linear, projection
 
 
 @dataclass
@@ -377,8 +377,9 @@ class GroupedQueryAttention(Mixer):
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         self.qkv = torch.cat([tensors[self.name("q_proj.weight")], tensors[self.name("k_proj.weight")],
-                              tensors[self.name("v_proj.weight")]], dim=0).contiguous()
-        self.o = tensors[self.name("o_proj.weight")].contiguous()
+                              tensors[self.name("v_proj.weight")]], dim=0)
+        self.qkv = projection(self.qkv, runtime)
+        self.o = projection(tensors[self.name("o_proj.weight")], runtime)
         self.position.bind(tensors, runtime)
         for norm in (self.q_norm, self.k_norm):
             if norm is not None:

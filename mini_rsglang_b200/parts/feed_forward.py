@@ -9,7 +9,7 @@ from .. import kernels
 from ..errors import InvalidRequest
 from ..weights.spec import WeightSpec
 from .base import FEED_FORWARDS, FeedForward, Prenormed, observing, plain
-from .linear import few_rows, linear
+from .linear import FourBitWeight, few_rows, linear, projection
 
 
 @FEED_FORWARDS.register("swiglu")
@@ -39,15 +39,15 @@ class SwiGLU(FeedForward):
         gate, up = tensors[self.name(self.leaf["gate"])], tensors[self.name(self.leaf["up"])]
         # When serving in bfloat16 and the width allows it, blocks of 64 gate rows alternate with the 64
         # matching up rows: a weight tile of the product for few rows then holds both halves of its outputs,
-        # and the product applies silu(gate) * up before it stores.
-        self.block = self.BLOCK if runtime.is_bf16 and self.inner % self.BLOCK == 0 else 0
+        # and the product applies silu(gate) * up before it stores.  (Weights in 4 bits have products of their own.)
+        self.block = self.BLOCK if runtime.is_bf16 and runtime.weight_format == "held" and self.inner % self.BLOCK == 0 else 0
         if self.block:
             b = self.block
             self.gate_up = torch.stack([gate.view(-1, b, self.width), up.view(-1, b, self.width)], dim=1) \
                 .reshape(2 * self.inner, self.width).contiguous()
         else:
-            self.gate_up = torch.cat([gate, up], dim=0).contiguous()
-        self.down = tensors[self.name(self.leaf["down"])].contiguous()
+            self.gate_up = projection(torch.cat([gate, up], dim=0), runtime)
+        self.down = projection(tensors[self.name(self.leaf["down"])], runtime)
 
     def forward(self, h, ctx, into=None):
         act = torch.empty((h.shape[0], self.inner), dtype=self.runtime.dtype, device=self.down.device)
@@ -89,8 +89,8 @@ class ClampedGLU(FeedForward):
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         n = self.leaf
-        self.gate_up = torch.cat([tensors[self.name(n["gate"])], tensors[self.name(n["up"])]], dim=0).contiguous()
-        self.down = tensors[self.name(n["down"])].contiguous()
+        self.gate_up = projection(torch.cat([tensors[self.name(n["gate"])], tensors[self.name(n["up"])]], dim=0), runtime)
+        self.down = projection(tensors[self.name(n["down"])], runtime)
 
     def forward(self, h, ctx):
         h = plain(h)
@@ -122,12 +122,12 @@ class DenseMLP(FeedForward):
 
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
-        self.up = tensors[self.name(self.leaf["up"])].contiguous()
-        self.down = tensors[self.name(self.leaf["down"])].contiguous()
+        self.up = projection(tensors[self.name(self.leaf["up"])], runtime)
+        self.down = projection(tensors[self.name(self.leaf["down"])], runtime)
 
     def forward(self, h, ctx):
         x = plain(h)
-        if kernels.gemm_act_rows_wins(x, self.up, self.activation):      # many rows: the activation in the product's epilogue
+        if not isinstance(self.up, FourBitWeight) and kernels.gemm_act_rows_wins(x, self.up, self.activation):      # many rows: the activation in the product's epilogue
             z = torch.empty((x.shape[0], self.inner), dtype=x.dtype, device=x.device)
             kernels.gemm_act_rows(x, self.up, z, self.activation)
         else:
@@ -167,14 +167,14 @@ class GatedMLP(FeedForward):
         super().bind(tensors, runtime)
         n = self.leaf
         gate, up = tensors[self.name(n["gate"])], tensors[self.name(n["up"])]
-        self.block = self.BLOCK if runtime.is_bf16 and self.inner % self.BLOCK == 0 else 0
+        self.block = self.BLOCK if runtime.is_bf16 and runtime.weight_format == "held" and self.inner % self.BLOCK == 0 else 0
         if self.block:
             b = self.block
             self.gate_up = torch.stack([gate.view(-1, b, self.width), up.view(-1, b, self.width)], dim=1) \
                 .reshape(2 * self.inner, self.width).contiguous()
         else:
-            self.gate_up = torch.cat([gate, up], dim=0).contiguous()
-        self.down = tensors[self.name(n["down"])].contiguous()
+            self.gate_up = projection(torch.cat([gate, up], dim=0), runtime)
+        self.down = projection(tensors[self.name(n["down"])], runtime)
 
     def forward(self, h, ctx):
         h = plain(h)

@@ -5,7 +5,10 @@ bfloat16 of every float32, so that no bit of the inputs is given up; no reduced-
 portions) go through the engine's tcgen05 kernel, which streams the weights once with bulk
 tensor copies; more rows go through the library (cuBLAS through torch.mm, float32
 accumulation, reduced-precision reductions switched off), as the reference uses cuBLAS for
-every projection (crates/kernels/src/lib.rs:298-321)."""
+every projection (crates/kernels/src/lib.rs:298-321).
+
+A projection may be held in 4 bits instead (`projection`, `FourBitWeight`): its products are the engine's own kernels for any
+number of rows."""
 from __future__ import annotations
 
 import torch
@@ -22,14 +25,39 @@ def configure_library_products() -> None:
     torch.backends.cuda.matmul.allow_tf32 = False
 
 
-def few_rows(x, weight: torch.Tensor) -> bool:
-    """Whether the engine's own tensor-core product takes this one."""
+class FourBitWeight:
+    """A projection's weights in microscaled 4-bit floating point, and whether what it reads is brought to 4 bits too."""
+
+    def __init__(self, weight: torch.Tensor, quantise: bool):
+        self.matrix = kernels.mxfp4_quantise(weight.contiguous()).settle()
+        self.quantise = bool(quantise)
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.matrix.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.matrix.device
+
+
+def projection(weight: torch.Tensor, runtime) -> "torch.Tensor | FourBitWeight":
+    """A projection's weights [out, in] as the runtime wants them held; `linear` takes either."""
+    if runtime.weight_format == "mxfp4":
+        return FourBitWeight(weight, runtime.activation_format == "mxfp4")
+    return weight.contiguous()
+
+
+def few_rows(x, weight) -> bool:
+    """Whether the engine's own tensor-core product for bfloat16 weights takes this one."""
+    if isinstance(weight, FourBitWeight):
+        return False
     scaled = x.scaled if isinstance(x, Prenormed) else x
     return scaled.shape[0] <= kernels.GEMM_TC_BEST_ROWS and kernels.gemm_tc_supported(scaled, weight)
 
 
-def linear(x, weight: torch.Tensor, out_dtype: torch.dtype | None = None, into: ResidualLink | None = None):
-    """x [M, K], weight [N, K] -> [M, N] in `out_dtype` (default: x's dtype).
+def linear(x, weight, out_dtype: torch.dtype | None = None, into: ResidualLink | None = None):
+    """x [M, K], weight [N, K] (a tensor or a `FourBitWeight`) -> [M, N] in `out_dtype` (default: x's dtype).
 
     `x` may be a `Prenormed`: the product for few rows finishes the norm in its epilogue; otherwise the
     norm's own kernel runs first.  With `into` and few rows the product adds its result to the stream and
@@ -40,6 +68,10 @@ def linear(x, weight: torch.Tensor, out_dtype: torch.dtype | None = None, into: 
             return _tensor_core(x.scaled, weight, out, x.row_sums, into)
         x = x.materialise()
     out_dtype = out_dtype or x.dtype
+    if isinstance(weight, FourBitWeight):
+        out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype, device=x.device)
+        kernels.mxfp4_gemm(x, weight.matrix, out, quantise=weight.quantise)
+        return out
     if x.dtype is torch.float32:
         out = torch.empty((x.shape[0], weight.shape[0]), dtype=torch.float32, device=x.device)
         kernels.gemm_f32(x, weight, out)

@@ -2,12 +2,12 @@
 import pytest
 import torch
 
-from mini_rsglang_b200 import kernels
+from mini_rsglang_b200 import RuntimeConfig, kernels
 from mini_rsglang_b200.errors import BackendError, InvalidRequest
 
 
 def matrix(rows, width):
-    return kernels.Mxfp4(*kernels._mxfp4_buffers(rows, width, "cpu"), rows, width)
+    return kernels._mxfp4_empty(rows, width, "cpu")
 
 
 @pytest.mark.parametrize("shape", [(4, 33), (4, 16), (4, 0), (32,), (2, 2, 32)])
@@ -62,3 +62,15 @@ def test_block_scales_reads_the_tiles():
                 m.scales[(r // 128 * tiles + b // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4] = want[r, b]
         assert torch.equal(m.block_scales(), want)
     assert matrix(0, 64).block_scales().shape == (0, 2)
+
+
+@pytest.mark.parametrize("kwargs", [dict(weight_format="int4"), dict(activation_format="mxfp4"), dict(weight_format="mxfp4", activation_format="fp8")])
+def test_runtime_config_refuses_other_formats(kwargs):
+    with pytest.raises(InvalidRequest):
+        RuntimeConfig(**kwargs).validate()
+
+
+def test_runtime_config_takes_both_formats():
+    RuntimeConfig().validate()
+    RuntimeConfig(weight_format="mxfp4").validate()
+    RuntimeConfig(weight_format="mxfp4", activation_format="mxfp4").validate()
