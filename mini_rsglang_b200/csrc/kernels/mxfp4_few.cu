@@ -13,10 +13,10 @@
 // be shared with its neighbours, whose sums meet in shared memory in the order of K.  Where x does not fit, the CTAs of a cluster
 // take a range of K each and their sums meet in the ranges' order.  A result does not depend on timing.
 //
-// x as halfs.  A CTA brings its part of x into the halfs' range by one power of two (for up to 128 pieces of 256 elements at a time),
-// which goes into the scales again.  Where that could lose a bit of any element (2^29 and more between the sizes of two), or x has an
-// element that is not finite, or the power is beyond [2^-20, 2^15], the CTA multiplies in bfloat16 instead, whose codes take more
-// steps to make: the same products and sums.
+// x as halfs.  A warp brings a stage of x, all tokens, into the halfs' range by one power of two, which goes into the stage's scales.
+// Where that could lose a bit of any element (2^29 and more between the sizes of two), or x has an element there that is not finite,
+// or the power is beyond [2^-20, 2^15], the stage is multiplied in bfloat16 instead, whose codes take more steps to make: the same
+// products and sums.
 #include "mxfp4.cuh"
 
 namespace {
@@ -27,9 +27,9 @@ constexpr int CODE_BYTES = 16 * 128, SCALE_BYTES = 16 * 8, STAGE_BYTES = CODE_BY
 constexpr int RING = 3;
 constexpr int FACTOR_BYTES = 16 * 8 * 4;           // a stage's scales as floats
 constexpr int X_PAD = 64;                          // bytes behind a row of x: two rows then fill all banks
-constexpr int HELD = 8;                            // pieces of 256 elements of x that a warp holds while their power is found
-constexpr int MAX_BATCHES = 64;
-constexpr int SMEM_MOST = 227 * 1024 - 1024;
+constexpr int TOKENS = 8, GROUP_SUMS = TOKENS * 16;      // the N of the MMA
+constexpr int MAX_STAGES = 512;                    // of x in shared memory
+constexpr int SMEM_MOST = 227 * 1024 - 2560;
 constexpr int ROUND_GROUPS = 16;                   // groups whose sums wait for the cluster's others at a time
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -74,9 +74,17 @@ struct Shapes {
     int cluster;            // CTAs that share their groups, a range of K each
     int x_stages;           // the longest of these ranges, in stages
     int early;              // w was there before the kernel before this one: it may be fetched while that runs
+    int groups_each, groups_over;      // of 16 rows a share (CTA or cluster): so many, and one more for the first `groups_over`
+    int stages_each, stages_over;      // of K a CTA of a cluster, likewise
 };
 
-__device__ __forceinline__ int range_start(int count, int ranges, int r) { return (int)((long long)count * r / ranges); }
+// Where range r begins: ranges of `each`, the first `over` of them one longer.  (Divisions in a kernel's first steps, 64-bit ones above
+// all, cost it more than a stage of products.)
+__device__ __forceinline__ int range_start(int each, int over, int r) { return each * r + min(r, over); }
+__device__ __forceinline__ int range_of(int each, int over, int index) {
+    const int longer = over * (each + 1);
+    return index < longer ? (int)((unsigned)index / (unsigned)(each + 1)) : over + (int)((unsigned)(index - longer) / (unsigned)max(each, 1));
+}
 
 __device__ __forceinline__ uint32_t shared_word(uint32_t address) {
     uint32_t v;
@@ -85,9 +93,9 @@ __device__ __forceinline__ uint32_t shared_word(uint32_t address) {
 }
 
 // One stage of a warp's rows joined to its sums.  `factors`: room for the stage's scales as floats.
-template <int NT, bool HALFS>
+template <bool HALFS>
 __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, const unsigned char* x_stage, int x_pitch, float factor,
-                                               int live, float (&sums)[NT][4]) {
+                                               int live, float (&sums)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     {
         // lane: row lane / 2, blocks 4 (lane % 2) to 4 (lane % 2) + 3.  Byte 0 is 2^-127; byte 255, not a number, stands beside codes of 0:
@@ -102,9 +110,7 @@ __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, c
         __syncwarp();
     }
     const uint32_t codes = stage + g * 128 + g * 16 + t * 4;                  // stages are multiples of 128 bytes: block b lies 16 b xor-ed further
-    const unsigned char* x_rows[NT];                                         // tokens that are not there read the first: nobody stores their sums
-#pragma unroll
-    for (int n = 0; n < NT; ++n) x_rows[n] = x_stage + (n * 8 + g < live ? n * 8 + g : 0) * x_pitch + t * 16;
+    const unsigned char* x_row = x_stage + (g < live ? g : 0) * x_pitch + t * 16;        // tokens that are not there read the first: nobody stores their sums
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const float4 f_low = *reinterpret_cast<const float4*>(factors + g * 8 + half * 4);
@@ -121,17 +127,14 @@ __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, c
                 for (int j = 0; j < 4; ++j) low[j] = as_bf16_pair(low[j]), high[j] = as_bf16_pair(high[j]);
             }
             const uint32_t a0[4] = {low[0], high[0], low[1], high[1]}, a1[4] = {low[2], high[2], low[3], high[3]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint4 xs = *reinterpret_cast<const uint4*>(x_rows[n] + b * 64);
-                float d[4];
-                mma_first<HALFS>(d, a0, xs.x, xs.y);
-                mma_more<HALFS>(d, a1, xs.z, xs.w);
-                sums[n][0] = fmaf(d[0], s_low[i], sums[n][0]);
-                sums[n][1] = fmaf(d[1], s_low[i], sums[n][1]);
-                sums[n][2] = fmaf(d[2], s_high[i], sums[n][2]);
-                sums[n][3] = fmaf(d[3], s_high[i], sums[n][3]);
-            }
+            const uint4 xs = *reinterpret_cast<const uint4*>(x_row + b * 64);
+            float d[4];
+            mma_first<HALFS>(d, a0, xs.x, xs.y);
+            mma_more<HALFS>(d, a1, xs.z, xs.w);
+            sums[0] = fmaf(d[0], s_low[i], sums[0]);
+            sums[1] = fmaf(d[1], s_low[i], sums[1]);
+            sums[2] = fmaf(d[2], s_high[i], sums[2]);
+            sums[3] = fmaf(d[3], s_high[i], sums[3]);
         }
     }
 }
@@ -162,45 +165,35 @@ __device__ __forceinline__ uint4 through_codes(uint4 raw) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Stages [from, to) of x's rows first_token .. + live into shared memory (what lies behind K as zeros), `to - from` times `live` pieces of
-// 256 elements, at most HELD a warp.  Returns the factor 2^(e - 15) of elements that lie there as halfs times 2^(15 - e), or 0 where
-// that might lose a bit and they lie there as they are.
+// A stage of x, the rows first_token .. + live, into shared memory by one warp (what lies behind K as zeros).  Returns the factor 2^(e - 15)
+// of elements that lie there as halfs times 2^(15 - e), or 0 where that might lose a bit and they lie there as they are.
 template <bool QUANTISE>
-__device__ __forceinline__ float bring_x(const bf16* __restrict__ x, unsigned char* x_smem, int x_pitch, int live, int first_token, const Shapes& s,
-                                         int from, int to, int x_from, uint32_t* scratch) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = (to - from) * live;
-    uint4 held[HELD];
+__device__ __forceinline__ float bring_x(const bf16* __restrict__ x, unsigned char* place, int x_pitch, int live, int column, int K) {
+    uint4 held[TOKENS];
     uint32_t largest = 0;                                                     // a pair
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) {
-        const int i = j * WARPS + warp, stage = i / live, row = i - stage * live, column = (from + stage) * STAGE_K + lane * 8;
+    for (int j = 0; j < TOKENS; ++j) {
         held[j] = make_uint4(0, 0, 0, 0);
-        if (i < pieces && column < s.K) held[j] = *reinterpret_cast<const uint4*>(x + (size_t)(first_token + row) * s.K + column);
+        if (j < live && column < K) held[j] = *reinterpret_cast<const uint4*>(x + (size_t)j * K + column);
     }
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) {
-        if (j * WARPS + warp >= pieces) break;                                // the same for the whole warp
+    for (int j = 0; j < TOKENS; ++j) {
+        if (j >= live) break;
         if constexpr (QUANTISE) held[j] = through_codes(held[j]);
         const uint32_t w[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
 #pragma unroll
         for (int p = 0; p < 4; ++p) largest = __viaddmax_s16x2(w[p] & 0x7FFF7FFFu, 0u, largest);
     }
     largest = __reduce_max_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16));
-    if (lane == 0) scratch[warp] = largest;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) largest = max(largest, scratch[w]);
     const int field = (int)(largest >> 7), e = largest == 0 ? 0 : field - 127;
-    const bool asked = e >= -20 && e <= 15;                                   // the same for the whole CTA; not with infinities or NaN
-    bool exact = asked;
-    if (asked) {
+    bool exact = e >= -20 && e <= 15;                                         // not with infinities or NaN
+    uint32_t lost = 0;
+    if (exact) {
         // a half's exponent field is the element's less that of the largest, plus 30; its mantissa the element's seven bits, then zeros
         const uint32_t down = (uint32_t)(-((e + 127 - 30) << 7)) & 0xFFFFu, both = down | down << 16;
-        uint32_t lost = 0;
 #pragma unroll
-        for (int j = 0; j < HELD; ++j) {
-            const int i = j * WARPS + warp, stage = i / live, row = i - stage * live;
-            if (i >= pieces) break;
+        for (int j = 0; j < TOKENS; ++j) {
+            if (j >= live) break;
             const uint32_t w[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
             uint32_t h[4];
 #pragma unroll
@@ -209,34 +202,27 @@ __device__ __forceinline__ float bring_x(const bf16* __restrict__ x, unsigned ch
                 lost |= (size + 0x7FFF7FFFu) & ~(r + 0x7F807F80u);            // highest bit of each half: not 0, and below the halfs' smallest ordinary number
                 h[p] = (r << 3) | (w[p] & 0x80008000u);
             }
-            *reinterpret_cast<uint4*>(x_smem + row * x_pitch + (from - x_from + stage) * (STAGE_K * 2) + lane * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(place + j * x_pitch) = make_uint4(h[0], h[1], h[2], h[3]);
         }
-        exact = (lost & 0x80008000u) == 0;
     }
-    if (!__syncthreads_or(!exact)) return __uint_as_float((uint32_t)(127 + e - 15) << 23);
+    exact = exact && !__any_sync(0xffffffffu, (lost & 0x80008000u) != 0u);
+    if (exact) return __uint_as_float((uint32_t)(127 + e - 15) << 23);
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) {
-        const int i = j * WARPS + warp, stage = i / live, row = i - stage * live;
-        if (i < pieces) *reinterpret_cast<uint4*>(x_smem + row * x_pitch + (from - x_from + stage) * (STAGE_K * 2) + lane * 16) = held[j];
-    }
+    for (int j = 0; j < TOKENS; ++j)
+        if (j < live) *reinterpret_cast<uint4*>(place + j * x_pitch) = held[j];
     return 0.0f;
 }
 
-template <int NT, bool QUANTISE, typename Out>
+template <bool QUANTISE, typename Out>
 __global__ void __launch_bounds__(THREADS, 1) few_rows_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, Out* __restrict__ out, const Shapes s) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t scratch[WARPS];
-    __shared__ float x_factors[MAX_BATCHES];
-    constexpr int TOKENS = NT * 8, GROUP_SUMS = TOKENS * 16;
+    __shared__ float x_factors[MAX_STAGES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % s.cluster, share = blockIdx.x / s.cluster, shares = gridDim.x / s.cluster;
-    const int groups = (s.N + 15) >> 4;
-    const int group_from = range_start(groups, shares, share), group_to = range_start(groups, shares, share + 1);
+    const int rank = blockIdx.x & (s.cluster - 1), share = blockIdx.x >> (31 - __clz(s.cluster));
+    const int group_from = range_start(s.groups_each, s.groups_over, share), group_to = range_start(s.groups_each, s.groups_over, share + 1);
     const int first_token = blockIdx.y * TOKENS, live = min(TOKENS, s.M - first_token);
-    const int stages = (s.K + STAGE_K - 1) / STAGE_K;
-    const int k_from = range_start(stages, s.cluster, rank), k_to = range_start(stages, s.cluster, rank + 1), depth = k_to - k_from;
-    const int batch_stages = HELD * WARPS / live;                             // of x, whose power is found together
+    const int k_from = range_start(s.stages_each, s.stages_over, rank), k_to = range_start(s.stages_each, s.stages_over, rank + 1), depth = k_to - k_from;
 
     unsigned char* place = smem;
     const uint32_t ring = smem_address(place + warp * (RING * STAGE_BYTES));
@@ -259,11 +245,13 @@ __global__ void __launch_bounds__(THREADS, 1) few_rows_kernel(const bf16* __rest
     bool waited = false;
     for (int first = group_from; first < group_to; first += round_groups) {
         const int count = min(round_groups, group_to - first), units = count * depth;
-        const int unit_from = range_start(units, WARPS, warp), unit_to = range_start(units, WARPS, warp + 1);
+        const int unit_each = units / WARPS, unit_over = units % WARPS;
+        const int unit_from = range_start(unit_each, unit_over, warp), unit_to = range_start(unit_each, unit_over, warp + 1);
+        const int first_index = depth ? (int)((unsigned)unit_from / (unsigned)depth) : 0, first_stage = unit_from - first_index * depth;
 
         // The copies' walk through this warp's units: four 16-byte copies and one of four scales a lane.  Rows behind N and columns behind K
         // are copies of the last (their sums are not stored; x is 0 there): nothing is read out of range.
-        int copy_group = depth ? first + unit_from / depth : 0, copy_stage = k_from + (depth ? unit_from % depth : 0), left = unit_to - unit_from;
+        int copy_group = first + first_index, copy_stage = k_from + first_stage, left = unit_to - unit_from;
         uint32_t copy_offset = 0, used_offset = 0;
         const uint8_t *from0, *from1, *from2, *from3, *from_scales;
         auto start_group = [&]() {
@@ -305,74 +293,68 @@ __global__ void __launch_bounds__(THREADS, 1) few_rows_kernel(const bf16* __rest
             pdl_launch_dependents();
             if (s.early) pdl_wait();
             waited = true;
-            for (int b = k_from; b < k_to; b += batch_stages) {
-                const float factor = bring_x<QUANTISE>(x, x_smem, x_pitch, live, first_token, s, b, min(b + batch_stages, k_to), k_from, scratch);
-                if (threadIdx.x == 0) x_factors[(b - k_from) / batch_stages] = factor;
+            for (int stage = warp; stage < depth; stage += WARPS) {
+                const float factor = bring_x<QUANTISE>(x + (size_t)first_token * s.K, x_smem + stage * (STAGE_K * 2) + lane * 16, x_pitch, live,
+                                                       (k_from + stage) * STAGE_K + lane * 8, s.K);
+                if (lane == 0) x_factors[stage] = factor;
             }
             __syncthreads();
         }
 
-        int group = depth ? first + unit_from / depth : 0, stage = depth ? unit_from % depth : 0;        // of the CTA's range
+        int group = first + first_index, stage = first_stage;                   // of the CTA's range
         for (int unit = unit_from; unit < unit_to; ++group, stage = 0) {
             const int stop = min(unit + depth - stage, unit_to);               // of this warp's piece of the group
             const bool alone = stage == 0 && stop - unit == depth;
-            float sums[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) sums[n][0] = sums[n][1] = sums[n][2] = sums[n][3] = 0.0f;
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             const int slot = unit == unit_from ? 0 : 1;
-            int batch = stage / batch_stages, batch_end = (batch + 1) * batch_stages;
-            float factor = x_factors[batch];
             const unsigned char* x_stage = x_smem + stage * (STAGE_K * 2);
             for (; unit < stop; ++unit, ++stage, x_stage += STAGE_K * 2) {
-                if (stage == batch_end) {
-                    factor = x_factors[++batch];
-                    batch_end += batch_stages;
-                }
+                const float factor = x_factors[stage];
                 copy_wait<RING - 2>();
                 __syncwarp();
                 copy_next();
-                if (factor != 0.0f) stage_products<NT, true>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
-                else stage_products<NT, false>(ring + used_offset, factors, x_stage, x_pitch, 1.0f, live, sums);
+                if (factor != 0.0f) stage_products<true>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
+                else stage_products<false>(ring + used_offset, factors, x_stage, x_pitch, 1.0f, live, sums);
                 used_offset = used_offset + STAGE_BYTES == RING * STAGE_BYTES ? 0 : used_offset + STAGE_BYTES;
                 __syncwarp();
             }
             const int g = lane >> 2, t = lane & 3;
             if (alone && s.cluster == 1) {                                      // these sums are the results
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int token = n * 8 + 2 * t + (i & 1);
-                        const long long row = (long long)group * 16 + g + (i >> 1) * 8;
-                        if (token < live && row < s.N) out[(size_t)(first_token + token) * s.N + row] = from_float<Out>(sums[n][i]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int token = 2 * t + (i & 1);
+                    const long long row = (long long)group * 16 + g + (i >> 1) * 8;
+                    if (token < live && row < s.N) out[(size_t)(first_token + token) * s.N + row] = from_float<Out>(sums[i]);
+                }
             } else {
                 float* mine = alone ? whole + (group - first) * GROUP_SUMS : pieces + (warp * 2 + slot) * GROUP_SUMS;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mine[(n * 8 + 2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = sums[n][i];
+                for (int i = 0; i < 4; ++i) mine[(2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = sums[i];
             }
         }
         copy_wait<0>();
         __syncthreads();
 
-        // groups that several warps share: their pieces in the order of K.  Unit u belongs to warp ((u + 1) * WARPS - 1) / units.
+        // groups that several warps share: their pieces in the order of K
         for (int index = warp; index < count; index += WARPS) {
             const int begin = index * depth;
-            const int low = units ? (int)(((long long)(begin + 1) * WARPS - 1) / units) : 0, high = units ? (int)(((long long)(begin + depth) * WARPS - 1) / units) : 0;
+            const int low = units ? range_of(unit_each, unit_over, begin) : 0, high = units ? range_of(unit_each, unit_over, begin + depth - 1) : 0;
             if (units && low == high) continue;
-            const float* first_piece = pieces + (low * 2 + (range_start(units, WARPS, low) >= begin ? 0 : 1)) * GROUP_SUMS;
-            for (int i = lane; i < live * 16; i += 32) {
-                float sum = 0.0f;
-                if (units) {
-                    sum = first_piece[i];
-                    for (int w = low + 1; w <= high; ++w)
-                        if (range_start(units, WARPS, w) < range_start(units, WARPS, w + 1)) sum += pieces[w * 2 * GROUP_SUMS + i];
-                }
-                const long long row = (long long)(first + index) * 16 + (i & 15);
-                if (s.cluster > 1) whole[index * GROUP_SUMS + i] = sum;
-                else if (row < s.N) out[(size_t)(first_token + (i >> 4)) * s.N + row] = from_float<Out>(sum);
+            float sum[GROUP_SUMS / 32];
+            const float* piece = pieces + (low * 2 + (range_start(unit_each, unit_over, low) >= begin ? 0 : 1)) * GROUP_SUMS + lane;
+#pragma unroll
+            for (int i = 0; i < GROUP_SUMS / 32; ++i) sum[i] = units ? piece[i * 32] : 0.0f;
+            for (int w = low + 1; w <= high; ++w) {
+                piece = pieces + w * 2 * GROUP_SUMS + lane;
+#pragma unroll
+                for (int i = 0; i < GROUP_SUMS / 32; ++i) sum[i] += piece[i * 32];
+            }
+            const long long row = (long long)(first + index) * 16 + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < GROUP_SUMS / 32; ++i) {
+                const int token = i * 2 + (lane >> 4);
+                if (s.cluster > 1) whole[index * GROUP_SUMS + i * 32 + lane] = sum[i];
+                else if (token < live && row < s.N) out[(size_t)(first_token + token) * s.N + row] = from_float<Out>(sum[i]);
             }
         }
         if (s.cluster > 1) {
@@ -399,29 +381,30 @@ __global__ void __launch_bounds__(THREADS, 1) few_rows_kernel(const bf16* __rest
 }
 
 // Bytes of shared memory; 0 where x does not fit.
-size_t shared_bytes(int tokens, int x_stages, int live, int cluster) {
-    const size_t bytes = (size_t)WARPS * (RING * STAGE_BYTES + FACTOR_BYTES) + (size_t)WARPS * 2 * tokens * 16 * 4 +
-                         (cluster > 1 ? (size_t)ROUND_GROUPS * tokens * 16 * 4 : 0) + (size_t)live * ((size_t)x_stages * STAGE_K * 2 + X_PAD);
-    const int batch = HELD * WARPS / live;
-    return bytes > SMEM_MOST || (x_stages + batch - 1) / batch > MAX_BATCHES ? 0 : bytes;
+size_t shared_bytes(int x_stages, int live, int cluster) {
+    const size_t bytes = (size_t)WARPS * (RING * STAGE_BYTES + FACTOR_BYTES) + (size_t)WARPS * 2 * GROUP_SUMS * 4 +
+                         (cluster > 1 ? (size_t)ROUND_GROUPS * GROUP_SUMS * 4 : 0) + (size_t)live * ((size_t)x_stages * STAGE_K * 2 + X_PAD);
+    return bytes > SMEM_MOST || x_stages > MAX_STAGES ? 0 : bytes;
 }
 
-template <int NT, bool QUANTISE, typename Out>
+template <bool QUANTISE, typename Out>
 int launch(const void* x, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
     const int stages = (s.K + STAGE_K - 1) / STAGE_K;
     s.x_stages = (stages + s.cluster - 1) / s.cluster;
-    const size_t bytes = shared_bytes(NT * 8, s.x_stages, s.M < NT * 8 ? s.M : NT * 8, s.cluster);
+    const size_t bytes = shared_bytes(s.x_stages, s.M < TOKENS ? s.M : TOKENS, s.cluster);
     if (!bytes) return MRS_BAD_ARGUMENT;
     static PerDevice configured;
     if (!configured.get()) {
-        cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<NT, QUANTISE, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
+        cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<QUANTISE, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
         if (e != cudaSuccess) return (int)e;
         configured.set(1);
     }
-    const int groups = (s.N + 15) / 16, most_shares = (ctas / s.cluster) > 1 ? ctas / s.cluster : 1;
+    const int groups = s.N / 16 + (s.N % 16 != 0), most_shares = (ctas / s.cluster) > 1 ? ctas / s.cluster : 1;
     const int shares = groups < most_shares ? groups : most_shares;
+    s.groups_each = groups / shares, s.groups_over = groups % shares;
+    s.stages_each = stages / s.cluster, s.stages_over = stages % s.cluster;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(shares * s.cluster), (unsigned)((s.M + NT * 8 - 1) / (NT * 8)));
+    config.gridDim = dim3((unsigned)(shares * s.cluster), (unsigned)((s.M + TOKENS - 1) / TOKENS));
     config.blockDim = dim3(THREADS);
     config.dynamicSmemBytes = bytes;
     config.stream = (cudaStream_t)stream;
@@ -432,25 +415,19 @@ int launch(const void* x, const void* codes, const void* scales, void* out, Shap
     attributes[1].val.clusterDim.x = s.cluster, attributes[1].val.clusterDim.y = 1, attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    cudaError_t e = cudaLaunchKernelEx(&config, few_rows_kernel<NT, QUANTISE, Out>, (const bf16*)x, (const uint8_t*)codes, (const uint8_t*)scales,
+    cudaError_t e = cudaLaunchKernelEx(&config, few_rows_kernel<QUANTISE, Out>, (const bf16*)x, (const uint8_t*)codes, (const uint8_t*)scales,
                                        (Out*)out, s);
     if (e != cudaSuccess) return (int)e;
     MRS_RETURN_LAUNCH_STATUS();
 }
 
-template <int NT, typename Out>
-int launch_x(const void* x, const void* codes, const void* scales, void* out, const Shapes& s, int quantise, int ctas, void* stream) {
-    return quantise ? launch<NT, true, Out>(x, codes, scales, out, s, ctas, stream) : launch<NT, false, Out>(x, codes, scales, out, s, ctas, stream);
-}
-
 }  // namespace
 
-// CTAs of a cluster (1, 2, 4 or 8) whose shared memory holds their ranges of up to 16 rows (tokens of 8 at a time for up to 8) of
-// K elements; 0 where none does.
+// CTAs of a cluster (1, 2, 4 or 8) whose shared memory holds their ranges of up to 8 rows of K elements; 0 where none does.
 MRS_EXPORT int mrs_mxfp4_few_rows_cluster(int M, int K) {
-    const int tokens = M <= 8 ? 8 : 16, stages = (K + STAGE_K - 1) / STAGE_K;
+    const int stages = (K + STAGE_K - 1) / STAGE_K;
     for (int c = 1; c <= 8; c *= 2)
-        if (shared_bytes(tokens, (stages + c - 1) / c, M < tokens ? M : tokens, c)) return c;
+        if (shared_bytes((stages + c - 1) / c, M < TOKENS ? M : TOKENS, c)) return c;
     return 0;
 }
 
@@ -462,8 +439,7 @@ MRS_EXPORT int mrs_mxfp4_few_rows(const void* x, const void* codes, const void* 
     if (M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || M > 65535 * 8 || ctas < 1 || !x || !codes || !scales || !out) return MRS_BAD_ARGUMENT;
     if ((((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1))) return MRS_BAD_ARGUMENT;
     if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return MRS_BAD_ARGUMENT;
-    Shapes s = {M, N, K, cluster, 0, early};
-    if (M <= 8)
-        return out_f32 ? launch_x<1, float>(x, codes, scales, out, s, quantise, ctas, stream) : launch_x<1, bf16>(x, codes, scales, out, s, quantise, ctas, stream);
-    return out_f32 ? launch_x<2, float>(x, codes, scales, out, s, quantise, ctas, stream) : launch_x<2, bf16>(x, codes, scales, out, s, quantise, ctas, stream);
+    Shapes s = {M, N, K, cluster, 0, early, 0, 0, 0, 0};
+    if (quantise) return out_f32 ? launch<true, float>(x, codes, scales, out, s, ctas, stream) : launch<true, bf16>(x, codes, scales, out, s, ctas, stream);
+    return out_f32 ? launch<false, float>(x, codes, scales, out, s, ctas, stream) : launch<false, bf16>(x, codes, scales, out, s, ctas, stream);
 }
