@@ -255,6 +255,69 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
     if (threadIdx.x == 0) exponents[row] = bad ? HALFS_LOST : empty ? 0 : field - 127 - 15;
 }
 
+// Up to `tokens` rows of bfloat16 as three parts of E5M2 (three bits of significand, exponents of -16 to 15) each, part p of row r at row
+// p * tokens + r, with a power of two for 32 neighbours in scale tiles (mxfp4.cuh) of these 3 * tokens rows.  With 2^(e - 14) for a block
+// whose largest size has the exponent e, x = (a + b + c 2^-8) 2^(e - 14): a is x rounded, b what is left of it rounded, c, with
+// a power 2^-8 further down, the rest: of eight bits three, three signed and two are enough down to 2^-26 of the largest.  Where that
+// is not so lost[r * stretches + stretch] is 1: the row cannot be had in parts.
+constexpr int PART_SHIFT = 8;
+__global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __restrict__ x, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
+                                                                int* __restrict__ lost, int rows, int width, int tokens, int stretches, int* __restrict__ zeros,
+                                                                int zero_count) {
+    pdl_launch_dependents();
+    pdl_wait();
+    clear(zeros, zero_count);
+    const int lane = threadIdx.x & 31, index = (int)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+    if (index >= rows * stretches) return;
+    const int row = index / stretches, stretch = index - row * stretches, column = stretch * 256 + lane * 8;
+    Eight held = {};
+    if (column < width) held.load(x + (size_t)row * width + column);
+    const uint32_t largest = held.largest_of_block();
+    const int e = (int)(largest >> 23) - 127;                    // 128: infinity or NaN
+    const bool empty = largest == 0, fits = empty || (e >= -105 && e < 128);
+    const uint32_t byte = fits && !empty ? (uint32_t)(e - 14 + 127) : 127u;
+    const float up = mx_inverse(byte), down = mx_scale(byte);
+    float v[8];
+    held.values(v);
+    uint32_t a[2] = {0, 0}, b[2] = {0, 0}, c[2] = {0, 0};
+    bool exact = fits;
+    auto part_of = [](float f) {
+        uint16_t two;
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.0f), "f"(f));
+        return (uint32_t)two & 255u;
+    };
+    auto value_of = [](uint32_t part) { return __half2float(__ushort_as_half((unsigned short)(part << 8))); };      // E5M2 is a half's upper byte
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float scaled = v[i] * up;
+        const uint32_t first = part_of(scaled);
+        const float left = scaled - value_of(first);
+        const uint32_t second = part_of(left);
+        const float rest = (left - value_of(second)) * (float)(1 << PART_SHIFT);
+        const uint32_t third = part_of(rest);
+        exact = exact && (value_of(first) + value_of(second) + value_of(third) * (1.0f / (1 << PART_SHIFT))) * down == v[i];
+        a[i >> 2] |= first << (8 * (i & 3));
+        b[i >> 2] |= second << (8 * (i & 3));
+        c[i >> 2] |= third << (8 * (i & 3));
+    }
+    if (column < width) {
+        *reinterpret_cast<uint2*>(parts + (size_t)row * width + column) = make_uint2(a[0], a[1]);
+        *reinterpret_cast<uint2*>(parts + (size_t)(tokens + row) * width + column) = make_uint2(b[0], b[1]);
+        *reinterpret_cast<uint2*>(parts + (size_t)(2 * tokens + row) * width + column) = make_uint2(c[0], c[1]);
+    }
+    uint32_t four = byte << (8 * ((lane >> 2) & 3));
+    four |= __shfl_xor_sync(0xffffffffu, four, 4);
+    four |= __shfl_xor_sync(0xffffffffu, four, 8);
+    if ((lane & 15) == 0) {
+        const int tiles = stretches * 2, q = stretch * 2 + (lane >> 4);
+        *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(row, q, tiles)) = four;
+        *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(tokens + row, q, tiles)) = four;
+        *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(2 * tokens + row, q, tiles)) = four - 0x01010101u * PART_SHIFT;
+    }
+    const bool all = __all_sync(0xffffffffu, exact);
+    if (lane == 0) lost[index] = all ? 0 : 1;
+}
+
 // Blocks of a launch over `items` threads of work: they loop where that is more than 64 blocks an SM.
 int blocks_for(long long items) {
     const long long want = (items + THREADS - 1) / THREADS, most = (long long)mrs_sm_count() * 64;
@@ -321,6 +384,19 @@ MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* exponen
     if (rows == 0) return 0;
     if (bad_sizes(rows, width) || (zero_count && !zeros) || rows > 0x7FFFFFFF || !x || !halfs || !exponents || (((uintptr_t)x | (uintptr_t)halfs) & 15) || ((uintptr_t)exponents & 3)) return MRS_BAD_ARGUMENT;
     MRS_LAUNCH(rows_to_halfs_kernel, (unsigned)rows, THREADS, 0, stream, (const bf16*)x, (uint16_t*)halfs, (int*)exponents, width, (int*)zeros, zero_count);
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+// x [rows, width] bfloat16, rows up to `tokens` (16 or 32), to parts [3 tokens, width], their scales and lost [rows * ceil(width / 256)] int32.
+MRS_EXPORT int mrs_mxfp4_rows_to_parts(const void* x, void* parts, void* scales, void* lost, int rows, int width, int tokens, void* zeros, int zero_count,
+                                       void* stream) {
+    if (rows == 0) return 0;
+    if (bad_sizes(rows, width) || rows > tokens || (tokens != 16 && tokens != 32) || (zero_count && !zeros) || !x || !parts || !scales || !lost ||
+        (((uintptr_t)x | (uintptr_t)parts | (uintptr_t)scales) & 15) || ((uintptr_t)lost & 3))
+        return MRS_BAD_ARGUMENT;
+    const int stretches = (width + 255) / 256;
+    MRS_LAUNCH(rows_to_parts_kernel, (rows * stretches + THREADS / 32 - 1) / (THREADS / 32), THREADS, 0, stream, (const bf16*)x, (uint8_t*)parts, (uint8_t*)scales,
+               (int*)lost, rows, width, tokens, stretches, (int*)zeros, zero_count);
     MRS_RETURN_LAUNCH_STATUS();
 }
 

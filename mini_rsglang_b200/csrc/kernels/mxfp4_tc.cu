@@ -15,6 +15,10 @@
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
 //                    tensor memory (tcgen05.cp) stage by stage.
 //
+//   parts_kernel     x in bfloat16 once more, up to 32 rows: as three parts of E5M2 (mxfp4.cu), 3 x 32 columns of kind::mxf8f6f4 MMAs whose A
+//                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
+//                    columns' sums are the result's.  Rows that three parts do not hold exactly are multiplied on the CUDA cores.
+//
 // Every wait is bounded (tma.cuh).
 #include <limits.h>
 
@@ -95,9 +99,9 @@ struct Walk {
 // An accumulator's results (lane: row of w, column: token) to memory.  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes
 // are those of its number modulo 4.  `halfs`: the rows' powers of two go into them (`factors`: 32 floats of shared memory for each warp).  A
 // tile that other CTAs share goes through scratch memory; `flag` is a word of shared memory.
-template <int TOKENS, int WARPS, typename Out>
+template <int TOKENS, int WARPS, typename Out, bool PARTS = false>
 __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors) {
-    constexpr int STEP = TOKENS < 32 ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
+    constexpr int STEP = TOKENS < 32 || PARTS ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
     const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
     const int token0 = walk.tile % s.token_tiles * TOKENS, live = min(TOKENS, s.M - token0);
     const uint32_t acc = accumulator + ((uint32_t)(quarter * 32) << 16);
@@ -136,6 +140,14 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
         if constexpr (STEP == 16) tmem_load_16_async(acc + c, v);
         else tmem_load_32_async(acc + c, v);
         tmem_load_wait();
+        if constexpr (PARTS) {                     // the other two parts' columns, the smallest sums first
+            float rest[STEP], least[STEP];
+            if constexpr (STEP == 16) tmem_load_16_async(acc + TOKENS + c, rest), tmem_load_16_async(acc + 2 * TOKENS + c, least);
+            else tmem_load_32_async(acc + TOKENS + c, rest), tmem_load_32_async(acc + 2 * TOKENS + c, least);
+            tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < STEP; ++e) v[e] += rest[e] + least[e];
+        }
         if (whole) {
             finish(c, v);
         } else {
@@ -627,6 +639,223 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------
+// x in three parts
+// ------------------------------------------------------------------------------------------
+// kind::mxf8f6f4: A E2M1 (a code a byte of shared memory, 16 codes in 8 bytes and 8 unused), B E5M2, one E8M0 scale for 32 elements, K 32;
+// `id`: which of a word's four scales.
+__host__ __device__ constexpr uint32_t mxf8f6f4_idesc(int m, int n, uint32_t id) {
+    return (id << 4)                      // scales of B
+           | (5u << 7) | (1u << 10)       // A: E2M1, B: E5M2
+           | ((uint32_t)(n >> 3) << 17)   // N / 8
+           | (1u << 23)                   // scales: E8M0
+           | ((uint32_t)(m >> 7) << 27)   // M / 128
+           | (id << 29);                  // scales of A
+}
+__device__ __forceinline__ void umma_mxf8f6f4(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, bool accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                 ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"((uint32_t)accumulate) : "memory");
+}
+
+constexpr int HALF_STAGE_K = 128;                          // elements of K of a 128-byte row of bytes
+constexpr int P_A_BYTES = BM * HALF_STAGE_K;               // half a stage of w in shared memory, of which the copies count half
+constexpr int P_STORERS = 8, P_THREADS = (3 + P_STORERS) * 32;
+constexpr int P_SCALE_COLUMNS = 16;                        // of a stage: 2 x 4 of w, 2 x 4 of the tokens' parts
+template <int TOKENS> constexpr int p_stages() { return TOKENS > 16 ? 3 : 4; }
+template <int TOKENS> constexpr int p_x_bytes() { return 3 * TOKENS * HALF_STAGE_K; }
+template <int TOKENS> constexpr size_t parts_smem() { return 1024 + (size_t)p_stages<TOKENS>() * (2 * P_A_BYTES + 2 * p_x_bytes<TOKENS>() + 2 * SCALE_BYTES) + 256; }
+
+template <int TOKENS, typename Out>
+__global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                                                             const bf16* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ w_scales,
+                                                             const uint8_t* __restrict__ x_scales, const int* __restrict__ lost, int lost_count,
+                                                             Out* __restrict__ out, const Shapes s) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int STAGES = p_stages<TOKENS>(), N_COLUMNS = 3 * TOKENS, ACCUMULATOR = 128, SCALES_FIRST = 2 * ACCUMULATOR;
+    unsigned char* w_ring = smem;
+    unsigned char* x_ring = w_ring + STAGES * 2 * P_A_BYTES;
+    unsigned char* s_ring = x_ring + STAGES * 2 * p_x_bytes<TOKENS>();
+    uint64_t* full = reinterpret_cast<uint64_t*>(s_ring + STAGES * 2 * SCALE_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    int* flag = reinterpret_cast<int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Walk walk(s);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&full[i], 2);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], P_STORERS);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, TMEM_COLUMNS);
+        tmem_relinquish_alloc_permit();
+    }
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    tcgen05_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+
+    // a stage of w: two halves of 128 elements, and its scales
+    auto load_w = [&](int n_tile, int stage, int slot) {
+        mbar_arrive_expect_tx(&full[slot], P_A_BYTES + SCALE_BYTES);                    // half of what two halves take in shared memory
+#pragma unroll
+        for (int h = 0; h < 2; ++h) tma_load_2d(w_ring + (slot * 2 + h) * P_A_BYTES, &w_map, &full[slot], stage * STAGE_K + h * HALF_STAGE_K, n_tile * BM);
+        bulk_load(s_ring + slot * 2 * SCALE_BYTES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[slot]);
+    };
+    const int ahead = s.early ? min(STAGES, walk.total) : 0;
+    if (warp == 2 + P_STORERS) {
+        if (elect_one())
+            for (int i = 0; i < ahead; ++i) load_w(walk.tile_of(s, i) / s.token_tiles, walk.stage_of(s, i), i);
+        __syncwarp();
+    }
+    pdl_wait();
+    bool bad = false;
+    for (int i = threadIdx.x; i < lost_count; i += P_THREADS) bad = bad || lost[i] != 0;
+    const bool slow = __syncthreads_or(bad);
+
+    if (slow) {
+        // Rows that three parts do not hold: a thread a row of w and every third token, the products of a bfloat16 and a code times its
+        // power of two exact, sums in float32.
+        if (warp == 2 + P_STORERS) {                                                    // what was fetched has to have come before the CTA ends
+            for (int i = 0; i < ahead; ++i) {
+                if (elect_one()) mbar_arrive(&full[i]);
+                __syncwarp();
+                warp_wait(&full[i], 0);
+            }
+        }
+        const long long code_pitch = s.K >> 1;
+        constexpr int LANES = P_THREADS / BM;                                           // threads a row
+        const int part = threadIdx.x / BM;
+        for (int tile = blockIdx.x; part < LANES && tile < s.units / s.depth; tile += gridDim.x) {
+            const long long n = (long long)tile * BM + (threadIdx.x & (BM - 1));
+            if (n >= s.N) continue;
+            for (int token = part; token < s.M; token += LANES) {
+                float sum = 0.0f;
+                for (int block = 0; block < s.K / MX_BLOCK; ++block) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(codes + n * code_pitch + block * 16);
+                    const float scale = mx_scale(w_scales[mx_scale_offset(n, block >> 2, s.w_tiles_of_a_row) + (block & 3)]);
+                    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+                    const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)token * s.K + block * MX_BLOCK);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[4];
+                        mx_decode_8(words[i], h);
+                        const uint4 raw = from[i];
+                        const uint32_t pairs[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            const float2 w = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
+                            sum = fmaf(__uint_as_float(pairs[p] << 16), w.x * scale, sum);
+                            sum = fmaf(__uint_as_float(pairs[p] & 0xFFFF0000u), w.y * scale, sum);
+                        }
+                    }
+                }
+                out[(size_t)token * s.N + n] = from_float<Out>(sum);
+            }
+        }
+    } else if (warp == 0) {
+        const bool leader = elect_one();
+        bool alive = true;
+        int slot = 0;
+        uint32_t phase = 1;
+        while (alive && walk.step(s)) {
+            for (int stage = walk.from; stage < walk.to; ++stage) {
+                if (!(alive = warp_wait(&empty[slot], phase))) break;
+                if (leader) {
+                    mbar_arrive_expect_tx(&full[slot], 2 * p_x_bytes<TOKENS>() + SCALE_BYTES);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_2d(x_ring + (slot * 2 + h) * p_x_bytes<TOKENS>(), &x_map, &full[slot], stage * STAGE_K + h * HALF_STAGE_K, 0);
+                    bulk_load(s_ring + slot * 2 * SCALE_BYTES + SCALE_BYTES, x_scales + (size_t)stage * SCALE_BYTES, SCALE_BYTES, &full[slot]);
+                }
+                __syncwarp();
+                if (++slot == STAGES) slot = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == 2 + P_STORERS) {
+        const bool leader = elect_one();
+        bool alive = true;
+        int slot = 0, count = 0;
+        uint32_t phase = 1;
+        while (alive && walk.step(s)) {
+            const int n_tile = walk.tile / s.token_tiles;
+            for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
+                if (count >= ahead) {
+                    if (!(alive = warp_wait(&empty[slot], phase))) break;
+                    if (leader) load_w(n_tile, stage, slot);
+                    __syncwarp();
+                }
+                if (++slot == STAGES) slot = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        const bool leader = elect_one();
+        bool alive = true;
+        int slot = 0, round = 0;
+        uint32_t phase = 0;
+        for (; alive && walk.step(s); ++round) {
+            const int buffer = round & 1;
+            if (!(alive = warp_wait(&acc_empty[buffer], ((round >> 1) & 1) ^ 1))) break;
+            tcgen05_fence_after_sync();
+            const uint32_t d_tmem = tmem + buffer * ACCUMULATOR;
+            for (int index = 0; index < walk.to - walk.from; ++index) {
+                if (!(alive = warp_wait(&full[slot], phase))) break;
+                tcgen05_fence_after_sync();
+                const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(w_ring + slot * 2 * P_A_BYTES));
+                const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + slot * 2 * p_x_bytes<TOKENS>()));
+                const uint32_t scales = smem_u32(s_ring + slot * 2 * SCALE_BYTES);
+                const uint32_t columns = tmem + SCALES_FIRST + slot * P_SCALE_COLUMNS;
+                if (leader) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {                                   // 128 elements of K
+                        scales_to_tmem(columns + q * 4, scales + q * MX_TILE_BYTES);
+                        scales_to_tmem(columns + 8 + q * 4, scales + SCALE_BYTES + q * MX_TILE_BYTES);
+                    }
+#pragma unroll
+                    for (int k = 0; k < STAGE_K / 32; ++k)
+                        umma_mxf8f6f4(d_tmem, a_desc + (k >> 2) * (P_A_BYTES / 16) + 2 * (k & 3), b_desc + (k >> 2) * (p_x_bytes<TOKENS>() / 16) + 2 * (k & 3),
+                                      mxf8f6f4_idesc(BM, N_COLUMNS, k & 3), columns + (k >> 2) * 4, columns + 8 + (k >> 2) * 4, index > 0 || k > 0);
+                    umma_commit(&empty[slot]);
+                }
+                __syncwarp();
+                if (++slot == STAGES) slot = 0, phase ^= 1;
+            }
+            if (leader) umma_commit(&acc_full[buffer]);
+            __syncwarp();
+        }
+    } else {
+        for (int round = 0; walk.step(s); ++round) {
+            const int buffer = round & 1;
+            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
+            tcgen05_fence_after_sync();
+            store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr);
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buffer]);
+        }
+    }
+    __syncwarp();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tcgen05_fence_after_sync();
+        tmem_dealloc(tmem, TMEM_COLUMNS);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------
 int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, long long row_bytes, long long columns, long long rows, int box_columns, int box_rows) {
@@ -684,6 +913,19 @@ int launch_both(const void* x_codes, const void* x_scales, const void* codes, co
                       (const uint8_t*)x_scales, (Out*)out, s);
 }
 
+template <int TOKENS, typename Out>
+int launch_parts(const void* x, const void* parts, const void* x_scales, const void* lost, const void* codes, const void* scales, void* out, Shapes s, int ctas,
+                 void* stream) {
+    CUtensorMap w_map, x_map;
+    int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, s.K / 2, s.K, s.N, HALF_STAGE_K, BM);
+    if (!code) code = make_map(&x_map, parts, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K, s.K, 3 * TOKENS, HALF_STAGE_K, 3 * TOKENS);
+    if (code) return code;
+    static PerDevice configured;
+    if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
+    return launch_run(parts_kernel<TOKENS, Out>, configured, P_THREADS, ctas, parts_smem<TOKENS>(), stream, w_map, x_map, (const bf16*)x, (const uint8_t*)codes,
+                      (const uint8_t*)scales, (const uint8_t*)x_scales, (const int*)lost, s.M * s.depth, (Out*)out, s);
+}
+
 bool bad(const void* x, const void* codes, const void* scales, const void* out, int out_f32, int M, int N, int K, int tokens, int ctas, const void* scratch,
          const void* arrived) {
     return M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || !x || !codes || !scales || !out ||
@@ -721,6 +963,21 @@ MRS_EXPORT int mrs_mxfp4_both_rows(const void* x_codes, const void* x_scales, co
     s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
 #define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_both<T, float>(x_codes, x_scales, codes, scales, out, s, ctas, stream) : launch_both<T, bf16>(x_codes, x_scales, codes, scales, out, s, ctas, stream)
     MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
+#undef MRS_TOKENS
+    return MRS_BAD_ARGUMENT;
+}
+
+// The same with x [M, K] in bfloat16 and in parts (mxfp4.cu), M up to `tokens` (16 or 32), K a multiple of 128.
+MRS_EXPORT int mrs_mxfp4_parts_rows(const void* x, const void* parts, const void* x_scales, const void* lost, const void* codes, const void* scales, void* out,
+                                    int out_f32, int M, int N, int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
+    if (M == 0 || N == 0) return 0;
+    if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived) || K % HALF_STAGE_K || ((uintptr_t)codes & 31) || !parts || !x_scales || !lost ||
+        (((uintptr_t)parts | (uintptr_t)x_scales) & 15) || ((uintptr_t)lost & 3))
+        return MRS_BAD_ARGUMENT;
+    Shapes s = {};
+    s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
+#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_parts<T, float>(x, parts, x_scales, lost, codes, scales, out, s, ctas, stream) : launch_parts<T, bf16>(x, parts, x_scales, lost, codes, scales, out, s, ctas, stream)
+    MRS_TOKENS(16); MRS_TOKENS(32);
 #undef MRS_TOKENS
     return MRS_BAD_ARGUMENT;
 }

@@ -2574,6 +2574,8 @@ _MXFP4_SIGNATURES = {
     "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp,
                                _c_int, _c_vp],
+    "mrs_mxfp4_rows_to_parts": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp],
+    "mrs_mxfp4_parts_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_take_error": [ctypes.POINTER(ctypes.c_uint)],
 }
@@ -2754,29 +2756,40 @@ def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
 
 @functools.lru_cache(maxsize=4096)
 def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
-    """How a product is launched: ("few", CTAs of a cluster) or ("many", tokens of a tile, CTAs, whether tiles may be shared)."""
+    """How a product is launched: ("few", CTAs of a cluster), or ("parts" | "many", tokens of a tile, CTAs, whether tiles are shared).
+
+    Measured on a B200 (us, weights [n, k] from a cold L2, the kernel that prepares x included; few / parts / many):
+      24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 17.4 / 22.1, 16 rows - / 16.9 / 21.6, 32 rows - / 20.0 / 25.3
+      4,096 x 12,288   1 row 9.8 / 14.8 / 19.0, 8 rows (x in four CTAs) 18.3 / 15.5 / 20.2
+      5,120 x 17,408   4 rows (x in two CTAs) 15.1 / 17.8 / 24.4, 8 rows (in four) 27.9 / 18.0 / 25.1
+    and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.6 / 14.5, 8 rows 16.1 / 14.5; 1,000 x 2,048 4 rows 3.6 / 6."""
     if m <= (4 if quantise else 8):
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
-        if cluster:
+        if 0 < cluster <= 2:
             return ("few", cluster)
-    tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128 if m <= 128 else 192
-    return mxfp4_many_plan(m, n, k, tokens, sms)
+    if m <= 32 and k % 128 == 0 and not quantise:
+        return ("parts", *mxfp4_tiles(m, n, k, 16 if m <= 16 else 32, sms, 11))
+    if m <= 128:
+        tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128
+    else:
+        tokens = min((192, 128), key=lambda t: -(-(-(-n // 128) * -(-m // t)) // sms) * t)
+    return ("many", *mxfp4_tiles(m, n, k, tokens, sms, 11 if tokens <= 32 and not quantise else 30))
 
 
-def mxfp4_many_plan(m: int, n: int, k: int, tokens: int, sms: int, shared: bool | None = None) -> tuple:
-    """Tiles of 128 rows of weights x `tokens`, on as many CTAs as there are SMs."""
+def mxfp4_tiles(m: int, n: int, k: int, tokens: int, sms: int, meeting: int, shared: bool | None = None) -> tuple:
+    """(tokens of a tile, CTAs, whether tiles are shared) of tiles of 128 rows of weights x `tokens` on as many CTAs as there are SMs.
+    Shared tiles cost a meeting of their CTAs, as long as `meeting` stages of 256 elements of K: measured 3 to 5 us, where a stage takes
+    0.43 us with a few tokens of bfloat16, 0.25 with 4 bits on both sides, and more columns have to meet with wide tiles."""
     tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
     if shared is None:
-        rounds = -(-tiles // sms)
-        shared = tiles < 0.9 * rounds * sms and depth > 1
-    if not shared:
-        return ("many", tokens, min(tiles, sms), False)
-    return ("many", tokens, min(sms, max(tiles, tiles * depth // 3)), True)
+        shared = tiles * depth / sms + meeting < -(-tiles // sms) * depth
+    return (tokens, min(sms, max(tiles, tiles * depth // 3)), True) if shared else (tokens, min(tiles, sms), False)
 
 
 def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool = False, plan: tuple | None = None) -> None:
     """out[M, N] = x[M, K] . weight[N, K]^T; x bfloat16, weight in 4 bits, sums in float32, `out` bfloat16 or float32.  With `quantise`
-    x's rows are brought to 4 bits first, as `mxfp4_quantise` does.  `plan`: another than `mxfp4_plan` only for measurements and tests."""
+    x's rows are brought to 4 bits first, as `mxfp4_quantise` does.  Up to 8 rows take one kernel, others two, the first of which
+    prepares x in a buffer of its own.  `plan`: another than `mxfp4_plan` only for measurements and tests."""
     global launch_count
     if x.dim() != 2 or out.dim() != 2:
         raise InvalidRequest("mxfp4_gemm: input and output are rows")
@@ -2805,9 +2818,15 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
                                           _stream())
         else:
             # one buffer: what x becomes, then, where tiles are shared, their sums and their counts (set to zero by the kernel before the product)
-            _, tokens, ctas, shared = plan
+            kind, tokens, ctas, shared = plan
             tiles = -(-n // 128) * -(-m // tokens) if shared else 0
-            x_bytes, side_bytes = _mxfp4_bytes(m, k) if quantise else (2 * m * k, -(-m // 4) * 16)
+            depth = -(-k // 256)
+            if quantise:
+                x_bytes, side_bytes = _mxfp4_bytes(m, k)
+            elif kind == "parts":
+                x_bytes, side_bytes = 3 * tokens * k, 1024 * depth + -(-m * depth // 4) * 16
+            else:
+                x_bytes, side_bytes = 2 * m * k, -(-m // 4) * 16
             scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
             work = torch.empty(x_bytes + side_bytes + scratch_bytes + 4 * tiles, dtype=torch.uint8, device=x.device)
             made = work.data_ptr()
@@ -2819,6 +2838,11 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
                 code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), made, side, m, k, arrived, tiles, stream)
                 code = code or lib.mrs_mxfp4_both_rows(made, side, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived,
                                                        early, stream)
+            elif kind == "parts":
+                lost = side + 1024 * depth
+                code = lib.mrs_mxfp4_rows_to_parts(x.data_ptr(), made, side, lost, m, k, tokens, arrived, tiles, stream)
+                code = code or lib.mrs_mxfp4_parts_rows(x.data_ptr(), made, side, lost, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas,
+                                                        scratch, arrived, early, stream)
             else:
                 fits = weight.half_exponent is not None
                 code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, m, k, arrived, tiles, stream)

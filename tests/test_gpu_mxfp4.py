@@ -128,7 +128,17 @@ def test_product_over_the_sizes(m, n, k, quantise):
 
 
 PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 5, False), ("many", 16, 7, True), ("many", 32, 1, False), ("many", 64, 3, True), ("many", 128, 148, False),
-         ("many", 128, 148, True), ("many", 128, 11, True), ("many", 192, 148, False), ("many", 192, 9, True)]
+         ("many", 128, 148, True), ("many", 128, 11, True), ("many", 192, 148, False), ("many", 192, 9, True), ("parts", 16, 5, False), ("parts", 16, 9, True),
+         ("parts", 32, 148, False), ("parts", 32, 7, True)]
+
+
+def takes(plan, m, k, quantise):
+    """Whether a kernel takes these rows."""
+    if plan[0] == "few":
+        return plan[1] >= kernels.mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k) > 0
+    if plan[0] == "parts":
+        return m <= plan[1] and k % 128 == 0 and not quantise
+    return plan[1] >= 128 or m <= plan[1]
 
 
 def fitting(plan, m, n, k):
@@ -141,12 +151,11 @@ def fitting(plan, m, n, k):
 
 @pytest.mark.parametrize("quantise", [False, True])
 @pytest.mark.parametrize("plan", PLANS)
-@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96), (400, 2500, 512)])
+@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96), (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096),
+                                   (32, 70, 640)])
 def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
-    if plan[0] == "many" and plan[1] < 128 and m > plan[1]:
-        pytest.skip("tiles of fewer than 128 tokens hold all of them")
-    if plan[0] == "few" and plan[1] < kernels.mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k):
-        pytest.skip("these rows do not fit the shared memory of so few CTAs")
+    if not takes(plan, m, k, quantise):
+        pytest.skip("not for these rows")
     g = torch.Generator(device=DEV).manual_seed(m * 31 + n * 7 + k)
     codes, scales, w = random_matrix(g, n, k)
     weight = kernels.mxfp4_matrix(codes, scales)
@@ -161,7 +170,7 @@ def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
         close_to_sums(out, want, size, k, f"{m} x {n} x {k} {plan}")
 
 
-SOME_PLANS = [("few", 1), ("few", 2), ("many", 64, 2, False), ("many", 128, 3, True), ("many", 192, 2, True)]
+SOME_PLANS = [("parts", 16, 2, False), ("few", 1), ("few", 2), ("many", 64, 2, False), ("many", 128, 3, True), ("many", 192, 2, True)]
 
 
 def check_product(x, weight, w, quantise, plan, what):
@@ -183,7 +192,9 @@ def check_product(x, weight, w, quantise, plan, what):
 def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
     """Elements of very different sizes in a row and in neighbouring rows, the ends of bfloat16's range, rows of zeros, infinities
     and NaN beside ordinary rows: exact products whatever the range, and nothing of one row in another."""
-    m, n, k = 11, 150, 800
+    m, n, k = 11, 150, 768 if plan[0] == "parts" else 800
+    if not takes(plan, m, k, quantise):
+        pytest.skip("not for these rows")
     g = torch.Generator(device=DEV).manual_seed(len(kind))
     codes, scales, w = random_matrix(g, n, k)
     weight = kernels.mxfp4_matrix(codes, scales)
@@ -199,7 +210,7 @@ def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
         x[::2] = 0.0
         x[1, 5:] = 0.0
     elif kind == "infinite":
-        x[2, 7], x[5, 300], x[8, 799] = math.inf, math.nan, -math.inf
+        x[2, 7], x[5, 300], x[8, k - 1] = math.inf, math.nan, -math.inf
     elif kind == "one_row":
         x[4, 10] = 1e30
         weight_column = (codes[:, 5] & 0xF0)                # column 10 of every row is 0: what is left of that row is its small elements
@@ -213,7 +224,9 @@ def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
 @pytest.mark.parametrize("plan", SOME_PLANS)
 @pytest.mark.parametrize("kind", ["wide", "nan", "zero_blocks", "small", "large", "unsettled"])
 def test_scales_of_every_size(kind, plan, quantise):
-    m, n, k = 9, 260, 544
+    m, n, k = 9, 260, 640 if plan[0] == "parts" else 544
+    if not takes(plan, m, k, quantise):
+        pytest.skip("not for these rows")
     g = torch.Generator(device=DEV).manual_seed(len(kind) + 50)
     codes, scales, w = random_matrix(g, n, k)
     if kind == "wide":

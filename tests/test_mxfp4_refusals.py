@@ -74,3 +74,14 @@ def test_runtime_config_takes_both_formats():
     RuntimeConfig().validate()
     RuntimeConfig(weight_format="mxfp4").validate()
     RuntimeConfig(weight_format="mxfp4", activation_format="mxfp4").validate()
+
+
+@pytest.mark.parametrize("m", [1, 8, 9, 16, 17, 33, 128, 129, 485, 4096])
+@pytest.mark.parametrize("n,k", [(1, 32), (128, 4096), (6145, 4096), (24576, 4096), (5120, 17408), (151936, 1024), (40, 65536)])
+@pytest.mark.parametrize("tokens,shared", [(16, None), (32, True), (192, None), (128, False)])
+def test_tiles_have_work_for_every_cta(m, n, k, tokens, shared):
+    """No more CTAs than SMs, and none without a stage (shared tiles) or a tile of its own."""
+    got, ctas, is_shared = kernels.mxfp4_tiles(m, n, k, tokens, 148, 11, shared)
+    tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
+    assert got == tokens and 1 <= ctas <= 148 and ctas <= (tiles * depth if is_shared else tiles)
+    assert shared is None or is_shared is shared
