@@ -401,6 +401,7 @@ MRS_EXPORT int mrs_mxfp4_rows_to_parts(const void* x, void* parts, void* scales,
 }
 
 MRS_EXPORT const char* mrs_mxfp4_error_string(int code) {
-    if (code == MRS_BAD_ARGUMENT) return "arguments outside what the kernels support (width no multiple of 32, unaligned base)";
+    if (code == MRS_BAD_ARGUMENT) return "arguments outside what the kernels support (width no multiple of 32, unaligned base, a plan for other sizes)";
+    if (code == -3) return "the driver refused the tensor map (address, sizes or strides)";
     return cudaGetErrorString((cudaError_t)code);
 }

@@ -414,7 +414,7 @@ int launch(const void* x, const void* codes, const void* scales, void* out, Shap
     attributes[1].id = cudaLaunchAttributeClusterDimension;
     attributes[1].val.clusterDim.x = s.cluster, attributes[1].val.clusterDim.y = 1, attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
-    config.numAttrs = 2;
+    config.numAttrs = s.cluster > 1 ? 2 : 1;
     cudaError_t e = cudaLaunchKernelEx(&config, few_rows_kernel<QUANTISE, Out>, (const bf16*)x, (const uint8_t*)codes, (const uint8_t*)scales,
                                        (Out*)out, s);
     if (e != cudaSuccess) return (int)e;

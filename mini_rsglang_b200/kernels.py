@@ -102,6 +102,8 @@ _sm_counts: dict[int, int] = {}
 
 def sm_count(device=None) -> int:
     """Multiprocessors of the device (asked once): what launch plans fill."""
+    if device in _sm_counts:                      # an index that has been asked for
+        return _sm_counts[device]
     index = torch.device(device).index if device is not None else None
     if index is None:
         index = torch.cuda.current_device()
@@ -2604,22 +2606,12 @@ def _mxfp4_check(code: int, what: str) -> None:
         raise BackendError(f"{what}: {mxfp4_library().mrs_mxfp4_error_string(code).decode()} (code {code})")
 
 
-class _OnDevice:
-    """The tensor's device as the current one, where it is not (`torch.cuda.device` costs microseconds)."""
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # the index, without asking whether CUDA is up
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device: torch.device):
-        index = device.index
-        self.guard = None if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _stream_here(index: int) -> int:
+    """The current stream of the current device `index`."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _mxfp4_bytes(rows: int, width: int) -> tuple[int, int]:
@@ -2669,11 +2661,13 @@ class Mxfp4:
     def settle(self) -> "Mxfp4":
         """Waits until the matrix is there and takes note of its scales' range.  For weights, once: products of settled weights are
         faster.  Whoever writes the data afterwards has to make a matrix anew.  Not while a graph is recorded."""
-        with _OnDevice(self.device):
+        with torch.cuda.device(self.device):
             span = torch.tensor([256, -1], dtype=torch.int32, device=self.device)
             codes, scales = self.addresses()
             _mxfp4_check(mxfp4_library().mrs_mxfp4_scale_range(codes, scales, span.data_ptr(), self.rows, self.width, _stream()), "mxfp4_scale_range")
             low, high = span.tolist()                        # waits for the stream
+        if 252 < high < 255:
+            raise InvalidRequest(f"4-bit matrix: a scale of 2^{high - 127} stands for values beyond float32; at most 2^125")
         # halfs hold 0.5 times 2^-23 to 6 times 2^13
         self.half_exponent = None if high == 255 or high - low > 36 else max(high, 0) - 127 - 13
         self.settled = True
@@ -2713,29 +2707,34 @@ def mxfp4_quantise(x: torch.Tensor) -> Mxfp4:
     bf16 = _is_bf16(x.dtype)
     _need(x, None, "mxfp4_quantise input")
     _mxfp4_aligned(x, "mxfp4_quantise input")
-    with _OnDevice(x.device):
-        out = _mxfp4_empty(rows, width, x.device)
-        codes, scales = out.addresses()
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes, scales, rows, width, None, 0, _stream()), "mxfp4_quantise")
+    here = x.get_device()
+    if here != _current_device():
+        with torch.cuda.device(here):
+            return mxfp4_quantise(x)
+    out = _mxfp4_empty(rows, width, x.device)
+    codes, scales = out.addresses()
+    _mxfp4_check(mxfp4_library().mrs_mxfp4_quantise(bf16, x.data_ptr(), codes, scales, rows, width, None, 0, _stream_here(here)), "mxfp4_quantise")
     return out
 
 
 def mxfp4_dequantise(matrix: Mxfp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """What the codes stand for, in bfloat16 or float32 (both hold every such value; a scale beyond 2^125 may make bfloat16's and
-    float32's infinity of a code)."""
+    """What the codes stand for, in bfloat16 or float32 (both hold every such value)."""
     bf16 = _is_bf16(dtype)
     _need(matrix.data, torch.uint8, "mxfp4 matrix")
-    with _OnDevice(matrix.device):
-        out = torch.empty((matrix.rows, matrix.width), dtype=dtype, device=matrix.device)
-        codes, scales = matrix.addresses()
-        _mxfp4_check(mxfp4_library().mrs_mxfp4_dequantise(bf16, codes, scales, out.data_ptr(), matrix.rows, matrix.width, _stream()), "mxfp4_dequantise")
+    here = matrix.data.get_device()
+    if here != _current_device():
+        with torch.cuda.device(here):
+            return mxfp4_dequantise(matrix, dtype)
+    out = torch.empty((matrix.rows, matrix.width), dtype=dtype, device=matrix.data.device)
+    codes, scales = matrix.addresses()
+    _mxfp4_check(mxfp4_library().mrs_mxfp4_dequantise(bf16, codes, scales, out.data_ptr(), matrix.rows, matrix.width, _stream_here(here)), "mxfp4_dequantise")
     return out
 
 
 def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
     """A matrix from elsewhere: `codes` uint8 [rows, width / 2], element 2 j of a row in the low half of byte j, and `scales` uint8
-    [rows, width / 32], a block's exponent + 127 (255: not a number).  Takes copies, and waits until they are made: what it
-    returns is settled.  For loading weights, not for a step."""
+    [rows, width / 32], a block's exponent + 127 (255: not a number; 253 and 254 are refused where the block is not all zeros).
+    Takes copies, and waits until they are made: what it returns is settled.  For loading weights, not for a step."""
     if codes.dim() != 2 or scales.dim() != 2:
         raise InvalidRequest("mxfp4_matrix: codes [rows, width / 2] and scales [rows, width / 32]")
     rows, width = codes.shape[0], 2 * codes.shape[1]
@@ -2746,7 +2745,7 @@ def mxfp4_matrix(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4:
     _need(scales, torch.uint8, "mxfp4 scales")
     if scales.device != codes.device:
         raise InvalidRequest("mxfp4_matrix: codes and scales are on different devices")
-    with _OnDevice(codes.device):
+    with torch.cuda.device(codes.device):
         out = _mxfp4_empty(rows, width, codes.device)
         out.codes.copy_(codes)
         held, tiles = out.addresses()
@@ -2801,51 +2800,52 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
         raise InvalidRequest("mxfp4_gemm: out must be bfloat16 or float32")
     _need(x, torch.bfloat16, "mxfp4_gemm input")
     _need(out, None, "mxfp4_gemm out", (m, n))
-    if x.device != weight.device or out.device != x.device:
+    here = x.get_device()
+    if here != weight.data.get_device() or here != out.get_device():
         raise InvalidRequest("mxfp4_gemm: input, weights and output are on different devices")
     if m == 0 or n == 0:
         return
     _mxfp4_aligned(x, "mxfp4_gemm input")
+    if here != _current_device():
+        with torch.cuda.device(here):
+            return mxfp4_gemm(x, weight, out, quantise, plan)
     lib = mxfp4_library()
     out_f32, early = int(out.dtype is torch.float32), int(weight.settled)
     w_codes, w_scales = weight.addresses()
-    with _OnDevice(x.device):
-        sms = sm_count(x.device)
-        if plan is None:
-            plan = mxfp4_plan(m, n, k, bool(quantise), sms)
-        if plan[0] == "few":
-            code = lib.mrs_mxfp4_few_rows(x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early,
-                                          _stream())
+    sms, stream = sm_count(here), _stream_here(here)
+    if plan is None:
+        plan = mxfp4_plan(m, n, k, bool(quantise), sms)
+    if plan[0] == "few":
+        code = lib.mrs_mxfp4_few_rows(x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early, stream)
+    else:
+        # one buffer: what x becomes, then, where tiles are shared, their sums and their counts (set to zero by the kernel before the product)
+        kind, tokens, ctas, shared = plan
+        tiles = -(-n // 128) * -(-m // tokens) if shared else 0
+        depth = -(-k // 256)
+        if quantise:
+            x_bytes, side_bytes = _mxfp4_bytes(m, k)
+        elif kind == "parts":
+            x_bytes, side_bytes = 3 * tokens * k, 1024 * depth + -(-m * depth // 4) * 16
         else:
-            # one buffer: what x becomes, then, where tiles are shared, their sums and their counts (set to zero by the kernel before the product)
-            kind, tokens, ctas, shared = plan
-            tiles = -(-n // 128) * -(-m // tokens) if shared else 0
-            depth = -(-k // 256)
-            if quantise:
-                x_bytes, side_bytes = _mxfp4_bytes(m, k)
-            elif kind == "parts":
-                x_bytes, side_bytes = 3 * tokens * k, 1024 * depth + -(-m * depth // 4) * 16
-            else:
-                x_bytes, side_bytes = 2 * m * k, -(-m // 4) * 16
-            scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
-            work = torch.empty(x_bytes + side_bytes + scratch_bytes + 4 * tiles, dtype=torch.uint8, device=x.device)
-            made = work.data_ptr()
-            side, scratch = made + x_bytes, made + x_bytes + side_bytes if shared else None
-            arrived = scratch + scratch_bytes if shared else None
-            stream = _stream()
-            launch_count += 1
-            if quantise:
-                code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), made, side, m, k, arrived, tiles, stream)
-                code = code or lib.mrs_mxfp4_both_rows(made, side, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived,
-                                                       early, stream)
-            elif kind == "parts":
-                lost = side + 1024 * depth
-                code = lib.mrs_mxfp4_rows_to_parts(x.data_ptr(), made, side, lost, m, k, tokens, arrived, tiles, stream)
-                code = code or lib.mrs_mxfp4_parts_rows(x.data_ptr(), made, side, lost, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas,
-                                                        scratch, arrived, early, stream)
-            else:
-                fits = weight.half_exponent is not None
-                code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, m, k, arrived, tiles, stream)
-                code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), made if fits else None, side if fits else None, weight.half_exponent or 0, w_codes,
-                                                          w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived, early, stream)
-        _mxfp4_check(code, "mxfp4_gemm")
+            x_bytes, side_bytes = 2 * m * k, -(-m // 4) * 16
+        scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
+        work = torch.empty(x_bytes + side_bytes + scratch_bytes + 4 * tiles, dtype=torch.uint8, device=x.device)
+        made = work.data_ptr()
+        side, scratch = made + x_bytes, made + x_bytes + side_bytes if shared else None
+        arrived = scratch + scratch_bytes if shared else None
+        launch_count += 1
+        if quantise:
+            code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), made, side, m, k, arrived, tiles, stream)
+            code = code or lib.mrs_mxfp4_both_rows(made, side, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived,
+                                                   early, stream)
+        elif kind == "parts":
+            lost = side + 1024 * depth
+            code = lib.mrs_mxfp4_rows_to_parts(x.data_ptr(), made, side, lost, m, k, tokens, arrived, tiles, stream)
+            code = code or lib.mrs_mxfp4_parts_rows(x.data_ptr(), made, side, lost, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas,
+                                                    scratch, arrived, early, stream)
+        else:
+            fits = weight.half_exponent is not None
+            code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, m, k, arrived, tiles, stream)
+            code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), made if fits else None, side if fits else None, weight.half_exponent or 0, w_codes,
+                                                      w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived, early, stream)
+    _mxfp4_check(code, "mxfp4_gemm")

@@ -261,3 +261,137 @@ def test_settle_knows_what_halfs_hold(rows, width, low, high):
     scales[-1, -1] = high
     weight = kernels.mxfp4_matrix(codes, scales)
     assert weight.settled and weight.half_exponent == (None if high == 255 or high - low > 36 else high - 140)
+
+
+ALL_KINDS = [(3, False), (3, True), (12, False), (12, True), (60, False), (60, True), (200, False), (200, True)]
+
+
+@pytest.mark.parametrize("m,quantise", ALL_KINDS)
+def test_nothing_but_the_output_is_written(m, quantise):
+    """Odd sizes inside a larger buffer: what stands before and behind the rows stays."""
+    n, k = 333, 1152
+    g = torch.Generator(device=DEV).manual_seed(m)
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    before = (x.clone(), weight.data.clone())
+    for dtype in (torch.bfloat16, torch.float32):
+        buffer = torch.full((m * n + 2 * n,), 7.0, device=DEV, dtype=dtype)
+        kernels.mxfp4_gemm(x, weight, buffer[n:-n].view(m, n), quantise=quantise)
+        assert (buffer[:n] == 7).all() and (buffer[-n:] == 7).all()
+        values = plain_quantise(x)[0] if quantise else x.double()
+        close_to_sums(buffer[n:-n].view(m, n), values @ w.T, values.abs() @ w.abs().T, k, "inside a buffer")
+    assert torch.equal(x, before[0]) and torch.equal(weight.data, before[1])
+
+
+@pytest.mark.parametrize("m,quantise", ALL_KINDS)
+def test_the_same_bits_every_time(m, quantise):
+    """Several CTAs add up a tile, in whatever order they end: a result depends on its inputs alone, on every stream."""
+    n, k = 1100, 5120
+    g = torch.Generator(device=DEV).manual_seed(m)
+    weight = kernels.mxfp4_matrix(*random_matrix(g, n, k)[:2])
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    first = torch.empty(m, n, device=DEV)
+    kernels.mxfp4_gemm(x, weight, first, quantise=quantise)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.empty_like(first) for _ in range(30)]
+    for i, out in enumerate(outs):
+        with torch.cuda.stream(streams[i % 3]):                 # three at a time, each with its own workspace
+            kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, out) for out in outs)
+    kernels.check_device_errors(certain=True)
+
+
+@pytest.mark.parametrize("m,quantise", ALL_KINDS)
+def test_recorded_and_replayed(m, quantise):
+    """Two recordings with the same weights, replayed in turn and beside eager calls, with new inputs."""
+    n, k = 700, 2304
+    g = torch.Generator(device=DEV).manual_seed(m + 1)
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    xs = [torch.zeros(m, k, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+    outs = [torch.empty(m, n, device=DEV) for _ in range(2)]
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for x, out in zip(xs, outs):
+            kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+    torch.cuda.synchronize()
+    graphs = []
+    for x, out in zip(xs, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+            if quantise:                                         # quantising and reading back in the same recording
+                back = kernels.mxfp4_dequantise(kernels.mxfp4_quantise(x), torch.float32)
+        graphs.append(graph)
+    for _ in range(3):
+        for x in xs:
+            x.copy_(torch.randn(m, k, device=DEV, generator=g))
+        eager = torch.empty(m, n, device=DEV)
+        for graph in graphs:
+            graph.replay()
+        kernels.mxfp4_gemm(xs[0], weight, eager, quantise=quantise)
+        torch.cuda.synchronize()
+        for x, out in zip(xs, outs):
+            values = plain_quantise(x)[0] if quantise else x.double()
+            close_to_sums(out, values @ w.T, values.abs() @ w.abs().T, k, "replayed")
+        assert torch.equal(outs[0], eager)
+        if quantise:
+            assert torch.equal(back.double(), plain_quantise(xs[1])[0])
+
+
+def test_offsets_beyond_32_bits():
+    """Codes of more than 2^31 bytes, results of more than 2^31 elements: the last rows and columns."""
+    n, k = 1_100_003, 4096
+    g = torch.Generator(device=DEV).manual_seed(5)
+    codes = torch.randint(0, 256, (n, k // 2), device=DEV, generator=g, dtype=torch.uint8)
+    scales = torch.randint(118, 124, (n, k // 32), device=DEV, generator=g, dtype=torch.uint8)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    places = torch.tensor([0, 524287, 524288, n - 130, n - 1], device=DEV)
+    w = plain_values(codes[places], scales[places])
+    del codes, scales
+    for m, quantise in ((1, False), (2, True), (9, False), (9, True), (130, False), (140, True)):
+        x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+        out = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
+        kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+        values = plain_quantise(x)[0] if quantise else x.double()
+        close_to_sums(out[:, places], values @ w.T, values.abs() @ w.abs().T, k, f"{m} rows")
+    values = kernels.mxfp4_dequantise(weight)
+    assert torch.equal(values[places].double(), w)
+    again = kernels.mxfp4_quantise(values)
+    assert torch.equal(kernels.mxfp4_dequantise(again)[places].double(), w)      # representable values stay
+    del values, again, weight, out
+    m, n, k = 20011, 120001, 32
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    rows = torch.tensor([0, 17895, 17896, m - 1], device=DEV)
+    for quantise in (False, True):
+        out = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
+        kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+        values = plain_quantise(x[rows])[0] if quantise else x[rows].double()
+        close_to_sums(out[rows], values @ w.T, values.abs() @ w.abs().T, k, "many results")
+        del out
+
+
+def test_refusals_on_the_gpu():
+    g = torch.Generator(device=DEV).manual_seed(1)
+    codes, scales, _ = random_matrix(g, 40, 64)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x, out = torch.zeros(4, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(4, 40, device=DEV)
+    odd = torch.zeros(4 * 64 + 1, device=DEV, dtype=torch.bfloat16)[1:].view(4, 64)
+    for bad_x, bad_out in ((x.float(), out), (x.half(), out), (torch.zeros(64, 4, device=DEV, dtype=torch.bfloat16).t(), out), (odd, out), (x[:3], out),
+                           (x, out.half()), (x, torch.zeros(4, 41, device=DEV)), (x, torch.zeros(40, 4, device=DEV).t()), (x[:, :32].contiguous(), out)):
+        with pytest.raises(InvalidRequest):
+            kernels.mxfp4_gemm(bad_x, weight, bad_out)
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_quantise(odd)
+    with pytest.raises(InvalidRequest):
+        kernels.mxfp4_quantise(x.t())
+    with pytest.raises(InvalidRequest, match="float32"):
+        kernels.mxfp4_matrix(codes, torch.full_like(scales, 253))
+    zeros = kernels.mxfp4_matrix(torch.zeros_like(codes), torch.full_like(scales, 254))         # blocks of zeros may have any scale
+    kernels.mxfp4_gemm(x, zeros, out)
+    assert (out == 0).all()
