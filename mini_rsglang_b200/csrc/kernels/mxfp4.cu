@@ -55,8 +55,8 @@ template <typename T> struct EightOf { typedef Eight Type; };
 template <> struct EightOf<float> { typedef EightFloats Type; };
 
 // A warp takes UNROLL stretches of 256 elements, one after the other in a row and then in the next, all loads first: with one load of
-// 16 bytes a thread in flight and a division for each, 2,048 x 17,408 bfloat16 took XXX us.  Stretches that reach over a row's end
-// write zero scales there.
+// 16 bytes a thread in flight and a division for each, 2,048 x 17,408 bfloat16 took 38 us, with four 22 (71 MB read and 19 MB
+// written; a copy of as much would take 14).  Stretches that reach over a row's end write zero scales there.
 template <typename T> constexpr int unroll() { return sizeof(T) == 2 ? 4 : 2; }
 
 struct Stretch {

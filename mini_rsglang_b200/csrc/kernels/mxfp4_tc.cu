@@ -5,7 +5,7 @@
 // memory, and the last to do so adds them in the order of K, so that a result does not depend on timing.
 //
 //   weights_kernel   x in bfloat16.  Bulk tensor copies bring 128 x 256 codes (128-byte swizzle) and their scales into a ring, x in
-//                    pieces of 128 elements into another.  Sixteen warps make the A operand of the codes, a thread a row and 64
+//                    pieces of 128 elements into another.  Eight warps make the A operand of the codes, a thread a row and 64
 //                    elements, in tensor memory; no shared memory is written for it.  One thread issues kind::f16 MMAs.
 //                    Making A is what a scheduler has to do for each MMA: halfs are a conversion and a multiplication for two codes (9
 //                    clocks for eight codes of a warp), bfloat16 goes through float32 (21 clocks).  So x comes as halfs, times a
@@ -39,7 +39,8 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 // A whole warp's bounded wait, whose outcome is the same for the whole warp and whose loop the compiler does not see: what the warp walks
 // through stays in uniform registers, which the MMA and copy instructions take their operands from.  (With the loop of mbar_wait and
-// breaks lane by lane a step of MMAs took 510 clocks to issue, with this one XXX.)
+// breaks lane by lane a step of MMAs took 510 clocks to issue, and 24,576 x 4,096 times 2,048 rows 320 us; with this one and steps of 128
+// elements instead of 64 301.)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     uint32_t done;
     asm volatile("{\n .reg .pred p, q;\n .reg .u64 start, now;\n"
@@ -69,27 +70,38 @@ struct Shapes {
 // A CTA's tiles; [from, to) are the stages of the tile at hand.  Shared tiles: the CTA's run of units.  Whole ones: every gridDim.x-th, so
 // that CTAs at work at the same time write neighbouring columns and read neighbouring weights.
 struct Walk {
-    int first, total, done, tile, from, to;        // `total` stages from unit `first` on (whole tiles: of this CTA's own)
-    __device__ __forceinline__ explicit Walk(const Shapes& s) : done(0), tile(0), from(0), to(0) {
+    int first, begin, total, done, from, to;       // `total` stages from unit `first` on, stage `begin` of its tile (whole tiles: of this CTA's own)
+    int n_tile, token_tile, n_step, token_step;    // the tile at hand, and how far to the next: no division a tile
+    __device__ __forceinline__ explicit Walk(const Shapes& s) : done(0), from(0), to(0) {
+        int tile = blockIdx.x, step = gridDim.x;
+        first = begin = 0;
         if (s.scratch) {
             first = start(s, blockIdx.x);
             total = start(s, blockIdx.x + 1) - first;
+            tile = first / s.depth, step = 1;
+            begin = first - tile * s.depth;
         } else {
-            first = 0;
-            total = ((s.units / s.depth - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * s.depth;
+            total = ((s.units / s.depth - 1 - tile) / step + 1) * s.depth;
         }
+        n_step = step / s.token_tiles, token_step = step - n_step * s.token_tiles;
+        n_tile = tile / s.token_tiles, token_tile = tile - n_tile * s.token_tiles;
     }
     __device__ static __forceinline__ int start(const Shapes& s, int cta) { return (int)((long long)s.units * cta / gridDim.x); }
     __device__ static __forceinline__ int owner(const Shapes& s, int unit) { return (int)(((long long)(unit + 1) * gridDim.x - 1) / s.units); }
-    __device__ __forceinline__ int tile_of(const Shapes& s, int position) const {
+    // Rows of w and stage of this CTA's `position`-th stage.
+    __device__ __forceinline__ int n_tile_of(const Shapes& s, int position) const {
         const int index = (first + position) / s.depth;
-        return s.scratch ? index : (int)blockIdx.x + index * (int)gridDim.x;
+        return (s.scratch ? index : (int)blockIdx.x + index * (int)gridDim.x) / s.token_tiles;
     }
     __device__ __forceinline__ int stage_of(const Shapes& s, int position) const { return (first + position) % s.depth; }
     __device__ __forceinline__ bool step(const Shapes& s) {
         if (done >= total) return false;
-        tile = tile_of(s, done);
-        from = stage_of(s, done);
+        from = begin;
+        if (done > 0) {
+            from = 0;
+            n_tile += n_step, token_tile += token_step;
+            if (token_tile >= s.token_tiles) token_tile -= s.token_tiles, ++n_tile;
+        }
         to = min(s.depth, from + total - done);
         done += to - from;
         return true;
@@ -103,9 +115,9 @@ template <int TOKENS, int WARPS, typename Out, bool PARTS = false>
 __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors) {
     constexpr int STEP = TOKENS < 32 || PARTS ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
     const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
-    const int token0 = walk.tile % s.token_tiles * TOKENS, live = min(TOKENS, s.M - token0);
+    const int token0 = walk.token_tile * TOKENS, live = min(TOKENS, s.M - token0), tile = walk.n_tile * s.token_tiles + walk.token_tile;
     const uint32_t acc = accumulator + ((uint32_t)(quarter * 32) << 16);
-    const long long n = (long long)(walk.tile / s.token_tiles) * BM + row;
+    const long long n = (long long)walk.n_tile * BM + row;
     const bool whole = walk.from == 0 && walk.to == s.depth;
     auto finish = [&](int c, float (&v)[STEP]) {
         if (halfs) {                               // powers of two in the floats' range, a lane each, by way of shared memory
@@ -156,10 +168,10 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
         }
     }
     if (whole) return;
-    const int first = Walk::owner(s, walk.tile * s.depth), last = Walk::owner(s, (walk.tile + 1) * s.depth - 1);
+    const int first = Walk::owner(s, tile * s.depth), last = Walk::owner(s, (tile + 1) * s.depth - 1);
     __threadfence();
     asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
-    if (index == 0 && (threadIdx.x & 31) == 0) *flag = atomicAdd(s.arrived + walk.tile, 1) == last - first;
+    if (index == 0 && (threadIdx.x & 31) == 0) *flag = atomicAdd(s.arrived + tile, 1) == last - first;
     asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
     const bool finisher = *flag != 0;
     asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");               // the flag is read by all before it is written again
@@ -193,7 +205,9 @@ constexpr int PIECE_K = 64;                        // a 128-byte row of x, and w
 // Elements of K of a step: a buffer of A and a slot of x.  The issuing warp's waits and commits cost some 400 clocks a step beside the
 // warps that make A, as much as 40 MMAs of 16 tokens or 4 of 192; tensor memory bounds the steps of wide tiles.
 template <int TOKENS> constexpr int step_k() { return TOKENS <= 64 ? 256 : 128; }
-constexpr int MAKERS = 16, STORERS = 4;            // warps that make bfloat16, and that store results
+// Warps that make A, and that store results.  Sixteen and four took 757 us for 151,936 x 1,024 times 2,048 rows (four storers need 13,000
+// to 22,000 clocks a tile, its MMAs 6,200), these 506; 24,576 x 4,096 took 301 and 305.
+constexpr int MAKERS = 8, STORERS = 8;
 constexpr int W_THREADS = (3 + MAKERS + STORERS) * 32;
 template <int TOKENS> constexpr int a_columns() { return step_k<TOKENS>() / 2; }
 template <int TOKENS> constexpr int x_bytes() { return TOKENS * step_k<TOKENS>() * 2; }
@@ -317,7 +331,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     };
     if (warp == 2 + MAKERS + STORERS) {
         if (elect_one())
-            for (int i = 0; i < ahead; ++i) load_codes(walk.tile_of(s, i) / s.token_tiles, walk.stage_of(s, i), i);
+            for (int i = 0; i < ahead; ++i) load_codes(walk.n_tile_of(s, i), walk.stage_of(s, i), i);
         __syncwarp();
     }
     pdl_wait();
@@ -339,7 +353,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         int slot = 0;
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
-            const int token0 = walk.tile % s.token_tiles * TOKENS, steps = steps_of();
+            const int token0 = walk.token_tile * TOKENS, steps = steps_of();
             for (int step = 0; step < steps; ++step) {
                 if (!(alive = warp_wait(&x_empty[slot], phase))) break;
                 if (leader) {
@@ -360,7 +374,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         uint32_t phase = 1;
         int count = 0;
         while (alive && walk.step(s)) {
-            const int n_tile = walk.tile / s.token_tiles;
+            const int n_tile = walk.n_tile;
             for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
                 if (count >= ahead) {                     // not even the wait before: the makers may be through with those stages
                     if (!(alive = warp_wait(&w_empty[slot], phase))) break;
@@ -402,35 +416,38 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
             __syncwarp();
         }
     } else if (warp < 2 + MAKERS) {
-        const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;        // group: a stage's quarter of K
+        const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;        // group: every GROUPS-th piece of a stage
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + A_FIRST;
-        const uint32_t first_chunk = ((group * 2) ^ (row & 7)) << 4, second_chunk = ((group * 2 + 1) ^ (row & 7)) << 4;
-        const int scale_place = (group >> 1) * MX_TILE_BYTES + lane * 16 + quarter * 4 + (group & 1) * 2;
+        constexpr int GROUPS = MAKERS / 4, STAGE_PIECES = STAGE_K / PIECE_K;
+        bool alive = true;
         int w_slot = 0;
         uint32_t w_phase = 0;
-        for (int step = group / STEP_PIECES; step < walk.total * STAGE_STEPS; step += STAGE_STEPS) {          // of the CTA's run
-            if (!warp_wait(&w_full[w_slot], w_phase)) break;
+        for (int stage = 0; stage < walk.total && alive; ++stage) {                              // of the CTA's run
+            if (!(alive = warp_wait(&w_full[w_slot], w_phase))) break;
             const unsigned char* codes = w_ring + w_slot * CODE_BYTES + row * 128;
-            const uint32_t two = *reinterpret_cast<const uint16_t*>(s_ring + w_slot * SCALE_BYTES + scale_place);
-            const uint4 first = *reinterpret_cast<const uint4*>(codes + first_chunk);
-            const uint4 second = *reinterpret_cast<const uint4*>(codes + second_chunk);
-            uint32_t words[32];
-            if (halfs) {
-                decode_block_halfs(first, two & 255u, s.w_exponent, words);
-                decode_block_halfs(second, two >> 8, s.w_exponent, words + 16);
-            } else {
-                decode_block(first, two & 255u, words);
-                decode_block(second, two >> 8, words + 16);
+            const unsigned char* scale_bytes = s_ring + w_slot * SCALE_BYTES + lane * 16 + quarter * 4;
+#pragma unroll 1
+            for (int piece = group; piece < STAGE_PIECES; piece += GROUPS) {
+                const uint32_t two = *reinterpret_cast<const uint16_t*>(scale_bytes + (piece >> 1) * MX_TILE_BYTES + (piece & 1) * 2);
+                const uint4 first = *reinterpret_cast<const uint4*>(codes + (((piece * 2) ^ (row & 7)) << 4));
+                const uint4 second = *reinterpret_cast<const uint4*>(codes + (((piece * 2 + 1) ^ (row & 7)) << 4));
+                uint32_t words[32];
+                if (halfs) {
+                    decode_block_halfs(first, two & 255u, s.w_exponent, words);
+                    decode_block_halfs(second, two >> 8, s.w_exponent, words + 16);
+                } else {
+                    decode_block(first, two & 255u, words);
+                    decode_block(second, two >> 8, words + 16);
+                }
+                const int step = stage * STAGE_STEPS + piece / STEP_PIECES, b = step % A_BUFFERS;
+                if (!(alive = warp_wait(&a_empty[b], ((step / A_BUFFERS) & 1) ^ 1))) break;
+                tcgen05_fence_after_sync();
+                tmem_store_32_words(lanes + b * A_COLUMNS + piece % STEP_PIECES * (PIECE_K / 2), words);
+                tmem_store_wait();
+                tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[b]);
             }
-            const int b = step % A_BUFFERS;
-            if (!warp_wait(&a_empty[b], ((step / A_BUFFERS) & 1) ^ 1)) break;
-            __syncwarp();
-            tcgen05_fence_after_sync();
-            tmem_store_32_words(lanes + b * A_COLUMNS + group % STEP_PIECES * (PIECE_K / 2), words);
-            tmem_store_wait();
-            tcgen05_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[b]);
             __syncwarp();
             if (lane == 0) mbar_arrive(&w_empty[w_slot]);
             if (++w_slot == W_STAGES) w_slot = 0, w_phase ^= 1;
@@ -540,7 +557,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
         int slot = 0;
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
-            const int token0 = walk.tile % s.token_tiles * TOKENS;
+            const int token0 = walk.token_tile * TOKENS;
             const uint8_t* tile_scales = x_scales + (size_t)(token0 >> 7) * s.w_tiles_of_a_row * MX_TILE_BYTES;
             // a tile behind the last token: nobody stores its sums
             const size_t second = (token0 >> 7) + 1 < s.x_row_tiles ? (size_t)s.w_tiles_of_a_row * MX_TILE_BYTES : 0;
@@ -564,7 +581,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
         int slot = 0;
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
-            const int n_tile = walk.tile / s.token_tiles;
+            const int n_tile = walk.n_tile;
             const uint8_t* tile_scales = w_scales + (size_t)n_tile * s.w_tiles_of_a_row * MX_TILE_BYTES;
             for (int stage = walk.from; stage < walk.to; ++stage) {
                 if (!(alive = warp_wait(&empty[slot], phase))) break;
@@ -589,7 +606,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
             tcgen05_fence_after_sync();
             const uint32_t d_tmem = tmem + buffer * B_ACCUMULATOR;
             // tiles of 192 tokens begin in the middle of a tile of scales every other time: two columns, 64 tokens, further in
-            const uint32_t shift = TOKENS == 192 ? (((uint32_t)(walk.tile % s.token_tiles) * TOKENS) & 127u) / 32 : 0u;
+            const uint32_t shift = TOKENS == 192 ? (((uint32_t)walk.token_tile * TOKENS) & 127u) / 32 : 0u;
             for (int index = 0; index < walk.to - walk.from; ++index) {
                 if (!(alive = warp_wait(&full[slot], phase))) break;
                 tcgen05_fence_after_sync();
@@ -717,7 +734,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     const int ahead = s.early ? min(STAGES, walk.total) : 0;
     if (warp == 2 + P_STORERS) {
         if (elect_one())
-            for (int i = 0; i < ahead; ++i) load_w(walk.tile_of(s, i) / s.token_tiles, walk.stage_of(s, i), i);
+            for (int i = 0; i < ahead; ++i) load_w(walk.n_tile_of(s, i), walk.stage_of(s, i), i);
         __syncwarp();
     }
     pdl_wait();
@@ -790,7 +807,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
         int slot = 0, count = 0;
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
-            const int n_tile = walk.tile / s.token_tiles;
+            const int n_tile = walk.n_tile;
             for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
                 if (count >= ahead) {
                     if (!(alive = warp_wait(&empty[slot], phase))) break;
