@@ -134,11 +134,9 @@ PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 5, False), ("many", 16
 
 def takes(plan, m, k, quantise):
     """Whether a kernel takes these rows."""
-    if plan[0] == "few":
-        return plan[1] >= kernels.mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k) > 0
     if plan[0] == "parts":
         return m <= plan[1] and k % 128 == 0 and not quantise
-    return plan[1] >= 128 or m <= plan[1]
+    return plan[0] == "few" or plan[1] >= 128 or m <= plan[1]
 
 
 def fitting(plan, m, n, k):
@@ -149,13 +147,13 @@ def fitting(plan, m, n, k):
     return (*plan[:2], min(plan[2], tiles * -(-k // 256) if plan[3] else tiles), plan[3])
 
 
-@pytest.mark.parametrize("quantise", [False, True])
-@pytest.mark.parametrize("plan", PLANS)
-@pytest.mark.parametrize("m,n,k", [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96), (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096),
-                                   (32, 70, 640)])
+SIZES = [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96),
+         (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096), (32, 70, 640)]
+
+
+@pytest.mark.parametrize("m,n,k,plan,quantise", [(m, n, k, plan, quantise) for m, n, k in SIZES for plan in PLANS for quantise in (False, True)
+                                                 if takes(plan, m, k, quantise)])
 def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
-    if not takes(plan, m, k, quantise):
-        pytest.skip("not for these rows")
     g = torch.Generator(device=DEV).manual_seed(m * 31 + n * 7 + k)
     codes, scales, w = random_matrix(g, n, k)
     weight = kernels.mxfp4_matrix(codes, scales)
@@ -186,15 +184,12 @@ def check_product(x, weight, w, quantise, plan, what):
     close_to_sums(out[finite], want[finite], size[finite], x.shape[1], what)
 
 
-@pytest.mark.parametrize("quantise", [False, True])
-@pytest.mark.parametrize("plan", SOME_PLANS)
+@pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS for q in (False, True) if takes(plan, 11, 128, q)])
 @pytest.mark.parametrize("kind", ["wide", "tiny", "huge", "zeros", "infinite", "one_row"])
 def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
     """Elements of very different sizes in a row and in neighbouring rows, the ends of bfloat16's range, rows of zeros, infinities
     and NaN beside ordinary rows: exact products whatever the range, and nothing of one row in another."""
     m, n, k = 11, 150, 768 if plan[0] == "parts" else 800
-    if not takes(plan, m, k, quantise):
-        pytest.skip("not for these rows")
     g = torch.Generator(device=DEV).manual_seed(len(kind))
     codes, scales, w = random_matrix(g, n, k)
     weight = kernels.mxfp4_matrix(codes, scales)
@@ -220,13 +215,10 @@ def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
     check_product(x.bfloat16(), weight, w, quantise, plan, kind)
 
 
-@pytest.mark.parametrize("quantise", [False, True])
-@pytest.mark.parametrize("plan", SOME_PLANS)
+@pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS for q in (False, True) if takes(plan, 11, 128, q)])
 @pytest.mark.parametrize("kind", ["wide", "nan", "zero_blocks", "small", "large", "unsettled"])
 def test_scales_of_every_size(kind, plan, quantise):
     m, n, k = 9, 260, 640 if plan[0] == "parts" else 544
-    if not takes(plan, m, k, quantise):
-        pytest.skip("not for these rows")
     g = torch.Generator(device=DEV).manual_seed(len(kind) + 50)
     codes, scales, w = random_matrix(g, n, k)
     if kind == "wide":
