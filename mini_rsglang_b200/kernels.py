@@ -2761,27 +2761,37 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
       24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 17.4 / 22.1, 16 rows - / 16.9 / 21.6, 32 rows - / 20.0 / 25.3
       4,096 x 12,288   1 row 9.8 / 14.8 / 19.0, 8 rows (x in four CTAs) 18.3 / 15.5 / 20.2
       5,120 x 17,408   4 rows (x in two CTAs) 15.1 / 17.8 / 24.4, 8 rows (in four) 27.9 / 18.0 / 25.1
-    and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.6 / 14.5, 8 rows 16.1 / 14.5; 1,000 x 2,048 4 rows 3.6 / 6."""
-    if m <= (4 if quantise else 8):
+    and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.8 / 14.0, 8 rows 16.4 / 14.6; 12,963 x 2,368 1 row 7.6 / 6.8; 4,096 x 12,288 4 rows 13.8 / 15.2;
+      8 rows: 6,144 x 4,096 8.9 / 8.1, 2,560 x 9,728 11.8 / 13.2, 4,096 x 2,560 6.8 / 6.8, 1,000 x 2,048 4.8 / 6.1."""
+    if m <= (8 if not quantise or n * k <= 3 << 23 else 4 if n <= 8192 else 0):
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
         if 0 < cluster <= 2:
             return ("few", cluster)
     if m <= 32 and k % 128 == 0 and not quantise:
         return ("parts", *mxfp4_tiles(m, n, k, 16 if m <= 16 else 32, sms, 11))
     if m <= 128:
-        tokens = 16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128
+        widths = (16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128,)
     else:
-        tokens = min((192, 128), key=lambda t: -(-(-(-n // 128) * -(-m // t)) // sms) * t)
-    return ("many", *mxfp4_tiles(m, n, k, tokens, sms, 11 if tokens <= 32 and not quantise else 30))
+        widths = (192, 128)
+    meeting = 36 if quantise else 6 if widths[0] <= 32 else 10
+    tokens = min(widths, key=lambda t: min(_mxfp4_stages(m, n, k, t, sms, meeting)) * (130 + t))          # a stage: 1.04 us with 128, 1.29 with 192
+    return ("many", *mxfp4_tiles(m, n, k, tokens, sms, meeting))
+
+
+def _mxfp4_stages(m: int, n: int, k: int, tokens: int, sms: int, meeting: int) -> tuple[float, float]:
+    """The stages of 256 elements of K that the product takes with whole tiles and with shared ones."""
+    tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
+    return -(-tiles // sms) * depth, 1.05 * tiles * depth / sms + meeting
 
 
 def mxfp4_tiles(m: int, n: int, k: int, tokens: int, sms: int, meeting: int, shared: bool | None = None) -> tuple:
     """(tokens of a tile, CTAs, whether tiles are shared) of tiles of 128 rows of weights x `tokens` on as many CTAs as there are SMs.
-    Shared tiles cost a meeting of their CTAs, as long as `meeting` stages of 256 elements of K: measured 3 to 5 us, where a stage takes
-    0.43 us with a few tokens of bfloat16, 0.25 with 4 bits on both sides, and more columns have to meet with wide tiles."""
+    Shared tiles cost a meeting of their CTAs, as long as `meeting` stages, and 1/20 of all since CTAs at work at the same time are further
+    apart in the matrix.  Measured whole / shared: 24,576 x 4,096 64 rows 34.5 / 30.2 us, 192 rows 43.0 / 41.4, 2,048 rows 305 / 310."""
     tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
     if shared is None:
-        shared = tiles * depth / sms + meeting < -(-tiles // sms) * depth
+        whole, together = _mxfp4_stages(m, n, k, tokens, sms, meeting)
+        shared = together < whole
     return (tokens, min(sms, max(tiles, tiles * depth // 3)), True) if shared else (tokens, min(tiles, sms), False)
 
 
