@@ -3,7 +3,7 @@
 // For a block of 32 neighbours with largest size a: e = floor(log2 a) - 2, code = the nearest E2M1 value to x 2^-e (ties to the
 // even code, above 6 to 6), scale = 2^e.  The power of two makes the multiplication exact, so a code is one rounding away from x.
 // Four lanes share a block (eight elements each: a 16-byte load of bfloat16), sixteen lanes the four blocks whose scales are one
-// word; two exchanges find a block's largest.  The kernels are bound by bytes.
+// word; two exchanges find a block's largest.  Bytes bound the kernels, once their instructions are few enough.
 #include <limits.h>
 
 #include "mxfp4.cuh"
@@ -17,18 +17,25 @@ __device__ __forceinline__ void clear(int* zeros, int count) {
     for (int i = blockIdx.x * THREADS + threadIdx.x; i < count; i += gridDim.x * THREADS) zeros[i] = 0;
 }
 
-// Eight elements as they come from memory, the float bits of their largest size, and they themselves.
+// Two 16-bit numbers a word, both at least 0: the larger ones.
+__device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b) { return __viaddmax_s16x2(a, 0u, b); }
+
+// Eight elements as they come from memory, their largest size, and they themselves.  Only exponents count for a scale, so that sizes are
+// compared as the upper 16 bits of float32; `of_two` gives those of two such eights in a word.
 struct Eight {
     uint4 raw;
     __device__ __forceinline__ void load(const bf16* p) { raw = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ uint32_t largest_of_block() const {            // of 32 elements: four lanes; two sizes a word
-        uint32_t m = __viaddmax_s16x2(raw.x & 0x7FFF7FFFu, 0u, raw.y & 0x7FFF7FFFu);
-        m = __viaddmax_s16x2(raw.z & 0x7FFF7FFFu, 0u, m);
-        m = __viaddmax_s16x2(raw.w & 0x7FFF7FFFu, 0u, m);
-        m = __viaddmax_s16x2(__shfl_xor_sync(0xffffffffu, m, 1), 0u, m);
-        m = __viaddmax_s16x2(__shfl_xor_sync(0xffffffffu, m, 2), 0u, m);
+    __device__ __forceinline__ uint32_t largest() const {
+        const uint32_t m = larger_pair(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu);
+        return larger_pair(raw.w & 0x7FFF7FFFu, larger_pair(raw.z & 0x7FFF7FFFu, m));
+    }
+    __device__ __forceinline__ uint32_t largest_of_block() const {             // the float bits, from four lanes
+        uint32_t m = largest();
+        m = larger_pair(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = larger_pair(m, __shfl_xor_sync(0xffffffffu, m, 2));
         return max(m << 16, m & 0xFFFF0000u);
     }
+    __device__ static __forceinline__ uint32_t of_two(uint32_t a, uint32_t b) { return larger_pair(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632)); }
     __device__ __forceinline__ void values(float (&v)[8]) const {
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
@@ -41,23 +48,18 @@ struct Eight {
 struct EightFloats {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
-    __device__ __forceinline__ uint32_t largest_of_block() const {
+    __device__ __forceinline__ uint32_t largest() const {
         const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        return m;
     }
+    __device__ static __forceinline__ uint32_t of_two(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
     __device__ __forceinline__ void values(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
 };
 template <typename T> struct EightOf { typedef Eight Type; };
 template <> struct EightOf<float> { typedef EightFloats Type; };
-
-// A warp takes UNROLL stretches of 256 elements, one after the other in a row and then in the next, all loads first: with one load of
-// 16 bytes a thread in flight and a division for each, 2,048 x 17,408 bfloat16 took 38 us, with four 22 (71 MB read and 19 MB
-// written; a copy of as much would take 14).  Stretches that reach over a row's end write zero scales there.
-template <typename T> constexpr int unroll() { return sizeof(T) == 2 ? 4 : 2; }
 
 struct Stretch {
     unsigned row, index;               // of its row
@@ -67,38 +69,65 @@ struct Stretch {
     }
 };
 
-template <typename T>
+// A warp takes four stretches of 256 elements, one after the other in a row and then in the next, all loads first.  What it does beside
+// loading and storing counts: with each stretch by itself it was 122 instructions a stretch, which filled the schedulers.  So largest sizes
+// are found for two stretches at a time, their scales for four, and in rows of whole stretches (WHOLE) an element's place follows from its
+// stretch's number: 80.  Stretches that reach over a row's end write zero scales there.
+// 2,048 x 17,408 bfloat16: 38 us with one stretch in flight, 22 with four, 17.8 with 80 instructions (90 MB: 13.7 at the bandwidth of a
+// copy); 5,003 x 5,120 float32 18.9 (17.7); dequantised 15.6 and 20.9.
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                            unsigned rows, unsigned width, unsigned of_a_row, int* __restrict__ zeros, int zero_count) {
-    constexpr int UNROLL = unroll<T>();
     pdl_launch_dependents();
     pdl_wait();
     clear(zeros, zero_count);
-    const unsigned lane = threadIdx.x & 31, half = lane >> 4, warps = gridDim.x * (THREADS / 32);
+    const unsigned lane = threadIdx.x & 31, warps = gridDim.x * (THREADS / 32);
+    const unsigned block = (lane >> 2) & 3, half = lane >> 4;                   // four lanes a block; blocks of half a stretch share a word of scales
     const unsigned stretches = rows * of_a_row;
-    for (unsigned first = (blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * UNROLL; first < stretches; first += warps * UNROLL) {
-        typename EightOf<T>::Type held[UNROLL];
+    for (unsigned first = (blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * 4; first < stretches; first += warps * 4) {
+        typename EightOf<T>::Type held[4];
+        size_t place[4];
+        bool here[4];
         Stretch at(first, of_a_row);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u, at.next(of_a_row)) {
+        for (int u = 0; u < 4; ++u) {
             const unsigned column = at.index * 256 + lane * 8;
+            place[u] = WHOLE ? (size_t)(first + u) * 256 + lane * 8 : (size_t)at.row * width + column;
+            here[u] = first + u < stretches && (WHOLE || column < width);
             held[u] = {};
-            if (first + u < stretches && column < width) held[u].load(x + (size_t)at.row * width + column);
+            if (here[u]) held[u].load(x + place[u]);
+            if (!WHOLE) at.next(of_a_row);
         }
-        at = Stretch(first, of_a_row);
+        uint32_t largest[2], bytes[2];                                          // stretches 0 and 1, 2 and 3
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u, at.next(of_a_row)) {
-            if (first + u >= stretches) break;                                 // the same for the whole warp
-            const unsigned column = at.index * 256 + lane * 8;
-            const uint32_t byte = mx_scale_byte(held[u].largest_of_block());
+        for (int p = 0; p < 2; ++p) {
+            largest[p] = EightOf<T>::Type::of_two(held[2 * p].largest(), held[2 * p + 1].largest());
+            largest[p] = larger_pair(largest[p], __shfl_xor_sync(0xffffffffu, largest[p], 1));
+            largest[p] = larger_pair(largest[p], __shfl_xor_sync(0xffffffffu, largest[p], 2));
+            bytes[p] = __viaddmax_s16x2((largest[p] >> 7) & 0x00FF00FFu, 0xFFFEFFFEu, 0u);      // exponents less two, at least 0
+        }
+        uint32_t four = __byte_perm(bytes[0], bytes[1], 0x6420);                // a byte a stretch
+        const uint32_t any = larger_pair(largest[0], largest[1]);
+        if ((any & 0xFFFFu) >= 0x7F80u || any >= 0x7F800000u) {                 // an infinity or NaN: no numbers, codes of zeros
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (((largest[u >> 1] >> (16 * (u & 1))) & 0xFFFFu) >= 0x7F80u) held[u] = {}, four |= 0xFFu << (8 * u);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
             float v[8];
             held[u].values(v);
-            const uint32_t word = byte == 255u ? 0u : mx_encode_8(v, mx_inverse(byte));
-            if (column < width) *reinterpret_cast<uint32_t*>(codes + (size_t)at.row * (width >> 1) + (column >> 1)) = word;
-            uint32_t four = byte << (8 * ((lane >> 2) & 3));
-            four |= __shfl_xor_sync(0xffffffffu, four, 4);
-            four |= __shfl_xor_sync(0xffffffffu, four, 8);
-            if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(at.row, at.index * 2 + half, of_a_row * 2)) = four;
+            const uint32_t word = mx_encode_8(v, mx_inverse((bytes[u >> 1] >> (16 * (u & 1))) & 0xFFu));
+            if (here[u]) *reinterpret_cast<uint32_t*>(codes + (place[u] >> 1)) = word;
+        }
+        // Four lanes' words of a byte a stretch become words of a byte a block, the lane of block u with stretch u.
+        uint32_t other = __shfl_xor_sync(0xffffffffu, four, 8);
+        four = __byte_perm(four, other, block & 2 ? 0x3276 : 0x5410);
+        other = __shfl_xor_sync(0xffffffffu, four, 4);
+        four = __byte_perm(four, other, block & 1 ? 0x3715 : 0x6240);
+        if ((lane & 3) == 0 && first + block < stretches) {
+            const Stretch mine(first + block, of_a_row);
+            *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(mine.row, mine.index * 2 + half, of_a_row * 2)) = four;
         }
     }
 }
@@ -341,13 +370,13 @@ MRS_EXPORT int mrs_mxfp4_quantise(int is_bf16, const void* x, void* codes, void*
     if (rows == 0) return 0;
     if (bad_sizes(rows, width) || (zero_count && !zeros) || !x || !codes || !scales || (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15)) return MRS_BAD_ARGUMENT;
     const unsigned of_a_row = (unsigned)((width + 255) / 256);
-    const long long threads = rows * of_a_row * 32;
-    if (is_bf16)
-        MRS_LAUNCH(quantise_kernel<bf16>, blocks_for(threads / unroll<bf16>()), THREADS, 0, stream, (const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, (unsigned)rows,
-                   (unsigned)width, of_a_row, (int*)zeros, zero_count);
-    else
-        MRS_LAUNCH(quantise_kernel<float>, blocks_for(threads / unroll<float>()), THREADS, 0, stream, (const float*)x, (uint8_t*)codes, (uint8_t*)scales, (unsigned)rows,
-                   (unsigned)width, of_a_row, (int*)zeros, zero_count);
+    const int blocks = blocks_for(rows * of_a_row * 8);
+#define MRS_QUANTISE(T, WHOLE) MRS_LAUNCH((quantise_kernel<T, WHOLE>), blocks, THREADS, 0, stream, (const T*)x, (uint8_t*)codes, (uint8_t*)scales, (unsigned)rows, (unsigned)width, of_a_row, (int*)zeros, zero_count)
+    if (is_bf16 && width % 256 == 0) MRS_QUANTISE(bf16, true);
+    else if (is_bf16) MRS_QUANTISE(bf16, false);
+    else if (width % 256 == 0) MRS_QUANTISE(float, true);
+    else MRS_QUANTISE(float, false);
+#undef MRS_QUANTISE
     MRS_RETURN_LAUNCH_STATUS();
 }
 
