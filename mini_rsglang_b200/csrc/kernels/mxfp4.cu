@@ -416,11 +416,11 @@ MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* exponen
     MRS_RETURN_LAUNCH_STATUS();
 }
 
-// x [rows, width] bfloat16, rows up to `tokens` (16 or 32), to parts [3 tokens, width], their scales and lost [rows * ceil(width / 256)] int32.
+// x [rows, width] bfloat16, rows up to `tokens` (16, 32 or 64), to parts [3 tokens, width], their scales and lost [rows * ceil(width / 256)] int32.
 MRS_EXPORT int mrs_mxfp4_rows_to_parts(const void* x, void* parts, void* scales, void* lost, int rows, int width, int tokens, void* zeros, int zero_count,
                                        void* stream) {
     if (rows == 0) return 0;
-    if (bad_sizes(rows, width) || rows > tokens || (tokens != 16 && tokens != 32) || (zero_count && !zeros) || !x || !parts || !scales || !lost ||
+    if (bad_sizes(rows, width) || rows > tokens || (tokens != 16 && tokens != 32 && tokens != 64) || (zero_count && !zeros) || !x || !parts || !scales || !lost ||
         (((uintptr_t)x | (uintptr_t)parts | (uintptr_t)scales) & 15) || ((uintptr_t)lost & 3))
         return MRS_BAD_ARGUMENT;
     const int stretches = (width + 255) / 256;

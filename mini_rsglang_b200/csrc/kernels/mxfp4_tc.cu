@@ -15,7 +15,7 @@
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
 //                    tensor memory (tcgen05.cp) stage by stage.
 //
-//   parts_kernel     x in bfloat16 once more, up to 32 rows: as three parts of E5M2 (mxfp4.cu), 3 x 32 columns of kind::mxf8f6f4 MMAs whose A
+//   parts_kernel     x in bfloat16 once more, up to 64 rows: as three parts of E5M2 (mxfp4.cu), 3 x 64 columns of kind::mxf8f6f4 MMAs whose A
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
 //                    columns' sums are the result's.  Rows that three parts do not hold exactly are multiplied on the CUDA cores.
 //
@@ -677,10 +677,16 @@ __device__ __forceinline__ void umma_mxf8f6f4(uint32_t d, uint64_t a_desc, uint6
 constexpr int HALF_STAGE_K = 128;                          // elements of K of a 128-byte row of bytes
 constexpr int P_A_BYTES = BM * HALF_STAGE_K;               // half a stage of w in shared memory, of which the copies count half
 constexpr int P_STORERS = 8, P_THREADS = (3 + P_STORERS) * 32;
-constexpr int P_SCALE_COLUMNS = 16;                        // of a stage: 2 x 4 of w, 2 x 4 of the tokens' parts
-template <int TOKENS> constexpr int p_stages() { return TOKENS > 16 ? 3 : 4; }
+// A slot of the ring holds a stage, with 64 tokens half of one: their parts are longer than the codes, and five halves in flight fit where
+// two stages would.
+template <int TOKENS> constexpr int p_halves() { return TOKENS > 32 ? 1 : 2; }
+template <int TOKENS> constexpr int p_stages() { return TOKENS > 32 ? 5 : TOKENS > 16 ? 3 : 4; }
 template <int TOKENS> constexpr int p_x_bytes() { return 3 * TOKENS * HALF_STAGE_K; }
-template <int TOKENS> constexpr size_t parts_smem() { return 1024 + (size_t)p_stages<TOKENS>() * (2 * P_A_BYTES + 2 * p_x_bytes<TOKENS>() + 2 * SCALE_BYTES) + 256; }
+template <int TOKENS> constexpr int p_x_tiles() { return (3 * TOKENS + 127) / 128; }                     // of scales
+template <int TOKENS> constexpr int p_slot_scale_bytes() { return p_halves<TOKENS>() * MX_TILE_BYTES * (1 + p_x_tiles<TOKENS>()); }
+template <int TOKENS> constexpr size_t parts_smem() {
+    return 1024 + (size_t)p_stages<TOKENS>() * (p_halves<TOKENS>() * (P_A_BYTES + p_x_bytes<TOKENS>()) + p_slot_scale_bytes<TOKENS>()) + 256;
+}
 
 template <int TOKENS, typename Out>
 __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
@@ -689,11 +695,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
                                                              Out* __restrict__ out, const Shapes s) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    constexpr int STAGES = p_stages<TOKENS>(), N_COLUMNS = 3 * TOKENS, ACCUMULATOR = 128, SCALES_FIRST = 2 * ACCUMULATOR;
+    constexpr int STAGES = p_stages<TOKENS>(), N_COLUMNS = 3 * TOKENS, ACCUMULATOR = N_COLUMNS > 128 ? 192 : 128, SCALES_FIRST = 2 * ACCUMULATOR;
+    constexpr int HALVES = p_halves<TOKENS>(), PIECES = 2 / HALVES, X_TILES = p_x_tiles<TOKENS>(), X_BYTES = p_x_bytes<TOKENS>();     // pieces: slots a stage
+    constexpr int W_SCALE_BYTES = HALVES * MX_TILE_BYTES, SLOT_SCALE_BYTES = p_slot_scale_bytes<TOKENS>();      // of a slot: w's scales, then the parts', tiles of 128 by tiles
+    constexpr int SCALE_COLUMNS = HALVES * 4 * (1 + X_TILES);                          // in tensor memory, of a slot
+    static_assert(SCALES_FIRST + STAGES * SCALE_COLUMNS <= TMEM_COLUMNS);
     unsigned char* w_ring = smem;
-    unsigned char* x_ring = w_ring + STAGES * 2 * P_A_BYTES;
-    unsigned char* s_ring = x_ring + STAGES * 2 * p_x_bytes<TOKENS>();
-    uint64_t* full = reinterpret_cast<uint64_t*>(s_ring + STAGES * 2 * SCALE_BYTES);
+    unsigned char* x_ring = w_ring + STAGES * HALVES * P_A_BYTES;
+    unsigned char* s_ring = x_ring + STAGES * HALVES * X_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(s_ring + STAGES * SLOT_SCALE_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
@@ -724,17 +734,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
 
-    // a stage of w: two halves of 128 elements, and its scales
-    auto load_w = [&](int n_tile, int stage, int slot) {
-        mbar_arrive_expect_tx(&full[slot], P_A_BYTES + SCALE_BYTES);                    // half of what two halves take in shared memory
+    // a piece of w: halves of 128 elements, and their scales
+    auto load_w = [&](int n_tile, int piece, int slot) {
+        mbar_arrive_expect_tx(&full[slot], HALVES * (P_A_BYTES / 2) + W_SCALE_BYTES);   // half of what the codes take in shared memory
 #pragma unroll
-        for (int h = 0; h < 2; ++h) tma_load_2d(w_ring + (slot * 2 + h) * P_A_BYTES, &w_map, &full[slot], stage * STAGE_K + h * HALF_STAGE_K, n_tile * BM);
-        bulk_load(s_ring + slot * 2 * SCALE_BYTES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + 2 * stage) * MX_TILE_BYTES, SCALE_BYTES, &full[slot]);
+        for (int h = 0; h < HALVES; ++h)
+            tma_load_2d(w_ring + (slot * HALVES + h) * P_A_BYTES, &w_map, &full[slot], (piece * HALVES + h) * HALF_STAGE_K, n_tile * BM);
+        bulk_load(s_ring + slot * SLOT_SCALE_BYTES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + piece * HALVES) * MX_TILE_BYTES, W_SCALE_BYTES, &full[slot]);
     };
-    const int ahead = s.early ? min(STAGES, walk.total) : 0;
+    const int ahead = s.early ? min(STAGES, walk.total * PIECES) : 0;
     if (warp == 2 + P_STORERS) {
         if (elect_one())
-            for (int i = 0; i < ahead; ++i) load_w(walk.n_tile_of(s, i), walk.stage_of(s, i), i);
+            for (int i = 0; i < ahead; ++i) load_w(walk.n_tile_of(s, i / PIECES), walk.stage_of(s, i / PIECES) * PIECES + i % PIECES, i);
         __syncwarp();
     }
     pdl_wait();
@@ -788,14 +799,17 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
         int slot = 0;
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
-            for (int stage = walk.from; stage < walk.to; ++stage) {
+            for (int piece = walk.from * PIECES; piece < walk.to * PIECES; ++piece) {
                 if (!(alive = warp_wait(&empty[slot], phase))) break;
                 if (leader) {
-                    mbar_arrive_expect_tx(&full[slot], 2 * p_x_bytes<TOKENS>() + SCALE_BYTES);
+                    mbar_arrive_expect_tx(&full[slot], HALVES * X_BYTES + X_TILES * W_SCALE_BYTES);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        tma_load_2d(x_ring + (slot * 2 + h) * p_x_bytes<TOKENS>(), &x_map, &full[slot], stage * STAGE_K + h * HALF_STAGE_K, 0);
-                    bulk_load(s_ring + slot * 2 * SCALE_BYTES + SCALE_BYTES, x_scales + (size_t)stage * SCALE_BYTES, SCALE_BYTES, &full[slot]);
+                    for (int h = 0; h < HALVES; ++h)
+                        tma_load_2d(x_ring + (slot * HALVES + h) * X_BYTES, &x_map, &full[slot], (piece * HALVES + h) * HALF_STAGE_K, 0);
+#pragma unroll
+                    for (int t = 0; t < X_TILES; ++t)
+                        bulk_load(s_ring + slot * SLOT_SCALE_BYTES + (1 + t) * W_SCALE_BYTES,
+                                  x_scales + ((size_t)t * s.w_tiles_of_a_row + piece * HALVES) * MX_TILE_BYTES, W_SCALE_BYTES, &full[slot]);
                 }
                 __syncwarp();
                 if (++slot == STAGES) slot = 0, phase ^= 1;
@@ -808,10 +822,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
         uint32_t phase = 1;
         while (alive && walk.step(s)) {
             const int n_tile = walk.n_tile;
-            for (int stage = walk.from; stage < walk.to; ++stage, ++count) {
+            for (int piece = walk.from * PIECES; piece < walk.to * PIECES; ++piece, ++count) {
                 if (count >= ahead) {
                     if (!(alive = warp_wait(&empty[slot], phase))) break;
-                    if (leader) load_w(n_tile, stage, slot);
+                    if (leader) load_w(n_tile, piece, slot);
                     __syncwarp();
                 }
                 if (++slot == STAGES) slot = 0, phase ^= 1;
@@ -827,23 +841,26 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
             if (!(alive = warp_wait(&acc_empty[buffer], ((round >> 1) & 1) ^ 1))) break;
             tcgen05_fence_after_sync();
             const uint32_t d_tmem = tmem + buffer * ACCUMULATOR;
-            for (int index = 0; index < walk.to - walk.from; ++index) {
+            for (int index = 0; index < (walk.to - walk.from) * PIECES; ++index) {
                 if (!(alive = warp_wait(&full[slot], phase))) break;
                 tcgen05_fence_after_sync();
-                const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(w_ring + slot * 2 * P_A_BYTES));
-                const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + slot * 2 * p_x_bytes<TOKENS>()));
-                const uint32_t scales = smem_u32(s_ring + slot * 2 * SCALE_BYTES);
-                const uint32_t columns = tmem + SCALES_FIRST + slot * P_SCALE_COLUMNS;
+                const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(w_ring + slot * HALVES * P_A_BYTES));
+                const uint64_t b_desc = umma_smem_desc_sw128(smem_u32(x_ring + slot * HALVES * X_BYTES));
+                const uint32_t scales = smem_u32(s_ring + slot * SLOT_SCALE_BYTES);
+                const uint32_t columns = tmem + SCALES_FIRST + slot * SCALE_COLUMNS;
                 if (leader) {
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {                                   // 128 elements of K
-                        scales_to_tmem(columns + q * 4, scales + q * MX_TILE_BYTES);
-                        scales_to_tmem(columns + 8 + q * 4, scales + SCALE_BYTES + q * MX_TILE_BYTES);
+                    for (int q = 0; q < HALVES; ++q) {                              // 128 elements of K: w, then the parts' tiles side by side
+                        scales_to_tmem(columns + q * 4 * (1 + X_TILES), scales + q * MX_TILE_BYTES);
+#pragma unroll
+                        for (int t = 0; t < X_TILES; ++t)
+                            scales_to_tmem(columns + q * 4 * (1 + X_TILES) + 4 * (1 + t), scales + (1 + t) * W_SCALE_BYTES + q * MX_TILE_BYTES);
                     }
 #pragma unroll
-                    for (int k = 0; k < STAGE_K / 32; ++k)
-                        umma_mxf8f6f4(d_tmem, a_desc + (k >> 2) * (P_A_BYTES / 16) + 2 * (k & 3), b_desc + (k >> 2) * (p_x_bytes<TOKENS>() / 16) + 2 * (k & 3),
-                                      mxf8f6f4_idesc(BM, N_COLUMNS, k & 3), columns + (k >> 2) * 4, columns + 8 + (k >> 2) * 4, index > 0 || k > 0);
+                    for (int k = 0; k < HALVES * 4; ++k)
+                        umma_mxf8f6f4(d_tmem, a_desc + (k >> 2) * (P_A_BYTES / 16) + 2 * (k & 3), b_desc + (k >> 2) * (X_BYTES / 16) + 2 * (k & 3),
+                                      mxf8f6f4_idesc(BM, N_COLUMNS, k & 3), columns + (k >> 2) * 4 * (1 + X_TILES), columns + (k >> 2) * 4 * (1 + X_TILES) + 4,
+                                      index > 0 || k > 0);
                     umma_commit(&empty[slot]);
                 }
                 __syncwarp();
@@ -984,7 +1001,7 @@ MRS_EXPORT int mrs_mxfp4_both_rows(const void* x_codes, const void* x_scales, co
     return MRS_BAD_ARGUMENT;
 }
 
-// The same with x [M, K] in bfloat16 and in parts (mxfp4.cu), M up to `tokens` (16 or 32), K a multiple of 128.
+// The same with x [M, K] in bfloat16 and in parts (mxfp4.cu), M up to `tokens` (16, 32 or 64), K a multiple of 128.
 MRS_EXPORT int mrs_mxfp4_parts_rows(const void* x, const void* parts, const void* x_scales, const void* lost, const void* codes, const void* scales, void* out,
                                     int out_f32, int M, int N, int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
@@ -994,7 +1011,7 @@ MRS_EXPORT int mrs_mxfp4_parts_rows(const void* x, const void* parts, const void
     Shapes s = {};
     s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
 #define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_parts<T, float>(x, parts, x_scales, lost, codes, scales, out, s, ctas, stream) : launch_parts<T, bf16>(x, parts, x_scales, lost, codes, scales, out, s, ctas, stream)
-    MRS_TOKENS(16); MRS_TOKENS(32);
+    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64);
 #undef MRS_TOKENS
     return MRS_BAD_ARGUMENT;
 }

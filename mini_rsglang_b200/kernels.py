@@ -2758,7 +2758,8 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
     """How a product is launched: ("few", CTAs of a cluster), or ("parts" | "many", tokens of a tile, CTAs, whether tiles are shared).
 
     Measured on a B200 (us, weights [n, k] from a cold L2, the kernel that prepares x included; few / parts / many):
-      24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 17.4 / 22.1, 16 rows - / 17.0 / 21.6, 24 rows - / 20.0 / 25.3
+      24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 17.4 / 22.1, 16 rows - / 17.0 / 21.6, 24 rows - / 20.0 / 25.3,
+                       64 rows - / 24.2 / 30.3
       4,096 x 12,288   1 row 9.8 / 14.8 / 19.0, 8 rows (x in four CTAs) 18.3 / 15.5 / 20.2
       5,120 x 17,408   4 rows (x in two CTAs) 15.1 / 17.8 / 24.4, 8 rows (in four) 27.9 / 18.0 / 25.1
     and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.8 / 14.0, 8 rows 16.4 / 14.6; 12,963 x 2,368 1 row 7.6 / 6.8; 4,096 x 12,288 4 rows 13.8 / 15.2;
@@ -2767,8 +2768,8 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
         if 0 < cluster <= 2:
             return ("few", cluster)
-    if m <= 32 and k % 128 == 0 and not quantise:
-        return ("parts", *mxfp4_tiles(m, n, k, 16 if m <= 16 else 32, sms, 9))
+    if m <= 64 and k % 128 == 0 and not quantise:
+        return ("parts", *mxfp4_tiles(m, n, k, 16 if m <= 16 else 32 if m <= 32 else 64, sms, 9 if m <= 32 else 10))
     if m <= 128:
         widths = (16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128,)
     else:
@@ -2835,7 +2836,8 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
         if quantise:
             x_bytes, side_bytes = _mxfp4_bytes(m, k)
         elif kind == "parts":
-            x_bytes, side_bytes = 3 * tokens * k, 1024 * depth + -(-m * depth // 4) * 16
+            x_bytes, scale_bytes = 3 * tokens * k, -(-3 * tokens // 128) * 1024 * depth
+            side_bytes = scale_bytes + -(-m * depth // 4) * 16
         else:
             x_bytes, side_bytes = 2 * m * k, -(-m // 4) * 16
         scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
@@ -2849,7 +2851,7 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
             code = code or lib.mrs_mxfp4_both_rows(made, side, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived,
                                                    early, stream)
         elif kind == "parts":
-            lost = side + 1024 * depth
+            lost = side + scale_bytes
             code = lib.mrs_mxfp4_rows_to_parts(x.data_ptr(), made, side, lost, m, k, tokens, arrived, tiles, stream)
             code = code or lib.mrs_mxfp4_parts_rows(x.data_ptr(), made, side, lost, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas,
                                                     scratch, arrived, early, stream)

@@ -129,7 +129,7 @@ def test_product_over_the_sizes(m, n, k, quantise):
 
 PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 5, False), ("many", 16, 7, True), ("many", 32, 1, False), ("many", 64, 3, True), ("many", 128, 148, False),
          ("many", 128, 148, True), ("many", 128, 11, True), ("many", 192, 148, False), ("many", 192, 9, True), ("parts", 16, 5, False), ("parts", 16, 9, True),
-         ("parts", 32, 148, False), ("parts", 32, 7, True)]
+         ("parts", 32, 148, False), ("parts", 32, 7, True), ("parts", 64, 3, False), ("parts", 64, 148, True)]
 
 
 def takes(plan, m, k, quantise):
@@ -148,7 +148,7 @@ def fitting(plan, m, n, k):
 
 
 SIZES = [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96),
-         (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096), (32, 70, 640)]
+         (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096), (32, 70, 640), (33, 300, 640), (50, 1000, 1152), (63, 129, 128)]
 
 
 @pytest.mark.parametrize("m,n,k,plan,quantise", [(m, n, k, plan, quantise) for m, n, k in SIZES for plan in PLANS for quantise in (False, True)
@@ -168,7 +168,7 @@ def test_every_kernel_over_the_sizes(m, n, k, plan, quantise):
         close_to_sums(out, want, size, k, f"{m} x {n} x {k} {plan}")
 
 
-SOME_PLANS = [("parts", 16, 2, False), ("few", 1), ("few", 2), ("many", 64, 2, False), ("many", 128, 3, True), ("many", 192, 2, True)]
+SOME_PLANS = [("parts", 16, 2, False), ("parts", 64, 2, True), ("few", 1), ("few", 2), ("many", 64, 2, False), ("many", 128, 3, True), ("many", 192, 2, True)]
 
 
 def check_product(x, weight, w, quantise, plan, what):
