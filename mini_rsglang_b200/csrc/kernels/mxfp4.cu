@@ -226,11 +226,13 @@ __global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __r
 
 // Rows of bfloat16 as halfs times a power of two of the row's own: row r holds x 2^-exponents[r], its largest in [2^15, 2^16).  An element's
 // exponent field becomes itself less that of the largest, plus 30, its mantissa its seven bits and three zeros: exact, but for elements
-// 2^30 and more below the largest, rows below 2^-96 and what is not finite; exponents[r] is then HALFS_LOST and the row is not to be used.
+// 2^30 and more below the largest, which become 0 and are noted (a few in a prompt's products of gate and up), rows below 2^-96 and what
+// is not finite.  factors[r] is twice the exponent, plus 1 where elements are noted; HALFS_LOST if there are more than fit or the row is
+// one of the others, and not to be used.
 constexpr int HELD = 4;
 constexpr int HALFS_LOST = INT_MIN;
-__global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __restrict__ x, uint16_t* __restrict__ halfs, int* __restrict__ exponents,
-                                                                long long width, int* __restrict__ zeros, int zero_count) {
+__global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __restrict__ x, uint16_t* __restrict__ halfs, int* __restrict__ factors,
+                                                                int* __restrict__ noted, long long width, int* __restrict__ zeros, int zero_count) {
     __shared__ uint32_t scratch[THREADS / 32];
     pdl_launch_dependents();
     pdl_wait();
@@ -263,32 +265,55 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
     const bool empty = largest == 0, ordinary = field >= 31 && field < 255;
     const uint32_t down = empty || !ordinary ? 0u : (uint32_t)(-((field - 30) << 7)) & 0xFFFFu, both = down | down << 16;
     uint32_t lost = 0;
-    auto convert = [&](const uint4& v) {
+    auto convert = [&](const uint4& v, uint32_t* gone) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t h[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             const uint32_t size = w[p] & 0x7FFF7FFFu, r = __viaddmax_s16x2(size, both, 0u);
-            lost |= (size + 0x7FFF7FFFu) & ~(r + 0x7F807F80u);                // highest bit of each half: not 0, and below the halfs' smallest ordinary number
             h[p] = (r << 3) | (w[p] & 0x80008000u);
+            gone[p] = (size + 0x7FFF7FFFu) & ~(r + 0x7F807F80u);              // highest bit of each half: not 0, and below the halfs' smallest ordinary number
+            lost |= gone[p];
         }
         return make_uint4(h[0], h[1], h[2], h[3]);
     };
+    uint32_t gone[4];
 #pragma unroll
     for (int j = 0; j < HELD; ++j) {
         const int i = j * THREADS + threadIdx.x;
-        if (i < chunks) to[i] = convert(held[j]);
+        if (i < chunks) to[i] = convert(held[j], gone);
     }
-    for (int i = HELD * THREADS + threadIdx.x; i < chunks; i += THREADS) to[i] = convert(from[i]);
-    const bool bad = __syncthreads_or((lost & 0x80008000u) != 0u) || !(empty || ordinary);
-    if (threadIdx.x == 0) exponents[row] = bad ? HALFS_LOST : empty ? 0 : field - 127 - 15;
+    for (int i = HELD * THREADS + threadIdx.x; i < chunks; i += THREADS) to[i] = convert(from[i], gone);
+    bool bad = !(empty || ordinary);
+    const bool some = __syncthreads_or((lost & 0x80008000u) != 0u);
+    if (some && !bad) {                                                       // once more, with zeros in their place; a warp's 32 eights are a stretch
+        const long long stretches = (width + 255) >> 8;
+        for (int i = threadIdx.x; (i & ~31) < chunks; i += THREADS) {
+            const uint4 v = i < chunks ? from[i] : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t mask = 0, h[4];
+            *reinterpret_cast<uint4*>(h) = convert(v, gone);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const uint32_t both_of = (gone[p] >> 15) & 0x00010001u;
+                h[p] &= ~(both_of * 0xFFFFu);
+                mask |= (both_of & 1u) << (2 * p) | (both_of >> 16) << (2 * p + 1);
+                if ((both_of & 1u) && field - (int)((w[p] >> 7) & 0xFFu) > 90) bad = true;       // so small that sums of halfs could not take it up
+                if ((both_of >> 16) && field - (int)((w[p] >> 23) & 0xFFu) > 90) bad = true;
+            }
+            if (mask) to[i] = *reinterpret_cast<uint4*>(h);
+            if (mx_note_lost(mask, v, row * stretches + (i >> 5), noted, gridDim.x * stretches)) bad = true;
+        }
+        bad = __syncthreads_or(bad);
+    }
+    if (threadIdx.x == 0) factors[row] = bad ? HALFS_LOST : 2 * (empty ? 0 : field - 127 - 15) + some;
 }
 
 // Up to `tokens` rows of bfloat16 as three parts of E5M2 (three bits of significand, exponents of -16 to 15) each, part p of row r at row
 // p * tokens + r, with a power of two for 32 neighbours in scale tiles (mxfp4.cuh) of these 3 * tokens rows.  With 2^(e - 14) for a block
 // whose largest size has the exponent e, x = (a + b + c 2^-8) 2^(e - 14): a is x rounded, b what is left of it rounded, c, with
-// a power 2^-8 further down, the rest: of eight bits three, three signed and two are enough down to 2^-26 of the largest.  Where that
-// is not so lost[r * stretches + stretch] is 1: the row cannot be had in parts.
+// a power 2^-8 further down, the rest: of eight bits three, three signed and two are enough down to 2^-26 of the largest.  Elements of
+// which that is not so, infinities and NaN among them, are 0 in all parts and noted.
 constexpr int PART_SHIFT = 8;
 __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __restrict__ x, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
                                                                 int* __restrict__ lost, int rows, int width, int tokens, int stretches, int* __restrict__ zeros,
@@ -303,13 +328,12 @@ __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __re
     if (column < width) held.load(x + (size_t)row * width + column);
     const uint32_t largest = held.largest_of_block();
     const int e = (int)(largest >> 23) - 127;                    // 128: infinity or NaN
-    const bool empty = largest == 0, fits = empty || (e >= -105 && e < 128);
-    const uint32_t byte = fits && !empty ? (uint32_t)(e - 14 + 127) : 127u;
+    const bool ordinary = largest != 0 && e >= -105 && e < 128;
+    const uint32_t byte = ordinary ? (uint32_t)(e - 14 + 127) : 127u;
     const float up = mx_inverse(byte), down = mx_scale(byte);
     float v[8];
     held.values(v);
-    uint32_t a[2] = {0, 0}, b[2] = {0, 0}, c[2] = {0, 0};
-    bool exact = fits;
+    uint32_t a[2] = {0, 0}, b[2] = {0, 0}, c[2] = {0, 0}, mask = 0;
     auto part_of = [](float f) {
         uint16_t two;
         asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.0f), "f"(f));
@@ -324,7 +348,10 @@ __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __re
         const uint32_t second = part_of(left);
         const float rest = (left - value_of(second)) * (float)(1 << PART_SHIFT);
         const uint32_t third = part_of(rest);
-        exact = exact && (value_of(first) + value_of(second) + value_of(third) * (1.0f / (1 << PART_SHIFT))) * down == v[i];
+        if ((value_of(first) + value_of(second) + value_of(third) * (1.0f / (1 << PART_SHIFT))) * down != v[i]) {
+            mask |= 1u << i;
+            continue;
+        }
         a[i >> 2] |= first << (8 * (i & 3));
         b[i >> 2] |= second << (8 * (i & 3));
         c[i >> 2] |= third << (8 * (i & 3));
@@ -343,8 +370,7 @@ __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __re
         *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(tokens + row, q, tiles)) = four;
         *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(2 * tokens + row, q, tiles)) = four - 0x01010101u * PART_SHIFT;
     }
-    const bool all = __all_sync(0xffffffffu, exact);
-    if (lane == 0) lost[index] = all ? 0 : 1;
+    mx_note_lost(mask, held.raw, index, lost, (long long)rows * stretches);
 }
 
 // Blocks of a launch over `items` threads of work: they loop where that is more than 64 blocks an SM.
@@ -407,16 +433,16 @@ MRS_EXPORT int mrs_mxfp4_scale_range(const void* codes, const void* scales, void
     MRS_RETURN_LAUNCH_STATUS();
 }
 
-// x [rows, width] bfloat16 to halfs [rows, width] and exponents [rows] int32.  `zeros`: `zero_count` ints that are set to 0, or null.
-MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* exponents, long long rows, long long width, void* zeros, int zero_count,
+// x [rows, width] bfloat16 to halfs [rows, width], factors [rows] int32 and lost (mxfp4.cuh; rows * ceil(width / 256) stretches).  `zeros`: `zero_count` ints that are set to 0, or null.
+MRS_EXPORT int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* factors, void* lost, long long rows, long long width, void* zeros, int zero_count,
                                        void* stream) {
     if (rows == 0) return 0;
-    if (bad_sizes(rows, width) || (zero_count && !zeros) || rows > 0x7FFFFFFF || !x || !halfs || !exponents || (((uintptr_t)x | (uintptr_t)halfs) & 15) || ((uintptr_t)exponents & 3)) return MRS_BAD_ARGUMENT;
-    MRS_LAUNCH(rows_to_halfs_kernel, (unsigned)rows, THREADS, 0, stream, (const bf16*)x, (uint16_t*)halfs, (int*)exponents, width, (int*)zeros, zero_count);
+    if (bad_sizes(rows, width) || (zero_count && !zeros) || rows > 0x7FFFFFFF || !x || !halfs || !factors || !lost || (((uintptr_t)x | (uintptr_t)halfs) & 15) || (((uintptr_t)factors | (uintptr_t)lost) & 3)) return MRS_BAD_ARGUMENT;
+    MRS_LAUNCH(rows_to_halfs_kernel, (unsigned)rows, THREADS, 0, stream, (const bf16*)x, (uint16_t*)halfs, (int*)factors, (int*)lost, width, (int*)zeros, zero_count);
     MRS_RETURN_LAUNCH_STATUS();
 }
 
-// x [rows, width] bfloat16, rows up to `tokens` (16, 32 or 64), to parts [3 tokens, width], their scales and lost [rows * ceil(width / 256)] int32.
+// x [rows, width] bfloat16, rows up to `tokens` (16, 32 or 64), to parts [3 tokens, width], their scales and lost (as above).
 MRS_EXPORT int mrs_mxfp4_rows_to_parts(const void* x, void* parts, void* scales, void* lost, int rows, int width, int tokens, void* zeros, int zero_count,
                                        void* stream) {
     if (rows == 0) return 0;

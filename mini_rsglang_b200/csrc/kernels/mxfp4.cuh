@@ -57,6 +57,31 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t largest) {
     const int exponent = (int)(largest >> 23);
     return exponent == 255 ? 255u : (uint32_t)max(exponent - 2, 0);
 }
+// Elements of x that another form of its rows (halfs, parts) does not hold, noted by stretches of 256 elements: how many a stretch has, or
+// MX_LOST_ALL if more than MX_LOST, and behind all counts MX_LOST words a stretch, place in it << 16 | bfloat16.  The product adds theirs.
+constexpr int MX_LOST = 8, MX_LOST_ALL = 255;
+__host__ __device__ __forceinline__ const uint32_t* mx_lost_entries(const int* counts, long long stretches) {
+    return reinterpret_cast<const uint32_t*>(counts) + (stretches + 3) / 4 * 4;
+}
+// By a whole warp, eight elements a lane, those of `mask` lost; true if they are too many.
+__device__ __forceinline__ bool mx_note_lost(uint32_t mask, const uint4& raw, long long stretch, int* counts, long long stretches) {
+    const int lane = threadIdx.x & 31;
+    int found = 0;
+    if (__any_sync(0xffffffffu, mask != 0)) {
+        uint32_t* entries = const_cast<uint32_t*>(mx_lost_entries(counts, stretches)) + stretch * MX_LOST;
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t all = __ballot_sync(0xffffffffu, (mask >> i) & 1u);
+            const int index = found + __popc(all & ((1u << lane) - 1u));
+            if (((mask >> i) & 1u) && index < MX_LOST) entries[index] = (uint32_t)(lane * 8 + i) << 16 | ((words[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+            found += __popc(all);
+        }
+    }
+    if (lane == 0) counts[stretch] = found > MX_LOST ? MX_LOST_ALL : found;
+    return found > MX_LOST;
+}
+
 // 2^-(byte - 127) for bytes up to 252: an ordinary number.
 __device__ __forceinline__ float mx_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 // 2^(byte - 127); byte 0 is under the ordinary numbers, byte 255 gives NaN.

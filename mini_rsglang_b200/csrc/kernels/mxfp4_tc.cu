@@ -10,14 +10,17 @@
 //                    Making A is what a scheduler has to do for each MMA: halfs are a conversion and a multiplication for two codes (9
 //                    clocks for eight codes of a warp), bfloat16 goes through float32 (21 clocks).  So x comes as halfs, times a
 //                    power of two a row, from a kernel before (mxfp4.cu), and w becomes halfs times one power of two of the matrix;
-//                    both powers go into the results.  All of it is exact: where a row of x does not fit the halfs' range without
-//                    losing a bit, or the matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead.
+//                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
+//                    for halfs are added one by one to the sums (lost_products), and where there are too many of them, or the
+//                    matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead.
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
 //                    tensor memory (tcgen05.cp) stage by stage.
 //
 //   parts_kernel     x in bfloat16 once more, up to 64 rows: as three parts of E5M2 (mxfp4.cu), 3 x 64 columns of kind::mxf8f6f4 MMAs whose A
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
-//                    columns' sums are the result's.  Rows that three parts do not hold exactly are multiplied on the CUDA cores.
+//                    columns' sums are the result's.  Elements that three parts do not hold are added one by one as well; with more than
+//                    8 of them in 256 elements of a row the CUDA cores do the whole product.  (In a decode step of 64 tokens some element
+//                    of silu(gate) * up nearly always is 2^26 below its neighbours: one of them, and the CUDA cores took 25 ms a step.)
 //
 // Every wait is bounded (tma.cuh).
 #include <limits.h>
@@ -61,8 +64,10 @@ struct Shapes {
     int units;                  // stages of all tiles
     int early;                  // w was there before the kernel before this one: it may be fetched while that runs
     long long w_tiles_of_a_row, x_row_tiles;
-    const int* x_exponents;     // of x as halfs, a row each; null: x is bfloat16
+    const int* x_factors;       // of x as halfs (mxfp4.cu), a row each; null: x is bfloat16
     int w_exponent;             // halfs are made of w times 2^-w_exponent
+    const int* lost;            // elements that halfs or parts do not hold (mxfp4.cuh)
+    const uint8_t *w_codes, *w_scales;
     float* scratch;             // where tiles are shared, for every CTA the sums of its first and of its last tile
     int* arrived;               // for every tile how many CTAs have left their sums; zeros to begin with
 };
@@ -108,12 +113,43 @@ struct Walk {
     }
 };
 
+// A number a row, added to a column of sums in tensor memory, by a warp of its rows.
+__device__ __forceinline__ void add_to_column(uint32_t column, float more) {
+    float sum;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;" : "=f"(sum) : "r"(column) : "memory");
+    sum += more;
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n tcgen05.wait::st.sync.aligned;" ::"r"(column), "f"(sum) : "memory");
+}
+// The sum of a token's lost elements times a row of w, for a whole warp with a row a lane (rarely called: apart, so that it takes no
+// registers of others).  `counts` and `entries`: of the token's `stretches`.
+__device__ __noinline__ float lost_products(const int* counts, const uint32_t* entries, int stretches, const uint8_t* codes, const uint8_t* scales) {
+    const int lane = threadIdx.x & 31;
+    float sum = 0.0f;
+    for (int base = 0; base < stretches; base += 32) {
+        const int count = base + lane < stretches ? __ldcg(counts + base + lane) : 0;
+        for (uint32_t left = __ballot_sync(0xffffffffu, count != 0); left; left &= left - 1) {
+            const int at = __ffs(left) - 1, n = __shfl_sync(0xffffffffu, count, at);
+            for (int i = 0; i < n; ++i) {
+                const uint32_t entry = __ldcg(entries + (size_t)(base + at) * MX_LOST + i);
+                const size_t k = (size_t)(base + at) * STAGE_K + (entry >> 16);
+                const uint32_t code = codes[k >> 1] >> (4 * (k & 1)), size = code & 7u;
+                const float w = size < 2 ? 0.5f * size : __uint_as_float((126u + (size >> 1)) << 23 | (size & 1u) << 22);
+                const float scale = mx_scale(scales[(k >> 7) * MX_TILE_BYTES + ((k >> 5) & 3)]);
+                sum = fmaf(__uint_as_float(entry << 16), (code & 8u ? -w : w) * scale, sum);
+            }
+        }
+    }
+    return sum;
+}
+
 // An accumulator's results (lane: row of w, column: token) to memory.  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes
 // are those of its number modulo 4.  `halfs`: the rows' powers of two go into them (`factors`: 32 floats of shared memory for each warp).  A
 // tile that other CTAs share goes through scratch memory; `flag` is a word of shared memory.
+// `lost`: null, or elements of x are missing in the sums; with parts, a bit for each token that has some, in shared memory.
 template <int TOKENS, int WARPS, typename Out, bool PARTS = false>
-__device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors) {
-    constexpr int STEP = TOKENS < 32 || PARTS ? 16 : 32, GROUPS = WARPS / 4;              // of four warps, that take the columns in turn
+__device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors,
+                                                  const uint32_t* lost = nullptr) {
+    constexpr int STEP = TOKENS < 32 || WARPS <= 8 ? 16 : 32, GROUPS = WARPS / 4;       // columns at a time (32: registers spill in kernels of 19 warps); of four warps
     const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
     const int token0 = walk.token_tile * TOKENS, live = min(TOKENS, s.M - token0), tile = walk.n_tile * s.token_tiles + walk.token_tile;
     const uint32_t acc = accumulator + ((uint32_t)(quarter * 32) << 16);
@@ -122,8 +158,9 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
     auto finish = [&](int c, float (&v)[STEP]) {
         if (halfs) {                               // powers of two in the floats' range, a lane each, by way of shared memory
             const int lane = threadIdx.x & 31;
+            const int factor = lane < STEP && c + lane < live ? __ldcg(s.x_factors + token0 + c + lane) : -2 * s.w_exponent;
             __syncwarp();
-            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (c + lane < live ? __ldcg(s.x_exponents + token0 + c + lane) : -s.w_exponent)) << 23);
+            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (factor >> 1)) << 23);
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < STEP; e += 4) {
@@ -143,6 +180,24 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
             }
         }
     };
+    // Lost elements go into the sums in tensor memory, where each warp takes up the columns that it reads; of a shared tile, the CTA with its beginning.
+    if (lost && walk.from == 0) {
+#pragma unroll 1
+        for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
+            const int lane = threadIdx.x & 31;
+            int factor = 0;
+            if constexpr (PARTS) factor = (lost[c >> 5] >> ((c + lane) & 31)) & (lane < STEP ? 1u : 0u);
+            else if (lane < STEP && c + lane < live) factor = __ldcg(s.x_factors + token0 + c + lane);
+            for (uint32_t some = __ballot_sync(0xffffffffu, factor & 1); some; some &= some - 1) {
+                const int at = __ffs(some) - 1;
+                const long long of = n < s.N ? n : s.N - 1, token = token0 + c + at;
+                float more = lost_products(s.lost + token * s.depth, mx_lost_entries(s.lost, (long long)s.M * s.depth) + token * s.depth * MX_LOST, s.depth,
+                                           s.w_codes + of * (s.K >> 1), s.w_scales + mx_scale_offset(of, 0, s.w_tiles_of_a_row));
+                if constexpr (!PARTS) more *= __uint_as_float((uint32_t)(127 - s.w_exponent - (__shfl_sync(0xffffffffu, factor, at) >> 1)) << 23);
+                add_to_column(acc + c + at, more);
+            }
+        }
+    }
     // a CTA's sums of a shared tile: [column / 4][row] of four columns
     auto place_of = [&](int cta, bool head) { return reinterpret_cast<float4*>(s.scratch + ((size_t)cta * 2 + (head ? 1 : 0)) * (TOKENS * BM)) + row; };
     float4* mine = place_of(blockIdx.x, walk.from == 0);
@@ -335,14 +390,16 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         __syncwarp();
     }
     pdl_wait();
-    bool halfs = false;
-    if (s.x_exponents) {
-        bool fit = true;
+    bool halfs = false, lost = false;
+    if (s.x_factors) {
+        bool fit = true, some = false;
         for (int i = threadIdx.x; i < s.M; i += W_THREADS) {
-            const int e = s.x_exponents[i];
-            fit = fit && e != INT_MIN && e + s.w_exponent >= -126 && e + s.w_exponent <= 127;
+            const int factor = s.x_factors[i], e = factor >> 1;
+            fit = fit && factor != INT_MIN && e + s.w_exponent >= -126 && e + s.w_exponent <= 126;
+            some = some || (factor & 1);
         }
         halfs = __syncthreads_and(fit);
+        lost = __syncthreads_or(some) && halfs;
     }
 
     // Codes and x come by the hands of two warps: a wait for the makers must not hold up x, whose pieces free up MMA by MMA.
@@ -457,7 +514,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2 - MAKERS, halfs, flag, factors + (warp - 2 - MAKERS) * 32);
+            store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2 - MAKERS, halfs, flag, factors + (warp - 2 - MAKERS) * 32,
+                                                   lost ? reinterpret_cast<const uint32_t*>(s.lost) : nullptr);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
@@ -690,9 +748,9 @@ template <int TOKENS> constexpr size_t parts_smem() {
 
 template <int TOKENS, typename Out>
 __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
-                                                             const bf16* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ w_scales,
-                                                             const uint8_t* __restrict__ x_scales, const int* __restrict__ lost, int lost_count,
-                                                             Out* __restrict__ out, const Shapes s) {
+                                                             const bf16* __restrict__ x, const uint8_t* __restrict__ x_scales, Out* __restrict__ out, const Shapes s) {
+    __shared__ uint32_t lost_tokens[2];
+    static_assert(TOKENS <= 64);
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int STAGES = p_stages<TOKENS>(), N_COLUMNS = 3 * TOKENS, ACCUMULATOR = N_COLUMNS > 128 ? 192 : 128, SCALES_FIRST = 2 * ACCUMULATOR;
@@ -713,6 +771,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Walk walk(s);
 
+    if (threadIdx.x < 2) lost_tokens[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&full[i], 2);
@@ -740,7 +799,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
             tma_load_2d(w_ring + (slot * HALVES + h) * P_A_BYTES, &w_map, &full[slot], (piece * HALVES + h) * HALF_STAGE_K, n_tile * BM);
-        bulk_load(s_ring + slot * SLOT_SCALE_BYTES, w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + piece * HALVES) * MX_TILE_BYTES, W_SCALE_BYTES, &full[slot]);
+        bulk_load(s_ring + slot * SLOT_SCALE_BYTES, s.w_scales + ((size_t)n_tile * s.w_tiles_of_a_row + piece * HALVES) * MX_TILE_BYTES, W_SCALE_BYTES, &full[slot]);
     };
     const int ahead = s.early ? min(STAGES, walk.total * PIECES) : 0;
     if (warp == 2 + P_STORERS) {
@@ -750,11 +809,16 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     }
     pdl_wait();
     bool bad = false;
-    for (int i = threadIdx.x; i < lost_count; i += P_THREADS) bad = bad || lost[i] != 0;
+    for (int i = threadIdx.x; i < s.M * s.depth; i += P_THREADS) {
+        const int count = s.lost[i];
+        if (count == 0) continue;
+        bad = bad || count == MX_LOST_ALL;
+        atomicOr(&lost_tokens[i / s.depth >> 5], 1u << (i / s.depth & 31));
+    }
     const bool slow = __syncthreads_or(bad);
 
     if (slow) {
-        // Rows that three parts do not hold: a thread a row of w and every third token, the products of a bfloat16 and a code times its
+        // Too many elements that three parts do not hold: a thread a row of w and every third token, the products of a bfloat16 and a code times its
         // power of two exact, sums in float32.
         if (warp == 2 + P_STORERS) {                                                    // what was fetched has to have come before the CTA ends
             for (int i = 0; i < ahead; ++i) {
@@ -772,8 +836,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
             for (int token = part; token < s.M; token += LANES) {
                 float sum = 0.0f;
                 for (int block = 0; block < s.K / MX_BLOCK; ++block) {
-                    const uint4 c = *reinterpret_cast<const uint4*>(codes + n * code_pitch + block * 16);
-                    const float scale = mx_scale(w_scales[mx_scale_offset(n, block >> 2, s.w_tiles_of_a_row) + (block & 3)]);
+                    const uint4 c = *reinterpret_cast<const uint4*>(s.w_codes + n * code_pitch + block * 16);
+                    const float scale = mx_scale(s.w_scales[mx_scale_offset(n, block >> 2, s.w_tiles_of_a_row) + (block & 3)]);
                     const uint32_t words[4] = {c.x, c.y, c.z, c.w};
                     const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)token * s.K + block * MX_BLOCK);
 #pragma unroll
@@ -874,7 +938,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr);
+            store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr, lost_tokens);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
@@ -927,7 +991,7 @@ int launch_weights(const void* x, const void* x_halfs, const void* codes, const 
     int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
     if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
     halfs_map = x_map;
-    if (!code && s.x_exponents) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
+    if (!code && s.x_factors) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
     if (code) return code;
     static PerDevice configured;
     if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
@@ -948,16 +1012,15 @@ int launch_both(const void* x_codes, const void* x_scales, const void* codes, co
 }
 
 template <int TOKENS, typename Out>
-int launch_parts(const void* x, const void* parts, const void* x_scales, const void* lost, const void* codes, const void* scales, void* out, Shapes s, int ctas,
-                 void* stream) {
+int launch_parts(const void* x, const void* parts, const void* x_scales, void* out, Shapes s, int ctas, void* stream) {
     CUtensorMap w_map, x_map;
-    int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, s.K / 2, s.K, s.N, HALF_STAGE_K, BM);
+    int code = make_map(&w_map, s.w_codes, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, s.K / 2, s.K, s.N, HALF_STAGE_K, BM);
     if (!code) code = make_map(&x_map, parts, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K, s.K, 3 * TOKENS, HALF_STAGE_K, 3 * TOKENS);
     if (code) return code;
     static PerDevice configured;
     if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
-    return launch_run(parts_kernel<TOKENS, Out>, configured, P_THREADS, ctas, parts_smem<TOKENS>(), stream, w_map, x_map, (const bf16*)x, (const uint8_t*)codes,
-                      (const uint8_t*)scales, (const uint8_t*)x_scales, (const int*)lost, s.M * s.depth, (Out*)out, s);
+    return launch_run(parts_kernel<TOKENS, Out>, configured, P_THREADS, ctas, parts_smem<TOKENS>(), stream, w_map, x_map, (const bf16*)x, (const uint8_t*)x_scales,
+                      (Out*)out, s);
 }
 
 bool bad(const void* x, const void* codes, const void* scales, const void* out, int out_f32, int M, int N, int K, int tokens, int ctas, const void* scratch,
@@ -969,19 +1032,22 @@ bool bad(const void* x, const void* codes, const void* scales, const void* out, 
 
 }  // namespace
 
-// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16, also as halfs with exponents (mxfp4.cu) or null; w as in mxfp4.cuh, whose blocks
+// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16, also as halfs with factors and lost elements (mxfp4.cu) or null; w as in mxfp4.cuh, whose blocks
 // other than zeros have scales of 2^(w_exponent - 23) to 2^(w_exponent + 13) if halfs are given.  `tokens` (16, 32, 64, 128, 192): of a tile,
 // below 128 only if they are all.  `ctas`: at most the GPU's SMs and the stages of 256 elements of K of all tiles.  With `scratch` (2 ctas
 // x tokens x 128 floats) and `arrived` (an int a tile, zero) the stages are cut into equal runs, without whole tiles are.  `early`: nothing
 // that still runs when this kernel starts writes w.
-MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const void* x_exponents, int w_exponent, const void* codes, const void* scales,
+MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const void* x_factors, const void* lost, int w_exponent, const void* codes, const void* scales,
                                       void* out, int out_f32, int M, int N, int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
     if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived)) return MRS_BAD_ARGUMENT;
-    if ((x_halfs == nullptr) != (x_exponents == nullptr) || ((uintptr_t)x_halfs & 15) || ((uintptr_t)x_exponents & 3)) return MRS_BAD_ARGUMENT;
+    if ((x_halfs == nullptr) != (x_factors == nullptr) || (x_halfs == nullptr) != (lost == nullptr) || ((uintptr_t)x_halfs & 15) ||
+        (((uintptr_t)x_factors | (uintptr_t)lost) & 3))
+        return MRS_BAD_ARGUMENT;
     Shapes s = {};
     s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K);
-    s.x_exponents = (const int*)x_exponents, s.w_exponent = w_exponent, s.scratch = (float*)scratch, s.arrived = (int*)arrived;
+    s.x_factors = (const int*)x_factors, s.w_exponent = w_exponent, s.lost = (const int*)lost;
+    s.w_codes = (const uint8_t*)codes, s.w_scales = (const uint8_t*)scales, s.scratch = (float*)scratch, s.arrived = (int*)arrived;
 #define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_weights<T, float>(x, x_halfs, codes, scales, out, s, ctas, stream) : launch_weights<T, bf16>(x, x_halfs, codes, scales, out, s, ctas, stream)
     MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
 #undef MRS_TOKENS
@@ -1010,7 +1076,8 @@ MRS_EXPORT int mrs_mxfp4_parts_rows(const void* x, const void* parts, const void
         return MRS_BAD_ARGUMENT;
     Shapes s = {};
     s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
-#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_parts<T, float>(x, parts, x_scales, lost, codes, scales, out, s, ctas, stream) : launch_parts<T, bf16>(x, parts, x_scales, lost, codes, scales, out, s, ctas, stream)
+    s.lost = (const int*)lost, s.w_codes = (const uint8_t*)codes, s.w_scales = (const uint8_t*)scales;
+#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_parts<T, float>(x, parts, x_scales, out, s, ctas, stream) : launch_parts<T, bf16>(x, parts, x_scales, out, s, ctas, stream)
     MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64);
 #undef MRS_TOKENS
     return MRS_BAD_ARGUMENT;

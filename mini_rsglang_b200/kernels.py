@@ -2573,8 +2573,8 @@ _MXFP4_SIGNATURES = {
     "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
     "mrs_mxfp4_few_rows_cluster": [_c_int, _c_int],
     "mrs_mxfp4_scale_range": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
-    "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
-    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp,
+    "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
+    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp,
                                _c_int, _c_vp],
     "mrs_mxfp4_rows_to_parts": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_parts_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp],
@@ -2617,6 +2617,11 @@ def _stream_here(index: int) -> int:
 def _mxfp4_bytes(rows: int, width: int) -> tuple[int, int]:
     """(bytes of codes, bytes of scales): scales in tiles of 128 rows x 4 blocks, an even number of tiles a row."""
     return rows * (width >> 1), -(-rows // 128) * (-(-width // 256) * 1024)
+
+
+def _mxfp4_lost_bytes(stretches: int) -> int:
+    """Of the elements that another form of x does not hold: a count and eight words for 256 elements."""
+    return -(-stretches // 4) * 16 + 32 * stretches
 
 
 class Mxfp4:
@@ -2837,9 +2842,10 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
             x_bytes, side_bytes = _mxfp4_bytes(m, k)
         elif kind == "parts":
             x_bytes, scale_bytes = 3 * tokens * k, -(-3 * tokens // 128) * 1024 * depth
-            side_bytes = scale_bytes + -(-m * depth // 4) * 16
+            side_bytes = scale_bytes + _mxfp4_lost_bytes(m * depth)
         else:
-            x_bytes, side_bytes = 2 * m * k, -(-m // 4) * 16
+            x_bytes, factor_bytes = 2 * m * k, -(-m // 4) * 16
+            side_bytes = factor_bytes + _mxfp4_lost_bytes(m * depth)
         scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
         work = torch.empty(x_bytes + side_bytes + scratch_bytes + 4 * tiles, dtype=torch.uint8, device=x.device)
         made = work.data_ptr()
@@ -2857,7 +2863,8 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
                                                     scratch, arrived, early, stream)
         else:
             fits = weight.half_exponent is not None
-            code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, m, k, arrived, tiles, stream)
-            code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), made if fits else None, side if fits else None, weight.half_exponent or 0, w_codes,
-                                                      w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived, early, stream)
+            lost = side + factor_bytes
+            code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, lost, m, k, arrived, tiles, stream)
+            code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), made if fits else None, side if fits else None, lost if fits else None,
+                                                      weight.half_exponent or 0, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived, early, stream)
     _mxfp4_check(code, "mxfp4_gemm")

@@ -215,6 +215,32 @@ def test_rows_that_halfs_do_not_hold(kind, plan, quantise):
     check_product(x.bfloat16(), weight, w, quantise, plan, kind)
 
 
+@pytest.mark.parametrize("plan", [("parts", 16, 2, False), ("parts", 32, 4, True), ("parts", 64, 1, False), ("parts", 64, 7, True), ("many", 16, 2, True), ("many", 32, 1, False),
+                                  ("many", 64, 2, False), ("many", 128, 3, True), ("many", 192, 2, True), ("many", 192, 1, False)])
+@pytest.mark.parametrize("count", [1, 8, 9, 200])
+def test_elements_far_below_the_others(plan, count):
+    """What stands beside much larger elements and is small enough for no form of x to hold both, `count` in 256: a few are added one
+    by one, many make another kernel or another path of it.  The large ones meet codes of zero, so that the result is the small ones'."""
+    m, n, k = 13, 150, 896
+    g = torch.Generator(device=DEV).manual_seed(count)
+    codes, scales, w = random_matrix(g, n, k)
+    x = torch.zeros(m, k, device=DEV)
+    codes = codes.clone()
+    for start in range(0, k, 256):
+        width = min(256, k - start)
+        order = torch.randperm(width, device=DEV, generator=g)
+        small, large = start + order[2:2 + min(count, width - 2)], start + order[:2]
+        rows = torch.arange(m, device=DEV) % 3 != 1                      # every third row has none of them
+        x[:, small] = rows[:, None] * torch.randn(m, small.numel(), device=DEV, generator=g) * 2.0 ** -40
+        x[:, large] = torch.randn(m, 2, device=DEV, generator=g)
+        for column in large.tolist():
+            codes[:, column // 2] &= 0x0F if column % 2 else 0xF0
+    x[:, -2:] = torch.tensor([1.0, 2.0 ** -40], device=DEV) * torch.randn(m, 2, device=DEV, generator=g)             # and the row's last two
+    codes[:, -1] = 0x50
+    w = plain_values(codes, scales)
+    check_product(x.bfloat16(), kernels.mxfp4_matrix(codes, scales), w, False, plan, f"{count}")
+
+
 @pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS for q in (False, True) if takes(plan, 11, 128, q)])
 @pytest.mark.parametrize("kind", ["wide", "nan", "zero_blocks", "small", "large", "unsettled"])
 def test_scales_of_every_size(kind, plan, quantise):
