@@ -150,6 +150,7 @@ template <int TOKENS, int WARPS, typename Out, bool PARTS = false>
 __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors,
                                                   const uint32_t* lost = nullptr) {
     constexpr int STEP = TOKENS < 32 || WARPS <= 8 ? 16 : 32, GROUPS = WARPS / 4;       // columns at a time (32: registers spill in kernels of 19 warps); of four warps
+    constexpr int TOGETHER = PARTS || (STEP == 16 && WARPS > 8) ? 4 : 2;
     const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
     const int token0 = walk.token_tile * TOKENS, live = min(TOKENS, s.M - token0), tile = walk.n_tile * s.token_tiles + walk.token_tile;
     const uint32_t acc = accumulator + ((uint32_t)(quarter * 32) << 16);
@@ -235,18 +236,27 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
 #pragma unroll 1
     for (int c = (index >> 2) * STEP; c < live; c += GROUPS * STEP) {
         float v[STEP];
+        // in the order of K, the first CTA's at the end of its run; TOGETHER pieces on the way at a time
 #pragma unroll 1
-        for (int cta = first; cta <= last; ++cta) {                             // in the order of K; the first's is at the end of its run
-            const float4* from = place_of(cta, cta == first) + (c >> 2) * BM;
-            float4 piece[STEP / 4];
+        for (int cta = first; cta <= last; cta += TOGETHER) {
+            float4 piece[TOGETHER][STEP / 4];
 #pragma unroll
-            for (int e = 0; e < STEP / 4; ++e) piece[e] = __ldcg(from + e * BM);
+            for (int t = 0; t < TOGETHER; ++t) {
+                const float4* from = place_of(min(cta + t, last), cta + t == first) + (c >> 2) * BM;
 #pragma unroll
-            for (int e = 0; e < STEP / 4; ++e) {
-                v[4 * e] = cta == first ? piece[e].x : v[4 * e] + piece[e].x;
-                v[4 * e + 1] = cta == first ? piece[e].y : v[4 * e + 1] + piece[e].y;
-                v[4 * e + 2] = cta == first ? piece[e].z : v[4 * e + 2] + piece[e].z;
-                v[4 * e + 3] = cta == first ? piece[e].w : v[4 * e + 3] + piece[e].w;
+                for (int e = 0; e < STEP / 4; ++e) piece[t][e] = __ldcg(from + e * BM);
+            }
+#pragma unroll
+            for (int t = 0; t < TOGETHER; ++t) {
+                if (cta + t > last) break;
+                const bool begin = cta + t == first;
+#pragma unroll
+                for (int e = 0; e < STEP / 4; ++e) {
+                    v[4 * e] = begin ? piece[t][e].x : v[4 * e] + piece[t][e].x;
+                    v[4 * e + 1] = begin ? piece[t][e].y : v[4 * e + 1] + piece[t][e].y;
+                    v[4 * e + 2] = begin ? piece[t][e].z : v[4 * e + 2] + piece[t][e].z;
+                    v[4 * e + 3] = begin ? piece[t][e].w : v[4 * e + 3] + piece[t][e].w;
+                }
             }
         }
         finish(c, v);
@@ -749,7 +759,7 @@ template <int TOKENS> constexpr size_t parts_smem() {
 template <int TOKENS, typename Out>
 __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                              const bf16* __restrict__ x, const uint8_t* __restrict__ x_scales, Out* __restrict__ out, const Shapes s) {
-    __shared__ uint32_t lost_tokens[2];
+    __shared__ uint32_t lost_tokens[3];             // a bit a token with elements to add; whether there are too many
     static_assert(TOKENS <= 64);
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -771,7 +781,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Walk walk(s);
 
-    if (threadIdx.x < 2) lost_tokens[threadIdx.x] = 0;
+    if (threadIdx.x < 3) lost_tokens[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&full[i], 2);
@@ -808,56 +818,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
         __syncwarp();
     }
     pdl_wait();
-    bool bad = false;
-    for (int i = threadIdx.x; i < s.M * s.depth; i += P_THREADS) {
-        const int count = s.lost[i];
-        if (count == 0) continue;
-        bad = bad || count == MX_LOST_ALL;
-        atomicOr(&lost_tokens[i / s.depth >> 5], 1u << (i / s.depth & 31));
-    }
-    const bool slow = __syncthreads_or(bad);
-
-    if (slow) {
-        // Too many elements that three parts do not hold: a thread a row of w and every third token, the products of a bfloat16 and a code times its
-        // power of two exact, sums in float32.
-        if (warp == 2 + P_STORERS) {                                                    // what was fetched has to have come before the CTA ends
-            for (int i = 0; i < ahead; ++i) {
-                if (elect_one()) mbar_arrive(&full[i]);
-                __syncwarp();
-                warp_wait(&full[i], 0);
-            }
-        }
-        const long long code_pitch = s.K >> 1;
-        constexpr int LANES = P_THREADS / BM;                                           // threads a row
-        const int part = threadIdx.x / BM;
-        for (int tile = blockIdx.x; part < LANES && tile < s.units / s.depth; tile += gridDim.x) {
-            const long long n = (long long)tile * BM + (threadIdx.x & (BM - 1));
-            if (n >= s.N) continue;
-            for (int token = part; token < s.M; token += LANES) {
-                float sum = 0.0f;
-                for (int block = 0; block < s.K / MX_BLOCK; ++block) {
-                    const uint4 c = *reinterpret_cast<const uint4*>(s.w_codes + n * code_pitch + block * 16);
-                    const float scale = mx_scale(s.w_scales[mx_scale_offset(n, block >> 2, s.w_tiles_of_a_row) + (block & 3)]);
-                    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-                    const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)token * s.K + block * MX_BLOCK);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t h[4];
-                        mx_decode_8(words[i], h);
-                        const uint4 raw = from[i];
-                        const uint32_t pairs[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            const float2 w = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
-                            sum = fmaf(__uint_as_float(pairs[p] << 16), w.x * scale, sum);
-                            sum = fmaf(__uint_as_float(pairs[p] & 0xFFFF0000u), w.y * scale, sum);
-                        }
-                    }
-                }
-                out[(size_t)token * s.N + n] = from_float<Out>(sum);
-            }
-        }
-    } else if (warp == 0) {
+    if (warp == 0) {
         const bool leader = elect_one();
         bool alive = true;
         int slot = 0;
@@ -934,11 +895,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
             __syncwarp();
         }
     } else {
+        for (int i = threadIdx.x - 64; i < s.M * s.depth; i += P_STORERS * 32) {
+            const int count = __ldcg(s.lost + i);
+            if (count == MX_LOST_ALL) atomicOr(&lost_tokens[2], 1u);
+            if (count != 0) atomicOr(&lost_tokens[i / s.depth >> 5], 1u << (i / s.depth & 31));
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(P_STORERS * 32) : "memory");
         for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr, lost_tokens);
+            if (lost_tokens[2] == 0)
+                store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr, lost_tokens);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
@@ -950,6 +918,40 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     if (warp == 1) {
         tcgen05_fence_after_sync();
         tmem_dealloc(tmem, TMEM_COLUMNS);
+    }
+    if (lost_tokens[2] != 0) {
+        // Too many elements that three parts do not hold: a thread a row of w and every third token, the products of a bfloat16 and a code
+        // times its power of two exact, sums in float32.
+        const long long code_pitch = s.K >> 1;
+        constexpr int LANES = P_THREADS / BM;                                           // threads a row
+        const int part = threadIdx.x / BM;
+        for (int tile = blockIdx.x; part < LANES && tile < s.units / s.depth; tile += gridDim.x) {
+            const long long n = (long long)tile * BM + (threadIdx.x & (BM - 1));
+            if (n >= s.N) continue;
+            for (int token = part; token < s.M; token += LANES) {
+                float sum = 0.0f;
+                for (int block = 0; block < s.K / MX_BLOCK; ++block) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(s.w_codes + n * code_pitch + block * 16);
+                    const float scale = mx_scale(s.w_scales[mx_scale_offset(n, block >> 2, s.w_tiles_of_a_row) + (block & 3)]);
+                    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+                    const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)token * s.K + block * MX_BLOCK);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[4];
+                        mx_decode_8(words[i], h);
+                        const uint4 raw = from[i];
+                        const uint32_t pairs[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            const float2 w = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
+                            sum = fmaf(__uint_as_float(pairs[p] << 16), w.x * scale, sum);
+                            sum = fmaf(__uint_as_float(pairs[p] & 0xFFFF0000u), w.y * scale, sum);
+                        }
+                    }
+                }
+                out[(size_t)token * s.N + n] = from_float<Out>(sum);
+            }
+        }
     }
 }
 
