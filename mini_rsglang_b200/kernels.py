@@ -2763,13 +2763,14 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
     """How a product is launched: ("few", CTAs of a cluster), or ("parts" | "many", tokens of a tile, CTAs, whether tiles are shared).
 
     Measured on a B200 (us, weights [n, k] from a cold L2, the kernel that prepares x included; few / parts / many):
-      24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 17.4 / 22.1, 16 rows - / 17.0 / 21.6, 24 rows - / 20.0 / 25.3,
-                       64 rows - / 24.2 / 30.3
-      4,096 x 12,288   1 row 9.8 / 14.8 / 19.0, 8 rows (x in four CTAs) 18.3 / 15.5 / 20.2
-      5,120 x 17,408   4 rows (x in two CTAs) 15.1 / 17.8 / 24.4, 8 rows (in four) 27.9 / 18.0 / 25.1
-    and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.8 / 14.0, 8 rows 16.4 / 14.6; 12,963 x 2,368 1 row 7.6 / 6.8; 4,096 x 12,288 4 rows 13.8 / 15.2;
-      8 rows: 6,144 x 4,096 8.9 / 8.1, 2,560 x 9,728 11.8 / 13.2, 4,096 x 2,560 6.8 / 6.8, 1,000 x 2,048 4.8 / 6.1."""
-    if m <= (8 if not quantise or n * k <= 3 << 23 else 4 if n <= 8192 else 0):
+      24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 16.9 / 22.1, 16 rows - / 16.6 / 21.6, 32 rows - / 19.5 / 25.3,
+                       64 rows - / 23.8 / 30.3
+      4,096 x 12,288   1 row 9.8 / 14.4 / 19.0, 8 rows (x in four CTAs) 18.3 / 14.5 / 20.2
+      5,120 x 17,408   4 rows (x in two CTAs) 15.1 / 17.1 / 24.4, 8 rows (in four) 27.9 / 17.1 / 25.1
+    and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.8 / 13.7, 8 rows 16.4 / 13.7;
+      12,963 x 2,368 1 row 7.6 / 6.8; 4,096 x 12,288 1 row 10.5 / 13.1, 4 rows 13.8 / 13.1;
+      8 rows: 6,144 x 4,096 8.9 / 7.6, 2,560 x 9,728 11.8 / 13.2, 4,096 x 2,560 6.8 / 6.8, 1,000 x 2,048 4.8 / 6.1."""
+    if m <= (8 if not quantise or n * k <= 3 << 22 else 4 if n <= 8192 else 0):
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
         if 0 < cluster <= 2:
             return ("few", cluster)
@@ -2779,21 +2780,26 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
         widths = (16 if m <= 16 else 32 if m <= 32 else 64 if m <= 64 else 128,)
     else:
         widths = (192, 128)
-    meeting = 36 if quantise else 6 if widths[0] <= 32 else 10
+    if quantise:
+        meeting = 30 if widths[0] <= 32 else 33 if widths[0] <= 64 else 48
+    else:
+        meeting = 6 if widths[0] <= 32 else 10 if widths[0] <= 64 else 11
     tokens = min(widths, key=lambda t: min(_mxfp4_stages(m, n, k, t, sms, meeting)) * (130 + t))          # a stage: 1.04 us with 128, 1.29 with 192
     return ("many", *mxfp4_tiles(m, n, k, tokens, sms, meeting))
 
 
 def _mxfp4_stages(m: int, n: int, k: int, tokens: int, sms: int, meeting: int) -> tuple[float, float]:
-    """The stages of 256 elements of K that the product takes with whole tiles and with shared ones."""
+    """The stages of 256 elements of K that the product takes with whole tiles and with shared ones, these only if half of L2 holds x."""
     tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
-    return -(-tiles // sms) * depth, 1.05 * tiles * depth / sms + meeting
+    return -(-tiles // sms) * depth, 1.05 * tiles * depth / sms + meeting if 2 * m * k <= 64 << 20 else math.inf
 
 
 def mxfp4_tiles(m: int, n: int, k: int, tokens: int, sms: int, meeting: int, shared: bool | None = None) -> tuple:
     """(tokens of a tile, CTAs, whether tiles are shared) of tiles of 128 rows of weights x `tokens` on as many CTAs as there are SMs.
     Shared tiles cost a meeting of their CTAs, as long as `meeting` stages, and 1/20 of all since CTAs at work at the same time are further
-    apart in the matrix.  Measured whole / shared: 24,576 x 4,096 64 rows 34.5 / 30.2 us, 192 rows 43.0 / 41.4, 2,048 rows 305 / 310."""
+    apart in the matrix; and an x longer than half of L2 would not stay there (3,357 rows of 14,912 with 3,256 outputs: 352 / 406 us).
+    Measured whole / shared, K 4,096: 24,576 outputs, 16 rows 18.4 / 16.6 us, 192 rows 43.0 / 41.4, 2,048 rows 305 / 310; 6,144 outputs, 128
+    rows 20.9 / 23.1; K 12,288: 4,096 outputs, 16 rows 20.9 / 14.0, 333 rows 54.0 / 46.7."""
     tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
     if shared is None:
         whole, together = _mxfp4_stages(m, n, k, tokens, sms, meeting)
