@@ -373,6 +373,12 @@ __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __re
     mx_note_lost(mask, held.raw, index, lost, (long long)rows * stretches);
 }
 
+__global__ void __launch_bounds__(THREADS) clear_kernel(int* __restrict__ zeros, int count) {
+    pdl_launch_dependents();
+    pdl_wait();
+    clear(zeros, count);
+}
+
 // Blocks of a launch over `items` threads of work: they loop where that is more than 64 blocks an SM.
 int blocks_for(long long items) {
     const long long want = (items + THREADS - 1) / THREADS, most = (long long)mrs_sm_count() * 64;
@@ -452,6 +458,14 @@ MRS_EXPORT int mrs_mxfp4_rows_to_parts(const void* x, void* parts, void* scales,
     const int stretches = (width + 255) / 256;
     MRS_LAUNCH(rows_to_parts_kernel, (rows * stretches + THREADS / 32 - 1) / (THREADS / 32), THREADS, 0, stream, (const bf16*)x, (uint8_t*)parts, (uint8_t*)scales,
                (int*)lost, rows, width, tokens, stretches, (int*)zeros, zero_count);
+    MRS_RETURN_LAUNCH_STATUS();
+}
+
+// `zero_count` ints that are set to 0.
+MRS_EXPORT int mrs_mxfp4_clear(void* zeros, int zero_count, void* stream) {
+    if (zero_count == 0) return 0;
+    if (zero_count < 0 || !zeros || ((uintptr_t)zeros & 3)) return MRS_BAD_ARGUMENT;
+    MRS_LAUNCH(clear_kernel, blocks_for(zero_count), THREADS, 0, stream, (int*)zeros, zero_count);
     MRS_RETURN_LAUNCH_STATUS();
 }
 

@@ -28,6 +28,15 @@
 #include "mxfp4.cuh"
 #include "tcgen05.cuh"
 
+// What is made of x, and counters set to zero on the way (mxfp4.cu).
+extern "C" {
+long long mrs_mxfp4_scale_bytes(long long rows, long long width);
+int mrs_mxfp4_quantise(int is_bf16, const void* x, void* codes, void* scales, long long rows, long long width, void* zeros, int zero_count, void* stream);
+int mrs_mxfp4_rows_to_halfs(const void* x, void* halfs, void* factors, void* lost, long long rows, long long width, void* zeros, int zero_count, void* stream);
+int mrs_mxfp4_rows_to_parts(const void* x, void* parts, void* scales, void* lost, int rows, int width, int tokens, void* zeros, int zero_count, void* stream);
+int mrs_mxfp4_clear(void* zeros, int zero_count, void* stream);
+}
+
 namespace {
 
 constexpr int BM = 128;                            // rows of w of a tile
@@ -988,28 +997,27 @@ int launch_run(void (*kernel)(KernelArgs...), PerDevice& configured, int threads
 }
 
 template <int TOKENS, typename Out>
-int launch_weights(const void* x, const void* x_halfs, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
+int launch_weights(const void* x, const void* x_halfs, void* out, Shapes s, int ctas, void* stream) {
     CUtensorMap w_map, x_map, halfs_map;
-    int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
+    int code = make_map(&w_map, s.w_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
     if (!code) code = make_map(&x_map, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
     halfs_map = x_map;
     if (!code && s.x_factors) code = make_map(&halfs_map, x_halfs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (long long)s.K * 2, s.K, s.M, PIECE_K, TOKENS);
     if (code) return code;
     static PerDevice configured;
     if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
-    return launch_run(weights_kernel<TOKENS, Out>, configured, W_THREADS, ctas, weights_smem<TOKENS>(), stream, w_map, x_map, halfs_map, (const uint8_t*)scales,
-                      (Out*)out, s);
+    return launch_run(weights_kernel<TOKENS, Out>, configured, W_THREADS, ctas, weights_smem<TOKENS>(), stream, w_map, x_map, halfs_map, s.w_scales, (Out*)out, s);
 }
 template <int TOKENS, typename Out>
-int launch_both(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, Shapes s, int ctas, void* stream) {
+int launch_both(const void* x_codes, const void* x_scales, void* out, Shapes s, int ctas, void* stream) {
     CUtensorMap w_map, x_map;
-    int code = make_map(&w_map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
+    int code = make_map(&w_map, s.w_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.N, 128, BM);
     if (!code) code = make_map(&x_map, x_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.K / 2, s.K / 2, s.M, 128, TOKENS);
     if (code) return code;
     static PerDevice configured;
     s.x_row_tiles = (s.M + 127) / 128;
     if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
-    return launch_run(both_kernel<TOKENS, Out>, configured, B_THREADS, ctas, both_smem<TOKENS>(), stream, w_map, x_map, (const uint8_t*)scales,
+    return launch_run(both_kernel<TOKENS, Out>, configured, B_THREADS, ctas, both_smem<TOKENS>(), stream, w_map, x_map, s.w_scales,
                       (const uint8_t*)x_scales, (Out*)out, s);
 }
 
@@ -1025,62 +1033,72 @@ int launch_parts(const void* x, const void* parts, const void* x_scales, void* o
                       (Out*)out, s);
 }
 
-bool bad(const void* x, const void* codes, const void* scales, const void* out, int out_f32, int M, int N, int K, int tokens, int ctas, const void* scratch,
-         const void* arrived) {
-    return M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || !x || !codes || !scales || !out ||
-           (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1)) || ctas < 1 || (tokens < 128 && M > tokens) ||
-           (scratch == nullptr) != (arrived == nullptr) || (((uintptr_t)scratch | (uintptr_t)arrived) & 3);
-}
+// What a product needs beside its operands, in one buffer: what x becomes and what belongs to it, elements that are lost on the way, and, where
+// tiles are shared, sums and counts.  All offsets are multiples of 16 bytes.
+enum Form { PARTS = 0, WEIGHTS = 1, BOTH = 2 };
+struct Work {
+    long long side = 0, lost = 0, scratch = 0, arrived = 0, tiles = 0, bytes = 0;
+    Work(int form, long long M, long long N, long long K, int tokens, int ctas, int shared) {
+        const long long depth = (K + STAGE_K - 1) / STAGE_K;
+        side = form == PARTS ? 3 * tokens * K : form == WEIGHTS ? 2 * M * K : M * (K / 2);
+        lost = side + (form == PARTS ? (3 * tokens + 127) / 128 * SCALE_BYTES * depth : form == WEIGHTS ? (M + 3) / 4 * 16 : mrs_mxfp4_scale_bytes(M, K));
+        scratch = lost + (form == BOTH ? 0 : (M * depth + 3) / 4 * 16 + M * depth * MX_LOST * 4);
+        arrived = scratch + (shared ? 2ll * ctas * tokens * BM * 4 : 0);
+        tiles = shared ? (N + BM - 1) / BM * ((M + tokens - 1) / tokens) : 0;
+        bytes = arrived + 4 * tiles;
+    }
+};
 
 }  // namespace
 
-// out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16, also as halfs with factors and lost elements (mxfp4.cu) or null; w as in mxfp4.cuh, whose blocks
-// other than zeros have scales of 2^(w_exponent - 23) to 2^(w_exponent + 13) if halfs are given.  `tokens` (16, 32, 64, 128, 192): of a tile,
-// below 128 only if they are all.  `ctas`: at most the GPU's SMs and the stages of 256 elements of K of all tiles.  With `scratch` (2 ctas
-// x tokens x 128 floats) and `arrived` (an int a tile, zero) the stages are cut into equal runs, without whole tiles are.  `early`: nothing
-// that still runs when this kernel starts writes w.
-MRS_EXPORT int mrs_mxfp4_weights_rows(const void* x, const void* x_halfs, const void* x_factors, const void* lost, int w_exponent, const void* codes, const void* scales,
-                                      void* out, int out_f32, int M, int N, int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
-    if (M == 0 || N == 0) return 0;
-    if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived)) return MRS_BAD_ARGUMENT;
-    if ((x_halfs == nullptr) != (x_factors == nullptr) || (x_halfs == nullptr) != (lost == nullptr) || ((uintptr_t)x_halfs & 15) ||
-        (((uintptr_t)x_factors | (uintptr_t)lost) & 3))
-        return MRS_BAD_ARGUMENT;
-    Shapes s = {};
-    s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K);
-    s.x_factors = (const int*)x_factors, s.w_exponent = w_exponent, s.lost = (const int*)lost;
-    s.w_codes = (const uint8_t*)codes, s.w_scales = (const uint8_t*)scales, s.scratch = (float*)scratch, s.arrived = (int*)arrived;
-#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_weights<T, float>(x, x_halfs, codes, scales, out, s, ctas, stream) : launch_weights<T, bf16>(x, x_halfs, codes, scales, out, s, ctas, stream)
-    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
-#undef MRS_TOKENS
-    return MRS_BAD_ARGUMENT;
-}
+// Bytes of the buffer for a product of `form` (0: x in parts, 1: as halfs or as it is, 2: in 4 bits).
+MRS_EXPORT long long mrs_mxfp4_work_bytes(int form, int M, int N, int K, int tokens, int ctas, int shared) { return Work(form, M, N, K, tokens, ctas, shared).bytes; }
 
-// The same with x in 4 bits.
-MRS_EXPORT int mrs_mxfp4_both_rows(const void* x_codes, const void* x_scales, const void* codes, const void* scales, void* out, int out_f32, int M, int N,
-                                   int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
+// out [M, N] bfloat16 or float32 (`out_f32`) = x [M, K] bfloat16 . w [N, K]^T, w as in mxfp4.cuh.  `tokens` of a tile: 16, 32, 64, 128 or 192, below
+// 128 only if they are all; with parts (K a multiple of 128) at most 64.  `ctas`: at most the GPU's SMs, and the tiles or, if they are `shared`,
+// cut into equal runs, the stages of 256 elements of K of all of them.  `fits`: w's blocks other than zeros have scales of 2^(w_exponent - 23) to
+// 2^(w_exponent + 13), so that halfs hold them.  `early`: nothing that still runs when the product starts writes w.
+MRS_EXPORT int mrs_mxfp4_rows(int form, const void* x, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int tokens, int ctas,
+                              int shared, int fits, int w_exponent, int early, void* work, void* stream) {
     if (M == 0 || N == 0) return 0;
-    if (bad(x_codes, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived) || !x_scales || ((uintptr_t)x_scales & 15)) return MRS_BAD_ARGUMENT;
+    if (M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || !x || !codes || !scales || !out || !work || ctas < 1 || (tokens < 128 && M > tokens) ||
+        (tokens != 16 && tokens != 32 && tokens != 64 && tokens != 128 && tokens != 192) ||
+        (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)work) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1)) || form < PARTS || form > BOTH ||
+        (form == PARTS && (K % HALF_STAGE_K || ((uintptr_t)codes & 31) || tokens > 64)))
+        return MRS_BAD_ARGUMENT;
+    const Work at(form, M, N, K, tokens, ctas, shared);
+    if (at.tiles > 0x7FFFFFFF) return MRS_BAD_ARGUMENT;
+    char* base = (char*)work;
+    void *side = base + at.side, *lost = base + at.lost, *scratch = shared ? base + at.scratch : nullptr, *arrived = shared ? base + at.arrived : nullptr;
+    int code;
+    if (form == BOTH) code = mrs_mxfp4_quantise(1, x, base, side, M, K, arrived, (int)at.tiles, stream);
+    else if (form == PARTS) code = mrs_mxfp4_rows_to_parts(x, base, side, lost, M, K, tokens, arrived, (int)at.tiles, stream);
+    else if (fits) code = mrs_mxfp4_rows_to_halfs(x, base, side, lost, M, K, arrived, (int)at.tiles, stream);
+    else code = mrs_mxfp4_clear(arrived, (int)at.tiles, stream);
+    if (code) return code;
     Shapes s = {};
     s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
-#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_both<T, float>(x_codes, x_scales, codes, scales, out, s, ctas, stream) : launch_both<T, bf16>(x_codes, x_scales, codes, scales, out, s, ctas, stream)
-    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64); MRS_TOKENS(128); MRS_TOKENS(192);
-#undef MRS_TOKENS
-    return MRS_BAD_ARGUMENT;
-}
-
-// The same with x [M, K] in bfloat16 and in parts (mxfp4.cu), M up to `tokens` (16, 32 or 64), K a multiple of 128.
-MRS_EXPORT int mrs_mxfp4_parts_rows(const void* x, const void* parts, const void* x_scales, const void* lost, const void* codes, const void* scales, void* out,
-                                    int out_f32, int M, int N, int K, int tokens, int ctas, void* scratch, void* arrived, int early, void* stream) {
-    if (M == 0 || N == 0) return 0;
-    if (bad(x, codes, scales, out, out_f32, M, N, K, tokens, ctas, scratch, arrived) || K % HALF_STAGE_K || ((uintptr_t)codes & 31) || !parts || !x_scales || !lost ||
-        (((uintptr_t)parts | (uintptr_t)x_scales) & 15) || ((uintptr_t)lost & 3))
-        return MRS_BAD_ARGUMENT;
-    Shapes s = {};
-    s.M = M, s.N = N, s.K = K, s.early = early, s.w_tiles_of_a_row = mx_tiles_of_a_row(K), s.scratch = (float*)scratch, s.arrived = (int*)arrived;
-    s.lost = (const int*)lost, s.w_codes = (const uint8_t*)codes, s.w_scales = (const uint8_t*)scales;
-#define MRS_TOKENS(T) if (tokens == T) return out_f32 ? launch_parts<T, float>(x, parts, x_scales, out, s, ctas, stream) : launch_parts<T, bf16>(x, parts, x_scales, out, s, ctas, stream)
-    MRS_TOKENS(16); MRS_TOKENS(32); MRS_TOKENS(64);
+    s.w_codes = (const uint8_t*)codes, s.w_scales = (const uint8_t*)scales;
+    if (form != BOTH) s.lost = (const int*)lost;
+    if (form == WEIGHTS && fits) s.x_factors = (const int*)side, s.w_exponent = w_exponent;
+#define MRS_TOKENS(T, LAUNCH, ...) if (tokens == T) return out_f32 ? LAUNCH<T, float>(__VA_ARGS__, out, s, ctas, stream) : LAUNCH<T, bf16>(__VA_ARGS__, out, s, ctas, stream)
+    if (form == PARTS) {
+        MRS_TOKENS(16, launch_parts, x, base, side);
+        MRS_TOKENS(32, launch_parts, x, base, side);
+        MRS_TOKENS(64, launch_parts, x, base, side);
+    } else if (form == WEIGHTS) {
+        MRS_TOKENS(16, launch_weights, x, base);
+        MRS_TOKENS(32, launch_weights, x, base);
+        MRS_TOKENS(64, launch_weights, x, base);
+        MRS_TOKENS(128, launch_weights, x, base);
+        MRS_TOKENS(192, launch_weights, x, base);
+    } else {
+        MRS_TOKENS(16, launch_both, base, side);
+        MRS_TOKENS(32, launch_both, base, side);
+        MRS_TOKENS(64, launch_both, base, side);
+        MRS_TOKENS(128, launch_both, base, side);
+        MRS_TOKENS(192, launch_both, base, side);
+    }
 #undef MRS_TOKENS
     return MRS_BAD_ARGUMENT;
 }

@@ -2573,12 +2573,7 @@ _MXFP4_SIGNATURES = {
     "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
     "mrs_mxfp4_few_rows_cluster": [_c_int, _c_int],
     "mrs_mxfp4_scale_range": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
-    "mrs_mxfp4_rows_to_halfs": [_c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
-    "mrs_mxfp4_weights_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp,
-                               _c_int, _c_vp],
-    "mrs_mxfp4_rows_to_parts": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp],
-    "mrs_mxfp4_parts_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp],
-    "mrs_mxfp4_both_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp],
+    "mrs_mxfp4_rows": [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, *[_c_int] * 10, _c_vp, _c_vp],
     "mrs_mxfp4_take_error": [ctypes.POINTER(ctypes.c_uint)],
 }
 _mxfp4_lib = None
@@ -2592,6 +2587,8 @@ def mxfp4_library() -> ctypes.CDLL:
         from .csrc.build import mxfp4_kernel_library
 
         lib = _typed(mxfp4_kernel_library(), _MXFP4_SIGNATURES)
+        lib.mrs_mxfp4_work_bytes.argtypes = [_c_int] * 7
+        lib.mrs_mxfp4_work_bytes.restype = ctypes.c_longlong
         lib.mrs_mxfp4_error_string.argtypes = [_c_int]
         lib.mrs_mxfp4_error_string.restype = ctypes.c_char_p
         _mxfp4_lib = lib
@@ -2614,14 +2611,15 @@ def _stream_here(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
+@functools.lru_cache(maxsize=4096)
 def _mxfp4_bytes(rows: int, width: int) -> tuple[int, int]:
     """(bytes of codes, bytes of scales): scales in tiles of 128 rows x 4 blocks, an even number of tiles a row."""
     return rows * (width >> 1), -(-rows // 128) * (-(-width // 256) * 1024)
 
 
-def _mxfp4_lost_bytes(stretches: int) -> int:
-    """Of the elements that another form of x does not hold: a count and eight words for 256 elements."""
-    return -(-stretches // 4) * 16 + 32 * stretches
+@functools.lru_cache(maxsize=4096)
+def _mxfp4_work_bytes(form: int, m: int, n: int, k: int, tokens: int, ctas: int, shared: bool) -> int:
+    return mxfp4_library().mrs_mxfp4_work_bytes(form, m, n, k, tokens, ctas, shared)
 
 
 class Mxfp4:
@@ -2685,6 +2683,7 @@ class Mxfp4:
         return by_row.reshape(row_tiles * 128, tiles * 4)[:self.rows, :self.width // MXFP4_BLOCK].contiguous()
 
 
+@functools.lru_cache(maxsize=4096)
 def _mxfp4_sizes(rows: int, width: int, what: str) -> None:
     if width <= 0 or width % MXFP4_BLOCK:
         raise InvalidRequest(f"{what}: rows of {width} elements; 4-bit rows are whole blocks of {MXFP4_BLOCK}")
@@ -2840,37 +2839,10 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
     if plan[0] == "few":
         code = lib.mrs_mxfp4_few_rows(x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early, stream)
     else:
-        # one buffer: what x becomes, then, where tiles are shared, their sums and their counts (set to zero by the kernel before the product)
         kind, tokens, ctas, shared = plan
-        tiles = -(-n // 128) * -(-m // tokens) if shared else 0
-        depth = -(-k // 256)
-        if quantise:
-            x_bytes, side_bytes = _mxfp4_bytes(m, k)
-        elif kind == "parts":
-            x_bytes, scale_bytes = 3 * tokens * k, -(-3 * tokens // 128) * 1024 * depth
-            side_bytes = scale_bytes + _mxfp4_lost_bytes(m * depth)
-        else:
-            x_bytes, factor_bytes = 2 * m * k, -(-m // 4) * 16
-            side_bytes = factor_bytes + _mxfp4_lost_bytes(m * depth)
-        scratch_bytes = 2 * ctas * tokens * 512 if shared else 0
-        work = torch.empty(x_bytes + side_bytes + scratch_bytes + 4 * tiles, dtype=torch.uint8, device=x.device)
-        made = work.data_ptr()
-        side, scratch = made + x_bytes, made + x_bytes + side_bytes if shared else None
-        arrived = scratch + scratch_bytes if shared else None
-        launch_count += 1
-        if quantise:
-            code = lib.mrs_mxfp4_quantise(1, x.data_ptr(), made, side, m, k, arrived, tiles, stream)
-            code = code or lib.mrs_mxfp4_both_rows(made, side, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived,
-                                                   early, stream)
-        elif kind == "parts":
-            lost = side + scale_bytes
-            code = lib.mrs_mxfp4_rows_to_parts(x.data_ptr(), made, side, lost, m, k, tokens, arrived, tiles, stream)
-            code = code or lib.mrs_mxfp4_parts_rows(x.data_ptr(), made, side, lost, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas,
-                                                    scratch, arrived, early, stream)
-        else:
-            fits = weight.half_exponent is not None
-            lost = side + factor_bytes
-            code = lib.mrs_mxfp4_rows_to_halfs(x.data_ptr(), made, side, lost, m, k, arrived, tiles, stream)
-            code = code or lib.mrs_mxfp4_weights_rows(x.data_ptr(), made if fits else None, side if fits else None, lost if fits else None,
-                                                      weight.half_exponent or 0, w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, scratch, arrived, early, stream)
+        form, fits = 2 if quantise else 0 if kind == "parts" else 1, weight.half_exponent is not None
+        work = torch.empty(_mxfp4_work_bytes(form, m, n, k, tokens, ctas, shared), dtype=torch.uint8, device=x.device)
+        launch_count += 1 if form != 1 or fits or shared else 0        # the kernel that prepares x
+        code = lib.mrs_mxfp4_rows(form, x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, shared, fits,
+                                  weight.half_exponent or 0, early, work.data_ptr(), stream)
     _mxfp4_check(code, "mxfp4_gemm")
