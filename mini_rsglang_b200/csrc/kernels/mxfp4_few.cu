@@ -17,6 +17,9 @@
 // Where that could lose a bit of any element (2^29 and more between the sizes of two), or x has an element there that is not finite,
 // or the power is beyond [2^-20, 2^15], the stage is multiplied in bfloat16 instead, whose codes take more steps to make: the same
 // products and sums.
+//
+// Measured from a cold L2: 24,576 x 4,096 (53 MB) 13.3 us for one token and 14.4 for eight, 6,144 x 4,096 6.0 and 7.2, 1,000 x 2,048 2.6 and
+// 3.4: 4.9 us to begin and to end, then 5.7 TB/s.  tcgen05 kernels (mxfp4_tc.cu) begin with a second kernel that prepares x.
 #include "mxfp4.cuh"
 
 namespace {

@@ -1,8 +1,9 @@
 // Products of many rows with a matrix in microscaled 4-bit floating point on the tcgen05 tensor cores: out[m, n] = sum_k x[m, k] w[n, k],
-// float32 sums.  A tile is 128 rows of w (the M of the MMA, so that a few tokens fill a narrow N) and up to 192 tokens.  All tiles' stages
-// of 256 elements of K, tile by tile, are cut into equal runs, one a CTA and SM.  A CTA has two accumulators in tensor memory: a tile's
-// results are stored while the next tile's MMAs run.  A tile at the end of a run is shared: its CTAs leave their sums in scratch
-// memory, and the last to do so adds them in the order of K, so that a result does not depend on timing.
+// float32 sums.  A tile is 128 rows of w (the M of the MMA, so that a few tokens fill a narrow N) and up to 192 tokens.  A CTA an SM
+// takes every 148th tile, or, where that leaves SMs without work (mxfp4_tiles in kernels.py), an equal run of all tiles' stages of 256 elements
+// of K, tile by tile.  It has two accumulators in tensor memory: a tile's results are stored while the next tile's MMAs run.  A
+// tile at the end of a run is shared: its CTAs leave their sums in scratch memory, and the last to do so adds them in the order of K, so
+// that a result does not depend on timing.
 //
 //   weights_kernel   x in bfloat16.  Bulk tensor copies bring 128 x 256 codes (128-byte swizzle) and their scales into a ring, x in
 //                    pieces of 128 elements into another.  Eight warps make the A operand of the codes, a thread a row and 64
@@ -13,14 +14,19 @@
 //                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
 //                    for halfs are added one by one to the sums (lost_products), and where there are too many of them, or the
 //                    matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead.
+//                    24,576 x 4,096 times 2,048 rows: 303 us, 1.36 PFLOP/s; a stage of 192 tokens takes 1.27 us, its MMAs 0.8 at 1,965 MHz.
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
-//                    tensor memory (tcgen05.cp) stage by stage.
+//                    tensor memory (tcgen05.cp) stage by stage.  24,576 x 4,096 times 16 rows 13.5 us (380 ns a stage, 6.8 TB/s, beyond
+//                    6 us), 2,048 rows 99 us, 4,096 rows 183 (4.5 PFLOP/s): 43 KB a stage of 192 tokens come to an SM in 0.41 us, 55
+//                    bytes a clock, which bounds it; its MMAs take 0.2.
 //
 //   parts_kernel     x in bfloat16 once more, up to 64 rows: as three parts of E5M2 (mxfp4.cu), 3 x 64 columns of kind::mxf8f6f4 MMAs whose A
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
 //                    columns' sums are the result's.  Elements that three parts do not hold are added one by one as well; with more than
 //                    8 of them in 256 elements of a row the CUDA cores do the whole product.  (In a decode step of 64 tokens some element
 //                    of silu(gate) * up nearly always is 2^26 below its neighbours: one of them, and the CUDA cores took 25 ms a step.)
+//                    24,576 x 4,096 times 16 rows 16.6 us, x's preparation included (430 ns a stage, 6 TB/s, beyond 6.5 us), 32 rows
+//                    19.5, 64 rows 23.8: the parts of 32 and 64 tokens, 24 and 48 KB a stage beside 17, come from L2 for every tile.
 //
 // Every wait is bounded (tma.cuh).
 #include <limits.h>
