@@ -26,7 +26,7 @@
 //                    8 of them in 256 elements of a row the CUDA cores do the whole product.  (In a decode step of 64 tokens some element
 //                    of silu(gate) * up nearly always is 2^26 below its neighbours: one of them, and the CUDA cores took 25 ms a step.)
 //                    24,576 x 4,096 times 16 rows 16.6 us, x's preparation included (430 ns a stage, 6 TB/s, beyond 6.5 us), 32 rows
-//                    19.5, 64 rows 23.8: the parts of 32 and 64 tokens, 24 and 48 KB a stage beside 17, come from L2 for every tile.
+//                    19.5, 64 rows 23.8 (the parts of 32 and 64 tokens, 24 and 48 KB a stage beside 17, leave room for three stages).
 //
 // Every wait is bounded (tma.cuh).
 #include <limits.h>

@@ -2634,8 +2634,17 @@ class Mxfp4:
     __slots__ = ("data", "rows", "width", "settled", "half_exponent")
 
     def __init__(self, data: torch.Tensor, rows: int, width: int):
+        _mxfp4_sizes(rows, width, "Mxfp4")
+        if data.dtype is not torch.uint8 or data.dim() != 1 or not data.is_contiguous() or data.numel() != sum(_mxfp4_bytes(rows, width)):
+            raise InvalidRequest(f"Mxfp4: {rows} rows of {width} elements are {sum(_mxfp4_bytes(rows, width))} bytes in one dimension")
+        if data.data_ptr() & 31:
+            raise InvalidRequest("Mxfp4: the data does not begin on a 32-byte boundary")
+        self._set(data, rows, width)
+
+    def _set(self, data: torch.Tensor, rows: int, width: int) -> "Mxfp4":
         self.data, self.rows, self.width = data, rows, width
         self.settled, self.half_exponent = False, None
+        return self
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -2692,7 +2701,7 @@ def _mxfp4_sizes(rows: int, width: int, what: str) -> None:
 
 
 def _mxfp4_empty(rows: int, width: int, device) -> Mxfp4:
-    return Mxfp4(torch.empty(sum(_mxfp4_bytes(rows, width)), dtype=torch.uint8, device=device), rows, width)
+    return Mxfp4.__new__(Mxfp4)._set(torch.empty(sum(_mxfp4_bytes(rows, width)), dtype=torch.uint8, device=device), rows, width)
 
 
 def _mxfp4_aligned(t: torch.Tensor, what: str) -> None:
@@ -2729,7 +2738,7 @@ def mxfp4_dequantise(matrix: Mxfp4, dtype: torch.dtype = torch.bfloat16) -> torc
     if here != _current_device():
         with torch.cuda.device(here):
             return mxfp4_dequantise(matrix, dtype)
-    out = torch.empty((matrix.rows, matrix.width), dtype=dtype, device=matrix.data.device)
+    out = matrix.data.new_empty((matrix.rows, matrix.width), dtype=dtype)
     codes, scales = matrix.addresses()
     _mxfp4_check(mxfp4_library().mrs_mxfp4_dequantise(bf16, codes, scales, out.data_ptr(), matrix.rows, matrix.width, _stream_here(here)), "mxfp4_dequantise")
     return out
@@ -2827,6 +2836,9 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
     if m == 0 or n == 0:
         return
     _mxfp4_aligned(x, "mxfp4_gemm input")
+    x_at, out_at = x.data_ptr(), out.data_ptr()
+    if x_at < out_at + out.element_size() * m * n and out_at < x_at + 2 * m * k:
+        raise InvalidRequest("mxfp4_gemm: the output overlaps the input")
     if here != _current_device():
         with torch.cuda.device(here):
             return mxfp4_gemm(x, weight, out, quantise, plan)
@@ -2837,12 +2849,12 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
     if plan is None:
         plan = mxfp4_plan(m, n, k, bool(quantise), sms)
     if plan[0] == "few":
-        code = lib.mrs_mxfp4_few_rows(x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early, stream)
+        code = lib.mrs_mxfp4_few_rows(x_at, w_codes, w_scales, out_at, out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early, stream)
     else:
         kind, tokens, ctas, shared = plan
         form, fits = 2 if quantise else 0 if kind == "parts" else 1, weight.half_exponent is not None
-        work = torch.empty(_mxfp4_work_bytes(form, m, n, k, tokens, ctas, shared), dtype=torch.uint8, device=x.device)
+        work = x.new_empty(_mxfp4_work_bytes(form, m, n, k, tokens, ctas, shared), dtype=torch.uint8)
         launch_count += 1 if form != 1 or fits or shared else 0        # the kernel that prepares x
-        code = lib.mrs_mxfp4_rows(form, x.data_ptr(), w_codes, w_scales, out.data_ptr(), out_f32, m, n, k, tokens, ctas, shared, fits,
+        code = lib.mrs_mxfp4_rows(form, x_at, w_codes, w_scales, out_at, out_f32, m, n, k, tokens, ctas, shared, fits,
                                   weight.half_exponent or 0, early, work.data_ptr(), stream)
     _mxfp4_check(code, "mxfp4_gemm")

@@ -129,7 +129,8 @@ def test_product_over_the_sizes(m, n, k, quantise):
 
 PLANS = [("few", 1), ("few", 2), ("few", 8), ("many", 16, 5, False), ("many", 16, 7, True), ("many", 32, 1, False), ("many", 64, 3, True), ("many", 128, 148, False),
          ("many", 128, 148, True), ("many", 128, 11, True), ("many", 192, 148, False), ("many", 192, 9, True), ("parts", 16, 5, False), ("parts", 16, 9, True),
-         ("parts", 32, 148, False), ("parts", 32, 7, True), ("parts", 64, 3, False), ("parts", 64, 148, True)]
+         ("parts", 32, 148, False), ("parts", 32, 7, True), ("parts", 64, 3, False), ("parts", 64, 148, True), ("parts", 16, 2, False), ("parts", 32, 1, False),
+         ("parts", 64, 2, False)]
 
 
 def takes(plan, m, k, quantise):
@@ -148,7 +149,8 @@ def fitting(plan, m, n, k):
 
 
 SIZES = [(1, 128, 256), (13, 100, 32), (16, 129, 288), (30, 200, 1056), (64, 64, 4096), (100, 300, 544), (260, 513, 768), (257, 130, 2080), (600, 24000, 96),
-         (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096), (32, 70, 640), (33, 300, 640), (50, 1000, 1152), (63, 129, 128)]
+         (400, 2500, 512), (9, 129, 128), (16, 500, 1152), (31, 1000, 4096), (32, 70, 640), (33, 300, 640), (50, 1000, 1152), (63, 129, 128),
+         (24, 700, 1024), (11, 900, 1920), (60, 500, 384)]
 
 
 @pytest.mark.parametrize("m,n,k,plan,quantise", [(m, n, k, plan, quantise) for m, n, k in SIZES for plan in PLANS for quantise in (False, True)
@@ -300,6 +302,18 @@ def test_nothing_but_the_output_is_written(m, quantise):
         values = plain_quantise(x)[0] if quantise else x.double()
         close_to_sums(buffer[n:-n].view(m, n), values @ w.T, values.abs() @ w.abs().T, k, "inside a buffer")
     assert torch.equal(x, before[0]) and torch.equal(weight.data, before[1])
+
+
+@pytest.mark.parametrize("m,quantise", ALL_KINDS)
+def test_an_output_over_the_input_is_refused(m, quantise):
+    weight = kernels.mxfp4_quantise(torch.randn(256, 256, device=DEV)).settle()
+    buffer = torch.zeros(3 * m * 256, device=DEV, dtype=torch.bfloat16)
+    x = buffer[m * 256:2 * m * 256].view(m, 256)
+    for out in (x, buffer[m * 256 - 2:2 * m * 256 - 2].view(m, 256), buffer[:2 * m * 256].view(torch.float32).view(m, 256)):
+        with pytest.raises(InvalidRequest):
+            kernels.mxfp4_gemm(x, weight, out, quantise=quantise)
+    kernels.mxfp4_gemm(x, weight, buffer[:m * 256].view(m, 256), quantise=quantise)
+    kernels.mxfp4_gemm(x, weight, buffer[2 * m * 256:].view(m, 256), quantise=quantise)
 
 
 @pytest.mark.parametrize("m,quantise", ALL_KINDS)

@@ -51,6 +51,21 @@ def test_product_refuses_sizes_and_types(x, out, dtype):
         kernels.mxfp4_gemm(torch.zeros(x, dtype=torch.bfloat16), matrix(8, 64), torch.zeros(out, dtype=dtype))
 
 
+@pytest.mark.parametrize("data,rows,width", [(torch.zeros(10, dtype=torch.uint8), 128, 256), (torch.zeros(1152 - 1, dtype=torch.uint8), 1, 256),
+                                             (torch.zeros(1152, dtype=torch.int8), 1, 256), (torch.zeros(1152 * 2, dtype=torch.uint8)[::2], 1, 256),
+                                             (torch.zeros(2, 576, dtype=torch.uint8), 1, 256), (torch.zeros(1152, dtype=torch.uint8), -1, 256),
+                                             (torch.zeros(1152, dtype=torch.uint8), 1, 250), (torch.zeros(1152 + 16, dtype=torch.uint8)[16:], 1, 256)])
+def test_a_matrix_has_the_bytes_of_its_sizes(data, rows, width):
+    with pytest.raises(InvalidRequest):
+        kernels.Mxfp4(data, rows, width)
+
+
+def test_a_matrix_of_given_bytes():
+    data = matrix(3, 320).data
+    held = kernels.Mxfp4(data, 3, 320)
+    assert held.data is data and held.shape == (3, 320) and not held.settled and held.codes.shape == (3, 160)
+
+
 def test_block_scales_reads_the_tiles():
     """A scale lies at byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of tile (r / 128, b / 4)."""
     for rows, width in ((1, 32), (129, 288), (300, 1056)):
