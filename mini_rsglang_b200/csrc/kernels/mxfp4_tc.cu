@@ -14,11 +14,12 @@
 //                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
 //                    for halfs are added one by one to the sums (lost_products), and where there are too many of them, or the
 //                    matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead.
-//                    24,576 x 4,096 times 2,048 rows: 303 us, 1.36 PFLOP/s; a stage of 192 tokens takes 1.27 us, its MMAs 0.8 at 1,965 MHz.
+//                    24,576 x 4,096 times 2,048 rows: 303 us, 1.36 PFLOP/s; the tensor pipe is busy 78% of the time at the 1.43 GHz that
+//                    the power cap leaves.
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
 //                    tensor memory (tcgen05.cp) stage by stage.  24,576 x 4,096 times 16 rows 13.5 us (380 ns a stage, 6.8 TB/s, beyond
-//                    6 us), 2,048 rows 99 us, 4,096 rows 183 (4.5 PFLOP/s): 43 KB a stage of 192 tokens come to an SM in 0.41 us, 55
-//                    bytes a clock, which bounds it; its MMAs take 0.2.
+//                    6 us), 2,048 rows 99 us, 4,096 rows 183 (4.5 PFLOP/s): 43 KB a stage of 192 tokens come to an SM in 0.41 us, 68
+//                    bytes a clock at 1.44 GHz, which bounds it; the tensor pipe is busy 65% of the time.
 //
 //   parts_kernel     x in bfloat16 once more, up to 64 rows: as three parts of E5M2 (mxfp4.cu), 3 x 64 columns of kind::mxf8f6f4 MMAs whose A
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
