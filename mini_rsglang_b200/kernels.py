@@ -2773,15 +2773,18 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
     Measured on a B200 (us, weights [n, k] from a cold L2, the kernel that prepares x included; few / parts / many):
       24,576 x 4,096   1 row 13.3 / 16.7 / 21.5, 8 rows 14.4 / 16.9 / 22.1, 16 rows - / 16.6 / 21.6, 32 rows - / 19.5 / 25.3,
                        64 rows - / 23.8 / 30.3
-      4,096 x 12,288   1 row 9.8 / 14.4 / 19.0, 8 rows (x in four CTAs) 18.3 / 14.5 / 20.2
-      5,120 x 17,408   4 rows (x in two CTAs) 15.1 / 17.1 / 24.4, 8 rows (in four) 27.9 / 17.1 / 25.1
+      4,096 x 12,288   1 row 9.9 / 14.4 / 19.0, 8 rows (x in four CTAs) 18.3 / 14.5 / 20.2
+      5,120 x 17,408   4 rows 15.8 / 17.1 / 24.4, 8 rows (in four) 27.9 / 17.1 / 25.1
     and with x brought to 4 bits (few / many): 24,576 x 4,096 4 rows 14.8 / 13.7, 8 rows 16.4 / 13.7;
-      12,963 x 2,368 1 row 7.6 / 6.8; 4,096 x 12,288 1 row 10.5 / 13.1, 4 rows 13.8 / 13.1;
+      12,963 x 2,368 1 row 7.6 / 6.8; 4,096 x 12,288 1 row 10.2 / 13.1, 4 rows 12.2 / 13.1;
       8 rows: 6,144 x 4,096 8.9 / 7.6, 2,560 x 9,728 11.8 / 13.2, 4,096 x 2,560 6.8 / 6.8, 1,000 x 2,048 4.8 / 6.1."""
     if m <= (8 if not quantise or n * k <= 3 << 22 else 4 if n <= 8192 else 0):
         cluster = mxfp4_library().mrs_mxfp4_few_rows_cluster(m, k)
-        if 0 < cluster <= 2:
-            return ("few", cluster)
+        if 0 < cluster <= (2 if quantise or k % 128 == 0 else 4):                # parts take whole 128 elements: 3,394 x 14,816 7 rows 20.3 / - / 24.1
+            # Two CTAs a cluster, half of K each, cost a meeting (0.8 us, one as long as a CTA has 16 groups of 16 outputs) and prepare half as
+            # much of x: 6,144 x 4,096 1 row 6.0 / 6.8, 4,096 x 12,288 4 rows 11.7 / 10.8 (x to 4 bits 13.9 / 12.2), 5,120 x 17,408 1 row 16.4 / 14.3.
+            halves = k > 4096 and n <= 128 * sms and (k >= 8192 or m * k >= 12288 if quantise else k >= 9216 or m * k >= 32768)
+            return ("few", 2 if halves else cluster)
     if m <= 64 and k % 128 == 0 and not quantise:
         return ("parts", *mxfp4_tiles(m, n, k, 16 if m <= 16 else 32 if m <= 32 else 64, sms, 9 if m <= 32 else 10))
     if m <= 128:
