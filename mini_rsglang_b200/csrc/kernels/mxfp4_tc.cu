@@ -12,8 +12,8 @@
 //                    clocks for eight codes of a warp), bfloat16 goes through float32 (21 clocks).  So x comes as halfs, times a
 //                    power of two a row, from a kernel before (mxfp4.cu), and w becomes halfs times one power of two of the matrix;
 //                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
-//                    for halfs are added one by one to the sums (lost_products), and where there are too many of them, or the
-//                    matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead.
+//                    for halfs are added one by one to the sums (lost_products), and where there are too many of them (LOST_SHARE),
+//                    or the matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead (a sixth slower).
 //                    24,576 x 4,096 times 2,048 rows: 303 us, 1.36 PFLOP/s; the tensor pipe is busy 78% of the time at the 1.43 GHz that
 //                    the power cap leaves.
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
@@ -23,8 +23,9 @@
 //
 //   parts_kernel     x in bfloat16 once more, up to 64 rows: as three parts of E5M2 (mxfp4.cu), 3 x 64 columns of kind::mxf8f6f4 MMAs whose A
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
-//                    columns' sums are the result's.  Elements that three parts do not hold are added one by one as well; with more than
-//                    8 of them in 256 elements of a row the CUDA cores do the whole product.  (In a decode step of 64 tokens some element
+//                    columns' sums are the result's.  Elements that three parts do not hold are added one by one as well (24,576 x 4,096
+//                    times 64 rows: none 24 us, in 1 row 26, in 16 rows 37, in all 72); with more than 8 of them in 256 elements of a row
+//                    the CUDA cores do the whole product.  (In a decode step of 64 tokens some element
 //                    of silu(gate) * up nearly always is 2^26 below its neighbours: one of them, and the CUDA cores took 25 ms a step.)
 //                    24,576 x 4,096 times 16 rows 16.6 us, x's preparation included (430 ns a stage, 6 TB/s, beyond 6.5 us), 32 rows
 //                    19.5, 64 rows 23.8 (the parts of 32 and 64 tokens, 24 and 48 KB a stage beside 17, leave room for three stages).
@@ -137,7 +138,7 @@ __device__ __forceinline__ void add_to_column(uint32_t column, float more) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n tcgen05.wait::st.sync.aligned;" ::"r"(column), "f"(sum) : "memory");
 }
 // The sum of a token's lost elements times a row of w, for a whole warp with a row a lane (rarely called: apart, so that it takes no
-// registers of others).  `counts` and `entries`: of the token's `stretches`.
+// registers of others; four tokens' side by side took a stack, 2 us of every call).  `counts` and `entries`: of the token's `stretches`.
 __device__ __noinline__ float lost_products(const int* counts, const uint32_t* entries, int stretches, const uint8_t* codes, const uint8_t* scales) {
     const int lane = threadIdx.x & 31;
     float sum = 0.0f;
@@ -175,9 +176,9 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
     auto finish = [&](int c, float (&v)[STEP]) {
         if (halfs) {                               // powers of two in the floats' range, a lane each, by way of shared memory
             const int lane = threadIdx.x & 31;
-            const int factor = lane < STEP && c + lane < live ? __ldcg(s.x_factors + token0 + c + lane) : -2 * s.w_exponent;
+            const int factor = lane < STEP && c + lane < live ? __ldcg(s.x_factors + token0 + c + lane) : -16 * s.w_exponent;
             __syncwarp();
-            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (factor >> 1)) << 23);
+            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (factor >> 4)) << 23);
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < STEP; e += 4) {
@@ -205,12 +206,12 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
             int factor = 0;
             if constexpr (PARTS) factor = (lost[c >> 5] >> ((c + lane) & 31)) & (lane < STEP ? 1u : 0u);
             else if (lane < STEP && c + lane < live) factor = __ldcg(s.x_factors + token0 + c + lane);
-            for (uint32_t some = __ballot_sync(0xffffffffu, factor & 1); some; some &= some - 1) {
+            for (uint32_t some = __ballot_sync(0xffffffffu, factor & 15); some; some &= some - 1) {
                 const int at = __ffs(some) - 1;
                 const long long of = n < s.N ? n : s.N - 1, token = token0 + c + at;
                 float more = lost_products(s.lost + token * s.depth, mx_lost_entries(s.lost, (long long)s.M * s.depth) + token * s.depth * MX_LOST, s.depth,
                                            s.w_codes + of * (s.K >> 1), s.w_scales + mx_scale_offset(of, 0, s.w_tiles_of_a_row));
-                if constexpr (!PARTS) more *= __uint_as_float((uint32_t)(127 - s.w_exponent - (__shfl_sync(0xffffffffu, factor, at) >> 1)) << 23);
+                if constexpr (!PARTS) more *= __uint_as_float((uint32_t)(127 - s.w_exponent - (__shfl_sync(0xffffffffu, factor, at) >> 4)) << 23);
                 add_to_column(acc + c + at, more);
             }
         }
@@ -290,6 +291,9 @@ template <int TOKENS> constexpr int step_k() { return TOKENS <= 64 ? 256 : 128; 
 // to 22,000 clocks a tile, its MMAs 6,200), these 506; 24,576 x 4,096 took 301 and 305.
 constexpr int MAKERS = 8, STORERS = 8;
 constexpr int W_THREADS = (3 + MAKERS + STORERS) * 32;
+// Bfloat16 is ahead of halfs when one in so many rows has an element to add (24,576 x 4,096 times 2,048 rows: none 300 us, one in 64 rows
+// 304, in 16 310, in 8 338, in 4 468; bfloat16 346.  4,096 x 12,288: 183, 189, 200, 223, 266; 206).
+constexpr int LOST_SHARE = 16;
 template <int TOKENS> constexpr int a_columns() { return step_k<TOKENS>() / 2; }
 template <int TOKENS> constexpr int x_bytes() { return TOKENS * step_k<TOKENS>() * 2; }
 template <int TOKENS> constexpr int x_stages() { return TOKENS > 128 ? 3 : 4; }
@@ -366,6 +370,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     int* flag = reinterpret_cast<int*>(tmem_slot + 1);
     __shared__ __align__(16) float factors[STORERS * 32];
+    __shared__ int lost_count;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Walk walk(s);
@@ -374,6 +379,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     auto steps_of = [&]() { return (walk.to - walk.from) * STAGE_STEPS; };
 
     if (threadIdx.x == 0) {
+        lost_count = 0;
         for (int i = 0; i < W_STAGES; ++i) {
             mbar_init(&w_full[i], 1);
             mbar_init(&w_empty[i], MAKERS);
@@ -418,14 +424,16 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     pdl_wait();
     bool halfs = false, lost = false;
     if (s.x_factors) {
-        bool fit = true, some = false;
+        bool fit = true;
+        int some = 0;
         for (int i = threadIdx.x; i < s.M; i += W_THREADS) {
-            const int factor = s.x_factors[i], e = factor >> 1;
+            const int factor = s.x_factors[i], e = factor >> 4;
             fit = fit && factor != INT_MIN && e + s.w_exponent >= -126 && e + s.w_exponent <= 126;
-            some = some || (factor & 1);
+            some += factor & 15;
         }
-        halfs = __syncthreads_and(fit);
-        lost = __syncthreads_or(some) && halfs;
+        if (some) atomicAdd(&lost_count, some);
+        halfs = __syncthreads_and(fit) && lost_count <= s.M / LOST_SHARE;
+        lost = halfs && lost_count != 0;
     }
 
     // Codes and x come by the hands of two warps: a wait for the makers must not hold up x, whose pieces free up MMA by MMA.

@@ -243,6 +243,28 @@ def test_elements_far_below_the_others(plan, count):
     check_product(x.bfloat16(), kernels.mxfp4_matrix(codes, scales), w, False, plan, f"{count}")
 
 
+@pytest.mark.parametrize("plan", [("parts", 64, 3, False), ("parts", 64, 5, True), ("many", 64, 2, False), ("many", 64, 5, True), ("many", 128, 3, False), ("many", 128, 7, True),
+                                  ("many", 192, 5, True), ("many", 192, 4, False)])
+@pytest.mark.parametrize("some", [1, 3, 7, 30])
+def test_a_few_rows_with_elements_far_below(plan, some):
+    """`some` rows among the others have up to eight such elements, which meet the only codes that are not zero."""
+    m, n, k = 64 if plan[1] == 64 else 300, 390, 1280
+    g = torch.Generator(device=DEV).manual_seed(some + plan[1])
+    codes, scales, _ = random_matrix(g, n, k)
+    x = torch.randn(m, k, device=DEV, generator=g)
+    nonzero = torch.tensor([3, 255, 256, 700, 1024, 1100, 1200, 1279], device=DEV)
+    keep = torch.zeros(k, dtype=torch.bool, device=DEV)
+    keep[nonzero] = True
+    mask = torch.where(keep[0::2], 0x0F, 0) | torch.where(keep[1::2], 0xF0, 0)
+    codes = codes & mask.to(torch.uint8)
+    rows = torch.randperm(m, device=DEV, generator=g)[:some]
+    for i, row in enumerate(rows.tolist()):
+        x[row, nonzero[:1 + i % 8]] *= 2.0 ** -50
+        x[row, nonzero[1 + i % 8:]] = 0.0
+    weight, w = kernels.mxfp4_matrix(codes, scales), plain_values(codes, scales)
+    check_product(x.bfloat16(), weight, w, False, plan, f"{some}")
+
+
 @pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS for q in (False, True) if takes(plan, 11, 128, q)])
 @pytest.mark.parametrize("kind", ["wide", "nan", "zero_blocks", "small", "large", "unsettled"])
 def test_scales_of_every_size(kind, plan, quantise):
