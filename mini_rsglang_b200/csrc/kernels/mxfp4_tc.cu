@@ -8,7 +8,7 @@
 //   weights_kernel   x in bfloat16.  Bulk tensor copies bring 128 x 256 codes (128-byte swizzle) and their scales into a ring, x in
 //                    pieces of 128 elements into another.  Eight warps make the A operand of the codes, a thread a row and 64
 //                    elements, in tensor memory; no shared memory is written for it.  One thread issues kind::f16 MMAs.
-//                    Making A is what a scheduler has to do for each MMA: halfs are a conversion and a multiplication for two codes (9
+//                    Making A is what a scheduler has to do for each MMA: halfs are a conversion and a multiplication for two codes (13
 //                    clocks for eight codes of a warp), bfloat16 goes through float32 (21 clocks).  So x comes as halfs, times a
 //                    power of two a row, from a kernel before (mxfp4.cu), and w becomes halfs times one power of two of the matrix;
 //                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
