@@ -2784,7 +2784,7 @@ def mxfp4_plan(m: int, n: int, k: int, quantise: bool, sms: int) -> tuple:
             # Two CTAs a cluster, half of K each, cost a meeting (0.8 us, one as long as a CTA has 16 groups of 16 outputs) and prepare half as
             # much of x: 6,144 x 4,096 1 row 6.0 / 6.8, 4,096 x 12,288 4 rows 11.7 / 10.8 (x to 4 bits 13.9 / 12.2), 5,120 x 17,408 1 row 16.4 / 14.3.
             halves = k > 4096 and n <= 128 * sms and (k >= 8192 or m * k >= 12288 if quantise else k >= 9216 or m * k >= 32768)
-            return ("few", 2 if halves else cluster)
+            return ("few", 2 if halves and cluster == 1 else cluster)            # no fewer than hold x
     if m <= 64 and k % 128 == 0 and not quantise:
         return ("parts", *mxfp4_tiles(m, n, k, 16 if m <= 16 else 32 if m <= 32 else 64, sms, 9 if m <= 32 else 10))
     if m <= 128:

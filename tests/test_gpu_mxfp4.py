@@ -449,3 +449,13 @@ def test_refusals_on_the_gpu():
     zeros = kernels.mxfp4_matrix(torch.zeros_like(codes), torch.full_like(scales, 254))         # blocks of zeros may have any scale
     kernels.mxfp4_gemm(x, zeros, out)
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("quantise", [False, True])
+@pytest.mark.parametrize("m,k", [(8, 11296), (8, 17376), (7, 12832), (7, 14816), (6, 15392), (6, 17376), (5, 18464), (4, 23072), (3, 30752), (1, 131104)])
+def test_few_rows_too_long_for_two_ctas(m, k, quantise):
+    """Rows that are no multiple of 128 elements and whose x only four CTAs' shared memory holds, as the plan launches them."""
+    n = 333
+    g = torch.Generator(device=DEV).manual_seed(m * 7 + k)
+    codes, scales, w = random_matrix(g, n, k)
+    check_product(torch.randn(m, k, device=DEV, generator=g).bfloat16(), kernels.mxfp4_matrix(codes, scales), w, quantise, None, f"{m} x {k}")

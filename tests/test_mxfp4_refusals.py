@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from mini_rsglang_b200 import RuntimeConfig, kernels
+from mini_rsglang_b200.csrc.build import mxfp4_kernel_library
 from mini_rsglang_b200.errors import BackendError, InvalidRequest
 
 
@@ -100,3 +101,16 @@ def test_tiles_have_work_for_every_cta(m, n, k, tokens, shared):
     tiles, depth = -(-n // 128) * -(-m // tokens), -(-k // 256)
     assert got == tokens and 1 <= ctas <= 148 and ctas <= (tiles * depth if is_shared else tiles)
     assert shared is None or is_shared is shared
+
+
+@pytest.mark.parametrize("quantise", [False, True])
+@pytest.mark.parametrize("m", range(1, 9))
+def test_few_rows_get_clusters_that_hold_them(m, quantise, monkeypatch):
+    """Whatever the plan weighs, the CTAs of a cluster of the kernel for few rows have shared memory for their ranges of x."""
+    lib = mxfp4_kernel_library()
+    monkeypatch.setattr(kernels, "mxfp4_library", lambda: lib)
+    for n in (1, 100, 3394, 5120, 8193, 18944, 18945, 30000):
+        for k in (*range(32, 1024, 32), *range(1024, 36000, 416), 11296, 12832, 14816, 15392, 17376, 18464, 23072, 30752, 65536, 131072, 131104, 1 << 20):
+            plan = kernels.mxfp4_plan(m, n, k, quantise, 148)
+            if plan[0] == "few":
+                assert 0 < lib.mrs_mxfp4_few_rows_cluster(m, k) <= plan[1], (m, n, k, plan)
