@@ -6,7 +6,8 @@
 // barrier stands in its loop.  A word of eight codes becomes four pairs of halfs (exact) that are A fragments of mma.m16n8k16 as
 // they stand: the order of K within a block is free as long as x has the same, so lane (g, t) takes the codes 8 t to 8 t + 7
 // of a block as its K indices of two MMAs and the same eight elements of x.  A block's two MMAs start from zero, and their sums are
-// multiplied by the block's power of two as they join the row's float32 sums: products of halfs are exact, every sum is float32.
+// multiplied by the powers of two of the block and of x as they join the row's float32 sums: products of halfs are exact, every sum is
+// float32.
 //
 // One CTA of 16 warps an SM takes an equal share of the groups of 16 rows and keeps x in shared memory for all of them.  Its
 // (group, stage of 256 elements) pairs, group by group, are cut into 16 equal runs, one a warp: a warp's first and last group may
@@ -14,11 +15,13 @@
 // take a range of K each and their sums meet in the ranges' order.  A result does not depend on timing.
 //
 // x as halfs.  A warp brings a stage of x, all tokens, into the halfs' range by one power of two, which goes into the stage's scales.
-// Where that could lose a bit of any element (2^29 and more between the sizes of two), or x has an element there that is not finite,
-// or the power is beyond [2^-20, 2^15], the stage is multiplied in bfloat16 instead, whose codes take more steps to make: the same
-// products and sums.
+// (Where it times a scale of w may be under float32's range, it goes into the sums before the scales do: 24,576 x 4,096 times one row 13.6
+// us instead of 13.0.)
+// Where halfs could lose a bit of any element (2^29 and more between the sizes of two), or x has an element there that is not finite,
+// or the power is beyond [2^-20, 2^15], the stage is multiplied in bfloat16 instead: x as it is, codes times their scale, which takes more
+// steps to make (18.6 us).  The same products, and no sum of them before the scales, which could leave float32's range on the way.
 //
-// Measured from a cold L2: 24,576 x 4,096 (53 MB) 13.3 us for one token and 14.4 for eight, 6,144 x 4,096 6.0 and 7.2, 1,000 x 2,048 2.6 and
+// Measured from a cold L2: 24,576 x 4,096 (53 MB) 12.9 us for one token and 14.4 for eight, 6,144 x 4,096 5.9 and 7.1, 1,000 x 2,048 2.6 and
 // 3.4: 4.9 us to begin and to end, then 5.7 TB/s.  tcgen05 kernels (mxfp4_tc.cu) begin with a second kernel that prepares x.
 #include "mxfp4.cuh"
 
@@ -45,19 +48,14 @@ __device__ __forceinline__ void copy_4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// d = a . b, and d += a . b
-template <bool HALFS>
+// d = a . b of halfs, and d += a . b
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (HALFS)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-template <bool HALFS>
+template <bool OF_HALFS>
 __device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (HALFS)
+    if constexpr (OF_HALFS)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
@@ -65,10 +63,11 @@ __device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], 
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A half pair of codes as a pair of bfloat16 (exact: both have the values 0.5 to 6).
-__device__ __forceinline__ uint32_t as_bf16_pair(uint32_t halfs) {
+// A half pair of codes times their scale as a pair of bfloat16 (exact: a code has two bits of significand; where the scale is not a
+// number, infinity beside codes of 0, it is none).
+__device__ __forceinline__ uint32_t as_bf16_pair(uint32_t halfs, __nv_bfloat162 scale) {
     const float2 v = __half22float2(*reinterpret_cast<__half2*>(&halfs));
-    __nv_bfloat162 pair = __floats2bfloat162_rn(v.x, v.y);
+    __nv_bfloat162 pair = __hmul2(__floats2bfloat162_rn(v.x, v.y), scale);
     return *reinterpret_cast<uint32_t*>(&pair);
 }
 
@@ -76,6 +75,7 @@ struct Shapes {
     int M, N, K;
     int cluster;            // CTAs that share their groups, a range of K each
     int x_stages;           // the longest of these ranges, in stages
+    float least_factor;     // that times any of w's scales is still a float; above 0
     int early;              // w was there before the kernel before this one: it may be fetched while that runs
     int groups_each, groups_over;      // of 16 rows a share (CTA or cluster): so many, and one more for the first `groups_over`
     int stages_each, stages_over;      // of K a CTA of a cluster, likewise
@@ -95,8 +95,12 @@ __device__ __forceinline__ uint32_t shared_word(uint32_t address) {
     return v;
 }
 
+// How a stage of x lies in shared memory (`factor` of bring_x): as halfs whose power goes into the scales, as halfs whose power is so small
+// that it goes into the sums, as it is.
+enum Form { HALFS, SMALL_HALFS, BFLOATS };
+
 // One stage of a warp's rows joined to its sums.  `factors`: room for the stage's scales as floats.
-template <bool HALFS>
+template <Form FORM>
 __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, const unsigned char* x_stage, int x_pitch, float factor,
                                                int live, float (&sums)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -105,10 +109,11 @@ __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, c
         // infinity times a sum of 0 is NaN.
         const uint32_t word = shared_word(stage + CODE_BYTES + lane * 4);
         float4 f;
-        f.x = __uint_as_float(max((word << 23) & 0x7F800000u, 0x00400000u)) * factor;
-        f.y = __uint_as_float(max((word << 15) & 0x7F800000u, 0x00400000u)) * factor;
-        f.z = __uint_as_float(max((word << 7) & 0x7F800000u, 0x00400000u)) * factor;
-        f.w = __uint_as_float(max((word >> 1) & 0x7F800000u, 0x00400000u)) * factor;
+        f.x = __uint_as_float(max((word << 23) & 0x7F800000u, 0x00400000u));
+        f.y = __uint_as_float(max((word << 15) & 0x7F800000u, 0x00400000u));
+        f.z = __uint_as_float(max((word << 7) & 0x7F800000u, 0x00400000u));
+        f.w = __uint_as_float(max((word >> 1) & 0x7F800000u, 0x00400000u));
+        if constexpr (FORM == HALFS) f.x *= factor, f.y *= factor, f.z *= factor, f.w *= factor;
         *reinterpret_cast<float4*>(factors + lane * 4) = f;
         __syncwarp();
     }
@@ -125,15 +130,22 @@ __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, c
             uint32_t low[4], high[4];
             mx_decode_8(shared_word(codes ^ (b * 16)), low);
             mx_decode_8(shared_word((codes ^ (b * 16)) + 8 * 128), high);
-            if constexpr (!HALFS) {
+            if constexpr (FORM == BFLOATS) {
+                const __nv_bfloat162 scale_low = __float2bfloat162_rn(s_low[i]), scale_high = __float2bfloat162_rn(s_high[i]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) low[j] = as_bf16_pair(low[j]), high[j] = as_bf16_pair(high[j]);
+                for (int j = 0; j < 4; ++j) low[j] = as_bf16_pair(low[j], scale_low), high[j] = as_bf16_pair(high[j], scale_high);
             }
             const uint32_t a0[4] = {low[0], high[0], low[1], high[1]}, a1[4] = {low[2], high[2], low[3], high[3]};
             const uint4 xs = *reinterpret_cast<const uint4*>(x_row + b * 64);
+            if constexpr (FORM == BFLOATS) {
+                mma_more<false>(sums, a0, xs.x, xs.y);
+                mma_more<false>(sums, a1, xs.z, xs.w);
+                continue;
+            }
             float d[4];
-            mma_first<HALFS>(d, a0, xs.x, xs.y);
-            mma_more<HALFS>(d, a1, xs.z, xs.w);
+            mma_first(d, a0, xs.x, xs.y);
+            mma_more<true>(d, a1, xs.z, xs.w);
+            if constexpr (FORM == SMALL_HALFS) d[0] *= factor, d[1] *= factor, d[2] *= factor, d[3] *= factor;         // exact
             sums[0] = fmaf(d[0], s_low[i], sums[0]);
             sums[1] = fmaf(d[1], s_low[i], sums[1]);
             sums[2] = fmaf(d[2], s_high[i], sums[2]);
@@ -316,8 +328,9 @@ __global__ void __launch_bounds__(THREADS, 1) few_rows_kernel(const bf16* __rest
                 copy_wait<RING - 2>();
                 __syncwarp();
                 copy_next();
-                if (factor != 0.0f) stage_products<true>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
-                else stage_products<false>(ring + used_offset, factors, x_stage, x_pitch, 1.0f, live, sums);
+                if (factor >= s.least_factor) stage_products<HALFS>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
+                else if (factor != 0.0f) stage_products<SMALL_HALFS>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
+                else stage_products<BFLOATS>(ring + used_offset, factors, x_stage, x_pitch, factor, live, sums);
                 used_offset = used_offset + STAGE_BYTES == RING * STAGE_BYTES ? 0 : used_offset + STAGE_BYTES;
                 __syncwarp();
             }
@@ -435,14 +448,16 @@ MRS_EXPORT int mrs_mxfp4_few_rows_cluster(int M, int K) {
 }
 
 // out [M, N] bfloat16 or float32 (`out_f32`); x [M, K] bfloat16; w as in mxfp4.cuh; `cluster` 1, 2, 4 or 8 ranges of K; `ctas`: the GPU's
-// SMs.  `early`: nothing that still runs when this kernel starts writes w.
+// SMs.  `fits`: w's blocks other than zeros have scales of 2^(w_exponent - 23) or more.  `early`: nothing that still runs when this kernel
+// starts writes w.
 MRS_EXPORT int mrs_mxfp4_few_rows(const void* x, const void* codes, const void* scales, void* out, int out_f32, int M, int N, int K, int quantise,
-                                  int cluster, int ctas, int early, void* stream) {
+                                  int cluster, int ctas, int fits, int w_exponent, int early, void* stream) {
     if (M == 0 || N == 0) return 0;
     if (M < 0 || N < 0 || K <= 0 || K % MX_BLOCK || K > (1 << 30) || M > 65535 * 8 || ctas < 1 || !x || !codes || !scales || !out) return MRS_BAD_ARGUMENT;
     if ((((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)out & (out_f32 ? 3 : 1))) return MRS_BAD_ARGUMENT;
     if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return MRS_BAD_ARGUMENT;
-    Shapes s = {M, N, K, cluster, 0, early, 0, 0, 0, 0};
+    const int least_scale = fits && w_exponent > -104 ? w_exponent - 23 : -127, least_factor = -149 - least_scale;
+    Shapes s = {M, N, K, cluster, 0, ldexpf(1.0f, least_factor > -126 ? least_factor : -126), early, 0, 0, 0, 0};
     if (quantise) return out_f32 ? launch<true, float>(x, codes, scales, out, s, ctas, stream) : launch<true, bf16>(x, codes, scales, out, s, ctas, stream);
     return out_f32 ? launch<false, float>(x, codes, scales, out, s, ctas, stream) : launch<false, bf16>(x, codes, scales, out, s, ctas, stream);
 }

@@ -2570,7 +2570,7 @@ _MXFP4_SIGNATURES = {
     "mrs_mxfp4_quantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp, _c_int, _c_vp],
     "mrs_mxfp4_dequantise": [_c_int, _c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_scales_to_tiles": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
-    "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    "mrs_mxfp4_few_rows": [_c_vp, _c_vp, _c_vp, _c_vp, *[_c_int] * 10, _c_vp],
     "mrs_mxfp4_few_rows_cluster": [_c_int, _c_int],
     "mrs_mxfp4_scale_range": [_c_vp, _c_vp, _c_vp, ctypes.c_longlong, ctypes.c_longlong, _c_vp],
     "mrs_mxfp4_rows": [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, *[_c_int] * 10, _c_vp, _c_vp],
@@ -2851,13 +2851,14 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
     sms, stream = sm_count(here), _stream_here(here)
     if plan is None:
         plan = mxfp4_plan(m, n, k, bool(quantise), sms)
+    fits, exponent = weight.half_exponent is not None, weight.half_exponent or 0
     if plan[0] == "few":
-        code = lib.mrs_mxfp4_few_rows(x_at, w_codes, w_scales, out_at, out_f32, m, n, k, int(bool(quantise)), plan[1], sms, early, stream)
+        code = lib.mrs_mxfp4_few_rows(x_at, w_codes, w_scales, out_at, out_f32, m, n, k, int(bool(quantise)), plan[1], sms, fits, exponent, early, stream)
     else:
         kind, tokens, ctas, shared = plan
-        form, fits = 2 if quantise else 0 if kind == "parts" else 1, weight.half_exponent is not None
+        form = 2 if quantise else 0 if kind == "parts" else 1
         work = x.new_empty(_mxfp4_work_bytes(form, m, n, k, tokens, ctas, shared), dtype=torch.uint8)
         launch_count += 1 if form != 1 or fits or shared else 0        # the kernel that prepares x
         code = lib.mrs_mxfp4_rows(form, x_at, w_codes, w_scales, out_at, out_f32, m, n, k, tokens, ctas, shared, fits,
-                                  weight.half_exponent or 0, early, work.data_ptr(), stream)
+                                  exponent, early, work.data_ptr(), stream)
     _mxfp4_check(code, "mxfp4_gemm")

@@ -459,3 +459,61 @@ def test_few_rows_too_long_for_two_ctas(m, k, quantise):
     g = torch.Generator(device=DEV).manual_seed(m * 7 + k)
     codes, scales, w = random_matrix(g, n, k)
     check_product(torch.randn(m, k, device=DEV, generator=g).bfloat16(), kernels.mxfp4_matrix(codes, scales), w, quantise, None, f"{m} x {k}")
+
+
+def close_to_small_sums(out, want, size, k, what):
+    """As `close_to_sums`; beside that, below float32's ordinary numbers each of the k products and each addition of 16 of them, of blocks and
+    of pieces is off by up to a step of 2^-149, which is all that float32 has there."""
+    limit = (k / 16 + 16) * size * 2.0 ** -23 + (k + k / 16 + 16) * 2.0 ** -149
+    off = (out.double() - want).abs()
+    assert (off <= limit).all(), f"{what}: {(off / limit).max().item():.3f} of the limit"
+
+
+def one_sign(x, codes, kind):
+    return (x.abs(), codes & 0x77) if kind else (x, codes)
+
+
+@pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS + [("few", 8)] for q in (False, True) if takes(plan, 3, 768, q)])
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("kind,top,low,high", [("all", 127, 97, 113), ("all", 120, 97, 120), ("all", 123, 97, 117), ("one", 127, 100, 122)])
+def test_large_rows_and_small_scales(kind, top, low, high, positive, plan, quantise):
+    """Elements up to 2^(top + 1) in every column, or in one column of 768 beside ordinary ones, against scales of 2^(low - 127) to 2^(high - 127):
+    no sum of sizes leaves float32's range (768 * 6 * 2^(top + 1 + high - 127) < 2^127 for all, 6 * 2^128 * 2^-5 and 768 ordinary products for one), and no
+    product may on its way."""
+    m, n, k = 3, 150, 768
+    g = torch.Generator(device=DEV).manual_seed(top + high)
+    codes, _, _ = random_matrix(g, n, k)
+    scales = torch.randint(low, high + 1, (n, k // 32), device=DEV, generator=g, dtype=torch.uint8)
+    x = torch.randn(m, k, device=DEV, generator=g)
+    large = (1 + torch.rand(m, k, device=DEV, generator=g) * 0.984375) * torch.sign(x) * 2.0 ** (top - 60) * 2.0 ** 60       # below 2^(top + 1) as bfloat16 too
+    columns = torch.arange(k, device=DEV) if kind == "all" else torch.tensor([517], device=DEV)
+    x[:, columns] = large[:, columns]
+    x, codes = one_sign(x, codes, positive)
+    w = plain_values(codes, scales)
+    check_product(x.bfloat16(), kernels.mxfp4_matrix(codes, scales), w, quantise, plan, f"{kind} {top}")
+
+
+@pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS + [("few", 8)] for q in (False, True) if takes(plan, 2, 768, q)])
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("low,high", [(0, 0), (0, 12), (12, 12)])
+@pytest.mark.parametrize("beside", [False, True])
+def test_small_rows_and_the_smallest_scales(beside, low, high, positive, plan, quantise):
+    """Stages of the smallest size that halfs take (2^-20) to 1 against scales of 2^-127 to 2^-115, where a long row's sum may be an ordinary
+    float and its products are not; `beside` them a much larger column that meets codes of zero."""
+    m, n, k = 2, 150, 12288
+    for size in (-20, -19, -12, -8, -7, 0):
+        g = torch.Generator(device=DEV).manual_seed(size + high + 100)
+        codes, _, _ = random_matrix(g, n, k)
+        scales = torch.randint(low, high + 1, (n, k // 32), device=DEV, generator=g, dtype=torch.uint8)
+        x = torch.randn(m, k, device=DEV, generator=g).clamp(-1.9, 1.9) * 2.0 ** size
+        if beside:
+            x[:, ::256] = 2.0 ** (size + 32)
+            codes = codes.clone()
+            codes[:, ::128] &= 0xF0
+        x, codes = one_sign(x, codes, positive)
+        w = plain_values(codes, scales)
+        x = x.bfloat16()
+        values = plain_quantise(x)[0] if quantise else x.double()
+        out = torch.full((m, n), 7.0, device=DEV)
+        kernels.mxfp4_gemm(x, kernels.mxfp4_matrix(codes, scales), out, quantise=quantise, plan=fitting(plan, m, n, k))
+        close_to_small_sums(out, values @ w.T, values.abs() @ w.abs().T, k, f"{size} {low} {high}")
