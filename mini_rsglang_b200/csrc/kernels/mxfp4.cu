@@ -204,17 +204,19 @@ __global__ void __launch_bounds__(THREADS) scales_to_tiles_kernel(const uint8_t*
     }
 }
 
-// The smallest and the largest scale byte of the blocks that are not all zeros, into range[0] and range[1] (which begin as 256 and -1).
+// The smallest and the largest scale byte below 255 of the blocks that are not all zeros, into range[0] and range[1] (which begin as 256
+// and -1), and whether any block is not a number, into range[2] (0).
 __global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int* __restrict__ range,
                                                               long long rows, long long width, long long tiles_of_a_row) {
     pdl_wait();
     const long long blocks = width / MX_BLOCK, total = rows * blocks;
-    int low = 256, high = -1;
+    int low = 256, high = -1, bad = 0;
     for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
         const long long row = i / blocks, block = i - row * blocks;
         const int byte = scales[mx_scale_offset(row, block >> 2, tiles_of_a_row) + (block & 3)];
         const uint4 c = *reinterpret_cast<const uint4*>(codes + i * 16);
-        if (((c.x | c.y | c.z | c.w) & 0x77777777u) != 0u || byte == 255) low = min(low, byte), high = max(high, byte);
+        if (byte == 255) bad = 1;
+        else if (((c.x | c.y | c.z | c.w) & 0x77777777u) != 0u) low = min(low, byte), high = max(high, byte);
     }
     low = __reduce_min_sync(0xffffffffu, low);
     high = __reduce_max_sync(0xffffffffu, high);
@@ -222,6 +224,7 @@ __global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __r
         atomicMin(&range[0], low);
         atomicMax(&range[1], high);
     }
+    if (bad) atomicOr(&range[2], 1);
 }
 
 // Rows of bfloat16 as halfs times a power of two of the row's own: row r holds x 2^-exponents[r], its largest in [2^15, 2^16).  An element's
@@ -433,7 +436,7 @@ MRS_EXPORT int mrs_mxfp4_scales_to_tiles(const void* plain, void* codes, void* s
     MRS_RETURN_LAUNCH_STATUS();
 }
 
-// range: two ints, 256 and -1 to begin with.
+// range: three ints, 256, -1 and 0 to begin with.
 MRS_EXPORT int mrs_mxfp4_scale_range(const void* codes, const void* scales, void* range, long long rows, long long width, void* stream) {
     if (rows == 0) return 0;
     if (bad_sizes(rows, width) || !range || !codes || !scales || (((uintptr_t)codes | (uintptr_t)scales) & 15) || ((uintptr_t)range & 3)) return MRS_BAD_ARGUMENT;

@@ -2674,14 +2674,14 @@ class Mxfp4:
         """Waits until the matrix is there and takes note of its scales' range.  For weights, once: products of settled weights are
         faster.  Whoever writes the data afterwards has to make a matrix anew.  Not while a graph is recorded."""
         with torch.cuda.device(self.device):
-            span = torch.tensor([256, -1], dtype=torch.int32, device=self.device)
+            span = torch.tensor([256, -1, 0], dtype=torch.int32, device=self.device)
             codes, scales = self.addresses()
             _mxfp4_check(mxfp4_library().mrs_mxfp4_scale_range(codes, scales, span.data_ptr(), self.rows, self.width, _stream()), "mxfp4_scale_range")
-            low, high = span.tolist()                        # waits for the stream
-        if 252 < high < 255:
+            low, high, bad = span.tolist()                   # waits for the stream; blocks that are not a number stand apart
+        if high > 252:
             raise InvalidRequest(f"4-bit matrix: a scale of 2^{high - 127} stands for values beyond float32; at most 2^125")
         # halfs hold 0.5 times 2^-23 to 6 times 2^13
-        self.half_exponent = None if high == 255 or high - low > 36 else max(high, 0) - 127 - 13
+        self.half_exponent = None if bad or high - low > 36 else max(high, 0) - 127 - 13
         self.settled = True
         return self
 

@@ -517,3 +517,18 @@ def test_small_rows_and_the_smallest_scales(beside, low, high, positive, plan, q
         out = torch.full((m, n), 7.0, device=DEV)
         kernels.mxfp4_gemm(x, kernels.mxfp4_matrix(codes, scales), out, quantise=quantise, plan=fitting(plan, m, n, k))
         close_to_small_sums(out, values @ w.T, values.abs() @ w.abs().T, k, f"{size} {low} {high}")
+
+
+@pytest.mark.parametrize("scale", [253, 254])
+def test_scales_beyond_float32_are_refused_beside_blocks_that_are_no_numbers(scale):
+    codes = torch.full((5, 64), 0x17, device=DEV, dtype=torch.uint8)
+    scales = torch.full((5, 4), 120, device=DEV, dtype=torch.uint8)
+    scales[1, 2] = 255
+    assert kernels.mxfp4_matrix(codes, scales).half_exponent is None
+    scales[4, 3] = scale
+    with pytest.raises(InvalidRequest, match="float32"):
+        kernels.mxfp4_matrix(codes, scales)
+    codes[4, 48:] = 0x80                                       # zeros may have any scale
+    weight = kernels.mxfp4_matrix(codes, scales)
+    assert torch.equal(weight.block_scales(), scales)
+    check_product(torch.ones(3, 128, device=DEV).bfloat16(), weight, plain_values(codes, scales), False, None, "beside no numbers")
