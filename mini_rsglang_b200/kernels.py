@@ -2840,14 +2840,17 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
         return
     _mxfp4_aligned(x, "mxfp4_gemm input")
     x_at, out_at = x.data_ptr(), out.data_ptr()
-    if x_at < out_at + out.element_size() * m * n and out_at < x_at + 2 * m * k:
+    w_codes, w_scales = weight.addresses()
+    out_end = out_at + out.element_size() * m * n
+    if x_at < out_end and out_at < x_at + 2 * m * k:
         raise InvalidRequest("mxfp4_gemm: the output overlaps the input")
+    if w_codes < out_end and out_at < w_codes + weight.bytes():
+        raise InvalidRequest("mxfp4_gemm: the output overlaps the weights")
     if here != _current_device():
         with torch.cuda.device(here):
             return mxfp4_gemm(x, weight, out, quantise, plan)
     lib = mxfp4_library()
     out_f32, early = int(out.dtype is torch.float32), int(weight.settled)
-    w_codes, w_scales = weight.addresses()
     sms, stream = sm_count(here), _stream_here(here)
     if plan is None:
         plan = mxfp4_plan(m, n, k, bool(quantise), sms)

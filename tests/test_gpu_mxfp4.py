@@ -532,3 +532,28 @@ def test_scales_beyond_float32_are_refused_beside_blocks_that_are_no_numbers(sca
     weight = kernels.mxfp4_matrix(codes, scales)
     assert torch.equal(weight.block_scales(), scales)
     check_product(torch.ones(3, 128, device=DEV).bfloat16(), weight, plain_values(codes, scales), False, None, "beside no numbers")
+
+
+@pytest.mark.parametrize("m,quantise", ALL_KINDS)
+def test_an_output_over_the_weights_is_refused(m, quantise):
+    """Over the first codes, the last scales, or all of them; right before and behind them is no overlap."""
+    n, k = 256, 512
+    x = torch.randn(m, k, device=DEV).bfloat16()
+    held = kernels.mxfp4_quantise(torch.randn(n, k, device=DEV))
+    size, bytes_ = 2 * m * n, held.bytes()
+    buffer = torch.zeros(2 * size + bytes_, device=DEV, dtype=torch.uint8)
+    buffer[size:size + bytes_] = held.data
+    weight = kernels.Mxfp4(buffer[size:size + bytes_], n, k).settle()
+
+    def out(begin):
+        return buffer[begin:begin + size].view(torch.bfloat16).view(m, n)
+
+    for begin in {2, size, size + bytes_ - 2, min(size + 4096, size + bytes_ - 2)}:
+        with pytest.raises(InvalidRequest, match="overlaps the weights"):
+            kernels.mxfp4_gemm(x, weight, out(begin), quantise=quantise)
+    before = weight.data.clone()
+    want = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
+    kernels.mxfp4_gemm(x, weight, want, quantise=quantise)
+    for begin in (0, size + bytes_):
+        kernels.mxfp4_gemm(x, weight, out(begin), quantise=quantise)
+        assert torch.equal(out(begin), want) and torch.equal(weight.data, before)

@@ -114,3 +114,24 @@ def test_few_rows_get_clusters_that_hold_them(m, quantise, monkeypatch):
             plan = kernels.mxfp4_plan(m, n, k, quantise, 148)
             if plan[0] == "few":
                 assert 0 < lib.mrs_mxfp4_few_rows_cluster(m, k) <= plan[1], (m, n, k, plan)
+
+
+def test_product_refuses_an_output_over_what_it_reads(monkeypatch):
+    """Over the input and over the weights, from either side, before the GPU is asked for anything."""
+    def gpu():
+        raise BackendError("asked for")
+
+    monkeypatch.setattr(kernels, "_need", lambda *_: None)
+    monkeypatch.setattr(kernels, "_current_device", gpu)
+    memory = torch.zeros(1 << 14, dtype=torch.uint8)
+    memory = memory[-memory.data_ptr() % 32:]
+    size = matrix(128, 64).bytes()
+    weight = kernels.Mxfp4(memory[4096:4096 + size], 128, 64)
+    x = memory[12288:12288 + 256].view(torch.bfloat16).view(2, 64)
+    for begin, end, over in ((4096, 4096 + size, "weights"), (12288, 12288 + 256, "input")):
+        for at in (begin - 510, begin - 2, begin, end - 2):
+            with pytest.raises(InvalidRequest, match=f"overlaps the {over}"):
+                kernels.mxfp4_gemm(x, weight, memory[at:at + 512].view(torch.bfloat16).view(2, 128))
+        for at in (begin - 512, end):
+            with pytest.raises(BackendError, match="asked for"):
+                kernels.mxfp4_gemm(x, weight, memory[at:at + 512].view(torch.bfloat16).view(2, 128))
