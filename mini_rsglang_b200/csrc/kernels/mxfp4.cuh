@@ -88,3 +88,9 @@ __device__ __forceinline__ float mx_inverse(uint32_t byte) { return __uint_as_fl
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
     return __uint_as_float(byte == 255u ? 0x7FC00000u : max(byte << 23, 0x00400000u));
 }
+
+// d += a . b of bfloat16, 16 rows x 8 columns x 16
+__device__ __forceinline__ void mx_mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}

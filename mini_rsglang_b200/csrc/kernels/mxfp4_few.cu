@@ -53,14 +53,9 @@ __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4],
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-template <bool OF_HALFS>
 __device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (OF_HALFS)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // A half pair of codes times their scale as a pair of bfloat16 (exact: a code has two bits of significand; where the scale is not a
@@ -138,13 +133,13 @@ __device__ __forceinline__ void stage_products(uint32_t stage, float* factors, c
             const uint32_t a0[4] = {low[0], high[0], low[1], high[1]}, a1[4] = {low[2], high[2], low[3], high[3]};
             const uint4 xs = *reinterpret_cast<const uint4*>(x_row + b * 64);
             if constexpr (FORM == BFLOATS) {
-                mma_more<false>(sums, a0, xs.x, xs.y);
-                mma_more<false>(sums, a1, xs.z, xs.w);
+                mx_mma_bf16(sums, a0, xs.x, xs.y);
+                mx_mma_bf16(sums, a1, xs.z, xs.w);
                 continue;
             }
             float d[4];
             mma_first(d, a0, xs.x, xs.y);
-            mma_more<true>(d, a1, xs.z, xs.w);
+            mma_more(d, a1, xs.z, xs.w);
             if constexpr (FORM == SMALL_HALFS) d[0] *= factor, d[1] *= factor, d[2] *= factor, d[3] *= factor;         // exact
             sums[0] = fmaf(d[0], s_low[i], sums[0]);
             sums[1] = fmaf(d[1], s_low[i], sums[1]);

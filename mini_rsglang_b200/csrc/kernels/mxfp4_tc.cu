@@ -23,10 +23,12 @@
 //
 //   parts_kernel     x in bfloat16 once more, up to 64 rows: as three parts of E5M2 (mxfp4.cu), 3 x 64 columns of kind::mxf8f6f4 MMAs whose A
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
-//                    columns' sums are the result's.  Elements that three parts do not hold are added one by one as well (24,576 x 4,096
-//                    times 64 rows: none 24 us, in 1 row 26, in 16 rows 37, in all 72); with more than 8 of them in 256 elements of a row
-//                    the CUDA cores do the whole product.  (In a decode step of 64 tokens some element
-//                    of silu(gate) * up nearly always is 2^26 below its neighbours: one of them, and the CUDA cores took 25 ms a step.)
+//                    columns' sums are the result's.  A few elements that three parts do not hold are added one by one as well; rows with
+//                    more than 8 of them in 256 elements, and all such rows where they are more than LOST_MOST, are computed from bfloat16
+//                    on mma.sync (wide_products), the others as ever: what one request's row holds costs its neighbours little.
+//                    24,576 x 4,096 times 64 rows: none 24 us, 1 element 25, 32 in as many rows 55, one such row 64, 64 such rows 206; 4,096 x
+//                    12,288: 22, 23, 43, 40, 101.  (In a decode step of 64 tokens some element of silu(gate) * up nearly always is 2^26
+//                    below its neighbours.  The CUDA cores took 3.5 and 5.3 ms for all rows as soon as one row had too many.)
 //                    24,576 x 4,096 times 16 rows 16.6 us, x's preparation included (430 ns a stage, 6 TB/s, beyond 6.5 us), 32 rows
 //                    19.5, 64 rows 23.8 (the parts of 32 and 64 tokens, 24 and 48 KB a stage beside 17, leave room for three stages).
 //
@@ -162,7 +164,8 @@ __device__ __noinline__ float lost_products(const int* counts, const uint32_t* e
 // An accumulator's results (lane: row of w, column: token) to memory.  Called by WARPS warps, `index` of them 0 to WARPS - 1; a warp's lanes
 // are those of its number modulo 4.  `halfs`: the rows' powers of two go into them (`factors`: 32 floats of shared memory for each warp).  A
 // tile that other CTAs share goes through scratch memory; `flag` is a word of shared memory.
-// `lost`: null, or elements of x are missing in the sums; with parts, a bit for each token that has some, in shared memory.
+// `lost`: null, or elements of x are missing in the sums; with parts, a bit for each token that has some, in shared memory, and behind these
+// two words two with a bit for each token whose results are computed and stored elsewhere (wide_products).
 template <int TOKENS, int WARPS, typename Out, bool PARTS = false>
 __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __restrict__ out, const Shapes& s, const Walk& walk, int index, bool halfs, int* flag, float* factors,
                                                   const uint32_t* lost = nullptr) {
@@ -188,13 +191,15 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
         }
         if (n < s.N) {
             Out* place = out + (size_t)(token0 + c) * s.N + n;
-            if (c + STEP <= live) {
+            uint32_t left = 0;
+            if constexpr (PARTS) left = lost[2 + (c >> 5)] >> (c & 31) & ((1ull << STEP) - 1);
+            if (c + STEP <= live && left == 0) {
 #pragma unroll
                 for (int e = 0; e < STEP; ++e) place[(size_t)e * s.N] = from_float<Out>(v[e]);
             } else {
 #pragma unroll
                 for (int e = 0; e < STEP; ++e)
-                    if (c + e < live) place[(size_t)e * s.N] = from_float<Out>(v[e]);
+                    if (c + e < live && !(left >> e & 1u)) place[(size_t)e * s.N] = from_float<Out>(v[e]);
             }
         }
     };
@@ -321,23 +326,28 @@ __device__ __forceinline__ void decode_block_halfs(uint4 codes, uint32_t byte, i
         }
     }
 }
+// 2^(byte - 127) as a pair of bfloat16: byte 0 under the ordinary numbers, byte 255 not a number.
+__device__ __forceinline__ __nv_bfloat162 scale_pair(uint32_t byte) {
+    const uint32_t bits = byte == 0u ? 0x0040u : byte == 255u ? 0x7FC0u : byte << 7, both = bits | bits << 16;
+    return *reinterpret_cast<const __nv_bfloat162*>(&both);
+}
+// Eight codes times their scale as four pairs of bfloat16.
+__device__ __forceinline__ void decode_eight(uint32_t codes, __nv_bfloat162 scale, uint32_t* words) {
+    uint32_t h[4];
+    mx_decode_8(codes, h);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const float2 v = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
+        const __nv_bfloat162 pair = __hmul2(__floats2bfloat162_rn(v.x, v.y), scale);
+        words[p] = *reinterpret_cast<const uint32_t*>(&pair);
+    }
+}
 // 32 codes of a row and their scale byte as 16 pairs of bfloat16.
 __device__ __forceinline__ void decode_block(uint4 codes, uint32_t byte, uint32_t* words) {
-    // 2^(byte - 127) as bfloat16: byte 0 under the ordinary numbers, byte 255 not a number
-    const uint32_t bits = byte == 0u ? 0x0040u : byte == 255u ? 0x7FC0u : byte << 7, both = bits | bits << 16;
-    const __nv_bfloat162 scale = *reinterpret_cast<const __nv_bfloat162*>(&both);
+    const __nv_bfloat162 scale = scale_pair(byte);
     const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t h[4];
-        mx_decode_8(w[i], h);
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const float2 v = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
-            const __nv_bfloat162 pair = __hmul2(__floats2bfloat162_rn(v.x, v.y), scale);
-            words[i * 4 + p] = *reinterpret_cast<const uint32_t*>(&pair);
-        }
-    }
+    for (int i = 0; i < 4; ++i) decode_eight(w[i], scale, words + 4 * i);
 }
 __device__ __forceinline__ void tmem_store_32_words(uint32_t address, const uint32_t (&v)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -780,10 +790,69 @@ template <int TOKENS> constexpr size_t parts_smem() {
     return 1024 + (size_t)p_stages<TOKENS>() * (p_halves<TOKENS>() * (P_A_BYTES + p_x_bytes<TOKENS>()) + p_slot_scale_bytes<TOKENS>()) + 256;
 }
 
+// With more elements to add than this for every 16 tokens that have some, these tokens take the products below (64 rows: an element costs 0.6
+// to 1 us, 16 tokens there 18 to 45).
+constexpr int LOST_MOST = 32;
+
+// The results of the tokens of a mask (bits of `low` and `high`) whose elements three parts do not hold, from x as it is and codes times their
+// scale in bfloat16 (both exact, mma.sync, sums in float32).  A CTA takes 16 rows of w and 16 of the tokens at a time, its warps a range of K
+// each, whose sums meet in shared memory (`pieces`: 1 KB a warp) in the order of K.  Of 128 elements of K lane (g, t) takes block t: of rows g
+// and g + 8 of w and of the tokens g and g + 8.  It decodes eight codes at a time: with a whole block the kernel has 147 registers a thread
+// instead of 121, the kernel that prepares the next x no longer fits beside it, and every product takes 2.3 us longer.
+template <int WARPS, typename Out>
+__device__ __forceinline__ void wide_products(const bf16* __restrict__ x, Out* __restrict__ out, const Shapes& s, uint32_t low, uint32_t high, float* pieces) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, count = __popc(low) + __popc(high), steps = s.K / HALF_STAGE_K;
+    const int from = (int)((long long)steps * warp / WARPS), to = (int)((long long)steps * (warp + 1) / WARPS);
+    auto token_of = [&](int index) {                // the index-th of them; behind the last the last
+        index = min(index, count - 1);
+        return index < __popc(low) ? (int)__fns(low, 0, index + 1) : 32 + (int)__fns(high, 0, index - __popc(low) + 1);
+    };
+    for (int group = blockIdx.x; group < (s.N + 15) / 16; group += gridDim.x) {
+        const long long n = (long long)group * 16, rows[2] = {min(n + g, (long long)s.N - 1), min(n + g + 8, (long long)s.N - 1)};
+        const uint8_t *codes[2], *scales[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) codes[r] = s.w_codes + rows[r] * (s.K >> 1) + t * 16, scales[r] = s.w_scales + mx_scale_offset(rows[r], 0, s.w_tiles_of_a_row) + t;
+        for (int base = 0; base < count; base += 16) {
+            const bf16 *first = x + (size_t)token_of(base + g) * s.K + t * MX_BLOCK, *second = x + (size_t)token_of(base + 8 + g) * s.K + t * MX_BLOCK;
+            float sums[2][4] = {};
+            for (int q = from; q < to; ++q) {
+                const uint4 held[2] = {*reinterpret_cast<const uint4*>(codes[0] + q * 64), *reinterpret_cast<const uint4*>(codes[1] + q * 64)};
+                const __nv_bfloat162 scale[2] = {scale_pair(scales[0][(size_t)q * MX_TILE_BYTES]), scale_pair(scales[1][(size_t)q * MX_TILE_BYTES])};
+                const uint32_t words[2][4] = {{held[0].x, held[0].y, held[0].z, held[0].w}, {held[1].x, held[1].y, held[1].z, held[1].w}};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {       // eight elements of the block
+                    const uint4 a = *reinterpret_cast<const uint4*>(first + q * HALF_STAGE_K + i * 8), b = *reinterpret_cast<const uint4*>(second + q * HALF_STAGE_K + i * 8);
+                    uint32_t w[2][4];
+                    decode_eight(words[0][i], scale[0], w[0]);
+                    decode_eight(words[1][i], scale[1], w[1]);
+                    const uint32_t even[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, odd[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
+                    mx_mma_bf16(sums[0], even, a.x, a.y);
+                    mx_mma_bf16(sums[1], even, b.x, b.y);
+                    mx_mma_bf16(sums[0], odd, a.z, a.w);
+                    mx_mma_bf16(sums[1], odd, b.z, b.w);
+                }
+            }
+            // [warp][token][row]
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pieces[warp * 256 + ((i >> 2) * 8 + 2 * t + (i & 1)) * 16 + g + (i >> 1 & 1) * 8] = sums[i >> 2][i & 3];
+            __syncthreads();
+            const int index = base + ((int)threadIdx.x >> 4);
+            if (threadIdx.x < 256 && index < count && n + (threadIdx.x & 15) < s.N) {
+                float sum = pieces[threadIdx.x];
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) sum += pieces[w * 256 + threadIdx.x];
+                out[(size_t)token_of(index) * s.N + n + (threadIdx.x & 15)] = from_float<Out>(sum);
+            }
+            __syncthreads();
+        }
+    }
+}
+
 template <int TOKENS, typename Out>
 __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                                                              const bf16* __restrict__ x, const uint8_t* __restrict__ x_scales, Out* __restrict__ out, const Shapes s) {
-    __shared__ uint32_t lost_tokens[3];             // a bit a token with elements to add; whether there are too many
+    __shared__ uint32_t lost_tokens[4];             // a bit a token with elements to add; a bit a token with too many
+    __shared__ int lost_count;                      // elements to add
     static_assert(TOKENS <= 64);
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -805,8 +874,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Walk walk(s);
 
-    if (threadIdx.x < 3) lost_tokens[threadIdx.x] = 0;
+    if (threadIdx.x < 4) lost_tokens[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
+        lost_count = 0;
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&full[i], 2);
             mbar_init(&empty[i], 1);
@@ -919,18 +989,29 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
             __syncwarp();
         }
     } else {
+        int some = 0;
         for (int i = threadIdx.x - 64; i < s.M * s.depth; i += P_STORERS * 32) {
-            const int count = __ldcg(s.lost + i);
-            if (count == MX_LOST_ALL) atomicOr(&lost_tokens[2], 1u);
-            if (count != 0) atomicOr(&lost_tokens[i / s.depth >> 5], 1u << (i / s.depth & 31));
+            const int count = __ldcg(s.lost + i), token = i / s.depth;
+            if (count == 0) continue;
+            atomicOr(&lost_tokens[(count == MX_LOST_ALL ? 2 : 0) + (token >> 5)], 1u << (token & 31));
+            some = min(some + count, 4 * LOST_MOST + 1);
+        }
+        if (some) atomicAdd(&lost_count, some);
+        asm volatile("bar.sync 1, %0;" ::"n"(P_STORERS * 32) : "memory");
+        if (threadIdx.x == 64) {                    // a token is in one of the two sets
+            const uint32_t all[2] = {lost_tokens[0] | lost_tokens[2], lost_tokens[1] | lost_tokens[3]};
+            const bool many = lost_count > LOST_MOST * ((__popc(all[0]) + __popc(all[1]) + 15) / 16);
+            for (int i = 0; i < 2; ++i) {
+                if (many) lost_tokens[2 + i] = all[i];
+                lost_tokens[i] = all[i] & ~lost_tokens[2 + i];
+            }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(P_STORERS * 32) : "memory");
         for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
             if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
             tcgen05_fence_after_sync();
-            if (lost_tokens[2] == 0)
-                store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr, lost_tokens);
+            store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr, lost_tokens);
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buffer]);
@@ -943,40 +1024,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
         tcgen05_fence_after_sync();
         tmem_dealloc(tmem, TMEM_COLUMNS);
     }
-    if (lost_tokens[2] != 0) {
-        // Too many elements that three parts do not hold: a thread a row of w and every third token, the products of a bfloat16 and a code
-        // times its power of two exact, sums in float32.
-        const long long code_pitch = s.K >> 1;
-        constexpr int LANES = P_THREADS / BM;                                           // threads a row
-        const int part = threadIdx.x / BM;
-        for (int tile = blockIdx.x; part < LANES && tile < s.units / s.depth; tile += gridDim.x) {
-            const long long n = (long long)tile * BM + (threadIdx.x & (BM - 1));
-            if (n >= s.N) continue;
-            for (int token = part; token < s.M; token += LANES) {
-                float sum = 0.0f;
-                for (int block = 0; block < s.K / MX_BLOCK; ++block) {
-                    const uint4 c = *reinterpret_cast<const uint4*>(s.w_codes + n * code_pitch + block * 16);
-                    const float scale = mx_scale(s.w_scales[mx_scale_offset(n, block >> 2, s.w_tiles_of_a_row) + (block & 3)]);
-                    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-                    const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)token * s.K + block * MX_BLOCK);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t h[4];
-                        mx_decode_8(words[i], h);
-                        const uint4 raw = from[i];
-                        const uint32_t pairs[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            const float2 w = __half22float2(*reinterpret_cast<__half2*>(&h[p]));
-                            sum = fmaf(__uint_as_float(pairs[p] << 16), w.x * scale, sum);
-                            sum = fmaf(__uint_as_float(pairs[p] & 0xFFFF0000u), w.y * scale, sum);
-                        }
-                    }
-                }
-                out[(size_t)token * s.N + n] = from_float<Out>(sum);
-            }
-        }
-    }
+    if (lost_tokens[2] | lost_tokens[3]) wide_products<P_THREADS / 32>(x, out, s, lost_tokens[2], lost_tokens[3], reinterpret_cast<float*>(smem));
 }
 
 // ------------------------------------------------------------------------------------------

@@ -557,3 +557,38 @@ def test_an_output_over_the_weights_is_refused(m, quantise):
     for begin in (0, size + bytes_):
         kernels.mxfp4_gemm(x, weight, out(begin), quantise=quantise)
         assert torch.equal(out(begin), want) and torch.equal(weight.data, before)
+
+
+WIDE_PLANS = [("parts", 16, 5, False), ("parts", 16, 9, True), ("parts", 32, 4, False), ("parts", 32, 7, True), ("parts", 64, 3, False), ("parts", 64, 6, True)]
+
+
+@pytest.mark.parametrize("plan", WIDE_PLANS)
+@pytest.mark.parametrize("kind", ["far", "infinite", "nan"])
+@pytest.mark.parametrize("n,k", [(390, 1280), (133, 128), (17, 640)])
+def test_rows_that_parts_do_not_hold_beside_others(n, k, kind, plan):
+    """One row, the last, a few, more than sixteen or all of a batch have elements that three parts do not hold, nine and more in 256, or two
+    each that are too many together: what belongs to each row is right, and the other rows' results have the bits that they have without."""
+    m = plan[1] - 1
+    g = torch.Generator(device=DEV).manual_seed(n + k + plan[1])
+    codes, scales, w = random_matrix(g, n, k)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    plan = fitting(plan, m, n, k)
+    plain = torch.randn(m, k, device=DEV, generator=g).bfloat16()
+    without = torch.full((m, n), 7.0, device=DEV)
+    kernels.mxfp4_gemm(plain, weight, without, plan=plan)
+    order = torch.randperm(m, device=DEV, generator=g).tolist()
+    for rows in ([m - 1], order[:1], order[:3], order[:17], order):
+        for each in (2, 9, k):
+            x = plain.float()
+            columns = torch.randperm(k, device=DEV, generator=g)[:each]
+            for row in rows:
+                if kind == "far":
+                    x[row, columns] *= 2.0 ** -45
+                else:
+                    x[row, columns[::2]] = math.inf if kind == "infinite" else math.nan
+                    x[row, columns[1::2]] *= 2.0 ** 60
+            check_product(x.bfloat16(), weight, w, False, plan, f"{len(rows)} rows {each}")
+            out = torch.full((m, n), 7.0, device=DEV)
+            kernels.mxfp4_gemm(x.bfloat16(), weight, out, plan=plan)
+            others = sorted(set(range(m)) - set(rows))
+            assert torch.equal(out[others], without[others]), f"{len(rows)} rows {each}"
