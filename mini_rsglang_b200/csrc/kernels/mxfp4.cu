@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __r
 // Rows of bfloat16 as halfs times a power of two of the row's own: row r holds x 2^-exponents[r], its largest in [2^15, 2^16).  An element's
 // exponent field becomes itself less that of the largest, plus 30, its mantissa its seven bits and three zeros: exact, but for elements
 // 2^30 and more below the largest, which become 0 and are noted (a few in a prompt's products of gate and up), rows below 2^-96 and what
-// is not finite.  factors[r] is 16 times the exponent plus the number of noted elements, up to 15; HALFS_LOST if there are more than fit or
-// the row is one of the others, and not to be used.
+// is not finite.  factors[r] is the exponent in the upper bits and the number of noted elements in the lower ones (mxfp4.cuh); HALFS_LOST if there
+// are more than fit or the row is one of the others, and not to be used.
 constexpr int HELD = 4;
 constexpr int HALFS_LOST = INT_MIN;
 __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __restrict__ x, uint16_t* __restrict__ halfs, int* __restrict__ factors,
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
         }
         bad = __syncthreads_or(bad);
     }
-    if (threadIdx.x == 0) factors[row] = bad ? HALFS_LOST : 16 * (empty ? 0 : field - 127 - 15) + min(number, 15);
+    if (threadIdx.x == 0) factors[row] = bad ? HALFS_LOST : (empty ? 0 : field - 127 - 15) * (1 << MX_NOTED_BITS) + min(number, MX_NOTED);
 }
 
 // Up to `tokens` rows of bfloat16 as three parts of E5M2 (three bits of significand, exponents of -16 to 15) each, part p of row r at row

@@ -63,6 +63,8 @@ constexpr int MX_LOST = 8, MX_LOST_ALL = 255;
 __host__ __device__ __forceinline__ const uint32_t* mx_lost_entries(const int* counts, long long stretches) {
     return reinterpret_cast<const uint32_t*>(counts) + (stretches + 3) / 4 * 4;
 }
+// What a row as halfs is described by: a power of two and how many of its elements are noted (up to MX_NOTED), in one number.
+constexpr int MX_NOTED_BITS = 10, MX_NOTED = (1 << MX_NOTED_BITS) - 1;
 // By a whole warp, eight elements a lane, those of `mask` lost; true if they are too many.
 __device__ __forceinline__ bool mx_note_lost(uint32_t mask, const uint4& raw, long long stretch, int* counts, long long stretches) {
     const int lane = threadIdx.x & 31;

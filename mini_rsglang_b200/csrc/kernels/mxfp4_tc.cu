@@ -12,7 +12,7 @@
 //                    clocks for eight codes of a warp), bfloat16 goes through float32 (21 clocks).  So x comes as halfs, times a
 //                    power of two a row, from a kernel before (mxfp4.cu), and w becomes halfs times one power of two of the matrix;
 //                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
-//                    for halfs are added one by one to the sums (lost_products), and where there are too many of them (LOST_SHARE),
+//                    for halfs are added one by one to the sums (lost_products), and where there are too many of them (most_lost),
 //                    or the matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead (a sixth slower).
 //                    24,576 x 4,096 times 2,048 rows: 303 us, 1.36 PFLOP/s; the tensor pipe is busy 78% of the time at the 1.43 GHz that
 //                    the power cap leaves.
@@ -84,6 +84,7 @@ struct Shapes {
     int early;                  // w was there before the kernel before this one: it may be fetched while that runs
     long long w_tiles_of_a_row, x_row_tiles;
     const int* x_factors;       // of x as halfs (mxfp4.cu), a row each; null: x is bfloat16
+    int lost_most;              // with more elements than this to add, bfloat16 operands are faster
     int w_exponent;             // halfs are made of w times 2^-w_exponent
     const int* lost;            // elements that halfs or parts do not hold (mxfp4.cuh)
     const uint8_t *w_codes, *w_scales;
@@ -179,9 +180,9 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
     auto finish = [&](int c, float (&v)[STEP]) {
         if (halfs) {                               // powers of two in the floats' range, a lane each, by way of shared memory
             const int lane = threadIdx.x & 31;
-            const int factor = lane < STEP && c + lane < live ? __ldcg(s.x_factors + token0 + c + lane) : -16 * s.w_exponent;
+            const int factor = lane < STEP && c + lane < live ? __ldcg(s.x_factors + token0 + c + lane) : -s.w_exponent * (1 << MX_NOTED_BITS);
             __syncwarp();
-            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (factor >> 4)) << 23);
+            if (lane < STEP) factors[lane] = __uint_as_float((uint32_t)(127 + s.w_exponent + (factor >> MX_NOTED_BITS)) << 23);
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < STEP; e += 4) {
@@ -211,12 +212,12 @@ __device__ __forceinline__ void store_accumulator(uint32_t accumulator, Out* __r
             int factor = 0;
             if constexpr (PARTS) factor = (lost[c >> 5] >> ((c + lane) & 31)) & (lane < STEP ? 1u : 0u);
             else if (lane < STEP && c + lane < live) factor = __ldcg(s.x_factors + token0 + c + lane);
-            for (uint32_t some = __ballot_sync(0xffffffffu, factor & 15); some; some &= some - 1) {
+            for (uint32_t some = __ballot_sync(0xffffffffu, factor & MX_NOTED); some; some &= some - 1) {
                 const int at = __ffs(some) - 1;
                 const long long of = n < s.N ? n : s.N - 1, token = token0 + c + at;
                 float more = lost_products(s.lost + token * s.depth, mx_lost_entries(s.lost, (long long)s.M * s.depth) + token * s.depth * MX_LOST, s.depth,
                                            s.w_codes + of * (s.K >> 1), s.w_scales + mx_scale_offset(of, 0, s.w_tiles_of_a_row));
-                if constexpr (!PARTS) more *= __uint_as_float((uint32_t)(127 - s.w_exponent - (__shfl_sync(0xffffffffu, factor, at) >> 4)) << 23);
+                if constexpr (!PARTS) more *= __uint_as_float((uint32_t)(127 - s.w_exponent - (__shfl_sync(0xffffffffu, factor, at) >> MX_NOTED_BITS)) << 23);
                 add_to_column(acc + c + at, more);
             }
         }
@@ -296,9 +297,18 @@ template <int TOKENS> constexpr int step_k() { return TOKENS <= 64 ? 256 : 128; 
 // to 22,000 clocks a tile, its MMAs 6,200), these 506; 24,576 x 4,096 took 301 and 305.
 constexpr int MAKERS = 8, STORERS = 8;
 constexpr int W_THREADS = (3 + MAKERS + STORERS) * 32;
-// Bfloat16 is ahead of halfs when one in so many rows has an element to add (24,576 x 4,096 times 2,048 rows: none 300 us, one in 64 rows
-// 304, in 16 310, in 8 338, in 4 468; bfloat16 346.  4,096 x 12,288: 183, 189, 200, 223, 266; 206).
-constexpr int LOST_SHARE = 16;
+// How many elements the storing warps may add one by one before bfloat16 operands are faster for all.  These cost 0.1 to 0.15 us for each of the
+// `stages` of the CTA with most of them, with up to 128 tokens, where making A counts for more, 0.3.  An element takes the warps that store its
+// tile of tokens 0.5 to 1 us, the first one 1 to 2 more; of several tiles a CTA only the last one's wait is not hidden behind MMAs, but for short
+// tiles, whose results take as long to store as they take.
+// Measured (us, without any / some in a row each, in few rows / bfloat16 operands):
+//   24,576 x 4,096: 2,048 rows 305 / 64: 314, 313 / 338, 512 rows 83 / 8: 86, 88 / 92, 200 rows 55 / 8: 61, 62 / 70, 100 rows 39 / 3: 43, 43 / 49;
+//   4,096 x 12,288: 2,048 rows 188 / 64: 199, 196 / 202, 512 rows 55 / 24: 66, 64 / 71, 200 rows 40 / 3: 45, 43 / 46;
+//   6,145 x 4,096: 485 rows 27.0 / 1: 29.2 / 28.3; 151,936 x 1,024: 700 rows 187 / 1: 237 / 203; 24,576 x 4,128: 24 rows 31 / 3: 37, 35 / 38.
+inline int most_lost(int tokens, int token_tiles, int stages, int depth) {
+    const int hidden = stages > depth ? depth - 6 : depth, tile = tokens > 128 ? stages / 10 - 2 : stages / 5 - 1;
+    return max(0, min(hidden, tile)) * token_tiles;
+}
 template <int TOKENS> constexpr int a_columns() { return step_k<TOKENS>() / 2; }
 template <int TOKENS> constexpr int x_bytes() { return TOKENS * step_k<TOKENS>() * 2; }
 template <int TOKENS> constexpr int x_stages() { return TOKENS > 128 ? 3 : 4; }
@@ -437,12 +447,12 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
         bool fit = true;
         int some = 0;
         for (int i = threadIdx.x; i < s.M; i += W_THREADS) {
-            const int factor = s.x_factors[i], e = factor >> 4;
+            const int factor = s.x_factors[i], e = factor >> MX_NOTED_BITS;
             fit = fit && factor != INT_MIN && e + s.w_exponent >= -126 && e + s.w_exponent <= 126;
-            some += factor & 15;
+            some = min(some + (factor & MX_NOTED), 1 << 20);
         }
         if (some) atomicAdd(&lost_count, some);
-        halfs = __syncthreads_and(fit) && lost_count <= s.M / LOST_SHARE;
+        halfs = __syncthreads_and(fit) && lost_count <= s.lost_most;
         lost = halfs && lost_count != 0;
     }
 
@@ -1069,6 +1079,8 @@ int launch_weights(const void* x, const void* x_halfs, void* out, Shapes s, int 
     if (code) return code;
     static PerDevice configured;
     if (!lay_out<TOKENS>(s, ctas)) return MRS_BAD_ARGUMENT;
+    const int stages = s.scratch ? (int)(((long long)s.units + ctas - 1) / ctas) : (s.units / s.depth + ctas - 1) / ctas * s.depth;
+    s.lost_most = most_lost(TOKENS, s.token_tiles, stages, s.depth);
     return launch_run(weights_kernel<TOKENS, Out>, configured, W_THREADS, ctas, weights_smem<TOKENS>(), stream, w_map, x_map, halfs_map, s.w_scales, (Out*)out, s);
 }
 template <int TOKENS, typename Out>

@@ -592,3 +592,26 @@ def test_rows_that_parts_do_not_hold_beside_others(n, k, kind, plan):
             kernels.mxfp4_gemm(x.bfloat16(), weight, out, plan=plan)
             others = sorted(set(range(m)) - set(rows))
             assert torch.equal(out[others], without[others]), f"{len(rows)} rows {each}"
+
+
+@pytest.mark.parametrize("m,n,k,rows,each", [(300, 390, 4096, 1, 40), (300, 390, 4096, 7, 3), (300, 390, 4096, 300, 1), (2048, 24576, 4096, 8, 12), (2048, 24576, 4096, 110, 1),
+                                             (2048, 24576, 4096, 111, 1), (2048, 24576, 4096, 8, 128), (100, 24576, 4096, 1, 5), (100, 24576, 4096, 3, 2), (11, 4096, 4128, 1, 1)])
+def test_either_operand_for_rows_with_elements_far_below(m, n, k, rows, each):
+    """Few elements in many rows and many in few (more in a row than a number of four bits counts), on both sides of what changes the whole
+    product's operands.  They alone meet codes that are not zero."""
+    g = torch.Generator(device=DEV).manual_seed(m + k + rows)
+    codes, scales, _ = random_matrix(g, n, k)
+    order = torch.randperm(k // 256, device=DEV, generator=g)                # no more than eight in 256 elements of a row
+    nonzero = (order[:, None] * 256 + torch.arange(3, 256, 32, device=DEV)[None, :]).T.reshape(-1)[:each]
+    keep = torch.zeros(k, dtype=torch.bool, device=DEV)
+    keep[nonzero] = True
+    codes = codes & (torch.where(keep[0::2], 0x0F, 0) | torch.where(keep[1::2], 0xF0, 0)).to(torch.uint8)
+    x = torch.randn(m, k, device=DEV, generator=g)
+    x[:, nonzero] = 0.0
+    for row in torch.randperm(m, device=DEV, generator=g)[:rows].tolist():
+        x[row, nonzero] = torch.randn(each, device=DEV, generator=g) * 2.0 ** -50
+    x = x.bfloat16()
+    weight, w = kernels.mxfp4_matrix(codes, scales), plain_values(codes, scales)[:, nonzero]
+    out = torch.full((m, n), 7.0, device=DEV)
+    kernels.mxfp4_gemm(x, weight, out)
+    close_to_sums(out, x[:, nonzero].double() @ w.T, x[:, nonzero].double().abs() @ w.abs().T, k, f"{rows} rows {each}")
