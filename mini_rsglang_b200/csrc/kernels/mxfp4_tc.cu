@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) weights_kernel(const __grid_cons
     } else {
         for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
-            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
+            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1) && !s.scratch) break;      // of shared tiles the others meet this warp at barriers
             tcgen05_fence_after_sync();
             store_accumulator<TOKENS, STORERS, Out>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2 - MAKERS, halfs, flag, factors + (warp - 2 - MAKERS) * 32,
                                                    lost ? reinterpret_cast<const uint32_t*>(s.lost) : nullptr);
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) both_kernel(const __grid_constan
         pdl_wait();
         for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
-            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
+            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1) && !s.scratch) break;      // of shared tiles the others meet this warp at barriers
             tcgen05_fence_after_sync();
             store_accumulator<TOKENS, B_STORERS, Out>(tmem + buffer * B_ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr);
             tcgen05_fence_before_sync();
@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) parts_kernel(const __grid_consta
         asm volatile("bar.sync 1, %0;" ::"n"(P_STORERS * 32) : "memory");
         for (int round = 0; walk.step(s); ++round) {
             const int buffer = round & 1;
-            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1)) break;
+            if (!warp_wait(&acc_full[buffer], (round >> 1) & 1) && !s.scratch) break;      // of shared tiles the others meet this warp at barriers
             tcgen05_fence_after_sync();
             store_accumulator<TOKENS, P_STORERS, Out, true>(tmem + buffer * ACCUMULATOR, out, s, walk, warp - 2, false, flag, nullptr, lost_tokens);
             tcgen05_fence_before_sync();
