@@ -2833,30 +2833,32 @@ def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool
         raise InvalidRequest("mxfp4_gemm: out must be bfloat16 or float32")
     _need(x, torch.bfloat16, "mxfp4_gemm input")
     _need(out, None, "mxfp4_gemm out", (m, n))
-    here = x.get_device()
-    if here != weight.data.get_device() or here != out.get_device():
+    here, held = x.get_device(), weight.data
+    if here != held.get_device() or here != out.get_device():
         raise InvalidRequest("mxfp4_gemm: input, weights and output are on different devices")
     if m == 0 or n == 0:
         return
     _mxfp4_aligned(x, "mxfp4_gemm input")
-    x_at, out_at = x.data_ptr(), out.data_ptr()
-    w_codes, w_scales = weight.addresses()
-    out_end = out_at + out.element_size() * m * n
+    x_at, out_at, w_codes = x.data_ptr(), out.data_ptr(), held.data_ptr()
+    w_scales, out_end = w_codes + n * (k >> 1), out_at + out.element_size() * m * n
     if x_at < out_end and out_at < x_at + 2 * m * k:
         raise InvalidRequest("mxfp4_gemm: the output overlaps the input")
-    if w_codes < out_end and out_at < w_codes + weight.bytes():
+    if w_codes < out_end and out_at < w_codes + held.numel():
         raise InvalidRequest("mxfp4_gemm: the output overlaps the weights")
     if here != _current_device():
         with torch.cuda.device(here):
             return mxfp4_gemm(x, weight, out, quantise, plan)
     lib = mxfp4_library()
-    out_f32, early = int(out.dtype is torch.float32), int(weight.settled)
+    out_f32, early, quantise = out.dtype is torch.float32, weight.settled, bool(quantise)
     sms, stream = sm_count(here), _stream_here(here)
     if plan is None:
-        plan = mxfp4_plan(m, n, k, bool(quantise), sms)
-    fits, exponent = weight.half_exponent is not None, weight.half_exponent or 0
+        plan = mxfp4_plan(m, n, k, quantise, sms)
+    exponent = weight.half_exponent
+    fits = exponent is not None
+    if not fits:
+        exponent = 0
     if plan[0] == "few":
-        code = lib.mrs_mxfp4_few_rows(x_at, w_codes, w_scales, out_at, out_f32, m, n, k, int(bool(quantise)), plan[1], sms, fits, exponent, early, stream)
+        code = lib.mrs_mxfp4_few_rows(x_at, w_codes, w_scales, out_at, out_f32, m, n, k, quantise, plan[1], sms, fits, exponent, early, stream)
     else:
         kind, tokens, ctas, shared = plan
         form = 2 if quantise else 0 if kind == "parts" else 1
