@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(THREADS) scale_range_kernel(const uint8_t* __r
 
 // Rows of bfloat16 as halfs times a power of two of the row's own: row r holds x 2^-exponents[r], its largest in [2^15, 2^16).  An element's
 // exponent field becomes itself less that of the largest, plus 30, its mantissa its seven bits and three zeros: exact, but for elements
-// 2^30 and more below the largest, which become 0 and are noted (a few in a prompt's products of gate and up), rows below 2^-96 and what
-// is not finite.  factors[r] is the exponent in the upper bits and the number of noted elements in the lower ones (mxfp4.cuh); HALFS_LOST if there
+// 2^30 and more below the largest, which become 0 and are noted (a few in a prompt's products of gate and up), and rows below 2^-96.  Of a row
+// with infinities or NaN these are held beside zeros (mxfp4.cuh).  factors[r] is the exponent in the upper bits and the number of noted elements in the lower ones (mxfp4.cuh); HALFS_LOST if there
 // are more than fit or the row is one of the others, and not to be used.
 constexpr int HELD = 4;
 constexpr int HALFS_LOST = INT_MIN;
@@ -269,6 +269,14 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
     const int field = (int)(largest >> 7);
     const bool empty = largest == 0, ordinary = field >= 31 && field < 255;
     const uint32_t down = empty || !ordinary ? 0u : (uint32_t)(-((field - 30) << 7)) & 0xFFFFu, both = down | down << 16;
+    if (field == 255) {
+        for (int i = threadIdx.x; i < chunks; i += THREADS) {
+            const uint4 v = from[i];
+            to[i] = make_uint4(mx_not_finite_pair(v.x), mx_not_finite_pair(v.y), mx_not_finite_pair(v.z), mx_not_finite_pair(v.w));
+        }
+        if (threadIdx.x == 0) factors[row] = 0;
+        return;
+    }
     uint32_t lost = 0;
     auto convert = [&](const uint4& v, uint32_t* gone) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -312,14 +320,14 @@ __global__ void __launch_bounds__(THREADS) rows_to_halfs_kernel(const bf16* __re
         }
         bad = __syncthreads_or(bad);
     }
-    if (threadIdx.x == 0) factors[row] = bad ? HALFS_LOST : (empty ? 0 : field - 127 - 15) * (1 << MX_NOTED_BITS) + min(number, MX_NOTED);
+    if (threadIdx.x == 0) factors[row] = bad ? HALFS_LOST : (ordinary ? field - 127 - 15 : 0) * (1 << MX_NOTED_BITS) + min(number, MX_NOTED);
 }
 
 // Up to `tokens` rows of bfloat16 as three parts of E5M2 (three bits of significand, exponents of -16 to 15) each, part p of row r at row
 // p * tokens + r, with a power of two for 32 neighbours in scale tiles (mxfp4.cuh) of these 3 * tokens rows.  With 2^(e - 14) for a block
 // whose largest size has the exponent e, x = (a + b + c 2^-8) 2^(e - 14): a is x rounded, b what is left of it rounded, c, with
 // a power 2^-8 further down, the rest: of eight bits three, three signed and two are enough down to 2^-26 of the largest.  Elements of
-// which that is not so, infinities and NaN among them, are 0 in all parts and noted.
+// which that is not so are 0 in all parts and noted.  Infinities and NaN are what they are in the first part, beside zeros in their block (mxfp4.cuh).
 constexpr int PART_SHIFT = 8;
 __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __restrict__ x, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
                                                                 int* __restrict__ lost, int rows, int width, int tokens, int stretches, int* __restrict__ zeros,
@@ -361,6 +369,12 @@ __global__ void __launch_bounds__(THREADS) rows_to_parts_kernel(const bf16* __re
         a[i >> 2] |= first << (8 * (i & 3));
         b[i >> 2] |= second << (8 * (i & 3));
         c[i >> 2] |= third << (8 * (i & 3));
+    }
+    if (e == 128) {
+        const uint32_t w[4] = {held.raw.x, held.raw.y, held.raw.z, held.raw.w};
+        mask = a[0] = a[1] = b[0] = b[1] = c[0] = c[1] = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) a[p >> 1] |= __byte_perm(mx_not_finite_pair(w[p]), 0, 0x4431) << (16 * (p & 1));
     }
     if (column < width) {
         *reinterpret_cast<uint2*>(parts + (size_t)row * width + column) = make_uint2(a[0], a[1]);

@@ -57,6 +57,20 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t largest) {
     const int exponent = (int)(largest >> 23);
     return exponent == 255 ? 255u : (uint32_t)max(exponent - 2, 0);
 }
+
+// An infinity or NaN of x decides its row's results by itself: the products of finite elements with finite weights change nothing of an
+// infinity or NaN among the others (an infinity times a weight of 0 is none either).  So halfs and parts hold the infinities and NaN of a row, or
+// of a block of it, beside zeros, and what a row has of them costs nothing.  A pair of bfloat16 as such halfs (halfs' upper bytes are E5M2):
+__device__ __forceinline__ uint32_t mx_not_finite_pair(uint32_t pair) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t v = (pair >> (16 * i)) & 0xFFFFu, size = v & 0x7FFFu;
+        if (size >= 0x7F80u) out |= ((v & 0x8000u) | (size == 0x7F80u ? 0x7C00u : 0x7E00u)) << (16 * i);
+    }
+    return out;
+}
+
 // Elements of x that another form of its rows (halfs, parts) does not hold, noted by stretches of 256 elements: how many a stretch has, or
 // MX_LOST_ALL if more than MX_LOST, and behind all counts MX_LOST words a stretch, place in it << 16 | bfloat16.  The product adds theirs.
 constexpr int MX_LOST = 8, MX_LOST_ALL = 255;

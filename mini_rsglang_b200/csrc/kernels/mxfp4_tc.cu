@@ -25,7 +25,8 @@
 //                    operand is the codes, brought into bytes by the bulk tensor copies: nobody makes anything of w.  The three
 //                    columns' sums are the result's.  A few elements that three parts do not hold are added one by one as well; rows with
 //                    more than 8 of them in 256 elements, and all such rows where they are more than LOST_MOST, are computed from bfloat16
-//                    on mma.sync (wide_products), the others as ever: what one request's row holds costs its neighbours little.
+//                    on mma.sync (wide_products), the others as ever: what one request's row holds costs its neighbours little, infinities
+//                    and NaN nothing (E5M2 has both).
 //                    24,576 x 4,096 times 64 rows: none 24 us, 1 element 25, 32 in as many rows 55, one such row 64, 64 such rows 206; 4,096 x
 //                    12,288: 22, 23, 43, 40, 101.  (In a decode step of 64 tokens some element of silu(gate) * up nearly always is 2^26
 //                    below its neighbours.  The CUDA cores took 3.5 and 5.3 ms for all rows as soon as one row had too many.)

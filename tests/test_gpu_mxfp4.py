@@ -615,3 +615,46 @@ def test_either_operand_for_rows_with_elements_far_below(m, n, k, rows, each):
     out = torch.full((m, n), 7.0, device=DEV)
     kernels.mxfp4_gemm(x, weight, out)
     close_to_sums(out, x[:, nonzero].double() @ w.T, x[:, nonzero].double().abs() @ w.abs().T, k, f"{rows} rows {each}")
+
+
+@pytest.mark.parametrize("plan,quantise", [(plan, q) for plan in SOME_PLANS + [("few", 8), ("parts", 32, 3, True), ("many", 16, 4, True)] for q in (False, True) if takes(plan, 8, 640, q)])
+@pytest.mark.parametrize("kind", ["infinity", "infinities", "nan", "all nan", "both", "all infinite", "beside far"])
+def test_rows_that_are_not_finite_beside_others(kind, plan, quantise):
+    """An infinity or NaN decides its own row, whatever else is in it and whether it meets weights of zero, and leaves the others what they are."""
+    m, n, k = 8, 150, 1408
+    g = torch.Generator(device=DEV).manual_seed(len(kind))
+    codes, scales, _ = random_matrix(g, n, k)
+    codes[::2, 100:140] = 0                                    # weights of zero: infinity times these is none
+    codes[1::4, 100:140] &= 0x70
+    scales[5, 7] = 255
+    w = plain_values(codes, scales)
+    weight = kernels.mxfp4_matrix(codes, scales)
+    x = torch.randn(m, k, device=DEV, generator=g)
+    x[:, 64:96] = 0.0
+    plain = torch.full((m, n), 7.0, device=DEV)
+    kernels.mxfp4_gemm(x.bfloat16(), weight, plain, quantise=quantise, plan=plan)
+    for row in (6, 2):                                         # first one such row, then two
+        if kind == "infinity":
+            x[row, 3] = -math.inf
+        elif kind == "infinities":
+            x[row, [5, 6, 900]] = math.inf
+            x[row, 1200] = -math.inf if row == 2 else math.inf
+        elif kind == "nan":
+            x[row, k - 1] = math.nan
+        elif kind == "all nan":
+            x[row] = -math.nan
+        elif kind == "both":
+            x[row, 200], x[row, 210], x[row, 700] = math.inf, -math.inf, math.nan
+        elif kind == "all infinite":
+            x[row] = math.inf
+        else:
+            x[row] *= torch.exp2(torch.randint(-60, 60, (k,), device=DEV, generator=g).float())
+            x[row, 77] = math.inf
+        check_product(x.bfloat16(), weight, w, quantise, plan, kind)
+        out = torch.full((m, n), 7.0, device=DEV)
+        kernels.mxfp4_gemm(x.bfloat16(), weight, out, quantise=quantise, plan=plan)
+        others = [i for i in range(m) if i != row and (i != 6 or row != 2)]
+        columns = [i for i in range(n) if i != 5]              # a row of w that is not a number is none for every row of x
+        assert out[:, 5].isnan().all()
+        if plan[0] != "few":                                   # there such a row brings the others' stages to bfloat16: another order of their sums
+            assert torch.equal(out[others][:, columns], plain[others][:, columns])
