@@ -36,6 +36,7 @@ class StepContext:
     # when every sequence brings one token: [B, 4] int32 attention tiles (sequence, row, 1, 0), zeros for padding
     decode_tiles: torch.Tensor | None = None
     real_sequences: int = 0            # sequences that are not padding (padding rows come last)
+    fixed_rows: bool = False           # its rows are filled up to a fixed number: the last ones may belong to no sequence
     want_every_row: bool = False       # `want_rows` is 0, 1, ..., T - 1
     # Layer-by-layer inspection (the reference's observer, crates/models/src/qwen3.rs:159-229): when set, the
     # model calls observe(label, tensor [T, width]) with what the reference's observer sees under the same

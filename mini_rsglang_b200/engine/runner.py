@@ -308,7 +308,7 @@ class ModelRunner:
             host_state_slots=[self.cache.slot(s.request_id) for s in sequences] + [-1] * pads if self._needs_host_slots else [],
             max_query_len=int(layout[13 + 3 * G]), max_context_len=int(layout[12 + 3 * G]),
             fresh=(starts == 0).tolist() + [True] * pads,
-            decode_tiles=dview(layout[11], 4 * B, (B, 4)) if decode else None, real_sequences=real,
+            decode_tiles=dview(layout[11], 4 * B, (B, 4)) if decode else None, real_sequences=real, fixed_rows=pad_to is not None,
             want_every_row=bool(decode) and R == T, facts=facts, plan_views=plan_views, layout_words=used)
 
     def forward(self, sequences: Sequence[SequenceStep], observe=None, carried=None) -> torch.Tensor | None:

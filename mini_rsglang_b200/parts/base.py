@@ -125,10 +125,19 @@ class Runtime:
     page_size: int = 16
     weight_format: str = "held"        # "mxfp4": projections that can be are held in 4 bits (`parts.linear.projection`)
     activation_format: str = "held"    # "mxfp4": and read their input in 4 bits
+    _standing: dict = field(default_factory=dict, repr=False, compare=False)
 
     @property
     def is_bf16(self) -> bool:
         return self.dtype is torch.bfloat16
+
+    def standing_rows(self, rows: int, width: int) -> torch.Tensor:
+        """Rows [rows, width] of this model's own, at one address for a number of rows: zeros to begin with, then what steps left there.  For what
+        is written and read within a layer and leaves rows of recorded steps out.  First asked for outside a recording."""
+        held = max(16, 1 << (rows - 1).bit_length())
+        if (held, width) not in self._standing:
+            self._standing[held, width] = torch.zeros((held, width), dtype=self.dtype, device=self.device)
+        return self._standing[held, width][:rows]
 
 
 @dataclass

@@ -158,3 +158,35 @@ def test_real_layer_sizes(real_size_folder):
     want = P.logits_of_sequence(P.PlainConfig.load(real_size_folder), plain_weights(real_size_folder), tokens)
     runner = ModelRunner.load(real_size_folder, limits=RuntimeConfig(max_seq_len=512, max_running=2, weight_format="mxfp4"), num_pages=32)
     T.check_rows(feed(runner, 1, tokens, [60, 1, 1, 8]), want, "bfloat16", "real sizes")
+
+
+@pytest.mark.parametrize("activations", ["held", "mxfp4"])
+def test_padding_rows_are_ordinary_numbers(folder, activations, monkeypatch):
+    """Recorded steps have rows that belong to no sequence and are in no attention tile.  What the memory held before reaches no product: one row far from
+    the others, or not finite, would choose the operands of all."""
+    monkeypatch.setattr(torch, "empty_like", lambda t, **kwargs: torch.full_like(t, float("nan"), **kwargs))
+    seen = {}
+    product = kernels.mxfp4_gemm
+
+    def watched(x, weight, out, quantise=False, plan=None):
+        product(x, weight, out, quantise=quantise, plan=plan)
+        if torch.cuda.is_current_stream_capturing():
+            seen.setdefault(x.shape[0], []).append(x.clone())
+
+    monkeypatch.setattr(kernels, "mxfp4_gemm", watched)
+    runner = runner_for(folder, activations)
+    tokens = [(29 * i + 3) % CONFIG["vocab_size"] for i in range(90)]
+
+    def step(batch, rows):
+        assert runner.step(batch).isfinite().all()
+        assert len(seen[rows]) == 4 * CONFIG["num_hidden_layers"] and all(x.isfinite().all() for x in seen[rows])
+
+    for request, n, rows in ((1, 30, 32), (2, 3, 16), (3, 17, 32)):
+        runner.cache.open(request)
+        runner.cache.extend(request, n)
+        step([SequenceStep(request, tokens[:n], 0, [n - 1])], rows)
+    for k in range(3):                                             # three decoded tokens in a step of four
+        for request, n in ((1, 30), (2, 3), (3, 17)):
+            runner.cache.extend(request, n + k + 1)
+        step([SequenceStep(request, [tokens[n + k]], n + k, [0]) for request, n in ((1, 30), (2, 3), (3, 17))], 4)
+    assert runner.recorded_steps == 6
