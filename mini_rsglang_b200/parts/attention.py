@@ -17,7 +17,7 @@ from .. import kernels
 from ..errors import InvalidRequest
 from ..weights.spec import WeightSpec
 from .base import MIXERS, NORMS, POSITION_ENCODINGS, KVNeed, Mixer, PartSpec, Prenormed, StepFacts, observing
-from .linear import FourBitWeight, few_rows, linear, projection
+from .linear import few_rows, linear, projection
 
 
 @dataclass
@@ -431,10 +431,7 @@ class GroupedQueryAttention(Mixer):
             self.q_norm.weight if self.q_norm else None, self.k_norm.weight if self.k_norm else None, eps,
             self.inv_freq, self.nq, self.nkv, self.d, cache.k.shape[2],
             rotations=self.position.rotations(ctx) if self.d in (64, 128, 256) else None)
-        # The last rows of a recorded step may be in no attention tile.  A product with weights in 4 bits looks at all rows' sizes before it
-        # chooses its operands, so what the memory held before must not be among them.
-        standing = ctx.fixed_rows and isinstance(self.o, FourBitWeight)
-        out = self.runtime.standing_rows(tokens, self.nq * self.d) if standing else torch.empty_like(q)
+        out = self.rows_of_sequences(ctx, "heads", tokens, self.nq * self.d, q.dtype)
         paged_attention(q, cache, ctx, out, self.nq, self.nkv, self.d, self.window)
         if observing(ctx):
             self._observe_rotated(q, out, cache, ctx, write_cache)

@@ -236,9 +236,7 @@ class BiasedWindowAttention(Mixer):
 
     def _attend(self, q, proj, gate, ctx, cache):
         """The attention over the pages and the output projection; `gate`: the heads' gates, if there are such."""
-        tokens = q.shape[0]
-        device, dtype = self.o.device, self.runtime.dtype
-        out = torch.empty((tokens, self.nq * self.e), dtype=dtype, device=device)
+        out = self.rows_of_sequences(ctx, "heads", q.shape[0], self.nq * self.e, self.runtime.dtype)
         table = ctx.block_tables[cache.group]
         arguments = self._tile_plan()
         if self._plain_scores():

@@ -164,7 +164,7 @@ class LatentAttention(Mixer):
         # the queries in the latent space: q_rows[:, head, :R] = q_plain[head] . W_uk[head]
         torch.bmm(q_plain, self.up_k, out=q_rows[:, :, :R].transpose(0, 1))
         q_rows = q_rows.view(tokens, H * row)
-        mixed = torch.empty((tokens, H * R), dtype=dtype, device=device)
+        mixed = self.rows_of_sequences(ctx, "mixed", tokens, H * R, dtype)
         table = ctx.block_tables[cache.group]
         arguments = self._tile_plan()
         if not arguments:

@@ -131,13 +131,14 @@ class Runtime:
     def is_bf16(self) -> bool:
         return self.dtype is torch.bfloat16
 
-    def standing_rows(self, rows: int, width: int) -> torch.Tensor:
-        """Rows [rows, width] of this model's own, at one address for a number of rows: zeros to begin with, then what steps left there.  For what
-        is written and read within a layer and leaves rows of recorded steps out.  First asked for outside a recording."""
+    def standing_rows(self, what: str, rows: int, width: int, dtype: torch.dtype) -> torch.Tensor:
+        """Rows [rows, width] of this model's own, at one address for a number of rows: zeros to begin with, then what steps left there.  First asked
+        for outside a recording."""
         held = max(16, 1 << (rows - 1).bit_length())
-        if (held, width) not in self._standing:
-            self._standing[held, width] = torch.zeros((held, width), dtype=self.dtype, device=self.device)
-        return self._standing[held, width][:rows]
+        key = (what, held, width, dtype)
+        if key not in self._standing:
+            self._standing[key] = torch.zeros((held, width), dtype=dtype, device=self.device)
+        return self._standing[key][:rows]
 
 
 @dataclass
@@ -316,6 +317,14 @@ class Mixer(Part):
         that product together with its own; `forward_projected(proj, offset, ctx, cache, write_cache)` then goes on from the
         float32 sums `proj`, this mixer's columns beginning at `offset`."""
         return None
+
+    def rows_of_sequences(self, ctx, what: str, rows: int, width: int, dtype: torch.dtype) -> torch.Tensor:
+        """[rows, width] for what is read before this mixer returns and what kernels write for the sequences' rows alone (`what`: one name for each that
+        a mixer has at a time).  A recorded step may have rows beside them.  Products with weights in 4 bits look at all rows' sizes before they
+        choose their operands, so these rows must not be what the memory held before: they are zeros, or what an earlier step computed."""
+        if self.runtime.weight_format != "held" and ctx.fixed_rows:
+            return self.runtime.standing_rows(what, rows, width, dtype)
+        return torch.empty((rows, width), dtype=dtype, device=self.runtime.device)
 
     def step_signature(self, facts: "StepFacts"):
         """What, beyond the shapes of a step, decides which kernels this mixer launches for it and with which

@@ -108,7 +108,7 @@ class Retention(LinearRecurrence):
         rotation = self.position.rotation() if self.position is not None else None
         if rotation is not None and rotation.rotary_dim:
             kernels.rotate_heads_(proj, offset, 2 * H, d, self.position.rotations(ctx), rotation.rotary_dim)
-        o = torch.empty((tokens, H * e), dtype=torch.float32, device=device)
+        o = self.rows_of_sequences(ctx, "heads", tokens, H * e, torch.float32)
         kernels.linear_scan(proj, offset, k_at, v_at, self.decay, None, self.matrix_state(cache), None, ctx.positions, ctx.q_start,
                             ctx.state_slots, o, None, H, d, e, write_state=write_cache)
         normed = torch.empty((tokens, H * e), dtype=self.runtime.dtype, device=device)
@@ -152,11 +152,11 @@ class MatrixMemory(LinearRecurrence):
         matrix, slots = H * d * e, cache.state.shape[0]
         n_state = cache.state[:, matrix:matrix + H * d].view(slots, H, d)
         m_state = cache.state[:, matrix + H * d:]
-        coef = torch.empty((tokens, 3 * H), dtype=torch.float32, device=device)
+        coef = self.rows_of_sequences(ctx, "gates", tokens, 3 * H, torch.float32)
         kernels.memory_gates(proj, i_at, i_at + H, self.i_bias, self.f_bias, self.gate_cap, m_state, ctx.positions, ctx.q_start,
                              ctx.state_slots, coef, write_state=write_cache)
-        o = torch.empty((tokens, H * e), dtype=torch.float32, device=device)
-        c = torch.empty((tokens, H), dtype=torch.float32, device=device)
+        o = self.rows_of_sequences(ctx, "heads", tokens, H * e, torch.float32)
+        c = self.rows_of_sequences(ctx, "normaliser", tokens, H, torch.float32)
         kernels.linear_scan(proj, offset, k_at, v_at, None, coef, self.matrix_state(cache), n_state, ctx.positions, ctx.q_start,
                             ctx.state_slots, o, c, H, d, e, write_state=write_cache)
         normed = torch.empty((tokens, H * e), dtype=self.runtime.dtype, device=device)
@@ -203,7 +203,7 @@ class GatedLinearAttention(LinearRecurrence):
         H, d, e = self.heads, self.d, self.e
         k_at, v_at = offset + H * d, offset + 2 * H * d
         g_at, low_at = v_at + H * e, v_at + 2 * H * e
-        o = torch.empty((tokens, H * e), dtype=torch.float32, device=device)
+        o = self.rows_of_sequences(ctx, "heads", tokens, H * e, torch.float32)
         kernels.channel_scan(proj, offset, k_at, v_at, low_at, self.a_up, self.a_bias, self.tau, self.matrix_state(cache), ctx.positions,
                              ctx.seq_of_token, ctx.q_start, ctx.state_slots, o, H, d, e, write_state=write_cache)
         normed = torch.empty((tokens, H * e), dtype=self.runtime.dtype, device=device)
