@@ -43,7 +43,8 @@ def build_parser() -> argparse.ArgumentParser:
                    help="do not share the cache pages of equal first tokens between requests")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     p.add_argument("--weight-format", choices=["held", "mxfp4"], default="held",
-                   help="mxfp4: projections of attention and dense feed-forwards in 4-bit floating point")
+                   help="mxfp4: projections of grouped-query attention and dense feed-forwards in 4-bit floating point "
+                        "(widths of whole 32s; other matrices stay as they are; prompts get slower unless activations are in 4 bits too)")
     p.add_argument("--activation-format", choices=["held", "mxfp4"], default="held", help="mxfp4: what they read in 4 bits too")
     p.add_argument("--num-pages", type=int, default=None, help="size of the page pool (overrides --kv-mib)")
     p.add_argument("--random-weights", type=int, default=None, metavar="SEED",

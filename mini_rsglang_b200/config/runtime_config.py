@@ -21,6 +21,7 @@ class RuntimeConfig:
     record_mixed_steps: bool = True   # steps with prompt portions are recorded with fixed shapes and replayed
     overlap_steps: bool = True        # a step is queued before the tokens of the step before it have reached the host
     weight_format: str = "held"       # "mxfp4": the projections of grouped-query attention and dense feed-forwards are held in 4 bits
+                                      # (their inputs whole blocks of 32 elements); all other matrices stay as they are
     activation_format: str = "held"   # "mxfp4": what these projections read is brought to 4 bits too
 
     def validate(self) -> None:

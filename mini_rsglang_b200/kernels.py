@@ -2627,7 +2627,8 @@ class Mxfp4:
     mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), for every 32 neighbours of a row one power of two.
 
     `data` uint8 holds the codes [rows, width / 2] (element 2 j in the low half of byte j) and behind them the scales in the tiles
-    that the tensor cores read (`csrc/kernels/mxfp4.cuh`).  `settled` (`settle()`): the matrix was there before anything
+    that the tensor cores read (`csrc/kernels/mxfp4.cuh`).  Scale bytes 253 and 254 stand for values beyond float32: `settle()` refuses
+    them, products of data that is not settled give infinities.  `settled` (`settle()`): the matrix was there before anything
     that is still queued, and nothing writes it any more, so that a product may fetch it while the kernel before still runs;
     `half_exponent` is then the power by which all of it fits halfs exactly, or None."""
 
@@ -2820,8 +2821,8 @@ def mxfp4_tiles(m: int, n: int, k: int, tokens: int, sms: int, meeting: int, sha
 
 def mxfp4_gemm(x: torch.Tensor, weight: Mxfp4, out: torch.Tensor, quantise: bool = False, plan: tuple | None = None) -> None:
     """out[M, N] = x[M, K] . weight[N, K]^T; x bfloat16, weight in 4 bits, sums in float32, `out` bfloat16 or float32.  With `quantise`
-    x's rows are brought to 4 bits first, as `mxfp4_quantise` does.  Up to 8 rows take one kernel, others two, the first of which
-    prepares x in a buffer of its own.  `plan`: another than `mxfp4_plan` only for measurements and tests."""
+    x's rows are brought to 4 bits first, as `mxfp4_quantise` does.  One to 8 rows take one kernel where `mxfp4_plan` says "few" (with
+    `quantise` not for many outputs of large matrices), everything else two, the first of which prepares x in a buffer of its own.  `plan`: another than `mxfp4_plan` only for measurements and tests."""
     global launch_count
     if x.dim() != 2 or out.dim() != 2:
         raise InvalidRequest("mxfp4_gemm: input and output are rows")

@@ -123,7 +123,7 @@ class Runtime:
     device: torch.device
     dtype: torch.dtype           # torch.bfloat16 (serving) or torch.float32 (the 32-bit path)
     page_size: int = 16
-    weight_format: str = "held"        # "mxfp4": projections that can be are held in 4 bits (`parts.linear.projection`)
+    weight_format: str = "held"        # "mxfp4": projections of grouped-query attention and dense feed-forwards are held in 4 bits (`parts.linear.projection`)
     activation_format: str = "held"    # "mxfp4": and read their input in 4 bits
     _standing: dict = field(default_factory=dict, repr=False, compare=False)
 

@@ -42,7 +42,8 @@ class FourBitWeight:
 
 
 def projection(weight: torch.Tensor, runtime) -> "torch.Tensor | FourBitWeight":
-    """A projection's weights [out, in] as the runtime wants them held; `linear` takes either."""
+    """A projection's weights [out, in] as the runtime wants them held; `linear` takes either.  In 4 bits `in` has to be whole blocks of
+    32 elements."""
     if runtime.weight_format == "mxfp4":
         return FourBitWeight(weight, runtime.activation_format == "mxfp4")
     return weight.contiguous()
