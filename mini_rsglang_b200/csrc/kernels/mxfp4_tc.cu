@@ -13,7 +13,7 @@
 //                    power of two a row, from a kernel before (mxfp4.cu), and w becomes halfs times one power of two of the matrix;
 //                    both powers go into the results.  All of it is exact: the few elements that lie too far below a row's largest
 //                    for halfs are added one by one to the sums (lost_products), and where there are too many of them (most_lost),
-//                    or the matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead (a sixth slower).
+//                    or the matrix's scales span more than 36 powers, the whole product is made of bfloat16 instead (4% to a quarter slower).
 //                    24,576 x 4,096 times 2,048 rows: 303 us, 1.36 PFLOP/s; the tensor pipe is busy 78% of the time at the 1.43 GHz that
 //                    the power cap leaves.
 //   both_kernel      x in 4 bits as well: codes of both sides go from shared memory into kind::mxf4 MMAs as they are, scales are copied into
@@ -801,8 +801,8 @@ template <int TOKENS> constexpr size_t parts_smem() {
     return 1024 + (size_t)p_stages<TOKENS>() * (p_halves<TOKENS>() * (P_A_BYTES + p_x_bytes<TOKENS>()) + p_slot_scale_bytes<TOKENS>()) + 256;
 }
 
-// With more elements to add than this for every 16 tokens that have some, these tokens take the products below (64 rows: an element costs 0.6
-// to 1 us, 16 tokens there 18 to 45).
+// With more elements to add than this for every 16 tokens that have some, these tokens take the products below (64 rows: an element costs 0.5
+// to 1 us, 16 tokens there 13 to 48).
 constexpr int LOST_MOST = 32;
 
 // The results of the tokens of a mask (bits of `low` and `high`) whose elements three parts do not hold, from x as it is and codes times their
