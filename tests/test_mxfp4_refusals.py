@@ -110,7 +110,7 @@ def test_few_rows_get_clusters_that_hold_them(m, quantise, monkeypatch):
     lib = mxfp4_kernel_library()
     monkeypatch.setattr(kernels, "mxfp4_library", lambda: lib)
     for n in (1, 100, 3394, 5120, 8193, 18944, 18945, 30000):
-        for k in (*range(32, 1024, 32), *range(1024, 36000, 416), 11296, 12832, 14816, 15392, 17376, 18464, 23072, 30752, 65536, 131072, 131104, 1 << 20):
+        for k in (*range(32, 1024, 32), *range(1024, 36000, 416), 11296, 12832, 14816, 15392, 17376, 18464, 23104, 30752, 65536, 131072, 131104, 1 << 20):
             plan = kernels.mxfp4_plan(m, n, k, quantise, 148)
             if plan[0] == "few":
                 assert 0 < lib.mrs_mxfp4_few_rows_cluster(m, k) <= plan[1], (m, n, k, plan)
